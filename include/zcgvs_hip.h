@@ -54,7 +54,9 @@ enum zcgvs_dtype {
     ZCGVS_DTYPE_F32 = 0,
     ZCGVS_DTYPE_F16 = 1,
     ZCGVS_DTYPE_I8 = 2,
-    ZCGVS_DTYPE_BINARY = 3
+    ZCGVS_DTYPE_BINARY = 3,
+    /* bfloat16: the embedding-model operators only; no store or search takes it */
+    ZCGVS_DTYPE_BF16 = 4
 };
 
 /* How an int8 corpus is scored.
@@ -421,6 +423,65 @@ int zcgvs_search_sketch_state(const zcgvs_search_desc* desc, void* d_workspace, 
  * ---------------------------------------------------------------------------------------- */
 int zcgvs_generate_normalized(float* d_out, int64_t rows, int dim, uint64_t seed,
                               int64_t row_offset, zcgvs_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Embedding-model operators: from token ids to query vectors on the device, and their gradients.
+ * No counterpart in the reference, whose QueryEmbedder runs a model outside its device code
+ * (include/zcgvs/embed/query_embedder.hpp:8-15). A model's call in front of a search:
+ * zcgvs_embedding_lookup (token rows, or the mean of each text's rows), zcgvs_gated_projection,
+ * zcgvs_adapted_projection with float32 output, which is the `queries` of zcgvs_search_topk.
+ *
+ * Types: float32, float16 or bfloat16 operands (ZCGVS_DTYPE_F32 / F16 / BF16). Products and sums are
+ * held in float32 whatever the type; results are rounded once, where they are written. Matrices are
+ * row-major with a row stride in elements (at least the row's length). Rows may start at any address
+ * that is aligned to their element; rows whose address and stride are multiples of 16 bytes take the
+ * faster kernels. The same inputs give the same bits on every call: no result depends on the order of
+ * atomic operations. Outputs must not overlap inputs, except where a function says so.
+ * Like the launchers, these functions are asynchronous on `stream`, allocate nothing, never
+ * synchronize and may be recorded into a HIP graph. Workspaces need no initialization and must not be
+ * shared by calls that can overlap; one of more bytes than asked for is fine.
+ * ---------------------------------------------------------------------------------------- */
+enum zcgvs_embedding_reduce { ZCGVS_EMBEDDING_SUM = 0, ZCGVS_EMBEDDING_MEAN = 1 };
+
+/* A table of token rows and the tokens to look up.
+ * A token counts when its id lies in [0, vocab) and differs from padding_id (-1: no padding id);
+ * any other token stands for a row of zeros and has no gradient.
+ * Without bags, output row j is scale * table[ids[j]]. With bag_offsets, output row r is scale times
+ * the sum (or the mean over the tokens that count) of the rows of tokens bag_offsets[r] ..
+ * bag_offsets[r + 1] - 1; a bag with no token that counts gives zeros. Offsets ascend and lie in
+ * [0, token_count]. */
+typedef struct zcgvs_embedding_desc {
+    const void* table;           /* [vocab, dim] rows of `dtype` (not read by the gradient)      */
+    int64_t table_stride;        /* elements from row to row; 0: dim                             */
+    int vocab;
+    int dim;
+    int dtype;                   /* of the table                                                 */
+    const int* ids;              /* [token_count]                                                */
+    int64_t token_count;         /* at most 2^29                                                 */
+    const int64_t* bag_offsets;  /* [bag_count + 1], or NULL: one output row per token           */
+    int64_t bag_count;           /* at most 2^31 - 1                                             */
+    int reduce;                  /* enum zcgvs_embedding_reduce (with bags)                      */
+    int padding_id;
+    float scale;
+} zcgvs_embedding_desc;
+
+/* d_out [token_count or bag_count, dim]; out_dtype is the table's type or ZCGVS_DTYPE_F32;
+ * out_stride 0: dim. */
+int zcgvs_embedding_lookup(const zcgvs_embedding_desc* desc, void* d_out, int64_t out_stride,
+                           int out_dtype, zcgvs_stream_t stream);
+
+/* The gradient of zcgvs_embedding_lookup with respect to the table, from the gradient of its output
+ * rows (d_out_gradient, of `gradient_dtype`): d_table_gradient[v] = scale * the sum of the output
+ * gradients of v's tokens (with ZCGVS_EMBEDDING_MEAN each over its bag's counting tokens). The tokens
+ * are sorted by id, stably, and each row's terms are added in a fixed grouping of that order.
+ * accumulate == 0: every row of d_table_gradient [vocab, dim] is written, those of tokens that do not
+ * occur with zeros. accumulate != 0: the sums are added to d_table_gradient and only rows of tokens
+ * that occur are touched. table_gradient_dtype is gradient_dtype or ZCGVS_DTYPE_F32. */
+size_t zcgvs_embedding_gradient_workspace_bytes(const zcgvs_embedding_desc* desc);
+int zcgvs_embedding_gradient(const zcgvs_embedding_desc* desc, const void* d_out_gradient,
+                             int64_t out_gradient_stride, int gradient_dtype, void* d_table_gradient,
+                             int64_t table_gradient_stride, int table_gradient_dtype, int accumulate,
+                             void* d_workspace, size_t workspace_bytes, zcgvs_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,8 @@ LIB_PATH = PKG / "lib" / "libzcgvs_hip.so"
 OK, ERR_INVALID_ARGUMENT, ERR_RUNTIME, ERR_HIP, ERR_UNSUPPORTED = 0, 1, 2, 3, 4
 COSINE, DOT, L2 = 0, 1, 2
 F32, F16, I8, BINARY = 0, 1, 2, 3
+BF16 = 4  # the embedding-model operators only
+EMBEDDING_SUM, EMBEDDING_MEAN = 0, 1
 INT8_REFERENCE, INT8_PER_VECTOR = 0, 1
 SEARCH_MATERIALIZE = 1
 SEARCH_UNSORTED_POSTINGS = 2
@@ -55,6 +57,12 @@ class SearchDesc(ctypes.Structure):
                 ("lex_weights", _vp), ("lex_doc_count", _i64), ("lex_vocab_size", _i32), ("query_terms", _vp),
                 ("lexical_stride", _i32), ("dense_weight", _f32), ("flags", _i32),
                 ("lex_slice_table", _vp)]
+
+
+class EmbeddingDesc(ctypes.Structure):
+    _fields_ = [("table", _vp), ("table_stride", _i64), ("vocab", _i32), ("dim", _i32), ("dtype", _i32), ("ids", _vp),
+                ("token_count", _i64), ("bag_offsets", _vp), ("bag_count", _i64), ("reduce", _i32),
+                ("padding_id", _i32), ("scale", _f32)]
 
 
 # name -> (restype, argtypes)
@@ -124,6 +132,10 @@ _SIGNATURES = {
     "zcgvs_search_phase_rows": (_i32, [ctypes.POINTER(SearchDesc), ctypes.POINTER(_i64), _i32,
                                        ctypes.POINTER(_i32)]),
     "zcgvs_generate_normalized": (_i32, [_vp, _i64, _i32, _u64, _i64, _vp]),
+    "zcgvs_embedding_lookup": (_i32, [ctypes.POINTER(EmbeddingDesc), _vp, _i64, _i32, _vp]),
+    "zcgvs_embedding_gradient_workspace_bytes": (_sz, [ctypes.POINTER(EmbeddingDesc)]),
+    "zcgvs_embedding_gradient": (_i32, [ctypes.POINTER(EmbeddingDesc), _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp,
+                                        _sz, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -512,3 +524,37 @@ def search(desc: SearchDesc, stream=None):
     call("zcgvs_memcpy_d2h", flags.ctypes.data, search_overflow_flags(desc, workspace), flags.nbytes, None)
     synchronize()
     return idx.to_host(), val.to_host(), flags
+
+
+# ---- embedding-model operators -------------------------------------------------------------
+
+def _workspace_bytes(name: str, desc) -> int:
+    size = int(getattr(library(), name)(ctypes.byref(desc)))
+    if size == 0:
+        raise ValueError(last_error())
+    return size
+
+
+def embedding_desc(table, vocab, dim, dtype, ids, token_count, *, bag_offsets=None, bag_count=0, reduce=EMBEDDING_SUM,
+                   padding_id=-1, scale=1.0, table_stride=0) -> EmbeddingDesc:
+    desc = EmbeddingDesc(ptr(table), table_stride, vocab, dim, dtype, ptr(ids), token_count, ptr(bag_offsets), bag_count,
+                         reduce, padding_id, scale)
+    return _keep_alive(desc, table, ids, bag_offsets)
+
+
+def embedding_lookup(desc: EmbeddingDesc, out, out_dtype, *, out_stride=0, stream=None) -> None:
+    """Rows of the token table times the scale, one per token or one per bag of tokens."""
+    call("zcgvs_embedding_lookup", ctypes.byref(desc), ptr(out), out_stride, out_dtype, getattr(stream, "handle", stream))
+
+
+def embedding_gradient_workspace_bytes(desc: EmbeddingDesc) -> int:
+    return _workspace_bytes("zcgvs_embedding_gradient_workspace_bytes", desc)
+
+
+def embedding_gradient(desc: EmbeddingDesc, out_gradient, gradient_dtype, table_gradient, table_gradient_dtype, workspace,
+                       workspace_bytes, *, out_gradient_stride=0, table_gradient_stride=0, accumulate=False,
+                       stream=None) -> None:
+    """The gradient of embedding_lookup with respect to the table."""
+    call("zcgvs_embedding_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, gradient_dtype,
+         ptr(table_gradient), table_gradient_stride, table_gradient_dtype, int(accumulate), ptr(workspace),
+         workspace_bytes, getattr(stream, "handle", stream))

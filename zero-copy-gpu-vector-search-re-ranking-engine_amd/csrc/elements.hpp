@@ -1,0 +1,76 @@
+// Element types of the embedding-model operators (float32, float16, bfloat16) and their checks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "common.hpp"
+
+namespace zcgvs_hip {
+
+inline bool validElement(int dtype) {
+    return dtype == ZCGVS_DTYPE_F32 || dtype == ZCGVS_DTYPE_F16 || dtype == ZCGVS_DTYPE_BF16;
+}
+
+__host__ __device__ constexpr int elementBytes(int dtype) { return dtype == ZCGVS_DTYPE_F32 ? 4 : 2; }
+
+// Calls body(T{}) with the C++ type of a valid element dtype.
+template <typename Body>
+int withElement(int dtype, Body&& body) {
+    switch (dtype) {
+        case ZCGVS_DTYPE_F16:
+            return body(_Float16{});
+        case ZCGVS_DTYPE_BF16:
+            return body(__bf16{});
+        default:
+            return body(float{});
+    }
+}
+
+// Whether rows that start at `base`, `stride` elements apart, can be read `bytes` at a time.
+inline bool alignedRows(const void* base, std::int64_t stride, int dtype, int bytes) {
+    return reinterpret_cast<std::uintptr_t>(base) % static_cast<std::uintptr_t>(bytes) == 0 &&
+           stride * elementBytes(dtype) % bytes == 0;
+}
+
+// kCount neighbouring elements as one load or store of the vector's natural size.
+template <typename T, int kCount>
+struct Pack {
+    typedef T type __attribute__((ext_vector_type(kCount)));
+};
+template <typename T>
+struct Pack<T, 1> {
+    typedef T type;
+};
+
+template <typename T, int kCount>
+__device__ __forceinline__ void loadPack(const T* from, float (&to)[kCount]) {
+    if constexpr (kCount == 1) {
+        to[0] = static_cast<float>(*from);
+    } else {
+        const auto v = *reinterpret_cast<const typename Pack<T, kCount>::type*>(from);
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            to[e] = static_cast<float>(v[e]);
+        }
+    }
+}
+
+// Rounds to nearest even where T is narrower than float32.
+template <typename T, int kCount>
+__device__ __forceinline__ void storePack(const float (&from)[kCount], T* to) {
+    if constexpr (kCount == 1) {
+        *to = static_cast<T>(from[0]);
+    } else {
+        typename Pack<T, kCount>::type v;
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            v[e] = static_cast<T>(from[e]);
+        }
+        *reinterpret_cast<typename Pack<T, kCount>::type*>(to) = v;
+    }
+}
+
+}  // namespace zcgvs_hip

@@ -1,0 +1,887 @@
+// Token-table lookup with scaling and pooling, and its gradient by sorted tokens.
+//
+// Lookup. out[r] = scale * w_r * sum of table[id] over the tokens of row r that count; w_r is 1, or
+// 1 / (the number of those tokens) for the mean. Nothing is computed that a copy would not need, so
+// the kernels are bound by memory: the rows of the tokens are read and the output is written.
+//
+// Gradient. d_table[v] = scale * sum of w_r(j) * d_out[r(j)] over the tokens j with id v. A scatter
+// with atomics would add in an order that changes from run to run and queue up on frequent tokens (the
+// most frequent token of a text holds several percent of all positions); here the positions are sorted
+// by id (a stable radix sort), runs of equal ids are summed in the order of the positions, in chunks
+// of a fixed length, and the chunks' partial sums of a run that crosses chunks are joined in order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "elements.hpp"
+
+namespace zcgvs_hip {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWavesPerBlock = kThreads / kWave;
+constexpr std::int64_t kMaxTokens = 1 << 29;          // sorted positions and chunks fit 32 bits
+constexpr long long kMaxBlocks = (1ll << 24) - 1;     // a launch has less than 2^32 threads
+
+__device__ __forceinline__ bool counts(int id, int vocab, int padding_id) {
+    return id >= 0 && id < vocab && id != padding_id;
+}
+
+// ---- lookup, one output row per token ---------------------------------------------------------
+
+// Output rows are cut into packs of kPack elements; a block writes kLookupPacks * 256 consecutive
+// packs of the whole output, each thread kLookupPacks of them with their loads in flight together.
+constexpr int kLookupPacks = 4;
+
+template <typename In, typename Out, int kPack>
+__global__ __launch_bounds__(kThreads) void lookupKernel(const In* __restrict__ table, std::int64_t table_stride,
+                                                         int vocab, int packs_per_row, const int* __restrict__ ids,
+                                                         long long packs, int padding_id, float scale,
+                                                         Out* __restrict__ out, std::int64_t out_stride) {
+    const long long first = static_cast<long long>(blockIdx.x) * (kThreads * kLookupPacks);
+    const long long first_row = first / packs_per_row;
+    const unsigned first_pack = static_cast<unsigned>(first - first_row * packs_per_row);
+    const int left = static_cast<int>(min(packs - first, static_cast<long long>(kThreads * kLookupPacks)));
+    float value[kLookupPacks][kPack];
+#pragma unroll
+    for (int u = 0; u < kLookupPacks; ++u) {
+        const int i = u * kThreads + static_cast<int>(threadIdx.x);
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            value[u][e] = 0.0f;
+        }
+        if (i < left) {
+            const unsigned at = first_pack + static_cast<unsigned>(i);
+            const unsigned row = at / static_cast<unsigned>(packs_per_row);
+            const unsigned pack = at - row * static_cast<unsigned>(packs_per_row);
+            const int id = ids[first_row + row];
+            if (counts(id, vocab, padding_id)) {
+                loadPack(table + id * table_stride + static_cast<std::int64_t>(pack) * kPack, value[u]);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kLookupPacks; ++u) {
+        const int i = u * kThreads + static_cast<int>(threadIdx.x);
+        if (i < left) {
+            const unsigned at = first_pack + static_cast<unsigned>(i);
+            const unsigned row = at / static_cast<unsigned>(packs_per_row);
+            const unsigned pack = at - row * static_cast<unsigned>(packs_per_row);
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                value[u][e] *= scale;
+            }
+            storePack(value[u], out + (first_row + row) * out_stride + static_cast<std::int64_t>(pack) * kPack);
+        }
+    }
+}
+
+// ---- lookup with bags -------------------------------------------------------------------------
+
+// A block pools one bag's columns of a slice: kBagColumns lanes side by side hold the slice's packs,
+// the block's 256 / kBagColumns groups of lanes take the bag's tokens in turn (kBagAhead of them in
+// flight each), and their sums are joined through LDS in the order of the groups.
+constexpr int kBagColumns = 32;
+constexpr int kBagGroups = kThreads / kBagColumns;
+constexpr int kBagAhead = 4;
+
+template <typename In, typename Out, int kPack>
+__global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ table, std::int64_t table_stride,
+                                                      int vocab, int packs_per_row, const int* __restrict__ ids,
+                                                      long long token_count,
+                                                      const std::int64_t* __restrict__ bag_offsets, int slices,
+                                                      bool mean, int padding_id, float scale, Out* __restrict__ out,
+                                                      std::int64_t out_stride) {
+    __shared__ float sums[kBagGroups][kBagColumns * kPack];
+    __shared__ int found[kBagGroups];
+    const long long bag = blockIdx.x / static_cast<unsigned>(slices);
+    const int slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(bag) * static_cast<unsigned>(slices));
+    const int column = threadIdx.x % kBagColumns;
+    const int group = threadIdx.x / kBagColumns;
+    const int pack = slice * kBagColumns + column;
+    const long long begin = min(max(static_cast<long long>(bag_offsets[bag]), 0ll), token_count);
+    const long long end = min(static_cast<long long>(bag_offsets[bag + 1]), token_count);
+    const In* from = table + static_cast<std::int64_t>(pack) * kPack;
+    const bool has_pack = pack < packs_per_row;
+
+    float sum[kPack] = {};
+    int count = 0;
+    for (long long j = begin + group; j < end; j += kBagGroups * kBagAhead) {
+        float value[kBagAhead][kPack];
+#pragma unroll
+        for (int u = 0; u < kBagAhead; ++u) {
+            const long long at = j + u * kBagGroups;
+            const int id = at < end ? ids[at] : -1;
+            const bool ok = at < end && counts(id, vocab, padding_id);
+            count += ok ? 1 : 0;
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                value[u][e] = 0.0f;
+            }
+            if (ok && has_pack) {
+                loadPack(from + id * table_stride, value[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBagAhead; ++u) {
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                sum[e] += value[u][e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kPack; ++e) {
+        sums[group][column * kPack + e] = sum[e];
+    }
+    if (column == 0) {
+        found[group] = count;
+    }
+    __syncthreads();
+    if (group == 0 && has_pack) {
+        int total = count;
+        for (int g = 1; g < kBagGroups; ++g) {
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                sum[e] += sums[g][column * kPack + e];
+            }
+            total += found[g];
+        }
+        const float weight = mean && total > 1 ? scale / static_cast<float>(total) : scale;
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            sum[e] *= weight;
+        }
+        storePack(sum, out + bag * out_stride + static_cast<std::int64_t>(pack) * kPack);
+    }
+}
+
+// ---- sorting the tokens -----------------------------------------------------------------------
+
+// Stable least-significant-digit radix sort of (id, output row) pairs, at most kDigitBits bits a pass.
+// A tile is a run of items that one block counts and then scatters, kSortItems at a time; there are at
+// most kMaxTiles tiles, so that the scatter can add up the counts of the tiles before it by itself (one
+// thread per digit, rows of the count table are contiguous): two launches a pass.
+// A token that does not count has the id `vocab`, past every row of the table.
+constexpr int kDigitBits = 9;
+constexpr int kDigits = 1 << kDigitBits;
+constexpr int kSortItems = 1024;
+constexpr int kSortRounds = kSortItems / kThreads;
+constexpr int kMaxTiles = 256;
+
+struct SortPass {
+    const int* keys_in;
+    const int* rows_in;  // null: the position itself
+    int* keys_out;
+    int* rows_out;
+    unsigned* tile_counts;  // [tiles, kDigits]
+    int count;
+    int tile_items;  // a multiple of kSortItems
+    int tiles;
+    int shift;
+    int bits;
+    int vocab;
+    int padding_id;
+    bool raw;  // keys_in holds token ids, not yet checked
+};
+
+__device__ __forceinline__ int sortKey(const SortPass& pass, int i) {
+    const int key = pass.keys_in[i];
+    return !pass.raw || counts(key, pass.vocab, pass.padding_id) ? key : pass.vocab;
+}
+
+__global__ __launch_bounds__(kThreads) void sortCountKernel(SortPass pass) {
+    __shared__ unsigned histogram[kDigits];
+    for (int d = threadIdx.x; d < kDigits; d += kThreads) {
+        histogram[d] = 0;
+    }
+    __syncthreads();
+    const int begin = static_cast<int>(blockIdx.x) * pass.tile_items;
+    const int end = min(begin + pass.tile_items, pass.count);
+    const unsigned mask = (1u << pass.bits) - 1u;
+    for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
+        atomicAdd(&histogram[(static_cast<unsigned>(sortKey(pass, i)) >> pass.shift) & mask], 1u);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < kDigits; d += kThreads) {
+        pass.tile_counts[static_cast<std::size_t>(blockIdx.x) * kDigits + d] = histogram[d];
+    }
+}
+
+// Orders a wavefront's LDS accesses before and after it.
+__device__ __forceinline__ void waveFence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Exclusive prefix sum over the block's threads; every thread of the block calls it.
+__device__ __forceinline__ unsigned blockPrefix(unsigned value, unsigned* wave_sums) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+    unsigned prefix = value;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const unsigned below = __shfl_up(prefix, d, kWave);
+        prefix += lane >= d ? below : 0u;
+    }
+    if (lane == kWave - 1) {
+        wave_sums[wave] = prefix;
+    }
+    __syncthreads();
+    unsigned base = 0;
+    for (int w = 0; w < wave; ++w) {
+        base += wave_sums[w];
+    }
+    __syncthreads();
+    return base + prefix - value;
+}
+
+// Places the items of [begin, end) stably behind start[digit], which it moves on. Every thread of the
+// block calls it; `start` and `wave_counts` are in LDS.
+template <typename Key, typename Emit>
+__device__ __forceinline__ void placeItems(int begin, int end, int shift, int bits, unsigned* start,
+                                           unsigned (*wave_counts)[kDigits], Key&& key_of, Emit&& emit) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+    const unsigned mask = (1u << bits) - 1u;
+    for (int base = begin; base < end; base += kSortItems) {
+        for (int d = threadIdx.x; d < kDigits * kWavesPerBlock; d += kThreads) {
+            (&wave_counts[0][0])[d] = 0;
+        }
+        __syncthreads();
+        // a wavefront owns kSortRounds * 64 consecutive items; the rank of an item among its
+        // wavefront's items of the same digit follows from ballots over the digit's bits
+        int key[kSortRounds];
+        unsigned rank[kSortRounds];
+#pragma unroll
+        for (int round = 0; round < kSortRounds; ++round) {
+            const int i = base + (wave * kSortRounds + round) * kWave + lane;
+            const bool ok = i < end;
+            key[round] = ok ? key_of(i) : 0;
+            const unsigned digit = (static_cast<unsigned>(key[round]) >> shift) & mask;
+            unsigned long long same = __ballot(ok);
+            for (int b = 0; b < bits; ++b) {
+                const unsigned long long set = __ballot((digit >> b) & 1u);
+                same &= ((digit >> b) & 1u) ? set : ~set;
+            }
+            if (ok) {
+                const unsigned before = wave_counts[wave][digit];
+                waveFence();
+                const int below = __popcll(same & ((1ull << lane) - 1ull));
+                rank[round] = before + static_cast<unsigned>(below);
+                if (below == 0) {
+                    wave_counts[wave][digit] = before + static_cast<unsigned>(__popcll(same));
+                }
+            }
+            waveFence();
+        }
+        __syncthreads();
+        for (int d = threadIdx.x; d < kDigits; d += kThreads) {
+            unsigned at = start[d];
+            for (int w = 0; w < kWavesPerBlock; ++w) {
+                const unsigned here = wave_counts[w][d];
+                wave_counts[w][d] = at;
+                at += here;
+            }
+            start[d] = at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int round = 0; round < kSortRounds; ++round) {
+            const int i = base + (wave * kSortRounds + round) * kWave + lane;
+            if (i < end) {
+                const unsigned digit = (static_cast<unsigned>(key[round]) >> shift) & mask;
+                emit(i, key[round], wave_counts[wave][digit] + rank[round]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void sortScatterKernel(SortPass pass) {
+    __shared__ unsigned start[kDigits];
+    __shared__ unsigned wave_counts[kWavesPerBlock][kDigits];
+    __shared__ unsigned wave_sums[kWavesPerBlock];
+    // digits of smaller value in all tiles, then the same digit in the tiles before this one; thread t
+    // holds the neighbouring digits 2 t and 2 t + 1
+    unsigned total[2] = {0, 0}, before[2] = {0, 0};
+    const uint2* counts_of = reinterpret_cast<const uint2*>(pass.tile_counts) + threadIdx.x;
+#pragma unroll 8
+    for (int t = 0; t < pass.tiles; ++t) {
+        const uint2 c = counts_of[static_cast<std::size_t>(t) * (kDigits / 2)];
+        total[0] += c.x;
+        total[1] += c.y;
+        if (t < static_cast<int>(blockIdx.x)) {
+            before[0] += c.x;
+            before[1] += c.y;
+        }
+    }
+    static_assert(kDigits == 2 * kThreads, "two digits a thread");
+    const unsigned base = blockPrefix(total[0] + total[1], wave_sums);
+    start[2 * threadIdx.x] = base + before[0];
+    start[2 * threadIdx.x + 1] = base + total[0] + before[1];
+    __syncthreads();
+    const int begin = static_cast<int>(blockIdx.x) * pass.tile_items;
+    const int end = min(begin + pass.tile_items, pass.count);
+    placeItems(
+        begin, end, pass.shift, pass.bits, start, wave_counts, [&](int i) { return sortKey(pass, i); },
+        [&](int i, int key, unsigned at) {
+            pass.keys_out[at] = key;
+            pass.rows_out[at] = pass.rows_in == nullptr ? i : pass.rows_in[i];
+        });
+}
+
+// Output row of every token of a bag list, and how many of each bag's tokens count.
+__global__ __launch_bounds__(kThreads) void bagRowsKernel(const int* __restrict__ ids, int count, int vocab,
+                                                          int padding_id,
+                                                          const std::int64_t* __restrict__ bag_offsets, int bags,
+                                                          int* __restrict__ keys, int* __restrict__ rows,
+                                                          unsigned* __restrict__ bag_counts) {
+    const int j = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+    if (j >= count) {
+        return;
+    }
+    // the last bag that starts at or before j
+    int low = -1, high = bags;
+    while (high - low > 1) {
+        const int middle = low + (high - low) / 2;
+        if (bag_offsets[middle] <= j) {
+            low = middle;
+        } else {
+            high = middle;
+        }
+    }
+    const bool ok = low >= 0 && j < bag_offsets[low + 1] && counts(ids[j], vocab, padding_id);
+    keys[j] = ok ? ids[j] : vocab;
+    rows[j] = ok ? low : 0;
+    if (ok) {
+        atomicAdd(bag_counts + low, 1u);  // an integer count: the same in any order
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void clearWordsKernel(unsigned* __restrict__ words, long long count) {
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < count;
+         i += static_cast<long long>(gridDim.x) * kThreads) {
+        words[i] = 0u;
+    }
+}
+
+// ---- gradient ---------------------------------------------------------------------------------
+
+struct GradientArgs {
+    const int* keys;  // sorted
+    const int* rows;
+    int count;
+    int chunk;  // sorted positions a block sums
+    int vocab;
+    int dim;
+    const void* out_gradient;
+    std::int64_t out_gradient_stride;
+    const unsigned* bag_counts;  // null: no mean
+    float scale;
+    void* table_gradient;
+    std::int64_t table_gradient_stride;
+    bool accumulate;
+    float* partials;  // [chunks, 2, dim]: sums of a chunk's first and last run where they cross chunks
+};
+
+template <typename Out, int kPack>
+__device__ __forceinline__ void finishRow(const GradientArgs& args, int key, int column, float (&sum)[kPack]) {
+    Out* to = static_cast<Out*>(args.table_gradient) + key * args.table_gradient_stride + column;
+    float old[kPack] = {};
+    if (args.accumulate) {
+        loadPack(static_cast<const Out*>(to), old);
+    }
+#pragma unroll
+    for (int e = 0; e < kPack; ++e) {
+        sum[e] = sum[e] * args.scale + old[e];
+    }
+    storePack(sum, to);
+}
+
+// A block sums the chunk's rows, thread t the columns kPack * t and on; the ids and rows are uniform.
+constexpr int kGradientAhead = 8;
+
+template <typename In, typename Out, int kPack>
+__global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs args) {
+    const int column = (static_cast<int>(blockIdx.y) * kThreads + static_cast<int>(threadIdx.x)) * kPack;
+    const int begin = static_cast<int>(blockIdx.x) * args.chunk;
+    const int end = min(begin + args.chunk, args.count);
+    if (column >= args.dim) {
+        return;
+    }
+    const In* from = static_cast<const In*>(args.out_gradient) + column;
+    float* partials = args.partials + static_cast<std::size_t>(blockIdx.x) * 2 * args.dim + column;
+    // the run so far began before this chunk
+    bool continued = begin > 0 && args.keys[begin - 1] == args.keys[begin];
+    int current = args.keys[begin];
+    float sum[kPack] = {};
+    for (int j = begin; j < end; j += kGradientAhead) {
+        float value[kGradientAhead][kPack];
+        int key[kGradientAhead];
+#pragma unroll
+        for (int u = 0; u < kGradientAhead; ++u) {
+            const int at = min(j + u, end - 1);
+            key[u] = args.keys[at];
+            const int row = args.rows[at];
+            float weight = 1.0f;
+            if (args.bag_counts != nullptr && key[u] < args.vocab) {
+                weight = 1.0f / static_cast<float>(args.bag_counts[row]);
+            }
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                value[u][e] = 0.0f;
+            }
+            if (key[u] < args.vocab) {
+                loadPack(from + row * args.out_gradient_stride, value[u]);
+            }
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                value[u][e] *= weight;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kGradientAhead; ++u) {
+            if (j + u < end) {
+                if (key[u] != current) {
+                    if (continued) {
+                        storePack(sum, partials);
+                    } else {
+                        finishRow<Out, kPack>(args, current, column, sum);
+                    }
+                    continued = false;
+                    current = key[u];
+#pragma unroll
+                    for (int e = 0; e < kPack; ++e) {
+                        sum[e] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < kPack; ++e) {
+                    sum[e] += value[u][e];
+                }
+            }
+        }
+    }
+    if (current >= args.vocab) {
+        return;  // tokens that do not count stand at the end
+    }
+    if (continued) {
+        storePack(sum, partials);
+    } else if (end < args.count && args.keys[end] == current) {
+        storePack(sum, partials + args.dim);
+    } else {
+        finishRow<Out, kPack>(args, current, column, sum);
+    }
+}
+
+// Joins a run that crosses chunks: the block of the chunk where it begins adds that chunk's last sum
+// and the first sums of the chunks it reaches, four wavefronts taking a quarter of those each.
+template <typename Out>
+__global__ __launch_bounds__(kThreads) void gradientJoinKernel(GradientArgs args) {
+    __shared__ float sums[kWavesPerBlock][kWave];
+    const int chunk = blockIdx.x;
+    const int next = (chunk + 1) * args.chunk;  // the grid ends before the last chunk
+    const int key = args.keys[next - 1];
+    if (key != args.keys[next] || key >= args.vocab) {
+        return;
+    }
+    const int begin = chunk * args.chunk;
+    if (args.keys[begin] == key && begin > 0 && args.keys[begin - 1] == key) {
+        return;  // the run began in an earlier chunk
+    }
+    const int chunks = (args.count + args.chunk - 1) / args.chunk;
+    // the last chunk whose first id is the run's
+    int last = chunk + 1, past = chunks;
+    while (past - last > 1) {
+        const int middle = last + (past - last) / 2;
+        if (args.keys[middle * args.chunk] == key) {
+            last = middle;
+        } else {
+            past = middle;
+        }
+    }
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+    const int column = static_cast<int>(blockIdx.y) * kWave + lane;
+    const int reached = last - chunk;
+    const int share = (reached + kWavesPerBlock - 1) / kWavesPerBlock;
+    const int from = chunk + 1 + wave * share;
+    const int to = min(from + share, last + 1);
+    const std::size_t stride = 2 * static_cast<std::size_t>(args.dim);
+    float sum = 0.0f;
+    if (column < args.dim) {
+        if (wave == 0) {
+            sum = args.partials[chunk * stride + args.dim + column];
+        }
+#pragma unroll 8
+        for (int c = from; c < to; ++c) {
+            sum += args.partials[c * stride + column];
+        }
+    }
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && column < args.dim) {
+        for (int w = 1; w < kWavesPerBlock; ++w) {
+            sum += sums[w][lane];
+        }
+        float one[1] = {sum};
+        finishRow<Out, 1>(args, key, column, one);
+    }
+}
+
+// Zeros for rows [0, vocab) of the gradient, in packs as in the lookup.
+template <typename Out, int kPack>
+__global__ __launch_bounds__(kThreads) void clearRowsKernel(Out* __restrict__ out, std::int64_t stride, long long packs,
+                                                            int packs_per_row) {
+    const float zeros[kPack] = {};
+    const long long first = static_cast<long long>(blockIdx.x) * (kThreads * kLookupPacks);
+    const long long first_row = first / packs_per_row;
+    const unsigned first_pack = static_cast<unsigned>(first - first_row * packs_per_row);
+    const int left = static_cast<int>(min(packs - first, static_cast<long long>(kThreads * kLookupPacks)));
+#pragma unroll
+    for (int u = 0; u < kLookupPacks; ++u) {
+        const int i = u * kThreads + static_cast<int>(threadIdx.x);
+        if (i < left) {
+            const unsigned at = first_pack + static_cast<unsigned>(i);
+            const unsigned row = at / static_cast<unsigned>(packs_per_row);
+            const unsigned pack = at - row * static_cast<unsigned>(packs_per_row);
+            storePack(zeros, out + (first_row + row) * stride + static_cast<std::int64_t>(pack) * kPack);
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+std::int64_t rowStride(std::int64_t stride, int length) { return stride == 0 ? length : stride; }
+
+int invalid(const char* message) {
+    return setError(ZCGVS_ERR_INVALID_ARGUMENT, std::string("zcgvs embedding: ") + message);
+}
+
+// Checks what lookup and gradient share.
+int checkEmbedding(const zcgvs_embedding_desc* desc) {
+    if (desc == nullptr) {
+        return invalid("null descriptor");
+    }
+    if (desc->vocab <= 0 || desc->dim <= 0) {
+        return invalid("vocab and dim must be positive");
+    }
+    if (desc->vocab == INT32_MAX) {
+        return invalid("vocab must be below 2^31 - 1");
+    }
+    if (desc->token_count < 0 || desc->token_count > kMaxTokens) {
+        return invalid("token_count must lie in [0, 2^29]");
+    }
+    if (desc->bag_offsets != nullptr && (desc->bag_count < 0 || desc->bag_count > INT32_MAX)) {
+        return invalid("bag_count must lie in [0, 2^31 - 1]");
+    }
+    if (desc->bag_offsets == nullptr && desc->bag_count > 0) {
+        return invalid("bag_count needs bag_offsets");
+    }
+    if (desc->reduce != ZCGVS_EMBEDDING_SUM && desc->reduce != ZCGVS_EMBEDDING_MEAN) {
+        return invalid("unknown reduction");
+    }
+    if (desc->token_count > 0 && desc->ids == nullptr) {
+        return invalid("null token ids");
+    }
+    return ZCGVS_OK;
+}
+
+// The widest pack (16 bytes of the wider type at most) that both sides' rows allow: 4 or 1 elements.
+int packElements(int dim, const void* a, std::int64_t a_stride, int a_dtype, const void* b, std::int64_t b_stride,
+                 int b_dtype) {
+    return dim % 4 == 0 && alignedRows(a, a_stride, a_dtype, 4 * elementBytes(a_dtype)) &&
+                   alignedRows(b, b_stride, b_dtype, 4 * elementBytes(b_dtype))
+               ? 4
+               : 1;
+}
+
+template <typename In, typename Out, int kPack>
+int lookupTyped(const zcgvs_embedding_desc& d, Out* out, std::int64_t out_stride, hipStream_t stream) {
+    const In* table = static_cast<const In*>(d.table);
+    const std::int64_t table_stride = rowStride(d.table_stride, d.dim);
+    const int packs_per_row = d.dim / kPack;
+    if (d.bag_offsets == nullptr) {
+        const long long packs = static_cast<long long>(d.token_count) * packs_per_row;
+        const long long blocks = (packs + kThreads * kLookupPacks - 1) / (kThreads * kLookupPacks);
+        if (blocks > kMaxBlocks) {
+            return invalid("more output than one launch can write");
+        }
+        lookupKernel<In, Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            table, table_stride, d.vocab, packs_per_row, d.ids, packs, d.padding_id, d.scale, out, out_stride);
+    } else {
+        const int slices = (packs_per_row + kBagColumns - 1) / kBagColumns;
+        const std::int64_t most = std::max<std::int64_t>(1, kMaxBlocks / slices);
+        for (std::int64_t bag = 0; bag < d.bag_count; bag += most) {
+            const unsigned bags = static_cast<unsigned>(std::min<std::int64_t>(most, d.bag_count - bag));
+            bagKernel<In, Out, kPack><<<bags * static_cast<unsigned>(slices), kThreads, 0, stream>>>(
+                table, table_stride, d.vocab, packs_per_row, d.ids, d.token_count, d.bag_offsets + bag, slices,
+                d.reduce == ZCGVS_EMBEDDING_MEAN, d.padding_id, d.scale, out + bag * out_stride, out_stride);
+        }
+    }
+    ZCGVS_LAUNCH_CHECK("embedding lookup");
+    return ZCGVS_OK;
+}
+
+// Parts of the gradient's workspace, 256-byte aligned.
+struct GradientSpace {
+    std::size_t keys[2];
+    std::size_t rows[2];
+    std::size_t tile_counts;
+    std::size_t bag_counts;
+    std::size_t partials;
+    std::size_t bytes;
+    int chunk;
+    int tile_items;
+    int tiles;
+};
+
+GradientSpace gradientSpace(const zcgvs_embedding_desc& d) {
+    GradientSpace s{};
+    std::size_t at = 0;
+    auto take = [&](std::size_t bytes) {
+        const std::size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const std::size_t n = static_cast<std::size_t>(d.token_count);
+    // enough chunks for the whole GPU where there are few tokens; long enough to read on beyond
+    s.chunk = 64;
+    while (s.chunk > 8 && n / static_cast<std::size_t>(s.chunk) < 1024) {
+        s.chunk /= 2;
+    }
+    const std::size_t tile = (n + kMaxTiles - 1) / kMaxTiles;
+    s.tile_items = static_cast<int>(std::max<std::size_t>(1, (tile + kSortItems - 1) / kSortItems)) * kSortItems;
+    s.tiles = static_cast<int>((n + static_cast<std::size_t>(s.tile_items) - 1) / static_cast<std::size_t>(s.tile_items));
+    for (int side = 0; side < 2; ++side) {
+        s.keys[side] = take(n * 4);
+        s.rows[side] = take(n * 4);
+    }
+    s.tile_counts = take(static_cast<std::size_t>(kMaxTiles) * kDigits * 4);
+    s.bag_counts = take(d.bag_offsets != nullptr ? static_cast<std::size_t>(d.bag_count) * 4 : 0);
+    const std::size_t chunks = (n + static_cast<std::size_t>(s.chunk) - 1) / static_cast<std::size_t>(s.chunk);
+    s.partials = take(chunks * 2 * static_cast<std::size_t>(d.dim) * 4);
+    s.bytes = std::max<std::size_t>(at, 256);
+    return s;
+}
+
+unsigned clearBlocks(long long words) {
+    return static_cast<unsigned>(std::max(1ll, std::min(2048ll, (words + kThreads - 1) / kThreads)));
+}
+
+// Sorts the tokens; *keys and *rows are where the sorted pairs stand.
+int sortTokens(const zcgvs_embedding_desc& d, const GradientSpace& s, char* workspace, const int** keys,
+               const int** rows, hipStream_t stream) {
+    const int n = static_cast<int>(d.token_count);
+    int* key_buffer[2] = {reinterpret_cast<int*>(workspace + s.keys[0]), reinterpret_cast<int*>(workspace + s.keys[1])};
+    int* row_buffer[2] = {reinterpret_cast<int*>(workspace + s.rows[0]), reinterpret_cast<int*>(workspace + s.rows[1])};
+    SortPass pass{};
+    pass.keys_in = d.ids;
+    pass.raw = true;
+    if (d.bag_offsets != nullptr) {
+        unsigned* bag_counts = reinterpret_cast<unsigned*>(workspace + s.bag_counts);
+        clearWordsKernel<<<clearBlocks(d.bag_count), kThreads, 0, stream>>>(bag_counts, d.bag_count);
+        ZCGVS_LAUNCH_CHECK("embedding gradient");
+        bagRowsKernel<<<static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
+            d.ids, n, d.vocab, d.padding_id, d.bag_offsets, static_cast<int>(d.bag_count), key_buffer[0], row_buffer[0],
+            bag_counts);
+        ZCGVS_LAUNCH_CHECK("embedding gradient");
+        pass.keys_in = key_buffer[0];
+        pass.rows_in = row_buffer[0];
+        pass.raw = false;
+    }
+    pass.tile_counts = reinterpret_cast<unsigned*>(workspace + s.tile_counts);
+    pass.count = n;
+    pass.tile_items = s.tile_items;
+    pass.tiles = s.tiles;
+    pass.vocab = d.vocab;
+    pass.padding_id = d.padding_id;
+    int bits = 1;
+    while ((static_cast<long long>(d.vocab) >> bits) != 0) {
+        ++bits;
+    }
+    const int passes = (bits + kDigitBits - 1) / kDigitBits;
+    const int per_pass = (bits + passes - 1) / passes;
+    int side = 1;
+    for (int p = 0; p < passes; ++p) {
+        pass.shift = p * per_pass;
+        pass.bits = std::min(per_pass, bits - pass.shift);
+        pass.keys_out = key_buffer[side];
+        pass.rows_out = row_buffer[side];
+        sortCountKernel<<<static_cast<unsigned>(s.tiles), kThreads, 0, stream>>>(pass);
+        ZCGVS_LAUNCH_CHECK("embedding gradient");
+        sortScatterKernel<<<static_cast<unsigned>(s.tiles), kThreads, 0, stream>>>(pass);
+        ZCGVS_LAUNCH_CHECK("embedding gradient");
+        pass.keys_in = pass.keys_out;
+        pass.rows_in = pass.rows_out;
+        pass.raw = false;
+        side ^= 1;
+    }
+    *keys = pass.keys_in;
+    *rows = pass.rows_in;
+    return ZCGVS_OK;
+}
+
+template <typename In, typename Out, int kPack>
+int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, GradientArgs args, hipStream_t stream) {
+    if (!args.accumulate) {
+        const int packs_per_row = d.dim / kPack;
+        const long long packs = static_cast<long long>(d.vocab) * packs_per_row;
+        const long long blocks = (packs + kThreads * kLookupPacks - 1) / (kThreads * kLookupPacks);
+        if (blocks > kMaxBlocks) {
+            return invalid("more output than one launch can write");
+        }
+        clearRowsKernel<Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
+            static_cast<Out*>(args.table_gradient), args.table_gradient_stride, packs, packs_per_row);
+        ZCGVS_LAUNCH_CHECK("embedding gradient");
+    }
+    if (args.count == 0) {
+        return ZCGVS_OK;
+    }
+    const int chunks = static_cast<int>((static_cast<long long>(args.count) + s.chunk - 1) / s.chunk);
+    const unsigned columns = static_cast<unsigned>((d.dim + kThreads * kPack - 1) / (kThreads * kPack));
+    gradientChunkKernel<In, Out, kPack><<<dim3(static_cast<unsigned>(chunks), columns), kThreads, 0, stream>>>(args);
+    ZCGVS_LAUNCH_CHECK("embedding gradient");
+    if (chunks > 1) {
+        const unsigned slices = static_cast<unsigned>((d.dim + kWave - 1) / kWave);
+        gradientJoinKernel<Out><<<dim3(static_cast<unsigned>(chunks - 1), slices), kThreads, 0, stream>>>(args);
+        ZCGVS_LAUNCH_CHECK("embedding gradient");
+    }
+    return ZCGVS_OK;
+}
+
+}  // namespace
+
+}  // namespace zcgvs_hip
+
+using namespace zcgvs_hip;
+
+extern "C" {
+
+int zcgvs_embedding_lookup(const zcgvs_embedding_desc* desc, void* d_out, std::int64_t out_stride, int out_dtype,
+                           zcgvs_stream_t stream) {
+    const int status = checkEmbedding(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_embedding_desc& d = *desc;
+    if (!validElement(d.dtype)) {
+        return invalid("the table must hold float32, float16 or bfloat16");
+    }
+    if (out_dtype != d.dtype && out_dtype != ZCGVS_DTYPE_F32) {
+        return invalid("the output type is the table's or float32");
+    }
+    const std::int64_t stride = rowStride(out_stride, d.dim);
+    const std::int64_t table_stride = rowStride(d.table_stride, d.dim);
+    if (stride < d.dim || table_stride < d.dim) {
+        return invalid("a row stride is smaller than dim");
+    }
+    const std::int64_t rows = d.bag_offsets != nullptr ? d.bag_count : d.token_count;
+    if (rows == 0) {
+        return clearError();
+    }
+    if (d.table == nullptr || d_out == nullptr) {
+        return invalid("null device pointer");
+    }
+    const int pack = packElements(d.dim, d.table, table_stride, d.dtype, d_out, stride, out_dtype);
+    const int launched = withElement(d.dtype, [&](auto in) {
+        using In = decltype(in);
+        return withElement(out_dtype, [&](auto element) {
+            using Out = decltype(element);
+            if constexpr (std::is_same_v<Out, In> || std::is_same_v<Out, float>) {
+                return pack == 4 ? lookupTyped<In, Out, 4>(d, static_cast<Out*>(d_out), stride, toStream(stream))
+                                 : lookupTyped<In, Out, 1>(d, static_cast<Out*>(d_out), stride, toStream(stream));
+            } else {
+                return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above
+            }
+        });
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+std::size_t zcgvs_embedding_gradient_workspace_bytes(const zcgvs_embedding_desc* desc) {
+    if (checkEmbedding(desc) != ZCGVS_OK) {
+        return 0;
+    }
+    clearError();
+    return gradientSpace(*desc).bytes;
+}
+
+int zcgvs_embedding_gradient(const zcgvs_embedding_desc* desc, const void* d_out_gradient,
+                             std::int64_t out_gradient_stride, int gradient_dtype, void* d_table_gradient,
+                             std::int64_t table_gradient_stride, int table_gradient_dtype, int accumulate,
+                             void* d_workspace, std::size_t workspace_bytes, zcgvs_stream_t stream) {
+    const int status = checkEmbedding(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_embedding_desc& d = *desc;
+    if (!validElement(gradient_dtype)) {
+        return invalid("the output gradient must hold float32, float16 or bfloat16");
+    }
+    if (table_gradient_dtype != gradient_dtype && table_gradient_dtype != ZCGVS_DTYPE_F32) {
+        return invalid("the table gradient's type is the output gradient's or float32");
+    }
+    const std::int64_t from_stride = rowStride(out_gradient_stride, d.dim);
+    const std::int64_t to_stride = rowStride(table_gradient_stride, d.dim);
+    if (from_stride < d.dim || to_stride < d.dim) {
+        return invalid("a row stride is smaller than dim");
+    }
+    const bool no_tokens = d.token_count == 0 || (d.bag_offsets != nullptr && d.bag_count == 0);
+    if (no_tokens && accumulate != 0) {
+        return clearError();
+    }
+    if (d_table_gradient == nullptr || (!no_tokens && d_out_gradient == nullptr)) {
+        return invalid("null device pointer");
+    }
+    const GradientSpace space = gradientSpace(d);
+    if (!no_tokens && (d_workspace == nullptr || workspace_bytes < space.bytes)) {
+        return invalid("the workspace is too small");
+    }
+    if (!no_tokens && !aligned16(d_workspace)) {
+        return invalid("the workspace must be aligned to 16 bytes");
+    }
+    char* workspace = static_cast<char*>(d_workspace);
+    GradientArgs args{};
+    if (!no_tokens) {
+        const int sorted = sortTokens(d, space, workspace, &args.keys, &args.rows, toStream(stream));
+        if (sorted != ZCGVS_OK) {
+            return sorted;
+        }
+        args.partials = reinterpret_cast<float*>(workspace + space.partials);
+    }
+    args.count = no_tokens ? 0 : static_cast<int>(d.token_count);
+    args.chunk = space.chunk;
+    args.vocab = d.vocab;
+    args.dim = d.dim;
+    args.out_gradient = d_out_gradient;
+    args.out_gradient_stride = from_stride;
+    args.bag_counts = d.bag_offsets != nullptr && d.reduce == ZCGVS_EMBEDDING_MEAN
+                          ? reinterpret_cast<const unsigned*>(workspace + space.bag_counts)
+                          : nullptr;
+    args.scale = d.scale;
+    args.table_gradient = d_table_gradient;
+    args.table_gradient_stride = to_stride;
+    args.accumulate = accumulate != 0;
+    const int pack = packElements(d.dim, d_out_gradient, from_stride, gradient_dtype, d_table_gradient, to_stride,
+                                  table_gradient_dtype);
+    const int launched = withElement(gradient_dtype, [&](auto in) {
+        using In = decltype(in);
+        return withElement(table_gradient_dtype, [&](auto element) {
+            using Out = decltype(element);
+            if constexpr (std::is_same_v<Out, In> || std::is_same_v<Out, float>) {
+                return pack == 4 ? gradientTyped<In, Out, 4>(d, space, args, toStream(stream))
+                                 : gradientTyped<In, Out, 1>(d, space, args, toStream(stream));
+            } else {
+                return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above
+            }
+        });
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+}  // extern "C"
