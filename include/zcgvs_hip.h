@@ -483,6 +483,42 @@ int zcgvs_embedding_gradient(const zcgvs_embedding_desc* desc, const void* d_out
                              int64_t table_gradient_stride, int table_gradient_dtype, int accumulate,
                              void* d_workspace, size_t workspace_bytes, zcgvs_stream_t stream);
 
+/* Activations of the gated block: x * sigmoid(x); x * Phi(x) with the normal distribution function
+ * Phi; and the latter's usual tanh approximation 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))). */
+enum zcgvs_activation { ZCGVS_ACT_SILU = 0, ZCGVS_ACT_GELU = 1, ZCGVS_ACT_GELU_TANH = 2 };
+
+/* The gated half of a feed-forward block: out = act(x gate^T) * (x up^T), both products, the
+ * activation and the product in one kernel. All matrices hold `dtype`. */
+typedef struct zcgvs_gated_desc {
+    const void* x;         /* [rows, dim]                                                  */
+    int64_t x_stride;      /* 0: dim                                                       */
+    const void* gate;      /* [hidden, dim]                                                */
+    const void* up;        /* [hidden, dim]; one [2 hidden, dim] matrix may hold both       */
+    int64_t weight_stride; /* of gate and up; 0: dim                                       */
+    int64_t rows;          /* at most 2^30                                                 */
+    int dim;
+    int hidden;
+    int dtype;
+    int activation;        /* enum zcgvs_activation                                        */
+} zcgvs_gated_desc;
+
+/* d_out [rows, hidden] of desc->dtype; out_stride 0: hidden. */
+int zcgvs_gated_projection(const zcgvs_gated_desc* desc, void* d_out, int64_t out_stride,
+                           zcgvs_stream_t stream);
+
+/* The gradient of zcgvs_gated_projection. With g = x gate^T and u = x up^T (computed again, nothing of
+ * the forward pass is kept): dg = d_out * u * act'(g), du = d_out * act(g), and
+ *     x_gradient [rows, dim] = dg gate + du up,
+ *     gate_gradient [hidden, dim] = dg^T x,   up_gradient [hidden, dim] = du^T x,
+ * all of desc->dtype. dg and du are rounded to desc->dtype between the products, as tensors of a model
+ * of that type are. x_gradient may be NULL (not wanted), and so may gate_gradient and up_gradient, both
+ * together. A stride of 0 is the row's length; gate_gradient and up_gradient share theirs. */
+size_t zcgvs_gated_gradient_workspace_bytes(const zcgvs_gated_desc* desc);
+int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradient,
+                         int64_t out_gradient_stride, void* d_x_gradient, int64_t x_gradient_stride,
+                         void* d_gate_gradient, void* d_up_gradient, int64_t weight_gradient_stride,
+                         void* d_workspace, size_t workspace_bytes, zcgvs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

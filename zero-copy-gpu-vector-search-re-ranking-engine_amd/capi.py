@@ -21,6 +21,7 @@ COSINE, DOT, L2 = 0, 1, 2
 F32, F16, I8, BINARY = 0, 1, 2, 3
 BF16 = 4  # the embedding-model operators only
 EMBEDDING_SUM, EMBEDDING_MEAN = 0, 1
+ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2
 INT8_REFERENCE, INT8_PER_VECTOR = 0, 1
 SEARCH_MATERIALIZE = 1
 SEARCH_UNSORTED_POSTINGS = 2
@@ -63,6 +64,11 @@ class EmbeddingDesc(ctypes.Structure):
     _fields_ = [("table", _vp), ("table_stride", _i64), ("vocab", _i32), ("dim", _i32), ("dtype", _i32), ("ids", _vp),
                 ("token_count", _i64), ("bag_offsets", _vp), ("bag_count", _i64), ("reduce", _i32),
                 ("padding_id", _i32), ("scale", _f32)]
+
+
+class GatedDesc(ctypes.Structure):
+    _fields_ = [("x", _vp), ("x_stride", _i64), ("gate", _vp), ("up", _vp), ("weight_stride", _i64), ("rows", _i64),
+                ("dim", _i32), ("hidden", _i32), ("dtype", _i32), ("activation", _i32)]
 
 
 # name -> (restype, argtypes)
@@ -136,6 +142,9 @@ _SIGNATURES = {
     "zcgvs_embedding_gradient_workspace_bytes": (_sz, [ctypes.POINTER(EmbeddingDesc)]),
     "zcgvs_embedding_gradient": (_i32, [ctypes.POINTER(EmbeddingDesc), _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp,
                                         _sz, _vp]),
+    "zcgvs_gated_projection": (_i32, [ctypes.POINTER(GatedDesc), _vp, _i64, _vp]),
+    "zcgvs_gated_gradient_workspace_bytes": (_sz, [ctypes.POINTER(GatedDesc)]),
+    "zcgvs_gated_gradient": (_i32, [ctypes.POINTER(GatedDesc), _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _sz, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -557,4 +566,26 @@ def embedding_gradient(desc: EmbeddingDesc, out_gradient, gradient_dtype, table_
     """The gradient of embedding_lookup with respect to the table."""
     call("zcgvs_embedding_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, gradient_dtype,
          ptr(table_gradient), table_gradient_stride, table_gradient_dtype, int(accumulate), ptr(workspace),
+         workspace_bytes, getattr(stream, "handle", stream))
+
+
+def gated_desc(x, rows, dim, gate, up, hidden, dtype, activation, *, x_stride=0, weight_stride=0) -> GatedDesc:
+    return _keep_alive(GatedDesc(ptr(x), x_stride, ptr(gate), ptr(up), weight_stride, rows, dim, hidden, dtype,
+                                 activation), x, gate, up)
+
+
+def gated_projection(desc: GatedDesc, out, *, out_stride=0, stream=None) -> None:
+    """act(x gate^T) * (x up^T)."""
+    call("zcgvs_gated_projection", ctypes.byref(desc), ptr(out), out_stride, getattr(stream, "handle", stream))
+
+
+def gated_gradient_workspace_bytes(desc: GatedDesc) -> int:
+    return _workspace_bytes("zcgvs_gated_gradient_workspace_bytes", desc)
+
+
+def gated_gradient(desc: GatedDesc, out_gradient, x_gradient, gate_gradient, up_gradient, workspace, workspace_bytes, *,
+                   out_gradient_stride=0, x_gradient_stride=0, weight_gradient_stride=0, stream=None) -> None:
+    """The gradients of gated_projection (x_gradient, or both weight gradients, may be None)."""
+    call("zcgvs_gated_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, ptr(x_gradient),
+         x_gradient_stride, ptr(gate_gradient), ptr(up_gradient), weight_gradient_stride, ptr(workspace),
          workspace_bytes, getattr(stream, "handle", stream))

@@ -28,6 +28,14 @@ __device__ __forceinline__ void copyToLds(const void* src, std::uint32_t lds_bas
                  : "memory");
 }
 
+// The same copy for data that other workgroups read too: no non-temporal hint.
+__device__ __forceinline__ void copySharedToLds(const void* src, std::uint32_t lds_base) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(src), "{m0}"(lds_base)
+                 : "memory");
+}
+
 // The same copy from a wave-uniform base address (SGPR pair) plus a per-lane 32-bit byte
 // offset, so no 64-bit address arithmetic runs per lane.
 __device__ __forceinline__ void copyToLds(const void* uniform_base, std::uint32_t lane_offset,

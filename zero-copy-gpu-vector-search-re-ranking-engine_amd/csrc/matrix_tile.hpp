@@ -1,0 +1,369 @@
+// Tiled matrix products on the matrix cores for the embedding-model operators.
+//
+// A workgroup forms a kM x kN tile of C[m, n] = sum_k A[m, k] B[n, k] in float32 accumulators. Each side
+// comes in one of two layouts: rows whose k are neighbours ("plain": the activations and weights of
+// a forward product), or k-rows whose m (or n) are neighbours ("turned": what the gradients contract).
+// A stage is 128 bytes of k a row (64 16-bit or 32 float32 values); two stages are in LDS, one being
+// read by the matrix cores while the next arrives.
+//
+// LDS layout. A plain side's row r takes 128 bytes; its 16-byte chunk c stands in slot
+// c ^ ((r >> 1) & 7), so that the 16 rows of one ds_read_b128 fall on 16 different 16-byte columns of
+// the 256 bytes that the 64 banks hold. A turned side's k-row takes its m (or n) in order, in granules
+// whose place is exchanged by the k-row's number (16-bit: 32-byte granules, read by
+// ds_read_b64_tr_b16, which hands lane i of 16 the column i of four k-rows; float32: 64-byte ones,
+// read a value at a time: their matrix instructions take sixteen times as long per value).
+//
+// Matrix instructions. 16-bit: v_mfma_f32_16x16x32, float32: v_mfma_f32_16x16x4. The first operand
+// holds B's rows and the second A's, so that lane l of a 16 x 16 result has the four neighbouring columns
+// n = 4 (l / 16) + e of row m = l % 16 and can store them together. Lane group h = l / 16 holds the
+// 16 bytes of chunk 4 t + h in step t, on both sides: every k meets itself whatever the order.
+//
+// Bounds. Rows past a side's end are read again from its last row (plain) or as zeros (turned); they
+// only reach results that are not stored. k past the end is read as zeros on both sides.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.hpp"
+#include "elements.hpp"
+#include "lds_copy.hpp"
+
+namespace zcgvs_hip {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kStageBytes = 128;  // of k in a plain side's row
+constexpr int kStageSteps = 2;    // matrix instruction steps of 64 bytes of k
+
+template <typename T>
+constexpr int kStageK = kStageBytes / static_cast<int>(sizeof(T));
+template <typename T>
+constexpr int kChunk = 16 / static_cast<int>(sizeof(T));  // values in 16 bytes
+
+template <typename T>
+struct Fragment {
+    typedef T type __attribute__((ext_vector_type(kChunk<T>)));
+};
+
+__device__ __forceinline__ f32x4 multiplyAdd(Fragment<_Float16>::type b, Fragment<_Float16>::type a, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(b, a, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 multiplyAdd(Fragment<__bf16>::type b, Fragment<__bf16>::type a, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 multiplyAdd(Fragment<float>::type b, Fragment<float>::type a, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(b[e], a[e], c, 0, 0, 0);
+    }
+    return c;
+}
+
+// What lanes read in the place of k past the end.
+static __device__ const u32x4 zero_chunk = {0u, 0u, 0u, 0u};
+
+// One side of a product: `rows` rows from `base` on, `stride` values apart (turned: `rows` columns of
+// k-rows that are `stride` values apart).
+template <typename T>
+struct MatrixSide {
+    const T* base;
+    std::int64_t stride;
+    int rows;
+};
+
+// Moves one side's stages into LDS: kRows rows of a tile, by a workgroup of kThreads threads.
+// kDirect: 16-byte copies past the registers; rows start at multiples of 16 bytes and hold whole
+// chunks. Otherwise through registers, from any alignment.
+template <typename T, int kRows, bool kTurned, bool kDirect, int kThreads>
+struct StageLoader {
+    static constexpr int kCopies = kRows * (kStageBytes / 16) / kThreads;
+    static constexpr int kBytes = kRows * kStageBytes;
+    static_assert(kCopies >= 1 && kRows * (kStageBytes / 16) % kThreads == 0, "a stage splits over the threads");
+
+    const char* src[kCopies];
+    int at[kCopies];     // k of the copy's first value within a stage
+    int count[kCopies];  // values of the copy that exist (turned)
+    std::int64_t step;   // bytes from stage to stage
+    int k_left;          // from the next stage to load on
+    u32x4 held[kDirect ? 1 : kCopies];
+
+    // row_of(r): the tile's row r of a plain side, at k = 0. A turned side starts at its tile's first column.
+    template <typename RowOf>
+    __device__ __forceinline__ void begin(RowOf&& row_of, std::int64_t stride, int columns, int k_total) {
+        const int tid = static_cast<int>(threadIdx.x);
+        k_left = k_total;
+        step = kTurned ? stride * kStageK<T> * static_cast<std::int64_t>(sizeof(T)) : kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int slot = i * kThreads + tid;
+            if constexpr (kTurned) {
+                constexpr int kSlots = kRows * static_cast<int>(sizeof(T)) / 16;
+                const int k = slot / kSlots;
+                const int chunk = sourceChunk(k, slot % kSlots);
+                at[i] = k;
+                count[i] = min(max(columns - chunk * kChunk<T>, 0), kChunk<T>);
+                src[i] = reinterpret_cast<const char*>(row_of(0) + k * stride + chunk * kChunk<T>);
+            } else {
+                const int row = slot / 8;
+                const int chunk = (slot % 8) ^ ((row >> 1) & 7);
+                at[i] = chunk * kChunk<T>;
+                count[i] = kChunk<T>;
+                src[i] = reinterpret_cast<const char*>(row_of(row) + chunk * kChunk<T>);
+            }
+        }
+    }
+
+    // Which chunk of k-row k stands in `slot` of its LDS row (an exchange, so also the reverse).
+    static __device__ __forceinline__ int sourceChunk(int k, int slot) {
+        if constexpr (sizeof(T) == 2) {
+            return slot ^ (2 * turnOf(k));
+        } else {
+            return slot ^ (4 * turnOf(k));
+        }
+    }
+    static __device__ __forceinline__ int turnOf(int k) {
+        if constexpr (sizeof(T) == 2) {
+            return ((k & 3) | ((k >> 1) & 4)) & (kRows / 16 - 1);
+        } else {
+            return (k >> 2) & 3;
+        }
+    }
+
+    // Starts the next stage's copies into `stage` (direct).
+    __device__ __forceinline__ void issue(const std::uint8_t* stage) {
+        const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+        const std::uint32_t base = ldsAddress(stage);
+        const bool whole = k_left >= kStageK<T>;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const char* from = src[i];
+            if ((!whole && at[i] >= k_left) || (kTurned && count[i] == 0)) {
+                from = reinterpret_cast<const char*>(&zero_chunk);
+            }
+            copySharedToLds(from, __builtin_amdgcn_readfirstlane(base + (i * kThreads + wave * kWave) * 16));
+            src[i] += step;
+        }
+        k_left -= kStageK<T>;
+    }
+
+    // Reads the next stage into registers, and later writes it to `stage` (not direct).
+    __device__ __forceinline__ void fetch() {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int valid = kTurned ? (at[i] < k_left ? count[i] : 0) : k_left - at[i];
+            if (valid >= kChunk<T>) {
+                __builtin_memcpy(&held[i], src[i], 16);
+            } else {
+                typename Fragment<T>::type v = {};
+                const T* from = reinterpret_cast<const T*>(src[i]);
+#pragma unroll
+                for (int e = 0; e < kChunk<T>; ++e) {
+                    if (e < valid) {
+                        v[e] = from[e];
+                    }
+                }
+                held[i] = __builtin_bit_cast(u32x4, v);
+            }
+            src[i] += step;
+        }
+        k_left -= kStageK<T>;
+    }
+    __device__ __forceinline__ void put(std::uint8_t* stage) const {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            *reinterpret_cast<u32x4*>(stage + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+        }
+    }
+
+    // The calling lane's fragment of rows 16 block .. 16 block + 15 in step t.
+    static __device__ __forceinline__ typename Fragment<T>::type read(const std::uint8_t* stage, int block, int t) {
+        const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+        const int r16 = lane & 15;
+        const int h = lane >> 4;
+        if constexpr (!kTurned) {
+            const int slot = (4 * t + h) ^ ((r16 >> 1) & 7);
+            return *reinterpret_cast<const typename Fragment<T>::type*>(stage + (16 * block + r16) * kStageBytes +
+                                                                        16 * slot);
+        } else if constexpr (sizeof(T) == 2) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* LdsPointer;
+            const int k = 32 * t + 8 * h + (r16 >> 2);
+            const std::uint32_t offset =
+                static_cast<std::uint32_t>(k * kRows * 2 + ((block ^ turnOf(k)) * 32) + (r16 & 3) * 8);
+            const std::uint32_t address = ldsAddress(stage) + offset;
+            const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(address));
+            const s16x4 high =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(address + 4 * kRows * 2));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            const s16x8 both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(typename Fragment<T>::type, both);
+        } else {
+            typename Fragment<T>::type v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = 16 * t + 4 * h + e;
+                v[e] = *reinterpret_cast<const float*>(stage + k * kRows * 4 + ((block ^ turnOf(k)) * 64) + r16 * 4);
+            }
+            return v;
+        }
+    }
+};
+
+// A tile's shape: kM x kN by kWavesM x kWavesN wavefronts, each (kM / kWavesM) x (kN / kWavesN).
+template <typename Element, int kTileM, int kTileN, int kSplitM, int kSplitN, bool kTurnedA, bool kTurnedB,
+          bool kDirectLoads>
+struct MatrixTile {
+    using T = Element;
+    static constexpr int kM = kTileM;
+    static constexpr int kN = kTileN;
+    static constexpr int kWavesM = kSplitM;
+    static constexpr int kWavesN = kSplitN;
+    static constexpr int kThreads = kWavesM * kWavesN * kWave;
+    static constexpr int kBlocksM = kM / kWavesM / 16;
+    static constexpr int kBlocksN = kN / kWavesN / 16;
+    static constexpr bool kDirect = kDirectLoads;
+    using SideA = StageLoader<T, kM, kTurnedA, kDirect, kThreads>;
+    using SideB = StageLoader<T, kN, kTurnedB, kDirect, kThreads>;
+    static constexpr int kLdsBytes = 2 * (SideA::kBytes + SideB::kBytes);
+
+    using Sums = f32x4[kBlocksM][kBlocksN];
+
+    static __device__ __forceinline__ int waveId() {
+        return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    }
+    static __device__ __forceinline__ int waveM() { return waveId() / kWavesN; }
+    static __device__ __forceinline__ int waveN() { return waveId() % kWavesN; }
+
+    static __device__ __forceinline__ void clear(Sums& sums) {
+#pragma unroll
+        for (int i = 0; i < kBlocksM; ++i) {
+#pragma unroll
+            for (int j = 0; j < kBlocksN; ++j) {
+                sums[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void multiplyStage(const std::uint8_t* stage, Sums& sums) {
+        const std::uint8_t* stage_b = stage + SideA::kBytes;
+        const int block_m = waveM() * kBlocksM;
+        const int block_n = waveN() * kBlocksN;
+#pragma unroll
+        for (int t = 0; t < kStageSteps; ++t) {
+            typename Fragment<T>::type a[kBlocksM], b[kBlocksN];
+#pragma unroll
+            for (int i = 0; i < kBlocksM; ++i) {
+                a[i] = SideA::read(stage, block_m + i, t);
+            }
+#pragma unroll
+            for (int j = 0; j < kBlocksN; ++j) {
+                b[j] = SideB::read(stage_b, block_n + j, t);
+            }
+#pragma unroll
+            for (int i = 0; i < kBlocksM; ++i) {
+#pragma unroll
+                for (int j = 0; j < kBlocksN; ++j) {
+                    sums[i][j] = multiplyAdd(b[j], a[i], sums[i][j]);
+                }
+            }
+        }
+    }
+
+    // Adds the tile's products over k to `sums`. Every thread of the workgroup calls it; `lds` holds
+    // kLdsBytes. Ends at a barrier: the LDS may be used for something else at once.
+    template <typename RowA, typename RowB>
+    static __device__ __forceinline__ void accumulate(std::uint8_t* lds, RowA&& row_a, std::int64_t stride_a,
+                                                      int columns_a, RowB&& row_b, std::int64_t stride_b, int columns_b,
+                                                      int k_total, Sums& sums) {
+        SideA a;
+        SideB b;
+        a.begin(row_a, stride_a, columns_a, k_total);
+        b.begin(row_b, stride_b, columns_b, k_total);
+        const int stages = (k_total + kStageK<T> - 1) / kStageK<T>;
+        constexpr int kStage = SideA::kBytes + SideB::kBytes;
+        if constexpr (kDirect) {
+            a.issue(lds);
+            b.issue(lds + SideA::kBytes);
+            for (int s = 0; s < stages; ++s) {
+                // this stage's copies have arrived, and every wavefront has read the other one
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                std::uint8_t* here = lds + (s & 1) * kStage;
+                std::uint8_t* next = lds + ((s & 1) ^ 1) * kStage;
+                if (s + 1 < stages) {
+                    a.issue(next);
+                    b.issue(next + SideA::kBytes);
+                }
+                multiplyStage(here, sums);
+            }
+        } else {
+            a.fetch();
+            b.fetch();
+            a.put(lds);
+            b.put(lds + SideA::kBytes);
+            __syncthreads();
+            for (int s = 0; s < stages; ++s) {
+                std::uint8_t* here = lds + (s & 1) * kStage;
+                std::uint8_t* next = lds + ((s & 1) ^ 1) * kStage;
+                if (s + 1 < stages) {
+                    a.fetch();
+                    b.fetch();
+                }
+                multiplyStage(here, sums);
+                if (s + 1 < stages) {
+                    a.put(next);
+                    b.put(next + SideA::kBytes);
+                }
+                __syncthreads();
+            }
+        }
+        if constexpr (kDirect) {
+            __syncthreads();
+        }
+    }
+};
+
+// Tile (m, n) of the launch's block: blocks of one XCD (every eighth one) take neighbouring tiles, in
+// bands of kBandRows tile rows walked column by column, so that an XCD's blocks share rows of both
+// sides in its L2.
+constexpr int kXcds = 8;
+constexpr int kBandRows = 4;
+
+__device__ __forceinline__ void tileOf(int tiles_m, int tiles_n, int& m, int& n) {
+    const int total = tiles_m * tiles_n;
+    const int block = static_cast<int>(blockIdx.x);
+    const int xcd = block % kXcds;
+    const int whole = total / kXcds;
+    const int more = total % kXcds;  // the first `more` XCDs have one block more
+    const int tile = xcd * whole + min(xcd, more) + block / kXcds;
+    const int band_tiles = kBandRows * tiles_n;
+    const int band = tile / band_tiles;
+    const int in_band = tile - band * band_tiles;
+    const int rows = min(kBandRows, tiles_m - band * kBandRows);
+    m = band * kBandRows + in_band % rows;
+    n = in_band / rows;
+}
+
+// Stores four neighbouring results of one row; `left` of them exist. `packed`: rows and their first
+// element allow stores of four.
+template <typename Out>
+__device__ __forceinline__ void storeFour(const f32x4& value, Out* to, int left, bool packed) {
+    if (packed && left >= 4) {
+        const float v[4] = {value[0], value[1], value[2], value[3]};
+        storePack(v, to);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e < left) {
+                to[e] = static_cast<Out>(value[e]);
+            }
+        }
+    }
+}
+
+}  // namespace zcgvs_hip
