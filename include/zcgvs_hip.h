@@ -519,6 +519,39 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
                          void* d_gate_gradient, void* d_up_gradient, int64_t weight_gradient_stride,
                          void* d_workspace, size_t workspace_bytes, zcgvs_stream_t stream);
 
+/* A projection that every row shares, beside low-rank adapters of which each row names one:
+ *     out[r] = x[r] weight^T + scales[a] * (x[r] down[a]^T) up[a]^T,   a = adapter_ids[r].
+ * A row whose id lies outside [0, adapter_count) has no adapter, as have all rows where adapter_ids is
+ * NULL. Of adapter a the first ranks[a] of max_rank rows of down[a] and columns of up[a] count; what
+ * lies beyond is not used. Rows may come in any order; rows of one adapter next to each other (the
+ * tokens of a request) cost least. A row's result does not depend on the other rows' adapters, also
+ * where those hold infinities or NaN. */
+typedef struct zcgvs_adapted_desc {
+    const void* x;          /* [rows, dim]                                                  */
+    int64_t x_stride;       /* 0: dim                                                       */
+    const void* weight;     /* [out_dim, dim]                                               */
+    int64_t weight_stride;  /* 0: dim                                                       */
+    int64_t rows;           /* at most 2^29                                                 */
+    int dim;
+    int out_dim;
+    int dtype;              /* of x, weight, down and up                                    */
+    const void* down;       /* [adapter_count, max_rank, dim]                               */
+    const void* up;         /* [adapter_count, out_dim, max_rank]                           */
+    int adapter_count;
+    int max_rank;           /* at most zcgvs_adapted_max_rank()                             */
+    const int* ranks;       /* [adapter_count], clamped to [0, max_rank]; NULL: max_rank    */
+    const float* scales;    /* [adapter_count]; NULL: 1                                     */
+    const int* adapter_ids; /* [rows]; NULL: no adapters (down and up are not read)         */
+} zcgvs_adapted_desc;
+
+int zcgvs_adapted_max_rank(void); /* 128 */
+/* d_out [rows, out_dim]; out_dtype is desc->dtype or ZCGVS_DTYPE_F32 (the `queries` of a search);
+ * out_stride 0: out_dim. */
+size_t zcgvs_adapted_projection_workspace_bytes(const zcgvs_adapted_desc* desc);
+int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, int64_t out_stride,
+                             int out_dtype, void* d_workspace, size_t workspace_bytes,
+                             zcgvs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

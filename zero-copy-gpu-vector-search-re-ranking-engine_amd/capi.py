@@ -71,6 +71,12 @@ class GatedDesc(ctypes.Structure):
                 ("dim", _i32), ("hidden", _i32), ("dtype", _i32), ("activation", _i32)]
 
 
+class AdaptedDesc(ctypes.Structure):
+    _fields_ = [("x", _vp), ("x_stride", _i64), ("weight", _vp), ("weight_stride", _i64), ("rows", _i64), ("dim", _i32),
+                ("out_dim", _i32), ("dtype", _i32), ("down", _vp), ("up", _vp), ("adapter_count", _i32),
+                ("max_rank", _i32), ("ranks", _vp), ("scales", _vp), ("adapter_ids", _vp)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "zcgvs_last_error": (ctypes.c_char_p, []),
@@ -145,6 +151,9 @@ _SIGNATURES = {
     "zcgvs_gated_projection": (_i32, [ctypes.POINTER(GatedDesc), _vp, _i64, _vp]),
     "zcgvs_gated_gradient_workspace_bytes": (_sz, [ctypes.POINTER(GatedDesc)]),
     "zcgvs_gated_gradient": (_i32, [ctypes.POINTER(GatedDesc), _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _sz, _vp]),
+    "zcgvs_adapted_max_rank": (_i32, []),
+    "zcgvs_adapted_projection_workspace_bytes": (_sz, [ctypes.POINTER(AdaptedDesc)]),
+    "zcgvs_adapted_projection": (_i32, [ctypes.POINTER(AdaptedDesc), _vp, _i64, _i32, _vp, _sz, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -588,4 +597,22 @@ def gated_gradient(desc: GatedDesc, out_gradient, x_gradient, gate_gradient, up_
     """The gradients of gated_projection (x_gradient, or both weight gradients, may be None)."""
     call("zcgvs_gated_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, ptr(x_gradient),
          x_gradient_stride, ptr(gate_gradient), ptr(up_gradient), weight_gradient_stride, ptr(workspace),
+         workspace_bytes, getattr(stream, "handle", stream))
+
+
+def adapted_desc(x, rows, dim, weight, out_dim, dtype, *, x_stride=0, weight_stride=0, down=None, up=None,
+                 adapter_count=0, max_rank=0, ranks=None, scales=None, adapter_ids=None) -> AdaptedDesc:
+    return _keep_alive(AdaptedDesc(ptr(x), x_stride, ptr(weight), weight_stride, rows, dim, out_dim, dtype, ptr(down),
+                                   ptr(up), adapter_count, max_rank, ptr(ranks), ptr(scales), ptr(adapter_ids)),
+                       x, weight, down, up, ranks, scales, adapter_ids)
+
+
+def adapted_projection_workspace_bytes(desc: AdaptedDesc) -> int:
+    return _workspace_bytes("zcgvs_adapted_projection_workspace_bytes", desc)
+
+
+def adapted_projection(desc: AdaptedDesc, out, out_dtype, workspace, workspace_bytes, *, out_stride=0,
+                       stream=None) -> None:
+    """x weight^T plus each row's own low-rank adapter."""
+    call("zcgvs_adapted_projection", ctypes.byref(desc), ptr(out), out_stride, out_dtype, ptr(workspace),
          workspace_bytes, getattr(stream, "handle", stream))

@@ -1,0 +1,567 @@
+// A projection shared by all rows beside low-rank adapters of which each row names one:
+//
+//     out[r] = x[r] weight^T + scale_a (x[r] down_a^T) up_a^T,   a = adapter_ids[r]
+//
+// The rows are sorted by adapter, so that rows of one adapter are next to each other in any batch, and
+// x and out are addressed through the order. `low` = scale_a x[r] down_a^T is formed first, one group of
+// up to 16 rows of one adapter at a time; the projection's kernel then starts each tile's sums with
+// low up_a^T and adds x weight^T on top: one read of x and one write of out for both.
+//
+// low between the two products. The products are the 16-bit matrix instructions', so low is handed over
+// in two parts of the operands' type, high + rest, which keeps 22 (float16) or 16 (bfloat16) bits of it
+// (one part alone would cost a float32 output most of its digits). Each row is scaled by a power of two
+// that brings its largest value to [2^14, 2^15), so that float16 neither overflows nor loses small
+// parts; its inverse is applied to the sums in float32. float32 operands need no parts.
+//
+// Rows are kept apart: a row's sums take the products with its own adapter only, chosen and not
+// multiplied by zero, so infinities and NaN in one adapter stay in its rows.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "common.hpp"
+#include "elements.hpp"
+#include "matrix_tile.hpp"
+#include "pair_sort.hpp"
+
+namespace zcgvs_hip {
+
+namespace {
+
+constexpr int kMaxRank = 128;
+constexpr int kRankStep = 32;  // low's rows are padded to whole steps of the matrix instructions
+
+template <typename T>
+constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+
+int paddedRank(int max_rank) { return (max_rank + kRankStep - 1) / kRankStep * kRankStep; }
+
+struct AdaptedArgs {
+    const void* x;
+    std::int64_t x_stride;
+    const void* weight;
+    std::int64_t weight_stride;
+    int rows;
+    int dim;
+    int out_dim;
+    const void* down;
+    const void* up;
+    int adapter_count;
+    int max_rank;
+    int padded_rank;
+    const int* ranks;
+    const float* scales;
+    const int* adapters;  // [rows] sorted, adapter_count: none; null: no row has one
+    const int* order;     // [rows] the row at each sorted position
+    void* low;            // [rows, parts, padded_rank] by sorted position
+    float* low_scale;     // [rows]
+    int tiles_m;
+    int tiles_n;
+    void* out;
+    std::int64_t out_stride;
+    bool out_packed;
+};
+
+__device__ __forceinline__ int rankOf(const AdaptedArgs& args, int adapter) {
+    return args.ranks == nullptr ? args.max_rank : min(max(args.ranks[adapter], 0), args.max_rank);
+}
+
+// 16 bytes of a row of which `valid` values from `from` on exist; the others are zeros.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::type loadChunk(const T* from, int valid) {
+    typename Fragment<T>::type v = {};
+    if (valid >= kChunk<T>) {
+        __builtin_memcpy(&v, from, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e) {
+            if (e < valid) {
+                v[e] = from[e];
+            }
+        }
+    }
+    return v;
+}
+
+// ---- low = scale x down^T -----------------------------------------------------------------------
+
+// A workgroup looks at kLowPositions sorted positions; each that begins a group (the first of its
+// adapter or of a block of 16) makes it form the group's rows of low. The four wavefronts take a quarter
+// of the steps over dim each and their sums are joined through LDS.
+constexpr int kLowThreads = 256;
+constexpr int kLowWaves = kLowThreads / kWave;
+
+template <typename T, int kRankBlocks>
+__global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int positions) {
+    constexpr int kRanks = kRankBlocks * 16;
+    __shared__ float joined[kLowWaves][16][kRanks];
+    __shared__ float row_peak[16][16];
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int r16 = lane & 15;
+    const int h = lane >> 4;
+    constexpr int kStepK = 4 * kChunk<T>;
+    const int steps = (args.dim + kStepK - 1) / kStepK;
+    const int share = (steps + kLowWaves - 1) / kLowWaves;
+    const int first_position = static_cast<int>(blockIdx.x) * positions;
+    const int past_position = min(first_position + positions, args.rows);
+    for (int p = first_position; p < past_position; ++p) {
+        const int adapter = args.adapters[p];
+        if (adapter >= args.adapter_count) {
+            return;  // rows without an adapter stand at the end
+        }
+        if (p % 16 != 0 && args.adapters[p - 1] == adapter) {
+            continue;
+        }
+        const int most = min(16 - p % 16, args.rows - p);
+        int length = 1;
+        while (length < most && args.adapters[p + length] == adapter) {
+            ++length;
+        }
+        const int rank = rankOf(args, adapter);
+        const T* x = static_cast<const T*>(args.x) + args.order[p + min(r16, length - 1)] * args.x_stride;
+        const T* down = static_cast<const T*>(args.down) +
+                        static_cast<std::int64_t>(adapter) * args.max_rank * args.dim;
+        f32x4 sums[kRankBlocks];
+#pragma unroll
+        for (int j = 0; j < kRankBlocks; ++j) {
+            sums[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int past_step = min((wave + 1) * share, steps);
+        for (int s = wave * share; s < past_step; ++s) {
+            const int k = s * kStepK + h * kChunk<T>;
+            const auto a = loadChunk(x + k, args.dim - k);
+#pragma unroll
+            for (int j = 0; j < kRankBlocks; ++j) {
+                const int r = j * 16 + r16;
+                const auto b = loadChunk(down + static_cast<std::int64_t>(min(r, args.max_rank - 1)) * args.dim + k,
+                                         r < rank ? args.dim - k : 0);
+                sums[j] = multiplyAdd(b, a, sums[j]);
+            }
+        }
+        __syncthreads();  // the last group's sums have been read
+#pragma unroll
+        for (int j = 0; j < kRankBlocks; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                joined[wave][r16][j * 16 + 4 * h + e] = sums[j][e];
+            }
+        }
+        __syncthreads();
+        // 16 threads a row
+        const int row = static_cast<int>(threadIdx.x) / 16;
+        const int column = static_cast<int>(threadIdx.x) % 16;
+        const float scale = args.scales == nullptr ? 1.0f : args.scales[adapter];
+        float value[kRankBlocks];
+        float peak = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kRankBlocks; ++j) {
+            const int r = j * 16 + column;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kLowWaves; ++w) {
+                sum += joined[w][row][r];
+            }
+            value[j] = r < rank ? sum * scale : 0.0f;
+            peak = fmaxf(peak, fabsf(value[j]));
+        }
+        if constexpr (sizeof(T) == 2) {
+            row_peak[row][column] = peak;
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                peak = fmaxf(peak, row_peak[row][c]);
+            }
+        }
+        if (row < length) {
+            const std::int64_t at = p + row;
+            if constexpr (sizeof(T) == 2) {
+                int exponent = 0;
+                if (peak > 0.0f && peak <= 3.402823466e+38f) {
+                    int e = 0;
+                    frexpf(peak, &e);  // peak = m 2^e, m in [0.5, 1)
+                    exponent = min(126, max(-126, 15 - e));
+                }
+                T* to = static_cast<T*>(args.low) + at * 2 * args.padded_rank;
+                const float up_by = ldexpf(1.0f, exponent);
+#pragma unroll
+                for (int j = 0; j < kRankBlocks; ++j) {
+                    const int r = j * 16 + column;
+                    const float scaled = value[j] * up_by;
+                    const T high = static_cast<T>(scaled);
+                    // an infinite value has no rest
+                    const float rest = fabsf(scaled) <= 3.402823466e+38f ? scaled - static_cast<float>(high) : 0.0f;
+                    if (r < args.padded_rank) {
+                        to[r] = high;
+                        to[args.padded_rank + r] = static_cast<T>(rest);
+                    }
+                }
+                for (int r = kRanks + column; r < args.padded_rank; r += 16) {
+                    to[r] = static_cast<T>(0.0f);
+                    to[args.padded_rank + r] = static_cast<T>(0.0f);
+                }
+                if (column == 0) {
+                    args.low_scale[at] = ldexpf(1.0f, -exponent);
+                }
+            } else {
+                float* to = static_cast<float*>(args.low) + at * args.padded_rank;
+#pragma unroll
+                for (int j = 0; j < kRankBlocks; ++j) {
+                    if (j * 16 + column < args.padded_rank) {
+                        to[j * 16 + column] = value[j];
+                    }
+                }
+                for (int r = kRanks + column; r < args.padded_rank; r += 16) {
+                    to[r] = 0.0f;
+                }
+                if (column == 0) {
+                    args.low_scale[at] = 1.0f;
+                }
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            __syncthreads();  // row_peak is written again
+        }
+    }
+}
+
+// ---- the projection -----------------------------------------------------------------------------
+
+// Starts a wavefront's sums with low up^T: one adapter of its rows after the other, for each the
+// products with the 16-row blocks that have rows of it, kept in those rows only.
+template <class Tile>
+__device__ __forceinline__ void addAdapters(const AdaptedArgs& args, int m0, int n0, typename Tile::Sums& sums) {
+    using T = typename Tile::T;
+    constexpr int kStepR = 4 * kChunk<T>;
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int r16 = lane & 15;
+    const int h = lane >> 4;
+    int adapter[Tile::kBlocksM];
+    float scale[Tile::kBlocksM];
+    int left = args.adapter_count;  // the smallest adapter of the wavefront's rows that is not done
+#pragma unroll
+    for (int i = 0; i < Tile::kBlocksM; ++i) {
+        const int p = m0 + i * 16 + r16;
+        adapter[i] = p < args.rows ? args.adapters[p] : args.adapter_count;
+        scale[i] = adapter[i] < args.adapter_count ? args.low_scale[p] : 0.0f;
+        left = min(left, adapter[i]);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        left = min(left, __shfl_xor(left, d, kWave));
+    }
+    left = __builtin_amdgcn_readfirstlane(left);
+    while (left < args.adapter_count) {
+        const int rank = rankOf(args, left);
+        const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(left) * args.out_dim * args.max_rank;
+        f32x4 part[Tile::kBlocksM][Tile::kBlocksN];
+        Tile::clear(part);
+        for (int r = 0; r < rank; r += kStepR) {
+            const int at = r + h * kChunk<T>;
+            typename Fragment<T>::type b[Tile::kBlocksN];
+#pragma unroll
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+                const int n = min(n0 + j * 16 + r16, args.out_dim - 1);
+                b[j] = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + at, rank - at);
+            }
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+                if (__ballot(adapter[i] == left) != 0) {
+                    const std::int64_t p = min(m0 + i * 16 + r16, args.rows - 1);
+#pragma unroll
+                    for (int half = 0; half < kParts<T>; ++half) {
+                        const T* low = static_cast<const T*>(args.low) + (p * kParts<T> + half) * args.padded_rank + at;
+                        const auto a = *reinterpret_cast<const typename Fragment<T>::type*>(low);
+#pragma unroll
+                        for (int j = 0; j < Tile::kBlocksN; ++j) {
+                            part[i][j] = multiplyAdd(b[j], a, part[i][j]);
+                        }
+                    }
+                }
+            }
+        }
+        int next = args.adapter_count;
+#pragma unroll
+        for (int i = 0; i < Tile::kBlocksM; ++i) {
+            const bool mine = adapter[i] == left;
+#pragma unroll
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sums[i][j][e] = mine ? part[i][j][e] * scale[i] : sums[i][j][e];
+                }
+            }
+            next = adapter[i] > left ? min(next, adapter[i]) : next;
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) {
+            next = min(next, __shfl_xor(next, d, kWave));
+        }
+        left = __builtin_amdgcn_readfirstlane(next);
+    }
+}
+
+template <class Tile, typename Out>
+__global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args) {
+    using T = typename Tile::T;
+    __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
+    int tile_m, tile_n;
+    tileOf(args.tiles_m, args.tiles_n, tile_m, tile_n);
+    const int m0 = tile_m * Tile::kM;
+    const int n0 = tile_n * Tile::kN;
+    const T* x = static_cast<const T*>(args.x);
+    const T* weight = static_cast<const T*>(args.weight);
+    const auto row_at = [&](int p) { return args.order == nullptr ? p : args.order[p]; };
+    typename Tile::Sums sums;
+    Tile::clear(sums);
+    if (args.adapters != nullptr) {
+        addAdapters<Tile>(args, m0 + Tile::waveM() * Tile::kBlocksM * 16, n0 + Tile::waveN() * Tile::kBlocksN * 16, sums);
+    }
+    Tile::accumulate(
+        lds, [&](int r) { return x + row_at(min(m0 + r, args.rows - 1)) * args.x_stride; }, args.x_stride, 0,
+        [&](int r) { return weight + min(n0 + r, args.out_dim - 1) * args.weight_stride; }, args.weight_stride, 0,
+        args.dim, sums);
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+#pragma unroll
+    for (int i = 0; i < Tile::kBlocksM; ++i) {
+        const int p = m0 + (Tile::waveM() * Tile::kBlocksM + i) * 16 + (lane & 15);
+        if (p >= args.rows) {
+            continue;
+        }
+        Out* out = static_cast<Out*>(args.out) + row_at(p) * args.out_stride;
+#pragma unroll
+        for (int j = 0; j < Tile::kBlocksN; ++j) {
+            const int n = n0 + (Tile::waveN() * Tile::kBlocksN + j) * 16 + 4 * (lane >> 4);
+            if (n < args.out_dim) {
+                storeFour(sums[i][j], out + n, args.out_dim - n, args.out_packed);
+            }
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+constexpr long long kMaxBlocks = (1ll << 22) - 1;  // a launch has less than 2^32 threads
+
+int invalid(const char* message) {
+    return setError(ZCGVS_ERR_INVALID_ARGUMENT, std::string("zcgvs adapted projection: ") + message);
+}
+
+std::int64_t rowStride(std::int64_t stride, int length) { return stride == 0 ? length : stride; }
+
+int divideUp(std::int64_t a, int b) { return static_cast<int>((a + b - 1) / b); }
+
+bool directRows(const void* base, std::int64_t stride, int length, int dtype) {
+    return alignedRows(base, stride, dtype, 16) && length * elementBytes(dtype) % 16 == 0;
+}
+
+int checkAdapted(const zcgvs_adapted_desc* desc) {
+    if (desc == nullptr) {
+        return invalid("null descriptor");
+    }
+    const zcgvs_adapted_desc& d = *desc;
+    if (!validElement(d.dtype)) {
+        return invalid("the operands must hold float32, float16 or bfloat16");
+    }
+    if (d.dim <= 0 || d.out_dim <= 0) {
+        return invalid("dim and out_dim must be positive");
+    }
+    if (d.dim > (1 << 24) || d.out_dim > (1 << 24)) {
+        return invalid("dim and out_dim must be at most 2^24");
+    }
+    if (d.rows < 0 || d.rows > (1 << 29)) {
+        return invalid("rows must lie in [0, 2^29]");
+    }
+    if (rowStride(d.x_stride, d.dim) < d.dim || rowStride(d.weight_stride, d.dim) < d.dim) {
+        return invalid("a row stride is smaller than dim");
+    }
+    if (d.rows > 0 && (d.x == nullptr || d.weight == nullptr)) {
+        return invalid("null device pointer");
+    }
+    if (d.adapter_ids != nullptr) {
+        if (d.adapter_count < 0 || d.adapter_count == INT32_MAX) {
+            return invalid("adapter_count must lie in [0, 2^31 - 2]");
+        }
+        if (d.adapter_count > 0 && (d.max_rank <= 0 || d.max_rank > kMaxRank)) {
+            return invalid("max_rank must lie in [1, 128]");
+        }
+        if (d.rows > 0 && d.adapter_count > 0 && (d.down == nullptr || d.up == nullptr)) {
+            return invalid("null adapter pointer");
+        }
+    }
+    return ZCGVS_OK;
+}
+
+bool hasAdapters(const zcgvs_adapted_desc& d) { return d.adapter_ids != nullptr && d.adapter_count > 0; }
+
+struct AdaptedSpace {
+    std::size_t sort;
+    std::size_t low;
+    std::size_t low_scale;
+    std::size_t bytes;
+};
+
+AdaptedSpace adaptedSpace(const zcgvs_adapted_desc& d) {
+    AdaptedSpace s{};
+    std::size_t at = 0;
+    if (hasAdapters(d)) {
+        const std::size_t rows = static_cast<std::size_t>(d.rows);
+        const std::size_t parts = d.dtype == ZCGVS_DTYPE_F32 ? 1 : 2;
+        s.sort = at;
+        at += pairSortBytes(rows);
+        s.low = at;
+        at += sortAligned(rows * parts * static_cast<std::size_t>(paddedRank(d.max_rank) * elementBytes(d.dtype)));
+        s.low_scale = at;
+        at += sortAligned(rows * 4);
+    }
+    s.bytes = std::max<std::size_t>(at, 256);
+    return s;
+}
+
+template <typename T>
+int launchLow(const AdaptedArgs& args, hipStream_t stream) {
+    // of many rows most begin no group
+    const int positions = args.rows <= 2048 ? 1 : 4;
+    const unsigned blocks = static_cast<unsigned>(divideUp(args.rows, positions));
+    if (blocks > (1u << 24) - 1u) {
+        return invalid("more rows than one launch can take");
+    }
+    const int rank_blocks = (args.max_rank + 15) / 16;
+    if (rank_blocks <= 1) {
+        lowKernel<T, 1><<<blocks, kLowThreads, 0, stream>>>(args, positions);
+    } else if (rank_blocks <= 2) {
+        lowKernel<T, 2><<<blocks, kLowThreads, 0, stream>>>(args, positions);
+    } else if (rank_blocks <= 4) {
+        lowKernel<T, 4><<<blocks, kLowThreads, 0, stream>>>(args, positions);
+    } else {
+        lowKernel<T, 8><<<blocks, kLowThreads, 0, stream>>>(args, positions);
+    }
+    ZCGVS_LAUNCH_CHECK("adapted projection");
+    return ZCGVS_OK;
+}
+
+template <class Tile, typename Out>
+int launchTile(AdaptedArgs args, hipStream_t stream) {
+    args.tiles_m = divideUp(args.rows, Tile::kM);
+    args.tiles_n = divideUp(args.out_dim, Tile::kN);
+    const long long blocks = static_cast<long long>(args.tiles_m) * args.tiles_n;
+    if (blocks > kMaxBlocks) {
+        return invalid("more output than one launch can write");
+    }
+    adaptedKernel<Tile, Out><<<static_cast<unsigned>(blocks), Tile::kThreads, 0, stream>>>(args);
+    ZCGVS_LAUNCH_CHECK("adapted projection");
+    return ZCGVS_OK;
+}
+
+template <typename T, typename Out>
+int launchAdapted(const AdaptedArgs& args, bool direct, hipStream_t stream) {
+    if (args.adapters != nullptr) {
+        const int status = launchLow<T>(args, stream);
+        if (status != ZCGVS_OK) {
+            return status;
+        }
+    }
+    const long long tiles = static_cast<long long>(divideUp(args.rows, 128)) * divideUp(args.out_dim, 128);
+    if (tiles >= deviceComputeUnits()) {
+        return direct ? launchTile<MatrixTile<T, 128, 128, 2, 2, false, false, true>, Out>(args, stream)
+                      : launchTile<MatrixTile<T, 128, 128, 2, 2, false, false, false>, Out>(args, stream);
+    }
+    return direct ? launchTile<MatrixTile<T, 64, 64, 2, 2, false, false, true>, Out>(args, stream)
+                  : launchTile<MatrixTile<T, 64, 64, 2, 2, false, false, false>, Out>(args, stream);
+}
+
+}  // namespace
+
+}  // namespace zcgvs_hip
+
+using namespace zcgvs_hip;
+
+extern "C" {
+
+int zcgvs_adapted_max_rank(void) { return kMaxRank; }
+
+std::size_t zcgvs_adapted_projection_workspace_bytes(const zcgvs_adapted_desc* desc) {
+    if (checkAdapted(desc) != ZCGVS_OK) {
+        return 0;
+    }
+    clearError();
+    return adaptedSpace(*desc).bytes;
+}
+
+int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::int64_t out_stride, int out_dtype,
+                             void* d_workspace, std::size_t workspace_bytes, zcgvs_stream_t stream) {
+    const int status = checkAdapted(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_adapted_desc& d = *desc;
+    if (out_dtype != d.dtype && out_dtype != ZCGVS_DTYPE_F32) {
+        return invalid("the output type is the operands' or float32");
+    }
+    const std::int64_t stride = rowStride(out_stride, d.out_dim);
+    if (stride < d.out_dim) {
+        return invalid("the output's row stride is smaller than out_dim");
+    }
+    if (d.rows == 0) {
+        return clearError();
+    }
+    if (d_out == nullptr) {
+        return invalid("null device pointer");
+    }
+    const AdaptedSpace space = adaptedSpace(d);
+    if (hasAdapters(d) && (d_workspace == nullptr || workspace_bytes < space.bytes)) {
+        return invalid("the workspace is too small");
+    }
+    if (hasAdapters(d) && !aligned16(d_workspace)) {
+        return invalid("the workspace must be aligned to 16 bytes");
+    }
+    AdaptedArgs args{};
+    args.x = d.x;
+    args.x_stride = rowStride(d.x_stride, d.dim);
+    args.weight = d.weight;
+    args.weight_stride = rowStride(d.weight_stride, d.dim);
+    args.rows = static_cast<int>(d.rows);
+    args.dim = d.dim;
+    args.out_dim = d.out_dim;
+    args.out = d_out;
+    args.out_stride = stride;
+    args.out_packed = alignedRows(d_out, stride, out_dtype, 4 * elementBytes(out_dtype));
+    if (hasAdapters(d)) {
+        char* workspace = static_cast<char*>(d_workspace);
+        args.down = d.down;
+        args.up = d.up;
+        args.adapter_count = d.adapter_count;
+        args.max_rank = d.max_rank;
+        args.padded_rank = paddedRank(d.max_rank);
+        args.ranks = d.ranks;
+        args.scales = d.scales;
+        args.low = workspace + space.low;
+        args.low_scale = reinterpret_cast<float*>(workspace + space.low_scale);
+        SortInput input{};
+        input.keys = d.adapter_ids;
+        input.count = args.rows;
+        input.key_end = d.adapter_count;
+        input.skipped = -1;
+        input.raw = true;
+        const int sorted = sortPairs(input, workspace + space.sort, &args.adapters, &args.order, toStream(stream));
+        if (sorted != ZCGVS_OK) {
+            return sorted;
+        }
+    }
+    const bool direct = directRows(d.x, args.x_stride, d.dim, d.dtype) &&
+                        directRows(d.weight, args.weight_stride, d.dim, d.dtype);
+    const int launched = withElement(d.dtype, [&](auto in) {
+        using T = decltype(in);
+        return withElement(out_dtype, [&](auto element) {
+            using Out = decltype(element);
+            if constexpr (std::is_same_v<Out, T> || std::is_same_v<Out, float>) {
+                return launchAdapted<T, Out>(args, direct, toStream(stream));
+            } else {
+                return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above
+            }
+        });
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@
 
 #include "common.hpp"
 #include "elements.hpp"
+#include "pair_sort.hpp"
 
 namespace zcgvs_hip {
 
@@ -25,10 +26,6 @@ constexpr int kThreads = 256;
 constexpr int kWavesPerBlock = kThreads / kWave;
 constexpr std::int64_t kMaxTokens = 1 << 29;          // sorted positions and chunks fit 32 bits
 constexpr long long kMaxBlocks = (1ll << 24) - 1;     // a launch has less than 2^32 threads
-
-__device__ __forceinline__ bool counts(int id, int vocab, int padding_id) {
-    return id >= 0 && id < vocab && id != padding_id;
-}
 
 // ---- lookup, one output row per token ---------------------------------------------------------
 
@@ -159,180 +156,7 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
     }
 }
 
-// ---- sorting the tokens -----------------------------------------------------------------------
-
-// Stable least-significant-digit radix sort of (id, output row) pairs, at most kDigitBits bits a pass.
-// A tile is a run of items that one block counts and then scatters, kSortItems at a time; there are at
-// most kMaxTiles tiles, so that the scatter can add up the counts of the tiles before it by itself (one
-// thread per digit, rows of the count table are contiguous): two launches a pass.
-// A token that does not count has the id `vocab`, past every row of the table.
-constexpr int kDigitBits = 9;
-constexpr int kDigits = 1 << kDigitBits;
-constexpr int kSortItems = 1024;
-constexpr int kSortRounds = kSortItems / kThreads;
-constexpr int kMaxTiles = 256;
-
-struct SortPass {
-    const int* keys_in;
-    const int* rows_in;  // null: the position itself
-    int* keys_out;
-    int* rows_out;
-    unsigned* tile_counts;  // [tiles, kDigits]
-    int count;
-    int tile_items;  // a multiple of kSortItems
-    int tiles;
-    int shift;
-    int bits;
-    int vocab;
-    int padding_id;
-    bool raw;  // keys_in holds token ids, not yet checked
-};
-
-__device__ __forceinline__ int sortKey(const SortPass& pass, int i) {
-    const int key = pass.keys_in[i];
-    return !pass.raw || counts(key, pass.vocab, pass.padding_id) ? key : pass.vocab;
-}
-
-__global__ __launch_bounds__(kThreads) void sortCountKernel(SortPass pass) {
-    __shared__ unsigned histogram[kDigits];
-    for (int d = threadIdx.x; d < kDigits; d += kThreads) {
-        histogram[d] = 0;
-    }
-    __syncthreads();
-    const int begin = static_cast<int>(blockIdx.x) * pass.tile_items;
-    const int end = min(begin + pass.tile_items, pass.count);
-    const unsigned mask = (1u << pass.bits) - 1u;
-    for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kThreads) {
-        atomicAdd(&histogram[(static_cast<unsigned>(sortKey(pass, i)) >> pass.shift) & mask], 1u);
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kThreads) {
-        pass.tile_counts[static_cast<std::size_t>(blockIdx.x) * kDigits + d] = histogram[d];
-    }
-}
-
-// Orders a wavefront's LDS accesses before and after it.
-__device__ __forceinline__ void waveFence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Exclusive prefix sum over the block's threads; every thread of the block calls it.
-__device__ __forceinline__ unsigned blockPrefix(unsigned value, unsigned* wave_sums) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = threadIdx.x / kWave;
-    unsigned prefix = value;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const unsigned below = __shfl_up(prefix, d, kWave);
-        prefix += lane >= d ? below : 0u;
-    }
-    if (lane == kWave - 1) {
-        wave_sums[wave] = prefix;
-    }
-    __syncthreads();
-    unsigned base = 0;
-    for (int w = 0; w < wave; ++w) {
-        base += wave_sums[w];
-    }
-    __syncthreads();
-    return base + prefix - value;
-}
-
-// Places the items of [begin, end) stably behind start[digit], which it moves on. Every thread of the
-// block calls it; `start` and `wave_counts` are in LDS.
-template <typename Key, typename Emit>
-__device__ __forceinline__ void placeItems(int begin, int end, int shift, int bits, unsigned* start,
-                                           unsigned (*wave_counts)[kDigits], Key&& key_of, Emit&& emit) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = threadIdx.x / kWave;
-    const unsigned mask = (1u << bits) - 1u;
-    for (int base = begin; base < end; base += kSortItems) {
-        for (int d = threadIdx.x; d < kDigits * kWavesPerBlock; d += kThreads) {
-            (&wave_counts[0][0])[d] = 0;
-        }
-        __syncthreads();
-        // a wavefront owns kSortRounds * 64 consecutive items; the rank of an item among its
-        // wavefront's items of the same digit follows from ballots over the digit's bits
-        int key[kSortRounds];
-        unsigned rank[kSortRounds];
-#pragma unroll
-        for (int round = 0; round < kSortRounds; ++round) {
-            const int i = base + (wave * kSortRounds + round) * kWave + lane;
-            const bool ok = i < end;
-            key[round] = ok ? key_of(i) : 0;
-            const unsigned digit = (static_cast<unsigned>(key[round]) >> shift) & mask;
-            unsigned long long same = __ballot(ok);
-            for (int b = 0; b < bits; ++b) {
-                const unsigned long long set = __ballot((digit >> b) & 1u);
-                same &= ((digit >> b) & 1u) ? set : ~set;
-            }
-            if (ok) {
-                const unsigned before = wave_counts[wave][digit];
-                waveFence();
-                const int below = __popcll(same & ((1ull << lane) - 1ull));
-                rank[round] = before + static_cast<unsigned>(below);
-                if (below == 0) {
-                    wave_counts[wave][digit] = before + static_cast<unsigned>(__popcll(same));
-                }
-            }
-            waveFence();
-        }
-        __syncthreads();
-        for (int d = threadIdx.x; d < kDigits; d += kThreads) {
-            unsigned at = start[d];
-            for (int w = 0; w < kWavesPerBlock; ++w) {
-                const unsigned here = wave_counts[w][d];
-                wave_counts[w][d] = at;
-                at += here;
-            }
-            start[d] = at;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int round = 0; round < kSortRounds; ++round) {
-            const int i = base + (wave * kSortRounds + round) * kWave + lane;
-            if (i < end) {
-                const unsigned digit = (static_cast<unsigned>(key[round]) >> shift) & mask;
-                emit(i, key[round], wave_counts[wave][digit] + rank[round]);
-            }
-        }
-        __syncthreads();
-    }
-}
-
-__global__ __launch_bounds__(kThreads) void sortScatterKernel(SortPass pass) {
-    __shared__ unsigned start[kDigits];
-    __shared__ unsigned wave_counts[kWavesPerBlock][kDigits];
-    __shared__ unsigned wave_sums[kWavesPerBlock];
-    // digits of smaller value in all tiles, then the same digit in the tiles before this one; thread t
-    // holds the neighbouring digits 2 t and 2 t + 1
-    unsigned total[2] = {0, 0}, before[2] = {0, 0};
-    const uint2* counts_of = reinterpret_cast<const uint2*>(pass.tile_counts) + threadIdx.x;
-#pragma unroll 8
-    for (int t = 0; t < pass.tiles; ++t) {
-        const uint2 c = counts_of[static_cast<std::size_t>(t) * (kDigits / 2)];
-        total[0] += c.x;
-        total[1] += c.y;
-        if (t < static_cast<int>(blockIdx.x)) {
-            before[0] += c.x;
-            before[1] += c.y;
-        }
-    }
-    static_assert(kDigits == 2 * kThreads, "two digits a thread");
-    const unsigned base = blockPrefix(total[0] + total[1], wave_sums);
-    start[2 * threadIdx.x] = base + before[0];
-    start[2 * threadIdx.x + 1] = base + total[0] + before[1];
-    __syncthreads();
-    const int begin = static_cast<int>(blockIdx.x) * pass.tile_items;
-    const int end = min(begin + pass.tile_items, pass.count);
-    placeItems(
-        begin, end, pass.shift, pass.bits, start, wave_counts, [&](int i) { return sortKey(pass, i); },
-        [&](int i, int key, unsigned at) {
-            pass.keys_out[at] = key;
-            pass.rows_out[at] = pass.rows_in == nullptr ? i : pass.rows_in[i];
-        });
-}
+// ---- gradient: the tokens and their output rows ------------------------------------------------
 
 // Output row of every token of a bag list, and how many of each bag's tokens count.
 __global__ __launch_bounds__(kThreads) void bagRowsKernel(const int* __restrict__ ids, int count, int vocab,
@@ -629,15 +453,13 @@ int lookupTyped(const zcgvs_embedding_desc& d, Out* out, std::int64_t out_stride
 
 // Parts of the gradient's workspace, 256-byte aligned.
 struct GradientSpace {
-    std::size_t keys[2];
-    std::size_t rows[2];
-    std::size_t tile_counts;
+    std::size_t sort;
+    std::size_t bag_keys;
+    std::size_t bag_rows;
     std::size_t bag_counts;
     std::size_t partials;
     std::size_t bytes;
     int chunk;
-    int tile_items;
-    int tiles;
 };
 
 GradientSpace gradientSpace(const zcgvs_embedding_desc& d) {
@@ -654,15 +476,11 @@ GradientSpace gradientSpace(const zcgvs_embedding_desc& d) {
     while (s.chunk > 8 && n / static_cast<std::size_t>(s.chunk) < 1024) {
         s.chunk /= 2;
     }
-    const std::size_t tile = (n + kMaxTiles - 1) / kMaxTiles;
-    s.tile_items = static_cast<int>(std::max<std::size_t>(1, (tile + kSortItems - 1) / kSortItems)) * kSortItems;
-    s.tiles = static_cast<int>((n + static_cast<std::size_t>(s.tile_items) - 1) / static_cast<std::size_t>(s.tile_items));
-    for (int side = 0; side < 2; ++side) {
-        s.keys[side] = take(n * 4);
-        s.rows[side] = take(n * 4);
-    }
-    s.tile_counts = take(static_cast<std::size_t>(kMaxTiles) * kDigits * 4);
-    s.bag_counts = take(d.bag_offsets != nullptr ? static_cast<std::size_t>(d.bag_count) * 4 : 0);
+    const bool bags = d.bag_offsets != nullptr;
+    s.sort = take(pairSortBytes(n));
+    s.bag_keys = take(bags ? n * 4 : 0);
+    s.bag_rows = take(bags ? n * 4 : 0);
+    s.bag_counts = take(bags ? static_cast<std::size_t>(d.bag_count) * 4 : 0);
     const std::size_t chunks = (n + static_cast<std::size_t>(s.chunk) - 1) / static_cast<std::size_t>(s.chunk);
     s.partials = take(chunks * 2 * static_cast<std::size_t>(d.dim) * 4);
     s.bytes = std::max<std::size_t>(at, 256);
@@ -677,53 +495,27 @@ unsigned clearBlocks(long long words) {
 int sortTokens(const zcgvs_embedding_desc& d, const GradientSpace& s, char* workspace, const int** keys,
                const int** rows, hipStream_t stream) {
     const int n = static_cast<int>(d.token_count);
-    int* key_buffer[2] = {reinterpret_cast<int*>(workspace + s.keys[0]), reinterpret_cast<int*>(workspace + s.keys[1])};
-    int* row_buffer[2] = {reinterpret_cast<int*>(workspace + s.rows[0]), reinterpret_cast<int*>(workspace + s.rows[1])};
-    SortPass pass{};
-    pass.keys_in = d.ids;
-    pass.raw = true;
+    SortInput input{};
+    input.keys = d.ids;
+    input.count = n;
+    input.key_end = d.vocab;
+    input.skipped = d.padding_id;
+    input.raw = true;
     if (d.bag_offsets != nullptr) {
         unsigned* bag_counts = reinterpret_cast<unsigned*>(workspace + s.bag_counts);
+        int* bag_keys = reinterpret_cast<int*>(workspace + s.bag_keys);
+        int* bag_rows = reinterpret_cast<int*>(workspace + s.bag_rows);
         clearWordsKernel<<<clearBlocks(d.bag_count), kThreads, 0, stream>>>(bag_counts, d.bag_count);
         ZCGVS_LAUNCH_CHECK("embedding gradient");
         bagRowsKernel<<<static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(
-            d.ids, n, d.vocab, d.padding_id, d.bag_offsets, static_cast<int>(d.bag_count), key_buffer[0], row_buffer[0],
+            d.ids, n, d.vocab, d.padding_id, d.bag_offsets, static_cast<int>(d.bag_count), bag_keys, bag_rows,
             bag_counts);
         ZCGVS_LAUNCH_CHECK("embedding gradient");
-        pass.keys_in = key_buffer[0];
-        pass.rows_in = row_buffer[0];
-        pass.raw = false;
+        input.keys = bag_keys;
+        input.rows = bag_rows;
+        input.raw = false;
     }
-    pass.tile_counts = reinterpret_cast<unsigned*>(workspace + s.tile_counts);
-    pass.count = n;
-    pass.tile_items = s.tile_items;
-    pass.tiles = s.tiles;
-    pass.vocab = d.vocab;
-    pass.padding_id = d.padding_id;
-    int bits = 1;
-    while ((static_cast<long long>(d.vocab) >> bits) != 0) {
-        ++bits;
-    }
-    const int passes = (bits + kDigitBits - 1) / kDigitBits;
-    const int per_pass = (bits + passes - 1) / passes;
-    int side = 1;
-    for (int p = 0; p < passes; ++p) {
-        pass.shift = p * per_pass;
-        pass.bits = std::min(per_pass, bits - pass.shift);
-        pass.keys_out = key_buffer[side];
-        pass.rows_out = row_buffer[side];
-        sortCountKernel<<<static_cast<unsigned>(s.tiles), kThreads, 0, stream>>>(pass);
-        ZCGVS_LAUNCH_CHECK("embedding gradient");
-        sortScatterKernel<<<static_cast<unsigned>(s.tiles), kThreads, 0, stream>>>(pass);
-        ZCGVS_LAUNCH_CHECK("embedding gradient");
-        pass.keys_in = pass.keys_out;
-        pass.rows_in = pass.rows_out;
-        pass.raw = false;
-        side ^= 1;
-    }
-    *keys = pass.keys_in;
-    *rows = pass.rows_in;
-    return ZCGVS_OK;
+    return sortPairs(input, workspace + s.sort, keys, rows, stream);
 }
 
 template <typename In, typename Out, int kPack>
