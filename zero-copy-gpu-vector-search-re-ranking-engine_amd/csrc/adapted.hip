@@ -21,6 +21,7 @@
 
 #include "common.hpp"
 #include "elements.hpp"
+#include "matrix_plan.hpp"
 #include "matrix_tile.hpp"
 #include "pair_sort.hpp"
 
@@ -254,43 +255,47 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, int m0, int
     while (left < args.adapter_count) {
         const int rank = rankOf(args, left);
         const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(left) * args.out_dim * args.max_rank;
-        f32x4 part[Tile::kBlocksM][Tile::kBlocksN];
-        Tile::clear(part);
-        for (int r = 0; r < rank; r += kStepR) {
-            const int at = r + h * kChunk<T>;
-            typename Fragment<T>::type b[Tile::kBlocksN];
+#pragma unroll
+        for (int i = 0; i < Tile::kBlocksM; ++i) {
+            const bool mine = adapter[i] == left;
+            if (__ballot(mine) == 0) {
+                continue;
+            }
+            const std::int64_t p = min(m0 + i * 16 + r16, args.rows - 1);
+            const T* low = static_cast<const T*>(args.low) + p * kParts<T> * args.padded_rank;
+            f32x4 part[Tile::kBlocksN];
 #pragma unroll
             for (int j = 0; j < Tile::kBlocksN; ++j) {
-                const int n = min(n0 + j * 16 + r16, args.out_dim - 1);
-                b[j] = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + at, rank - at);
+                part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
+            for (int r = 0; r < rank; r += kStepR) {
+                const int at = r + h * kChunk<T>;
+                typename Fragment<T>::type a[kParts<T>];
 #pragma unroll
-            for (int i = 0; i < Tile::kBlocksM; ++i) {
-                if (__ballot(adapter[i] == left) != 0) {
-                    const std::int64_t p = min(m0 + i * 16 + r16, args.rows - 1);
+                for (int half = 0; half < kParts<T>; ++half) {
+                    a[half] = *reinterpret_cast<const typename Fragment<T>::type*>(low + half * args.padded_rank + at);
+                }
+#pragma unroll
+                for (int j = 0; j < Tile::kBlocksN; ++j) {
+                    const int n = min(n0 + j * 16 + r16, args.out_dim - 1);
+                    const auto b = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + at, rank - at);
 #pragma unroll
                     for (int half = 0; half < kParts<T>; ++half) {
-                        const T* low = static_cast<const T*>(args.low) + (p * kParts<T> + half) * args.padded_rank + at;
-                        const auto a = *reinterpret_cast<const typename Fragment<T>::type*>(low);
-#pragma unroll
-                        for (int j = 0; j < Tile::kBlocksN; ++j) {
-                            part[i][j] = multiplyAdd(b[j], a, part[i][j]);
-                        }
+                        part[j] = multiplyAdd(b, a[half], part[j]);
                     }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sums[i][j][e] = mine ? part[j][e] * scale[i] : sums[i][j][e];
                 }
             }
         }
         int next = args.adapter_count;
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
-            const bool mine = adapter[i] == left;
-#pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sums[i][j][e] = mine ? part[i][j][e] * scale[i] : sums[i][j][e];
-                }
-            }
             next = adapter[i] > left ? min(next, adapter[i]) : next;
         }
 #pragma unroll
@@ -306,21 +311,24 @@ __global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args
     using T = typename Tile::T;
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;
-    tileOf(args.tiles_m, args.tiles_n, tile_m, tile_n);
+    tileOf(static_cast<int>(blockIdx.x), args.tiles_m, args.tiles_n, tile_m, tile_n);
     const int m0 = tile_m * Tile::kM;
     const int n0 = tile_n * Tile::kN;
     const T* x = static_cast<const T*>(args.x);
     const T* weight = static_cast<const T*>(args.weight);
     const auto row_at = [&](int p) { return args.order == nullptr ? p : args.order[p]; };
+    // the first stage is on its way while the adapters' part is formed
+    typename Tile::Loads loads;
+    loads.begin([&](int r) { return x + row_at(min(m0 + r, args.rows - 1)) * args.x_stride; }, args.x_stride, 0,
+                [&](int r) { return weight + min(n0 + r, args.out_dim - 1) * args.weight_stride; },
+                args.weight_stride, 0, args.dim);
+    loads.start(lds);
     typename Tile::Sums sums;
     Tile::clear(sums);
     if (args.adapters != nullptr) {
         addAdapters<Tile>(args, m0 + Tile::waveM() * Tile::kBlocksM * 16, n0 + Tile::waveN() * Tile::kBlocksN * 16, sums);
     }
-    Tile::accumulate(
-        lds, [&](int r) { return x + row_at(min(m0 + r, args.rows - 1)) * args.x_stride; }, args.x_stride, 0,
-        [&](int r) { return weight + min(n0 + r, args.out_dim - 1) * args.weight_stride; }, args.weight_stride, 0,
-        args.dim, sums);
+    Tile::accumulate(lds, loads, args.dim, sums, [] {});
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
 #pragma unroll
     for (int i = 0; i < Tile::kBlocksM; ++i) {
@@ -341,18 +349,8 @@ __global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args
 
 // ---- host ---------------------------------------------------------------------------------------
 
-constexpr long long kMaxBlocks = (1ll << 22) - 1;  // a launch has less than 2^32 threads
-
 int invalid(const char* message) {
     return setError(ZCGVS_ERR_INVALID_ARGUMENT, std::string("zcgvs adapted projection: ") + message);
-}
-
-std::int64_t rowStride(std::int64_t stride, int length) { return stride == 0 ? length : stride; }
-
-int divideUp(std::int64_t a, int b) { return static_cast<int>((a + b - 1) / b); }
-
-bool directRows(const void* base, std::int64_t stride, int length, int dtype) {
-    return alignedRows(base, stride, dtype, 16) && length * elementBytes(dtype) % 16 == 0;
 }
 
 int checkAdapted(const zcgvs_adapted_desc* desc) {
@@ -454,20 +452,17 @@ int launchTile(AdaptedArgs args, hipStream_t stream) {
 }
 
 template <typename T, typename Out>
-int launchAdapted(const AdaptedArgs& args, bool direct, hipStream_t stream) {
+int launchAdapted(const AdaptedArgs& args, int dtype, bool direct, hipStream_t stream) {
     if (args.adapters != nullptr) {
         const int status = launchLow<T>(args, stream);
         if (status != ZCGVS_OK) {
             return status;
         }
     }
-    const long long tiles = static_cast<long long>(divideUp(args.rows, 128)) * divideUp(args.out_dim, 128);
-    if (tiles >= deviceComputeUnits()) {
-        return direct ? launchTile<MatrixTile<T, 128, 128, 2, 2, false, false, true>, Out>(args, stream)
-                      : launchTile<MatrixTile<T, 128, 128, 2, 2, false, false, false>, Out>(args, stream);
-    }
-    return direct ? launchTile<MatrixTile<T, 64, 64, 2, 2, false, false, true>, Out>(args, stream)
-                  : launchTile<MatrixTile<T, 64, 64, 2, 2, false, false, false>, Out>(args, stream);
+    const ProductPlan plan = planProduct(args.rows, args.out_dim, args.dim, 1, dtype, 0, LargestTile::k128x128);
+    return withTile<T, false, false, LargestTile::k128x128, false>(plan.shape, direct, [&](auto tile) {
+        return launchTile<decltype(tile), Out>(args, stream);
+    });
 }
 
 }  // namespace
@@ -555,7 +550,7 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
         return withElement(out_dtype, [&](auto element) {
             using Out = decltype(element);
             if constexpr (std::is_same_v<Out, T> || std::is_same_v<Out, float>) {
-                return launchAdapted<T, Out>(args, direct, toStream(stream));
+                return launchAdapted<T, Out>(args, d.dtype, direct, toStream(stream));
             } else {
                 return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above
             }

@@ -16,6 +16,7 @@
 
 #include "common.hpp"
 #include "elements.hpp"
+#include "matrix_plan.hpp"
 #include "matrix_tile.hpp"
 
 namespace zcgvs_hip {
@@ -75,6 +76,7 @@ struct GatedArgs {
     // past hidden written as zeros
     const void* out_gradient;
     std::int64_t out_gradient_stride;
+    bool gradient_packed;
     std::int64_t du_offset;
 };
 
@@ -85,64 +87,112 @@ __global__ __launch_bounds__(Tile::kThreads) void gatedKernel(GatedArgs args) {
     constexpr int kWaveN = Tile::kN / Tile::kWavesN;
     constexpr int kHalf = kWaveN / 2;
     constexpr int kPairs = Tile::kBlocksN / 2;
-    int tile_m, tile_n;
-    tileOf(args.tiles_m, args.tiles_n, tile_m, tile_n);
-    const int m0 = tile_m * Tile::kM;
-    const int n0 = tile_n * (Tile::kN / 2);
+    static_assert(Tile::kBlocksN % 2 == 0, "a wavefront's columns are whole blocks of gate and of up rows");
     const T* x = static_cast<const T*>(args.x);
     const T* gate = static_cast<const T*>(args.gate);
     const T* up = static_cast<const T*>(args.up);
-
-    typename Tile::Sums sums;
-    Tile::clear(sums);
-    Tile::accumulate(
-        lds, [&](int r) { return x + min(m0 + r, args.rows - 1) * args.x_stride; }, args.x_stride, 0,
-        [&](int r) {
-            const int j = r % kWaveN;
-            const int n = min(n0 + r / kWaveN * kHalf + j % kHalf, args.hidden - 1);
-            return (j < kHalf ? gate : up) + n * args.weight_stride;
-        },
-        args.weight_stride, 0, args.dim, sums);
-
+    const int total = args.tiles_m * args.tiles_n;
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    typename Tile::Loads loads;
+    auto begin = [&](int index) {
+        int tile_m, tile_n;
+        tileOf(index, args.tiles_m, args.tiles_n, tile_m, tile_n);
+        const int m0 = tile_m * Tile::kM;
+        const int n0 = tile_n * (Tile::kN / 2);
+        loads.begin([&](int r) { return x + min(m0 + r, args.rows - 1) * args.x_stride; }, args.x_stride, 0,
+                    [&](int r) {
+                        const int j = r % kWaveN;
+                        const int n = min(n0 + r / kWaveN * kHalf + j % kHalf, args.hidden - 1);
+                        return (j < kHalf ? gate : up) + n * args.weight_stride;
+                    },
+                    args.weight_stride, 0, args.dim);
+        loads.start(lds);
+    };
+    begin(static_cast<int>(blockIdx.x));
+    for (int index = static_cast<int>(blockIdx.x); index < total; index += static_cast<int>(gridDim.x)) {
+        typename Tile::Sums sums;
+        Tile::clear(sums);
+        Tile::accumulate(lds, loads, args.dim, sums, [&] {
+            if (index + static_cast<int>(gridDim.x) < total) {
+                begin(index + static_cast<int>(gridDim.x));
+            }
+        });
+        int tile_m, tile_n;
+        tileOf(index, args.tiles_m, args.tiles_n, tile_m, tile_n);
+        const int m0 = tile_m * Tile::kM + Tile::waveM() * Tile::kBlocksM * 16 + (lane & 15);
+        const int n0 = tile_n * (Tile::kN / 2) + Tile::waveN() * kHalf + 4 * (lane >> 4);
+        if constexpr (!kGradient) {
 #pragma unroll
-    for (int i = 0; i < Tile::kBlocksM; ++i) {
-        const int m = m0 + (Tile::waveM() * Tile::kBlocksM + i) * 16 + (lane & 15);
-        if (m >= args.rows) {
-            continue;
-        }
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-            const int n = n0 + Tile::waveN() * kHalf + j * 16 + 4 * (lane >> 4);
-            const f32x4 g = sums[i][j];
-            const f32x4 u = sums[i][j + kPairs];
-            T* to = static_cast<T*>(args.out) + m * args.out_stride + n;
-            if constexpr (!kGradient) {
-                if (n < args.hidden) {
-                    f32x4 h;
+                for (int j = 0; j < kPairs; ++j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        h[e] = activate<kActivation>(g[e]) * u[e];
+                        sums[i][j][e] = activate<kActivation>(sums[i][j][e]) * sums[i][j + kPairs][e];
                     }
-                    storeFour(h, to, args.hidden - n, args.out_packed);
                 }
-            } else if (n < args.out_stride) {
-                const T* d = static_cast<const T*>(args.out_gradient) + m * args.out_gradient_stride + n;
-                f32x4 dg, du;
+            }
+            loads.land();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float from = n + e < args.hidden ? static_cast<float>(d[e]) : 0.0f;
-                    float value, slope;
-                    activateBoth<kActivation>(g[e], value, slope);
-                    dg[e] = n + e < args.hidden ? from * u[e] * slope : 0.0f;
-                    du[e] = n + e < args.hidden ? from * value : 0.0f;
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const int m = m0 + i * 16;
+                    const int n = n0 + j * 16;
+                    if (m < args.rows && n < args.hidden) {
+                        storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.hidden - n,
+                                  args.out_packed);
+                    }
                 }
-                storeFour(dg, to, 4, true);
-                storeFour(du, to + args.du_offset, 4, true);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+                const int m = m0 + i * 16;
+                f32x4 from[kPairs];
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const int n = n0 + j * 16;
+                    from[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (m < args.rows && n < args.hidden) {
+                        from[j] = loadFour(static_cast<const T*>(args.out_gradient) + m * args.out_gradient_stride + n,
+                                           args.hidden - n, args.gradient_packed);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const int n = n0 + j * 16;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float value, slope;
+                        activateBoth<kActivation>(sums[i][j][e], value, slope);
+                        // columns past hidden are zeros whatever stands in for their weights
+                        const bool inside = n + e < args.hidden;
+                        sums[i][j][e] = inside ? from[j][e] * sums[i][j + kPairs][e] * slope : 0.0f;
+                        sums[i][j + kPairs][e] = inside ? from[j][e] * value : 0.0f;
+                    }
+                }
+            }
+            loads.land();
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const int m = m0 + i * 16;
+                    const int n = n0 + j * 16;
+                    if (m < args.rows && n < args.out_stride) {
+                        T* to = static_cast<T*>(args.out) + m * args.out_stride + n;
+                        storeFour(sums[i][j], to, 4, true);
+                        storeFour(sums[i][j + kPairs], to + args.du_offset, 4, true);
+                    }
+                }
             }
         }
     }
 }
+
+// A product with too few tiles for the GPU is split over k as well: every split writes float32 partial
+// sums, which joinKernel adds in the order of the splits.
 
 // x_gradient [rows, dim] = dg gate + du up.
 struct InputGradientArgs {
@@ -157,6 +207,9 @@ struct InputGradientArgs {
     int hidden;
     int tiles_m;
     int tiles_n;
+    int splits;      // 1: both products in one; otherwise even, the first half of them for dg gate
+    int split_k;     // values of k of a split
+    float* partials;  // [splits, rows, dim]
     void* out;
     std::int64_t out_stride;
     bool out_packed;
@@ -167,18 +220,32 @@ __global__ __launch_bounds__(Tile::kThreads) void inputGradientKernel(InputGradi
     using T = typename Tile::T;
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;
-    tileOf(args.tiles_m, args.tiles_n, tile_m, tile_n);
+    tileOf(static_cast<int>(blockIdx.x), args.tiles_m, args.tiles_n, tile_m, tile_n);
+    const int split = static_cast<int>(blockIdx.y);
     const int m0 = tile_m * Tile::kM;
     const int n0 = tile_n * Tile::kN;
+    const int half = args.splits / 2;
+    int part = args.splits > 1 && split >= half ? 1 : 0;
+    const int past_part = args.splits > 1 ? part + 1 : 2;
+    const int k0 = args.splits > 1 ? (split - part * half) * args.split_k : 0;
+    const int k_total = args.splits > 1 ? min(args.split_k, args.hidden - k0) : args.hidden;
     typename Tile::Sums sums;
     Tile::clear(sums);
+    typename Tile::Loads loads;
+    const T* d = static_cast<const T*>(args.dg) + (part == 0 ? 0 : args.du_offset) + k0;
+    const T* weight = static_cast<const T*>(part == 0 ? args.gate : args.up) + k0 * args.weight_stride;
+    loads.begin([&](int r) { return d + min(m0 + r, args.rows - 1) * args.d_stride; }, args.d_stride, 0,
+                [&](int) { return weight + n0; }, args.weight_stride, args.dim - n0, k_total);
+    loads.start(lds);
 #pragma unroll 1
-    for (int part = 0; part < 2; ++part) {
-        const T* d = static_cast<const T*>(args.dg) + (part == 0 ? 0 : args.du_offset);
-        const T* weight = static_cast<const T*>(part == 0 ? args.gate : args.up);
-        Tile::accumulate(
-            lds, [&](int r) { return d + min(m0 + r, args.rows - 1) * args.d_stride; }, args.d_stride, 0,
-            [&](int) { return weight + n0; }, args.weight_stride, args.dim - n0, args.hidden, sums);
+    for (; part < past_part; ++part) {
+        Tile::accumulate(lds, loads, k_total, sums, [&] {
+            if (part + 1 < past_part) {
+                loads.moveOn(args.du_offset * static_cast<std::int64_t>(sizeof(T)),
+                             static_cast<const char*>(args.up) - static_cast<const char*>(args.gate), k_total);
+                loads.start(lds);
+            }
+        });
     }
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
 #pragma unroll
@@ -188,8 +255,13 @@ __global__ __launch_bounds__(Tile::kThreads) void inputGradientKernel(InputGradi
         for (int j = 0; j < Tile::kBlocksN; ++j) {
             const int n = n0 + (Tile::waveN() * Tile::kBlocksN + j) * 16 + 4 * (lane >> 4);
             if (m < args.rows && n < args.dim) {
-                storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.dim - n,
-                          args.out_packed);
+                if (args.splits > 1) {
+                    float* to = args.partials + (static_cast<std::int64_t>(split) * args.rows + m) * args.dim + n;
+                    storeFour(sums[i][j], to, args.dim - n, args.dim % 4 == 0);
+                } else {
+                    storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.dim - n,
+                              args.out_packed);
+                }
             }
         }
     }
@@ -207,6 +279,9 @@ struct WeightGradientArgs {
     int hidden;
     int tiles_m;  // of one of the two
     int tiles_n;
+    int splits;
+    int split_k;
+    float* partials;  // [splits, 2, hidden, dim]
     void* gate_out;
     void* up_out;
     std::int64_t out_stride;
@@ -218,18 +293,23 @@ __global__ __launch_bounds__(Tile::kThreads) void weightGradientKernel(WeightGra
     using T = typename Tile::T;
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;
-    tileOf(2 * args.tiles_m, args.tiles_n, tile_m, tile_n);
+    tileOf(static_cast<int>(blockIdx.x), 2 * args.tiles_m, args.tiles_n, tile_m, tile_n);
+    const int split = static_cast<int>(blockIdx.y);
+    const int k0 = split * args.split_k;
+    const int k_total = min(args.split_k, args.rows - k0);
     const bool second = tile_m >= args.tiles_m;
     const int m0 = (second ? tile_m - args.tiles_m : tile_m) * Tile::kM;
     const int n0 = tile_n * Tile::kN;
-    const T* d = static_cast<const T*>(args.dg) + (second ? args.du_offset : 0);
-    const T* x = static_cast<const T*>(args.x);
+    const T* d = static_cast<const T*>(args.dg) + (second ? args.du_offset : 0) + k0 * args.d_stride;
+    const T* x = static_cast<const T*>(args.x) + k0 * args.x_stride;
     typename Tile::Sums sums;
     Tile::clear(sums);
     // the rows of dg and du are padded to whole chunks
-    Tile::accumulate(
-        lds, [&](int) { return d + m0; }, args.d_stride, static_cast<int>(args.d_stride) - m0,
-        [&](int) { return x + n0; }, args.x_stride, args.dim - n0, args.rows, sums);
+    typename Tile::Loads loads;
+    loads.begin([&](int) { return d + m0; }, args.d_stride, static_cast<int>(args.d_stride) - m0,
+                [&](int) { return x + n0; }, args.x_stride, args.dim - n0, k_total);
+    loads.start(lds);
+    Tile::accumulate(lds, loads, k_total, sums, [] {});
     T* out = static_cast<T*>(second ? args.up_out : args.gate_out);
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
 #pragma unroll
@@ -239,27 +319,52 @@ __global__ __launch_bounds__(Tile::kThreads) void weightGradientKernel(WeightGra
         for (int j = 0; j < Tile::kBlocksN; ++j) {
             const int n = n0 + (Tile::waveN() * Tile::kBlocksN + j) * 16 + 4 * (lane >> 4);
             if (m < args.hidden && n < args.dim) {
-                storeFour(sums[i][j], out + m * args.out_stride + n, args.dim - n, args.out_packed);
+                if (args.splits > 1) {
+                    const std::int64_t row = (2 * static_cast<std::int64_t>(split) + (second ? 1 : 0)) * args.hidden + m;
+                    storeFour(sums[i][j], args.partials + row * args.dim + n, args.dim - n, args.dim % 4 == 0);
+                } else {
+                    storeFour(sums[i][j], out + m * args.out_stride + n, args.dim - n, args.out_packed);
+                }
             }
         }
     }
 }
 
-// ---- host ---------------------------------------------------------------------------------------
+// out = the sum of the splits' partials [splits, rows, columns]; rows from `rows_first` on go to `second`.
+constexpr int kJoinThreads = 256;
 
-constexpr long long kMaxBlocks = (1ll << 22) - 1;  // a launch has less than 2^32 threads
+template <typename T, int kPack>
+__global__ __launch_bounds__(kJoinThreads) void joinKernel(const float* __restrict__ partials, int splits,
+                                                           long long rows, int columns, long long rows_first,
+                                                           T* __restrict__ first, T* __restrict__ second,
+                                                           std::int64_t stride) {
+    const long long packs = rows * (columns / kPack);
+    const int packs_per_row = columns / kPack;
+    const long long split_values = rows * columns;
+    for (long long p = static_cast<long long>(blockIdx.x) * kJoinThreads + threadIdx.x; p < packs;
+         p += static_cast<long long>(gridDim.x) * kJoinThreads) {
+        float sum[kPack];
+        loadPack(partials + p * kPack, sum);
+#pragma unroll 4
+        for (int s = 1; s < splits; ++s) {
+            float more[kPack];
+            loadPack(partials + s * split_values + p * kPack, more);
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                sum[e] += more[e];
+            }
+        }
+        const long long row = p / packs_per_row;
+        const int column = static_cast<int>(p - row * packs_per_row) * kPack;
+        T* to = row < rows_first ? first + row * stride : second + (row - rows_first) * stride;
+        storePack(sum, to + column);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
 
 int invalid(const char* message) {
     return setError(ZCGVS_ERR_INVALID_ARGUMENT, std::string("zcgvs gated projection: ") + message);
-}
-
-std::int64_t rowStride(std::int64_t stride, int length) { return stride == 0 ? length : stride; }
-
-int divideUp(std::int64_t a, int b) { return static_cast<int>((a + b - 1) / b); }
-
-// Rows that the 16-byte copies can read: whole aligned chunks.
-bool directRows(const void* base, std::int64_t stride, int length, int dtype) {
-    return alignedRows(base, stride, dtype, 16) && length * elementBytes(dtype) % 16 == 0;
 }
 
 int checkGated(const zcgvs_gated_desc* desc) {
@@ -304,22 +409,6 @@ int withActivation(int activation, Body&& body) {
     }
 }
 
-// Calls body(Tile{}) with the tile for an m x n product: 128 x 128 where that fills the GPU, 64 x 64
-// otherwise; loads past the registers where the rows allow.
-template <typename T, bool kTurnedA, bool kTurnedB, typename Body>
-int withTile(long long tiles_128, bool direct, Body&& body) {
-    if (tiles_128 >= deviceComputeUnits()) {
-        return direct ? body(MatrixTile<T, 128, 128, 2, 2, kTurnedA, kTurnedB, true>{})
-                      : body(MatrixTile<T, 128, 128, 2, 2, kTurnedA, kTurnedB, false>{});
-    }
-    return direct ? body(MatrixTile<T, 64, 64, 2, 2, kTurnedA, kTurnedB, true>{})
-                  : body(MatrixTile<T, 64, 64, 2, 2, kTurnedA, kTurnedB, false>{});
-}
-
-long long tilesOf(std::int64_t m, std::int64_t n, int side) {
-    return static_cast<long long>(divideUp(m, side)) * divideUp(n, side);
-}
-
 template <typename T, bool kGradient>
 int launchGated(const zcgvs_gated_desc& d, GatedArgs args, hipStream_t stream) {
     args.x = d.x;
@@ -333,15 +422,21 @@ int launchGated(const zcgvs_gated_desc& d, GatedArgs args, hipStream_t stream) {
     const bool direct = directRows(args.x, args.x_stride, d.dim, d.dtype) &&
                         directRows(args.gate, args.weight_stride, d.dim, d.dtype) &&
                         directRows(args.up, args.weight_stride, d.dim, d.dtype);
-    return withTile<T, false, false>(tilesOf(d.rows, 2 * static_cast<std::int64_t>(d.hidden), 128), direct, [&](auto tile) {
-        using Tile = decltype(tile);
-        return withActivation(d.activation, [&](auto activation) {
+    return withActivation(d.activation, [&](auto activation) {
+        // the error function's terms do not fit the registers beside the sums of 256 x 256
+        constexpr LargestTile kLargest = decltype(activation)::value == ZCGVS_ACT_GELU ? LargestTile::k256x192
+                                                                                        : LargestTile::k256x256;
+        const ProductPlan plan =
+            planProduct(d.rows, 2 * static_cast<std::int64_t>(d.hidden), d.dim, 1, d.dtype, 0, kLargest);
+        return withTile<T, false, false, kLargest, true>(plan.shape, direct, [&](auto tile) {
+            using Tile = decltype(tile);
             args.tiles_m = divideUp(d.rows, Tile::kM);
             args.tiles_n = divideUp(d.hidden, Tile::kN / 2);
-            const long long blocks = static_cast<long long>(args.tiles_m) * args.tiles_n;
-            if (blocks > kMaxBlocks) {
+            const long long tiles = static_cast<long long>(args.tiles_m) * args.tiles_n;
+            if (tiles > INT32_MAX) {
                 return invalid("more output than one launch can write");
             }
+            const long long blocks = std::min(tiles, static_cast<long long>(persistentBlocks(plan.shape)));
             gatedKernel<Tile, decltype(activation)::value, kGradient>
                 <<<static_cast<unsigned>(blocks), Tile::kThreads, 0, stream>>>(args);
             ZCGVS_LAUNCH_CHECK("gated projection");
@@ -350,14 +445,62 @@ int launchGated(const zcgvs_gated_desc& d, GatedArgs args, hipStream_t stream) {
     });
 }
 
-// Elements from row to row of dg and du in the workspace.
+// Elements from row to row of dg and du in the workspace; the partial sums follow them.
 std::int64_t gradientStride(const zcgvs_gated_desc& d) { return (static_cast<std::int64_t>(d.hidden) + 7) / 8 * 8; }
+
+std::size_t partialsOffset(const zcgvs_gated_desc& d) {
+    const std::size_t both = 2 * static_cast<std::size_t>(d.rows) * static_cast<std::size_t>(gradientStride(d));
+    return (both * static_cast<std::size_t>(elementBytes(d.dtype)) + 255) / 256 * 256;
+}
+
+ProductPlan inputPlan(const zcgvs_gated_desc& d) {
+    // an even number of splits, each within one of the two products; 256 x 256 tiles of two products one
+    // after the other do not fit the registers (measured 140 us for what 256 x 192 take 93)
+    return planProduct(d.rows, d.dim, 2 * static_cast<std::int64_t>(d.hidden), 1, d.dtype, 2,
+                       LargestTile::k256x192);
+}
+
+ProductPlan weightPlan(const zcgvs_gated_desc& d) {
+    return planProduct(d.hidden, d.dim, d.rows, 2, d.dtype, 1, LargestTile::k256x256);
+}
+
+// float32 partial sums of the two products, one after the other in the same place.
+std::size_t partialValues(const zcgvs_gated_desc& d) {
+    const ProductPlan input = inputPlan(d);
+    const ProductPlan weight = weightPlan(d);
+    const std::size_t for_input = input.splits > 1 ? static_cast<std::size_t>(input.splits) * static_cast<std::size_t>(d.rows) : 0;
+    const std::size_t for_weight = weight.splits > 1 ? static_cast<std::size_t>(weight.splits) * 2 * static_cast<std::size_t>(d.hidden) : 0;
+    return std::max(for_input, for_weight) * static_cast<std::size_t>(d.dim);
+}
+
+template <typename T>
+int launchJoin(const float* partials, int splits, std::int64_t rows, int columns, std::int64_t rows_first, void* first,
+               void* second, std::int64_t stride, bool packed, hipStream_t stream) {
+    const bool four = packed && columns % 4 == 0;
+    const long long packs = static_cast<long long>(rows) * (columns / (four ? 4 : 1));
+    const unsigned blocks = static_cast<unsigned>(std::min(8192ll, (packs + kJoinThreads - 1) / kJoinThreads));
+    if (four) {
+        joinKernel<T, 4><<<blocks, kJoinThreads, 0, stream>>>(partials, splits, rows, columns, rows_first,
+                                                              static_cast<T*>(first), static_cast<T*>(second), stride);
+    } else {
+        joinKernel<T, 1><<<blocks, kJoinThreads, 0, stream>>>(partials, splits, rows, columns, rows_first,
+                                                              static_cast<T*>(first), static_cast<T*>(second), stride);
+    }
+    ZCGVS_LAUNCH_CHECK("gated gradient");
+    return ZCGVS_OK;
+}
 
 template <typename T>
 int launchInputGradient(const zcgvs_gated_desc& d, InputGradientArgs args, hipStream_t stream) {
     const bool direct = directRows(args.gate, args.weight_stride, d.dim, d.dtype) &&
                         directRows(args.up, args.weight_stride, d.dim, d.dtype);
-    return withTile<T, false, true>(tilesOf(d.rows, d.dim, 128), direct, [&](auto tile) {
+    const ProductPlan plan = inputPlan(d);
+    args.splits = plan.splits;
+    args.split_k = plan.splits > 1 ? divideUp(divideUp(d.hidden, plan.splits / 2), kStageK<T>) * kStageK<T> : d.hidden;
+    if (plan.splits > 1) {
+        args.splits = 2 * divideUp(d.hidden, args.split_k);  // rounding to whole stages may leave fewer
+    }
+    const int launched = withTile<T, false, true, LargestTile::k256x192, false>(plan.shape, direct, [&](auto tile) {
         using Tile = decltype(tile);
         args.tiles_m = divideUp(d.rows, Tile::kM);
         args.tiles_n = divideUp(d.dim, Tile::kN);
@@ -365,16 +508,25 @@ int launchInputGradient(const zcgvs_gated_desc& d, InputGradientArgs args, hipSt
         if (blocks > kMaxBlocks) {
             return invalid("more output than one launch can write");
         }
-        inputGradientKernel<Tile><<<static_cast<unsigned>(blocks), Tile::kThreads, 0, stream>>>(args);
+        inputGradientKernel<Tile><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(args.splits)),
+                                    Tile::kThreads, 0, stream>>>(args);
         ZCGVS_LAUNCH_CHECK("gated gradient");
         return static_cast<int>(ZCGVS_OK);
     });
+    if (launched != ZCGVS_OK || args.splits == 1) {
+        return launched;
+    }
+    return launchJoin<T>(args.partials, args.splits, d.rows, d.dim, d.rows, args.out, nullptr, args.out_stride,
+                         args.out_packed, stream);
 }
 
 template <typename T>
 int launchWeightGradient(const zcgvs_gated_desc& d, WeightGradientArgs args, hipStream_t stream) {
     const bool direct = directRows(args.x, args.x_stride, d.dim, d.dtype);
-    return withTile<T, true, true>(2 * tilesOf(d.hidden, d.dim, 128), direct, [&](auto tile) {
+    const ProductPlan plan = weightPlan(d);
+    args.split_k = divideUp(divideUp(d.rows, plan.splits), kStageK<T>) * kStageK<T>;
+    args.splits = divideUp(d.rows, args.split_k);
+    const int launched = withTile<T, true, true, LargestTile::k256x256, false>(plan.shape, direct, [&](auto tile) {
         using Tile = decltype(tile);
         args.tiles_m = divideUp(d.hidden, Tile::kM);
         args.tiles_n = divideUp(d.dim, Tile::kN);
@@ -382,10 +534,16 @@ int launchWeightGradient(const zcgvs_gated_desc& d, WeightGradientArgs args, hip
         if (blocks > kMaxBlocks) {
             return invalid("more output than one launch can write");
         }
-        weightGradientKernel<Tile><<<static_cast<unsigned>(blocks), Tile::kThreads, 0, stream>>>(args);
+        weightGradientKernel<Tile><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(args.splits)),
+                                     Tile::kThreads, 0, stream>>>(args);
         ZCGVS_LAUNCH_CHECK("gated gradient");
         return static_cast<int>(ZCGVS_OK);
     });
+    if (launched != ZCGVS_OK || args.splits == 1) {
+        return launched;
+    }
+    return launchJoin<T>(args.partials, args.splits, 2 * static_cast<std::int64_t>(d.hidden), d.dim, d.hidden,
+                         args.gate_out, args.up_out, args.out_stride, args.out_packed, stream);
 }
 
 // Zeros for the weight gradients of a batch without rows.
@@ -436,8 +594,7 @@ std::size_t zcgvs_gated_gradient_workspace_bytes(const zcgvs_gated_desc* desc) {
         return 0;
     }
     clearError();
-    const std::size_t one = static_cast<std::size_t>(desc->rows) * static_cast<std::size_t>(gradientStride(*desc));
-    return std::max<std::size_t>(256, 2 * one * static_cast<std::size_t>(elementBytes(desc->dtype)));
+    return desc->rows == 0 ? 256 : partialsOffset(*desc) + partialValues(*desc) * sizeof(float);
 }
 
 int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradient, std::int64_t out_gradient_stride,
@@ -496,6 +653,8 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
         form.out_packed = true;
         form.out_gradient = d_out_gradient;
         form.out_gradient_stride = from_stride;
+        form.gradient_packed = alignedRows(d_out_gradient, from_stride, d.dtype, 4 * elementBytes(d.dtype));
+        float* partials = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + partialsOffset(d));
         form.du_offset = d.rows * form.out_stride;
         int done = launchGated<T, true>(d, form, toStream(stream));
         if (done == ZCGVS_OK && d_x_gradient != nullptr) {
@@ -509,6 +668,7 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
             args.rows = static_cast<int>(d.rows);
             args.dim = d.dim;
             args.hidden = d.hidden;
+            args.partials = partials;
             args.out = d_x_gradient;
             args.out_stride = x_out_stride;
             args.out_packed = alignedRows(d_x_gradient, x_out_stride, d.dtype, 4 * elementBytes(d.dtype));
@@ -524,6 +684,7 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
             args.rows = static_cast<int>(d.rows);
             args.dim = d.dim;
             args.hidden = d.hidden;
+            args.partials = partials;
             args.gate_out = d_gate_gradient;
             args.up_out = d_up_gradient;
             args.out_stride = weight_out_stride;

@@ -18,7 +18,7 @@
 // n = 4 (l / 16) + e of row m = l % 16 and can store them together. Lane group h = l / 16 holds the
 // 16 bytes of chunk 4 t + h in step t, on both sides: every k meets itself whatever the order.
 //
-// Bounds. Rows past a side's end are read again from its last row (plain) or as zeros (turned); they
+// Bounds. Past a side's end its last row (plain) or chunk of columns (turned) is read again; those
 // only reach results that are not stored. k past the end is read as zeros on both sides.
 #pragma once
 
@@ -80,41 +80,74 @@ struct MatrixSide {
 // chunks. Otherwise through registers, from any alignment.
 template <typename T, int kRows, bool kTurned, bool kDirect, int kThreads>
 struct StageLoader {
-    static constexpr int kCopies = kRows * (kStageBytes / 16) / kThreads;
+    // 16-byte copies of a stage, by wavefronts of 64; where they do not split evenly the last ones have
+    // one round less
+    static constexpr int kWaves = kThreads / kWave;
+    static constexpr int kWaveCopies = kRows * (kStageBytes / 16) / kWave;
+    static constexpr int kCopies = (kWaveCopies + kWaves - 1) / kWaves;
+    static constexpr bool kEven = kWaveCopies % kWaves == 0;
     static constexpr int kBytes = kRows * kStageBytes;
-    static_assert(kCopies >= 1 && kRows * (kStageBytes / 16) % kThreads == 0, "a stage splits over the threads");
+
+    static __device__ __forceinline__ bool hasCopy(int i) {
+        return kEven || i + 1 < kCopies ||
+               i * kWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave) < kWaveCopies;
+    }
+
+    static constexpr int kSlots = kRows * static_cast<int>(sizeof(T)) / 16;  // 16-byte chunks of a turned k-row
 
     const char* src[kCopies];
-    int at[kCopies];     // k of the copy's first value within a stage
-    int count[kCopies];  // values of the copy that exist (turned)
-    std::int64_t step;   // bytes from stage to stage
-    int k_left;          // from the next stage to load on
+    std::int64_t step;  // bytes from stage to stage
+    int k_left;         // from the next stage to load on
+    int columns_left;   // that exist from the tile's first on (turned, not direct)
     u32x4 held[kDirect ? 1 : kCopies];
 
-    // row_of(r): the tile's row r of a plain side, at k = 0. A turned side starts at its tile's first column.
+    // Row (plain) or k-row (turned) and chunk of the i-th copy of this thread.
+    static __device__ __forceinline__ void placeOf(int i, int& row, int& chunk) {
+        const int slot = i * kThreads + static_cast<int>(threadIdx.x);
+        if constexpr (kTurned) {
+            row = slot / kSlots;
+            chunk = sourceChunk(row, slot % kSlots);
+        } else {
+            row = slot / 8;
+            chunk = (slot % 8) ^ ((row >> 1) & 7);
+        }
+    }
+    // k of the i-th copy's first value within a stage.
+    static __device__ __forceinline__ int kOf(int i) {
+        int row, chunk;
+        placeOf(i, row, chunk);
+        return kTurned ? row : chunk * kChunk<T>;
+    }
+
+    // row_of(r): the tile's row r of a plain side, at k = 0. A turned side starts at its tile's first
+    // column, of which `columns` (at least one) exist; direct copies read the last chunk again past them.
     template <typename RowOf>
     __device__ __forceinline__ void begin(RowOf&& row_of, std::int64_t stride, int columns, int k_total) {
-        const int tid = static_cast<int>(threadIdx.x);
         k_left = k_total;
+        columns_left = columns;
         step = kTurned ? stride * kStageK<T> * static_cast<std::int64_t>(sizeof(T)) : kStageBytes;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const int slot = i * kThreads + tid;
+            int row, chunk;
+            placeOf(i, row, chunk);
             if constexpr (kTurned) {
-                constexpr int kSlots = kRows * static_cast<int>(sizeof(T)) / 16;
-                const int k = slot / kSlots;
-                const int chunk = sourceChunk(k, slot % kSlots);
-                at[i] = k;
-                count[i] = min(max(columns - chunk * kChunk<T>, 0), kChunk<T>);
-                src[i] = reinterpret_cast<const char*>(row_of(0) + k * stride + chunk * kChunk<T>);
+                const int from = kDirect ? min(chunk, (columns - 1) / kChunk<T>) : chunk;
+                src[i] = reinterpret_cast<const char*>(row_of(0) + row * stride + from * kChunk<T>);
             } else {
-                const int row = slot / 8;
-                const int chunk = (slot % 8) ^ ((row >> 1) & 7);
-                at[i] = chunk * kChunk<T>;
-                count[i] = kChunk<T>;
                 src[i] = reinterpret_cast<const char*>(row_of(row) + chunk * kChunk<T>);
             }
         }
+    }
+
+    // From the end of k (whose last stage, where it is not a whole one, does not advance) to k = 0 of an
+    // operand `bytes` further on.
+    __device__ __forceinline__ void moveOn(std::int64_t bytes, int k_total) {
+        const std::int64_t by = bytes - (k_total / kStageK<T>)*step;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            src[i] += by;
+        }
+        k_left = k_total;
     }
 
     // Which chunk of k-row k stands in `slot` of its LDS row (an exchange, so also the reverse).
@@ -136,16 +169,23 @@ struct StageLoader {
     // Starts the next stage's copies into `stage` (direct).
     __device__ __forceinline__ void issue(const std::uint8_t* stage) {
         const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
-        const std::uint32_t base = ldsAddress(stage);
-        const bool whole = k_left >= kStageK<T>;
+        const std::uint32_t base = ldsAddress(stage) + static_cast<std::uint32_t>(wave * kWave * 16);
+        if (k_left >= kStageK<T>) {
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const char* from = src[i];
-            if ((!whole && at[i] >= k_left) || (kTurned && count[i] == 0)) {
-                from = reinterpret_cast<const char*>(&zero_chunk);
+            for (int i = 0; i < kCopies; ++i) {
+                if (hasCopy(i)) {
+                    copySharedToLds(src[i], __builtin_amdgcn_readfirstlane(base + i * kThreads * 16));
+                }
+                src[i] += step;
             }
-            copySharedToLds(from, __builtin_amdgcn_readfirstlane(base + (i * kThreads + wave * kWave) * 16));
-            src[i] += step;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const char* from = kOf(i) < k_left ? src[i] : reinterpret_cast<const char*>(&zero_chunk);
+                if (hasCopy(i)) {
+                    copySharedToLds(from, __builtin_amdgcn_readfirstlane(base + i * kThreads * 16));
+                }
+            }
         }
         k_left -= kStageK<T>;
     }
@@ -154,7 +194,10 @@ struct StageLoader {
     __device__ __forceinline__ void fetch() {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const int valid = kTurned ? (at[i] < k_left ? count[i] : 0) : k_left - at[i];
+            int row, chunk;
+            placeOf(i, row, chunk);
+            int valid = kTurned ? (row < k_left ? columns_left - chunk * kChunk<T> : 0) : k_left - chunk * kChunk<T>;
+            valid = hasCopy(i) ? valid : 0;
             if (valid >= kChunk<T>) {
                 __builtin_memcpy(&held[i], src[i], 16);
             } else {
@@ -168,14 +211,16 @@ struct StageLoader {
                 }
                 held[i] = __builtin_bit_cast(u32x4, v);
             }
-            src[i] += step;
+            src[i] += k_left >= kStageK<T> ? step : 0;
         }
         k_left -= kStageK<T>;
     }
     __device__ __forceinline__ void put(std::uint8_t* stage) const {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            *reinterpret_cast<u32x4*>(stage + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+            if (hasCopy(i)) {
+                *reinterpret_cast<u32x4*>(stage + (i * kThreads + static_cast<int>(threadIdx.x)) * 16) = held[i];
+            }
         }
     }
 
@@ -228,7 +273,8 @@ struct MatrixTile {
     static constexpr bool kDirect = kDirectLoads;
     using SideA = StageLoader<T, kM, kTurnedA, kDirect, kThreads>;
     using SideB = StageLoader<T, kN, kTurnedB, kDirect, kThreads>;
-    static constexpr int kLdsBytes = 2 * (SideA::kBytes + SideB::kBytes);
+    static constexpr int kStageLds = SideA::kBytes + SideB::kBytes;
+    static constexpr int kLdsBytes = 2 * kStageLds;
 
     using Sums = f32x4[kBlocksM][kBlocksN];
 
@@ -273,80 +319,137 @@ struct MatrixTile {
         }
     }
 
-    // Adds the tile's products over k to `sums`. Every thread of the workgroup calls it; `lds` holds
-    // kLdsBytes. Ends at a barrier: the LDS may be used for something else at once.
-    template <typename RowA, typename RowB>
-    static __device__ __forceinline__ void accumulate(std::uint8_t* lds, RowA&& row_a, std::int64_t stride_a,
-                                                      int columns_a, RowB&& row_b, std::int64_t stride_b, int columns_b,
-                                                      int k_total, Sums& sums) {
+    // The loads of both sides. A workgroup that forms several tiles (or a tile of several products)
+    // starts the next one's first stage while it multiplies the last stage of the one before, so that
+    // it arrives behind that stage and the tile's results.
+    struct Loads {
         SideA a;
         SideB b;
-        a.begin(row_a, stride_a, columns_a, k_total);
-        b.begin(row_b, stride_b, columns_b, k_total);
+        int buffer = 0;       // of the next stage
+        bool landed = false;  // the next stage is known to have arrived
+
+        template <typename RowA, typename RowB>
+        __device__ __forceinline__ void begin(RowA&& row_a, std::int64_t stride_a, int columns_a, RowB&& row_b,
+                                              std::int64_t stride_b, int columns_b, int k_total) {
+            a.begin(row_a, stride_a, columns_a, k_total);
+            b.begin(row_b, stride_b, columns_b, k_total);
+        }
+        __device__ __forceinline__ void issue(std::uint8_t* lds, int to) {
+            a.issue(lds + to * kStageLds);
+            b.issue(lds + to * kStageLds + SideA::kBytes);
+        }
+        // Goes on with a second product over the same k, its operands so many bytes from the first's.
+        __device__ __forceinline__ void moveOn(std::int64_t a_bytes, std::int64_t b_bytes, int k_total) {
+            a.moveOn(a_bytes, k_total);
+            b.moveOn(b_bytes, k_total);
+        }
+        // Starts the first stage after begin() or moveOn().
+        __device__ __forceinline__ void start(std::uint8_t* lds) {
+            if constexpr (kDirect) {
+                issue(lds, buffer);
+            }
+        }
+        // Waits for a started first stage; called before a tile's results are stored, so that the next
+        // tile does not wait for the stores.
+        __device__ __forceinline__ void land() {
+            if constexpr (kDirect) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                landed = true;
+            }
+        }
+    };
+
+    // Adds the products over k_total values of k to `sums`, from the stage that `loads` has started on.
+    // next(): called in the last stage; may begin and start what comes after (`loads.start(lds)`).
+    // Every thread of the workgroup calls it; `lds` holds kLdsBytes.
+    template <typename Next>
+    static __device__ __forceinline__ void accumulate(std::uint8_t* lds, Loads& loads, int k_total, Sums& sums,
+                                                      Next&& next) {
         const int stages = (k_total + kStageK<T> - 1) / kStageK<T>;
-        constexpr int kStage = SideA::kBytes + SideB::kBytes;
         if constexpr (kDirect) {
-            a.issue(lds);
-            b.issue(lds + SideA::kBytes);
             for (int s = 0; s < stages; ++s) {
-                // this stage's copies have arrived, and every wavefront has read the other one
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                // this stage's copies have arrived, and every wavefront has read the other buffer
+                if (loads.landed) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    loads.landed = false;
+                } else {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                }
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                std::uint8_t* here = lds + (s & 1) * kStage;
-                std::uint8_t* next = lds + ((s & 1) ^ 1) * kStage;
+                const std::uint8_t* here = lds + loads.buffer * kStageLds;
+                loads.buffer ^= 1;
                 if (s + 1 < stages) {
-                    a.issue(next);
-                    b.issue(next + SideA::kBytes);
+                    loads.issue(lds, loads.buffer);
+                } else {
+                    next();
                 }
                 multiplyStage(here, sums);
             }
         } else {
-            a.fetch();
-            b.fetch();
-            a.put(lds);
-            b.put(lds + SideA::kBytes);
+            __syncthreads();  // the LDS may still be read for the tile before
+            loads.a.fetch();
+            loads.b.fetch();
+            loads.a.put(lds);
+            loads.b.put(lds + SideA::kBytes);
             __syncthreads();
             for (int s = 0; s < stages; ++s) {
-                std::uint8_t* here = lds + (s & 1) * kStage;
-                std::uint8_t* next = lds + ((s & 1) ^ 1) * kStage;
+                std::uint8_t* here = lds + (s & 1) * kStageLds;
+                std::uint8_t* other = lds + ((s & 1) ^ 1) * kStageLds;
                 if (s + 1 < stages) {
-                    a.fetch();
-                    b.fetch();
+                    loads.a.fetch();
+                    loads.b.fetch();
                 }
                 multiplyStage(here, sums);
                 if (s + 1 < stages) {
-                    a.put(next);
-                    b.put(next + SideA::kBytes);
+                    loads.a.put(other);
+                    loads.b.put(other + SideA::kBytes);
                 }
                 __syncthreads();
             }
-        }
-        if constexpr (kDirect) {
-            __syncthreads();
+            next();
         }
     }
 };
 
-// Tile (m, n) of the launch's block: blocks of one XCD (every eighth one) take neighbouring tiles, in
-// bands of kBandRows tile rows walked column by column, so that an XCD's blocks share rows of both
-// sides in its L2.
+// The index-th tile (m, n) of a launch whose block b forms the tiles b, b + gridDim.x, ... (a multiple of
+// kXcds apart where there are several). Blocks of one XCD (every eighth one) take neighbouring tiles, in
+// bands of kBandRows tile rows walked column by column, so that an XCD's blocks share rows of both sides in
+// its L2.
 constexpr int kXcds = 8;
 constexpr int kBandRows = 4;
 
-__device__ __forceinline__ void tileOf(int tiles_m, int tiles_n, int& m, int& n) {
+__device__ __forceinline__ void tileOf(int index, int tiles_m, int tiles_n, int& m, int& n) {
     const int total = tiles_m * tiles_n;
-    const int block = static_cast<int>(blockIdx.x);
-    const int xcd = block % kXcds;
+    const int xcd = index % kXcds;
     const int whole = total / kXcds;
-    const int more = total % kXcds;  // the first `more` XCDs have one block more
-    const int tile = xcd * whole + min(xcd, more) + block / kXcds;
+    const int more = total % kXcds;  // the first `more` XCDs have one tile more
+    const int tile = xcd * whole + min(xcd, more) + index / kXcds;
     const int band_tiles = kBandRows * tiles_n;
     const int band = tile / band_tiles;
     const int in_band = tile - band * band_tiles;
     const int rows = min(kBandRows, tiles_m - band * kBandRows);
     m = band * kBandRows + in_band % rows;
     n = in_band / rows;
+}
+
+// Reads four neighbouring values of one row of which `left` exist; the others are zeros.
+template <typename T>
+__device__ __forceinline__ f32x4 loadFour(const T* from, int left, bool packed) {
+    f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (packed && left >= 4) {
+        float v[4];
+        loadPack(from, v);
+        value = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e < left) {
+                value[e] = static_cast<float>(from[e]);
+            }
+        }
+    }
+    return value;
 }
 
 // Stores four neighbouring results of one row; `left` of them exist. `packed`: rows and their first
