@@ -457,7 +457,7 @@ typedef struct zcgvs_embedding_desc {
     int dim;
     int dtype;                   /* of the table                                                 */
     const int* ids;              /* [token_count]                                                */
-    int64_t token_count;         /* at most 2^29                                                 */
+    int64_t token_count;         /* at most 2^28                                                 */
     const int64_t* bag_offsets;  /* [bag_count + 1], or NULL: one output row per token           */
     int64_t bag_count;           /* at most 2^31 - 1                                             */
     int reduce;                  /* enum zcgvs_embedding_reduce (with bags)                      */

@@ -8,8 +8,8 @@
 // low up_a^T and adds x weight^T on top: one read of x and one write of out for both.
 //
 // low between the two products. The products are the 16-bit matrix instructions', so low is handed over
-// in two parts of the operands' type, high + rest, which keeps 22 (float16) or 16 (bfloat16) bits of it
-// (one part alone would cost a float32 output most of its digits). Each row is scaled by a power of two
+// in parts of the operands' type, high + rest (+ rest of that), as many as keep a float32 output's digits:
+// two of float16 hold 22 bits, three of bfloat16 all 24; a bfloat16 output takes two, of 16 bits. Each row is scaled by a power of two
 // that brings its largest value to [2^14, 2^15), so that float16 neither overflows nor loses small
 // parts; its inverse is applied to the sums in float32. float32 operands need no parts.
 //
@@ -32,8 +32,9 @@ namespace {
 constexpr int kMaxRank = 128;
 constexpr int kRankStep = 32;  // low's rows are padded to whole steps of the matrix instructions
 
-template <typename T>
-constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+template <typename T, typename Out>
+constexpr int kParts = std::is_same_v<T, float> ? 1 : std::is_same_v<T, __bf16> && std::is_same_v<Out, float> ? 3 : 2;
+constexpr int kMostParts = 3;
 
 int paddedRank(int max_rank) { return (max_rank + kRankStep - 1) / kRankStep * kRankStep; }
 
@@ -54,6 +55,7 @@ struct AdaptedArgs {
     const float* scales;
     const int* adapters;  // [rows] sorted, adapter_count: none; null: no row has one
     const int* order;     // [rows] the row at each sorted position
+    int parts;
     void* low;            // [rows, parts, padded_rank] by sorted position
     float* low_scale;     // [rows]
     int tiles_m;
@@ -94,6 +96,7 @@ constexpr int kLowWaves = kLowThreads / kWave;
 
 template <typename T, int kRankBlocks>
 __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int positions) {
+    constexpr int kLowAhead = kRankBlocks <= 4 ? 4 : 2;  // steps whose loads are in flight
     constexpr int kRanks = kRankBlocks * 16;
     __shared__ float joined[kLowWaves][16][kRanks];
     __shared__ float row_peak[16][16];
@@ -124,20 +127,40 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
         const T* down = static_cast<const T*>(args.down) +
                         static_cast<std::int64_t>(adapter) * args.max_rank * args.dim;
         f32x4 sums[kRankBlocks];
+        const T* rows_of[kRankBlocks];  // a row past the rank gives sums that are not used
 #pragma unroll
         for (int j = 0; j < kRankBlocks; ++j) {
             sums[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            rows_of[j] = down + static_cast<std::int64_t>(min(j * 16 + r16, max(rank, 1) - 1)) * args.dim;
         }
         const int past_step = min((wave + 1) * share, steps);
-        for (int s = wave * share; s < past_step; ++s) {
+        const int past_whole = min(past_step, args.dim / kStepK);
+        int s = wave * share;
+        for (; s + kLowAhead <= past_whole; s += kLowAhead) {
+            typename Fragment<T>::type a[kLowAhead], b[kLowAhead][kRankBlocks];
+#pragma unroll
+            for (int u = 0; u < kLowAhead; ++u) {
+                const int k = (s + u) * kStepK + h * kChunk<T>;
+                __builtin_memcpy(&a[u], x + k, 16);
+#pragma unroll
+                for (int j = 0; j < kRankBlocks; ++j) {
+                    __builtin_memcpy(&b[u][j], rows_of[j] + k, 16);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kLowAhead; ++u) {
+#pragma unroll
+                for (int j = 0; j < kRankBlocks; ++j) {
+                    sums[j] = multiplyAdd(b[u][j], a[u], sums[j]);
+                }
+            }
+        }
+        for (; s < past_step; ++s) {
             const int k = s * kStepK + h * kChunk<T>;
             const auto a = loadChunk(x + k, args.dim - k);
 #pragma unroll
             for (int j = 0; j < kRankBlocks; ++j) {
-                const int r = j * 16 + r16;
-                const auto b = loadChunk(down + static_cast<std::int64_t>(min(r, args.max_rank - 1)) * args.dim + k,
-                                         r < rank ? args.dim - k : 0);
-                sums[j] = multiplyAdd(b, a, sums[j]);
+                sums[j] = multiplyAdd(loadChunk(rows_of[j] + k, args.dim - k), a, sums[j]);
             }
         }
         __syncthreads();  // the last group's sums have been read
@@ -183,23 +206,25 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
                     frexpf(peak, &e);  // peak = m 2^e, m in [0.5, 1)
                     exponent = min(126, max(-126, 15 - e));
                 }
-                T* to = static_cast<T*>(args.low) + at * 2 * args.padded_rank;
+                T* to = static_cast<T*>(args.low) + at * args.parts * args.padded_rank;
                 const float up_by = ldexpf(1.0f, exponent);
 #pragma unroll
                 for (int j = 0; j < kRankBlocks; ++j) {
                     const int r = j * 16 + column;
-                    const float scaled = value[j] * up_by;
-                    const T high = static_cast<T>(scaled);
-                    // an infinite value has no rest
-                    const float rest = fabsf(scaled) <= 3.402823466e+38f ? scaled - static_cast<float>(high) : 0.0f;
+                    float rest = value[j] * up_by;
                     if (r < args.padded_rank) {
-                        to[r] = high;
-                        to[args.padded_rank + r] = static_cast<T>(rest);
+                        for (int part = 0; part < args.parts; ++part) {
+                            const T here = static_cast<T>(rest);
+                            to[part * args.padded_rank + r] = here;
+                            // an infinite value has no rest
+                            rest = fabsf(rest) <= 3.402823466e+38f ? rest - static_cast<float>(here) : 0.0f;
+                        }
                     }
                 }
                 for (int r = kRanks + column; r < args.padded_rank; r += 16) {
-                    to[r] = static_cast<T>(0.0f);
-                    to[args.padded_rank + r] = static_cast<T>(0.0f);
+                    for (int part = 0; part < args.parts; ++part) {
+                        to[part * args.padded_rank + r] = static_cast<T>(0.0f);
+                    }
                 }
                 if (column == 0) {
                     args.low_scale[at] = ldexpf(1.0f, -exponent);
@@ -228,74 +253,126 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
 
 // ---- the projection -----------------------------------------------------------------------------
 
-// Starts a wavefront's sums with low up^T: one adapter of its rows after the other, for each the
-// products with the 16-row blocks that have rows of it, kept in those rows only.
-template <class Tile>
+// Starts a wavefront's sums with low up^T, in one of two ways.
+// By adapter: one adapter of the wavefront's rows after the other, for each the matrix products of all its
+// rows with the adapter's up, kept in the rows that are the adapter's. An adapter costs about 1.2 us, the
+// latency of its rank and of its up.
+// By row: every lane forms its own results, 4 columns of a row, from its row's adapter. That costs a fused
+// multiply-add for each rank and result (64 x 32 results of rank 32 about 3 us), whatever the adapters, and
+// is taken where the wavefront's rows have many of them.
+template <class Tile, typename Out>
 __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, int m0, int n0, typename Tile::Sums& sums) {
     using T = typename Tile::T;
     constexpr int kStepR = 4 * kChunk<T>;
+    constexpr int kHere = kParts<T, Out>;
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int r16 = lane & 15;
     const int h = lane >> 4;
     int adapter[Tile::kBlocksM];
     float scale[Tile::kBlocksM];
-    int left = args.adapter_count;  // the smallest adapter of the wavefront's rows that is not done
+    int first = args.adapter_count;  // the smallest adapter of the wavefront's rows
+    int changes = 0;                 // rows whose adapter is not that of the row before
 #pragma unroll
     for (int i = 0; i < Tile::kBlocksM; ++i) {
         const int p = m0 + i * 16 + r16;
         adapter[i] = p < args.rows ? args.adapters[p] : args.adapter_count;
+        const int before = p > 0 && p < args.rows ? args.adapters[p - 1] : adapter[i];
         scale[i] = adapter[i] < args.adapter_count ? args.low_scale[p] : 0.0f;
-        left = min(left, adapter[i]);
+        changes += __popcll(__ballot(adapter[i] < args.adapter_count && adapter[i] != before)) / 4;
+        first = min(first, adapter[i]);
     }
 #pragma unroll
     for (int d = 1; d < 16; d *= 2) {
-        left = min(left, __shfl_xor(left, d, kWave));
+        first = min(first, __shfl_xor(first, d, kWave));
     }
-    left = __builtin_amdgcn_readfirstlane(left);
-    while (left < args.adapter_count) {
-        const int rank = rankOf(args, left);
-        const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(left) * args.out_dim * args.max_rank;
+    int left = __builtin_amdgcn_readfirstlane(first);
+    if (changes > 2 + args.max_rank / 8) {
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
-            const bool mine = adapter[i] == left;
-            if (__ballot(mine) == 0) {
-                continue;
-            }
-            const std::int64_t p = min(m0 + i * 16 + r16, args.rows - 1);
-            const T* low = static_cast<const T*>(args.low) + p * kParts<T> * args.padded_rank;
-            f32x4 part[Tile::kBlocksN];
+            const int p = min(m0 + i * 16 + r16, args.rows - 1);
+            const bool has = adapter[i] < args.adapter_count;
+            const int mine = has ? adapter[i] : 0;
+            const int rank = has ? rankOf(args, mine) : 0;
+            const T* low = static_cast<const T*>(args.low) + static_cast<std::int64_t>(p) * kHere * args.padded_rank;
+            const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(mine) * args.out_dim * args.max_rank;
+            for (int r = 0; r < rank; r += kChunk<T>) {
+                float values[kChunk<T>];
 #pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-            for (int r = 0; r < rank; r += kStepR) {
-                const int at = r + h * kChunk<T>;
-                typename Fragment<T>::type a[kParts<T>];
+                for (int part = 0; part < kHere; ++part) {
+                    const auto v = *reinterpret_cast<const typename Fragment<T>::type*>(low + part * args.padded_rank + r);
 #pragma unroll
-                for (int half = 0; half < kParts<T>; ++half) {
-                    a[half] = *reinterpret_cast<const typename Fragment<T>::type*>(low + half * args.padded_rank + at);
+                    for (int e = 0; e < kChunk<T>; ++e) {
+                        values[e] = (part == 0 ? 0.0f : values[e]) + static_cast<float>(v[e]);
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < Tile::kBlocksN; ++j) {
-                    const int n = min(n0 + j * 16 + r16, args.out_dim - 1);
-                    const auto b = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + at, rank - at);
+                    typename Fragment<T>::type b[4];
 #pragma unroll
-                    for (int half = 0; half < kParts<T>; ++half) {
-                        part[j] = multiplyAdd(b, a[half], part[j]);
+                    for (int e = 0; e < 4; ++e) {
+                        const int n = min(n0 + j * 16 + 4 * h + e, args.out_dim - 1);
+                        b[e] = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + r, rank - r);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int c = 0; c < kChunk<T>; ++c) {
+                            sums[i][j][e] += values[c] * static_cast<float>(b[e][c]);
+                        }
                     }
                 }
             }
 #pragma unroll
             for (int j = 0; j < Tile::kBlocksN; ++j) {
+                sums[i][j] *= scale[i];
+            }
+        }
+        return;
+    }
+    while (left < args.adapter_count) {
+        const int rank = rankOf(args, left);
+        const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(left) * args.out_dim * args.max_rank;
+        typename Tile::Sums part;
+        Tile::clear(part);
+        for (int r = 0; r < rank; r += kStepR) {
+            const int at = r + h * kChunk<T>;
+            typename Fragment<T>::type a[Tile::kBlocksM][kHere], b[Tile::kBlocksN];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sums[i][j][e] = mine ? part[j][e] * scale[i] : sums[i][j][e];
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+                const int n = min(n0 + j * 16 + r16, args.out_dim - 1);
+                b[j] = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + at, rank - at);
+            }
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+                const std::int64_t p = min(m0 + i * 16 + r16, args.rows - 1);
+#pragma unroll
+                for (int e = 0; e < kHere; ++e) {
+                    a[i][e] = *reinterpret_cast<const typename Fragment<T>::type*>(
+                        static_cast<const T*>(args.low) + (p * kHere + e) * args.padded_rank + at);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+                for (int e = 0; e < kHere; ++e) {
+#pragma unroll
+                    for (int j = 0; j < Tile::kBlocksN; ++j) {
+                        part[i][j] = multiplyAdd(b[j], a[i][e], part[i][j]);
+                    }
                 }
             }
         }
         int next = args.adapter_count;
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
+            const bool mine = adapter[i] == left;
+#pragma unroll
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sums[i][j][e] = mine ? part[i][j][e] * scale[i] : sums[i][j][e];
+                }
+            }
             next = adapter[i] > left ? min(next, adapter[i]) : next;
         }
 #pragma unroll
@@ -326,7 +403,7 @@ __global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args
     typename Tile::Sums sums;
     Tile::clear(sums);
     if (args.adapters != nullptr) {
-        addAdapters<Tile>(args, m0 + Tile::waveM() * Tile::kBlocksM * 16, n0 + Tile::waveN() * Tile::kBlocksN * 16, sums);
+        addAdapters<Tile, Out>(args, m0 + Tile::waveM() * Tile::kBlocksM * 16, n0 + Tile::waveN() * Tile::kBlocksN * 16, sums);
     }
     Tile::accumulate(lds, loads, args.dim, sums, [] {});
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
@@ -345,6 +422,111 @@ __global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args
             }
         }
     }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------
+
+// Up to 16 rows in one launch: a workgroup forms 16 columns of all of them. Its wavefronts first form low, a
+// row each (every workgroup does: low is small, and another launch would cost more), then an eighth of the
+// products over dim each; 256 threads add those up, and their result's share of low up^T to it. All of low
+// stays in float32.
+constexpr int kFewRows = 16;
+constexpr int kFewThreads = 512;
+constexpr int kFewWaves = kFewThreads / kWave;
+
+// Products of 16 rows of `a_row` and 16 rows of `b_row` (a lane has its row l % 16 of each) over the steps
+// [step, past).
+template <typename T>
+__device__ __forceinline__ f32x4 multiplyRows(const T* a_row, const T* b_row, int step, int past, int dim) {
+    constexpr int kStepK = 4 * kChunk<T>;
+    constexpr int kAhead = 4;
+    const int h = (static_cast<int>(threadIdx.x) & (kWave - 1)) >> 4;
+    const int past_whole = min(past, dim / kStepK);
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (; step + kAhead <= past_whole; step += kAhead) {
+        typename Fragment<T>::type a[kAhead], b[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int k = (step + u) * kStepK + h * kChunk<T>;
+            __builtin_memcpy(&a[u], a_row + k, 16);
+            __builtin_memcpy(&b[u], b_row + k, 16);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            sum = multiplyAdd(b[u], a[u], sum);
+        }
+    }
+    for (; step < past; ++step) {
+        const int k = step * kStepK + h * kChunk<T>;
+        sum = multiplyAdd(loadChunk(b_row + k, dim - k), loadChunk(a_row + k, dim - k), sum);
+    }
+    return sum;
+}
+
+template <typename T, typename Out>
+__global__ __launch_bounds__(kFewThreads) void adaptedFewKernel(AdaptedArgs args, const int* adapter_ids) {
+    __shared__ float low[kFewRows][kMaxRank + 4];
+    __shared__ float parts[kFewWaves][16][17];
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int r16 = lane & 15;
+    const int h = lane >> 4;
+    const int n0 = static_cast<int>(blockIdx.x) * 16;
+    const int steps = (args.dim + 4 * kChunk<T> - 1) / (4 * kChunk<T>);
+    const int share = (steps + kFewWaves - 1) / kFewWaves;
+    const T* x_row = static_cast<const T*>(args.x) + min(r16, args.rows - 1) * args.x_stride;
+    const T* weight_row = static_cast<const T*>(args.weight) + min(n0 + r16, args.out_dim - 1) * args.weight_stride;
+    const f32x4 product = multiplyRows(x_row, weight_row, wave * share, min((wave + 1) * share, steps), args.dim);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        parts[wave][r16][4 * h + e] = product[e];
+    }
+    if (adapter_ids != nullptr) {
+        for (int row = wave; row < args.rows; row += kFewWaves) {
+            const int adapter = adapter_ids[row];
+            if (!counts(adapter, args.adapter_count, -1)) {
+                continue;
+            }
+            const int rank = rankOf(args, adapter);
+            const float scale = args.scales == nullptr ? 1.0f : args.scales[adapter];
+            const T* down = static_cast<const T*>(args.down) + static_cast<std::int64_t>(adapter) * args.max_rank * args.dim;
+            for (int r = 0; r < rank; r += 16) {
+                const f32x4 sum = multiplyRows(x_row, down + static_cast<std::int64_t>(min(r + r16, rank - 1)) * args.dim, 0,
+                                               steps, args.dim);
+                if (r16 == row) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        low[row][r + 4 * h + e] = sum[e] * scale;
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int row = static_cast<int>(threadIdx.x) / 16;
+    const int n = n0 + static_cast<int>(threadIdx.x) % 16;
+    if (row >= args.rows || n >= args.out_dim) {
+        return;
+    }
+    float sum = 0.0f;
+    const int adapter = adapter_ids == nullptr ? -1 : adapter_ids[row];
+    if (counts(adapter, args.adapter_count, -1)) {
+        const int rank = rankOf(args, adapter);
+        const T* up = static_cast<const T*>(args.up) +
+                      (static_cast<std::int64_t>(adapter) * args.out_dim + n) * args.max_rank;
+        for (int r = 0; r < rank; r += kChunk<T>) {
+            const auto b = loadChunk(up + r, rank - r);
+#pragma unroll
+            for (int e = 0; e < kChunk<T>; ++e) {
+                sum += r + e < rank ? low[row][r + e] * static_cast<float>(b[e]) : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+        sum += parts[w][row][static_cast<int>(threadIdx.x) % 16];
+    }
+    static_cast<Out*>(args.out)[row * args.out_stride + n] = static_cast<Out>(sum);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -404,7 +586,7 @@ AdaptedSpace adaptedSpace(const zcgvs_adapted_desc& d) {
     std::size_t at = 0;
     if (hasAdapters(d)) {
         const std::size_t rows = static_cast<std::size_t>(d.rows);
-        const std::size_t parts = d.dtype == ZCGVS_DTYPE_F32 ? 1 : 2;
+        const std::size_t parts = d.dtype == ZCGVS_DTYPE_F32 ? 1 : kMostParts;
         s.sort = at;
         at += pairSortBytes(rows);
         s.low = at;
@@ -521,6 +703,7 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
     args.out = d_out;
     args.out_stride = stride;
     args.out_packed = alignedRows(d_out, stride, out_dtype, 4 * elementBytes(out_dtype));
+    const bool few = d.rows <= kFewRows;
     if (hasAdapters(d)) {
         char* workspace = static_cast<char*>(d_workspace);
         args.down = d.down;
@@ -532,13 +715,16 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
         args.scales = d.scales;
         args.low = workspace + space.low;
         args.low_scale = reinterpret_cast<float*>(workspace + space.low_scale);
+    }
+    if (hasAdapters(d) && !few) {
         SortInput input{};
         input.keys = d.adapter_ids;
         input.count = args.rows;
         input.key_end = d.adapter_count;
         input.skipped = -1;
         input.raw = true;
-        const int sorted = sortPairs(input, workspace + space.sort, &args.adapters, &args.order, toStream(stream));
+        const int sorted = sortPairs(input, static_cast<char*>(d_workspace) + space.sort, &args.adapters, &args.order,
+                                     NoSideWork{}, toStream(stream));
         if (sorted != ZCGVS_OK) {
             return sorted;
         }
@@ -550,6 +736,13 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
         return withElement(out_dtype, [&](auto element) {
             using Out = decltype(element);
             if constexpr (std::is_same_v<Out, T> || std::is_same_v<Out, float>) {
+                if (few) {
+                    adaptedFewKernel<T, Out><<<static_cast<unsigned>(divideUp(d.out_dim, 16)), kFewThreads, 0,
+                                               toStream(stream)>>>(args, hasAdapters(d) ? d.adapter_ids : nullptr);
+                    ZCGVS_LAUNCH_CHECK("adapted projection");
+                    return static_cast<int>(ZCGVS_OK);
+                }
+                args.parts = kParts<T, Out>;
                 return launchAdapted<T, Out>(args, d.dtype, direct, toStream(stream));
             } else {
                 return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above

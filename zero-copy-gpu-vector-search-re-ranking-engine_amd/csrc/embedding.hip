@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWavesPerBlock = kThreads / kWave;
-constexpr std::int64_t kMaxTokens = 1 << 29;          // sorted positions and chunks fit 32 bits
+constexpr std::int64_t kMaxTokens = 1 << 28;          // a launch a chunk of 64 has less than 2^32 threads
 constexpr long long kMaxBlocks = (1ll << 24) - 1;     // a launch has less than 2^32 threads
 
 // ---- lookup, one output row per token ---------------------------------------------------------
@@ -78,76 +78,88 @@ __global__ __launch_bounds__(kThreads) void lookupKernel(const In* __restrict__ 
 
 // ---- lookup with bags -------------------------------------------------------------------------
 
-// A block pools one bag's columns of a slice: kBagColumns lanes side by side hold the slice's packs,
-// the block's 256 / kBagColumns groups of lanes take the bag's tokens in turn (kBagAhead of them in
-// flight each), and their sums are joined through LDS in the order of the groups.
-constexpr int kBagColumns = 32;
-constexpr int kBagGroups = kThreads / kBagColumns;
-constexpr int kBagAhead = 4;
+// A wavefront pools a share of one bag's tokens over a slice of 64 packs. It reads 64 ids at a time, a lane
+// each, and hands them on as scalars, so that the rows' loads wait for nothing but each other: kBagAhead of
+// them are in flight. kShares wavefronts of a workgroup share a bag's tokens, every kShares-th one each, and
+// their sums are joined through LDS in the order of the shares.
+constexpr int kBagAhead = 16;
 
-template <typename In, typename Out, int kPack>
+template <typename In, typename Out, int kPack, int kShares>
 __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ table, std::int64_t table_stride,
                                                       int vocab, int packs_per_row, const int* __restrict__ ids,
                                                       long long token_count,
-                                                      const std::int64_t* __restrict__ bag_offsets, int slices,
-                                                      bool mean, int padding_id, float scale, Out* __restrict__ out,
-                                                      std::int64_t out_stride) {
-    __shared__ float sums[kBagGroups][kBagColumns * kPack];
-    __shared__ int found[kBagGroups];
-    const long long bag = blockIdx.x / static_cast<unsigned>(slices);
-    const int slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(bag) * static_cast<unsigned>(slices));
-    const int column = threadIdx.x % kBagColumns;
-    const int group = threadIdx.x / kBagColumns;
-    const int pack = slice * kBagColumns + column;
+                                                      const std::int64_t* __restrict__ bag_offsets, long long items,
+                                                      int slices, bool mean, int padding_id, float scale,
+                                                      Out* __restrict__ out, std::int64_t out_stride) {
+    constexpr int kItems = kWavesPerBlock / kShares;  // of a workgroup
+    __shared__ float sums[kShares > 1 ? kWavesPerBlock : 1][kWave * kPack];
+    __shared__ int found[kWavesPerBlock];
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int share = wave % kShares;
+    const long long item = static_cast<long long>(blockIdx.x) * kItems + wave / kShares;
+    const bool has_item = item < items;
+    const long long bag = has_item ? item / slices : 0;
+    const int pack = static_cast<int>(item - bag * slices) * kWave + lane;
+    const bool has_pack = has_item && pack < packs_per_row;
     const long long begin = min(max(static_cast<long long>(bag_offsets[bag]), 0ll), token_count);
-    const long long end = min(static_cast<long long>(bag_offsets[bag + 1]), token_count);
-    const In* from = table + static_cast<std::int64_t>(pack) * kPack;
-    const bool has_pack = pack < packs_per_row;
+    const long long end = has_item ? min(static_cast<long long>(bag_offsets[bag + 1]), token_count) : begin;
+    const In* from = table + static_cast<std::int64_t>(has_pack ? pack : 0) * kPack;
 
     float sum[kPack] = {};
     int count = 0;
-    for (long long j = begin + group; j < end; j += kBagGroups * kBagAhead) {
-        float value[kBagAhead][kPack];
+    for (long long j = begin + share; j < end; j += kWave * kShares) {
+        // 64 of this share's tokens, those that count first and in their order
+        const long long mine = j + static_cast<long long>(lane) * kShares;
+        const int id = mine < end ? ids[mine] : -1;
+        unsigned long long left = __ballot(counts(id, vocab, padding_id));
+        count += __popcll(left);
+        while (left != 0) {
+            float value[kBagAhead][kPack];
+            int taken = 0;
 #pragma unroll
-        for (int u = 0; u < kBagAhead; ++u) {
-            const long long at = j + u * kBagGroups;
-            const int id = at < end ? ids[at] : -1;
-            const bool ok = at < end && counts(id, vocab, padding_id);
-            count += ok ? 1 : 0;
-#pragma unroll
-            for (int e = 0; e < kPack; ++e) {
-                value[u][e] = 0.0f;
+            for (int u = 0; u < kBagAhead; ++u) {
+                if (left != 0) {
+                    const int next = __builtin_ctzll(left);
+                    left &= left - 1;
+                    const std::int64_t row = __builtin_amdgcn_readlane(id, next);
+                    loadPack(from + row * table_stride, value[u]);
+                    ++taken;
+                }
             }
-            if (ok && has_pack) {
-                loadPack(from + id * table_stride, value[u]);
-            }
-        }
 #pragma unroll
-        for (int u = 0; u < kBagAhead; ++u) {
+            for (int u = 0; u < kBagAhead; ++u) {
+                if (u < taken) {
 #pragma unroll
-            for (int e = 0; e < kPack; ++e) {
-                sum[e] += value[u][e];
+                    for (int e = 0; e < kPack; ++e) {
+                        sum[e] += value[u][e];
+                    }
+                }
             }
         }
     }
+    if constexpr (kShares > 1) {
 #pragma unroll
-    for (int e = 0; e < kPack; ++e) {
-        sums[group][column * kPack + e] = sum[e];
-    }
-    if (column == 0) {
-        found[group] = count;
-    }
-    __syncthreads();
-    if (group == 0 && has_pack) {
-        int total = count;
-        for (int g = 1; g < kBagGroups; ++g) {
+        for (int e = 0; e < kPack; ++e) {
+            sums[wave][lane * kPack + e] = sum[e];
+        }
+        if (lane == 0) {
+            found[wave] = count;
+        }
+        __syncthreads();
+        if (share != 0) {
+            return;
+        }
+        for (int w = 1; w < kShares; ++w) {
 #pragma unroll
             for (int e = 0; e < kPack; ++e) {
-                sum[e] += sums[g][column * kPack + e];
+                sum[e] += sums[wave + w][lane * kPack + e];
             }
-            total += found[g];
+            count += found[wave + w];
         }
-        const float weight = mean && total > 1 ? scale / static_cast<float>(total) : scale;
+    }
+    if (has_pack) {
+        const float weight = mean && count > 1 ? scale / static_cast<float>(count) : scale;
 #pragma unroll
         for (int e = 0; e < kPack; ++e) {
             sum[e] *= weight;
@@ -226,76 +238,85 @@ __device__ __forceinline__ void finishRow(const GradientArgs& args, int key, int
     storePack(sum, to);
 }
 
-// A block sums the chunk's rows, thread t the columns kPack * t and on; the ids and rows are uniform.
-constexpr int kGradientAhead = 8;
+// A wavefront sums one chunk's rows over 64 packs of columns: it reads the chunk's ids and rows at once, a
+// lane each (a chunk is at most 64 positions), and hands them on as scalars; kGradientAhead rows are in
+// flight.
+constexpr int kGradientAhead = 16;
 
 template <typename In, typename Out, int kPack>
-__global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs args) {
-    const int column = (static_cast<int>(blockIdx.y) * kThreads + static_cast<int>(threadIdx.x)) * kPack;
-    const int begin = static_cast<int>(blockIdx.x) * args.chunk;
-    const int end = min(begin + args.chunk, args.count);
-    if (column >= args.dim) {
+__global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs args, long long items, int slices) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const long long item = static_cast<long long>(blockIdx.x) * kWavesPerBlock + wave;
+    if (item >= items) {
         return;
     }
-    const In* from = static_cast<const In*>(args.out_gradient) + column;
-    float* partials = args.partials + static_cast<std::size_t>(blockIdx.x) * 2 * args.dim + column;
-    // the run so far began before this chunk
-    bool continued = begin > 0 && args.keys[begin - 1] == args.keys[begin];
-    int current = args.keys[begin];
+    const int chunk = static_cast<int>(item / slices);
+    const int column = (static_cast<int>(item - static_cast<long long>(chunk) * slices) * kWave + lane) * kPack;
+    const bool has_column = column < args.dim;
+    const int begin = chunk * args.chunk;
+    const int length = min(args.chunk, args.count - begin);
+    const int at = begin + min(lane, length - 1);
+    const int my_key = args.keys[at];
+    const int my_row = args.rows[at];
+    // tokens that do not count stand at the end
+    const int valid = __popcll(__ballot(lane < length && my_key < args.vocab));
+    if (valid == 0) {
+        return;
+    }
+    float my_weight = 1.0f;
+    if (args.bag_counts != nullptr && my_key < args.vocab) {
+        my_weight = 1.0f / static_cast<float>(args.bag_counts[my_row]);
+    }
+    const int key_before = begin > 0 ? args.keys[begin - 1] : -1;
+    const int key_after = begin + length < args.count ? args.keys[begin + length] : args.vocab;
+    const In* from = static_cast<const In*>(args.out_gradient) + (has_column ? column : 0);
+    float* partials = args.partials + static_cast<std::size_t>(chunk) * 2 * args.dim + column;
+    int current = __builtin_amdgcn_readlane(my_key, 0);
+    bool continued = key_before == current;  // the run so far began before this chunk
     float sum[kPack] = {};
-    for (int j = begin; j < end; j += kGradientAhead) {
+    for (int j = 0; j < valid; j += kGradientAhead) {
         float value[kGradientAhead][kPack];
-        int key[kGradientAhead];
 #pragma unroll
         for (int u = 0; u < kGradientAhead; ++u) {
-            const int at = min(j + u, end - 1);
-            key[u] = args.keys[at];
-            const int row = args.rows[at];
-            float weight = 1.0f;
-            if (args.bag_counts != nullptr && key[u] < args.vocab) {
-                weight = 1.0f / static_cast<float>(args.bag_counts[row]);
-            }
-#pragma unroll
-            for (int e = 0; e < kPack; ++e) {
-                value[u][e] = 0.0f;
-            }
-            if (key[u] < args.vocab) {
+            if (j + u < valid) {
+                const std::int64_t row = __builtin_amdgcn_readlane(my_row, j + u);
                 loadPack(from + row * args.out_gradient_stride, value[u]);
-            }
-#pragma unroll
-            for (int e = 0; e < kPack; ++e) {
-                value[u][e] *= weight;
             }
         }
 #pragma unroll
         for (int u = 0; u < kGradientAhead; ++u) {
-            if (j + u < end) {
-                if (key[u] != current) {
-                    if (continued) {
-                        storePack(sum, partials);
-                    } else {
-                        finishRow<Out, kPack>(args, current, column, sum);
+            if (j + u < valid) {
+                const int key = __builtin_amdgcn_readlane(my_key, j + u);
+                if (key != current) {
+                    if (has_column) {
+                        if (continued) {
+                            storePack(sum, partials);
+                        } else {
+                            finishRow<Out, kPack>(args, current, column, sum);
+                        }
                     }
                     continued = false;
-                    current = key[u];
+                    current = key;
 #pragma unroll
                     for (int e = 0; e < kPack; ++e) {
                         sum[e] = 0.0f;
                     }
                 }
+                const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), j + u));
 #pragma unroll
                 for (int e = 0; e < kPack; ++e) {
-                    sum[e] += value[u][e];
+                    sum[e] += value[u][e] * weight;
                 }
             }
         }
     }
-    if (current >= args.vocab) {
-        return;  // tokens that do not count stand at the end
+    if (!has_column) {
+        return;
     }
     if (continued) {
         storePack(sum, partials);
-    } else if (end < args.count && args.keys[end] == current) {
+    } else if (valid == length && key_after == current) {
         storePack(sum, partials + args.dim);
     } else {
         finishRow<Out, kPack>(args, current, column, sum);
@@ -303,10 +324,13 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
 }
 
 // Joins a run that crosses chunks: the block of the chunk where it begins adds that chunk's last sum
-// and the first sums of the chunks it reaches, four wavefronts taking a quarter of those each.
-template <typename Out>
-__global__ __launch_bounds__(kThreads) void gradientJoinKernel(GradientArgs args) {
-    __shared__ float sums[kWavesPerBlock][kWave];
+// and the first sums of the chunks it reaches, its wavefronts taking an equal share of those each.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinWaves = kJoinThreads / kWave;
+
+template <typename Out, int kPack>
+__global__ __launch_bounds__(kJoinThreads) void gradientJoinKernel(GradientArgs args) {
+    __shared__ float sums[kJoinWaves][kWave * kPack];
     const int chunk = blockIdx.x;
     const int next = (chunk + 1) * args.chunk;  // the grid ends before the last chunk
     const int key = args.keys[next - 1];
@@ -330,52 +354,82 @@ __global__ __launch_bounds__(kThreads) void gradientJoinKernel(GradientArgs args
     }
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = threadIdx.x / kWave;
-    const int column = static_cast<int>(blockIdx.y) * kWave + lane;
+    const int column = (static_cast<int>(blockIdx.y) * kWave + lane) * kPack;
     const int reached = last - chunk;
-    const int share = (reached + kWavesPerBlock - 1) / kWavesPerBlock;
+    const int share = (reached + kJoinWaves - 1) / kJoinWaves;
     const int from = chunk + 1 + wave * share;
     const int to = min(from + share, last + 1);
     const std::size_t stride = 2 * static_cast<std::size_t>(args.dim);
-    float sum = 0.0f;
+    float sum[kPack] = {};
     if (column < args.dim) {
         if (wave == 0) {
-            sum = args.partials[chunk * stride + args.dim + column];
+            loadPack(args.partials + chunk * stride + args.dim + column, sum);
         }
 #pragma unroll 8
         for (int c = from; c < to; ++c) {
-            sum += args.partials[c * stride + column];
+            float more[kPack];
+            loadPack(args.partials + c * stride + column, more);
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                sum[e] += more[e];
+            }
         }
     }
-    sums[wave][lane] = sum;
+#pragma unroll
+    for (int e = 0; e < kPack; ++e) {
+        sums[wave][lane * kPack + e] = sum[e];
+    }
     __syncthreads();
     if (wave == 0 && column < args.dim) {
-        for (int w = 1; w < kWavesPerBlock; ++w) {
-            sum += sums[w][lane];
+        for (int w = 1; w < min(kJoinWaves, reached); ++w) {
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                sum[e] += sums[w][lane * kPack + e];
+            }
         }
-        float one[1] = {sum};
-        finishRow<Out, 1>(args, key, column, one);
+        finishRow<Out, kPack>(args, key, column, sum);
     }
 }
 
-// Zeros for rows [0, vocab) of the gradient, in packs as in the lookup.
+// Zeros for the rows of the gradient, written beside the sort: launch l of the sort's takes an equal part
+// of the packs.
 template <typename Out, int kPack>
-__global__ __launch_bounds__(kThreads) void clearRowsKernel(Out* __restrict__ out, std::int64_t stride, long long packs,
-                                                            int packs_per_row) {
-    const float zeros[kPack] = {};
-    const long long first = static_cast<long long>(blockIdx.x) * (kThreads * kLookupPacks);
-    const long long first_row = first / packs_per_row;
-    const unsigned first_pack = static_cast<unsigned>(first - first_row * packs_per_row);
-    const int left = static_cast<int>(min(packs - first, static_cast<long long>(kThreads * kLookupPacks)));
-#pragma unroll
-    for (int u = 0; u < kLookupPacks; ++u) {
-        const int i = u * kThreads + static_cast<int>(threadIdx.x);
-        if (i < left) {
-            const unsigned at = first_pack + static_cast<unsigned>(i);
-            const unsigned row = at / static_cast<unsigned>(packs_per_row);
-            const unsigned pack = at - row * static_cast<unsigned>(packs_per_row);
-            storePack(zeros, out + (first_row + row) * stride + static_cast<std::int64_t>(pack) * kPack);
+struct ClearRows {
+    static constexpr int kBlocks = 768;
+    Out* out;  // null: nothing to clear
+    std::int64_t stride;
+    long long packs;
+    int packs_per_row;
+
+    __device__ void run(int block, int blocks, int launch, int launches) const {
+        if (out == nullptr) {
+            return;
+        }
+        const long long begin = packs * launch / launches;
+        const long long end = packs * (launch + 1) / launches;
+        const float zeros[kPack] = {};
+        const long long step = static_cast<long long>(blocks) * blockDim.x;
+        long long at = begin + static_cast<long long>(block) * blockDim.x + threadIdx.x;
+        long long row = at / packs_per_row;
+        int pack = static_cast<int>(at - row * packs_per_row);
+        const long long row_step = step / packs_per_row;
+        const int pack_step = static_cast<int>(step - row_step * packs_per_row);
+        for (; at < end; at += step) {
+            storePack(zeros, out + row * stride + static_cast<std::int64_t>(pack) * kPack);
+            row += row_step;
+            pack += pack_step;
+            if (pack >= packs_per_row) {
+                pack -= packs_per_row;
+                ++row;
+            }
         }
     }
+};
+
+// The same without a sort, for a gradient of no tokens.
+template <typename Out, int kPack>
+__global__ __launch_bounds__(kThreads) void clearRowsKernel(ClearRows<Out, kPack> clear) {
+    clear.run(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), 0, 1);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -398,7 +452,7 @@ int checkEmbedding(const zcgvs_embedding_desc* desc) {
         return invalid("vocab must be below 2^31 - 1");
     }
     if (desc->token_count < 0 || desc->token_count > kMaxTokens) {
-        return invalid("token_count must lie in [0, 2^29]");
+        return invalid("token_count must lie in [0, 2^28]");
     }
     if (desc->bag_offsets != nullptr && (desc->bag_count < 0 || desc->bag_count > INT32_MAX)) {
         return invalid("bag_count must lie in [0, 2^31 - 1]");
@@ -438,13 +492,19 @@ int lookupTyped(const zcgvs_embedding_desc& d, Out* out, std::int64_t out_stride
         lookupKernel<In, Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
             table, table_stride, d.vocab, packs_per_row, d.ids, packs, d.padding_id, d.scale, out, out_stride);
     } else {
-        const int slices = (packs_per_row + kBagColumns - 1) / kBagColumns;
-        const std::int64_t most = std::max<std::int64_t>(1, kMaxBlocks / slices);
+        const int slices = (packs_per_row + kWave - 1) / kWave;
+        // a wavefront a bag where that keeps the GPU's memory busy, else four
+        const bool alone = d.bag_count * slices >= 16ll * deviceComputeUnits();
+        const int items_per_block = alone ? kWavesPerBlock : 1;
+        const std::int64_t most = std::max<std::int64_t>(1, kMaxBlocks * items_per_block / slices);
         for (std::int64_t bag = 0; bag < d.bag_count; bag += most) {
-            const unsigned bags = static_cast<unsigned>(std::min<std::int64_t>(most, d.bag_count - bag));
-            bagKernel<In, Out, kPack><<<bags * static_cast<unsigned>(slices), kThreads, 0, stream>>>(
-                table, table_stride, d.vocab, packs_per_row, d.ids, d.token_count, d.bag_offsets + bag, slices,
-                d.reduce == ZCGVS_EMBEDDING_MEAN, d.padding_id, d.scale, out + bag * out_stride, out_stride);
+            const long long items = std::min<std::int64_t>(most, d.bag_count - bag) * slices;
+            const unsigned blocks = static_cast<unsigned>((items + items_per_block - 1) / items_per_block);
+            const auto kernel = alone ? bagKernel<In, Out, kPack, 1> : bagKernel<In, Out, kPack, kWavesPerBlock>;
+            kernel<<<blocks, kThreads, 0, stream>>>(table, table_stride, d.vocab, packs_per_row, d.ids, d.token_count,
+                                                    d.bag_offsets + bag, items, slices,
+                                                    d.reduce == ZCGVS_EMBEDDING_MEAN, d.padding_id, d.scale,
+                                                    out + bag * out_stride, out_stride);
         }
     }
     ZCGVS_LAUNCH_CHECK("embedding lookup");
@@ -492,8 +552,9 @@ unsigned clearBlocks(long long words) {
 }
 
 // Sorts the tokens; *keys and *rows are where the sorted pairs stand.
+template <class Side>
 int sortTokens(const zcgvs_embedding_desc& d, const GradientSpace& s, char* workspace, const int** keys,
-               const int** rows, hipStream_t stream) {
+               const int** rows, const Side& side, hipStream_t stream) {
     const int n = static_cast<int>(d.token_count);
     SortInput input{};
     input.keys = d.ids;
@@ -515,32 +576,43 @@ int sortTokens(const zcgvs_embedding_desc& d, const GradientSpace& s, char* work
         input.rows = bag_rows;
         input.raw = false;
     }
-    return sortPairs(input, workspace + s.sort, keys, rows, stream);
+    return sortPairs(input, workspace + s.sort, keys, rows, side, stream);
 }
 
 template <typename In, typename Out, int kPack>
-int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, GradientArgs args, hipStream_t stream) {
+int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, GradientArgs args, char* workspace,
+                  hipStream_t stream) {
+    ClearRows<Out, kPack> clear{};
     if (!args.accumulate) {
-        const int packs_per_row = d.dim / kPack;
-        const long long packs = static_cast<long long>(d.vocab) * packs_per_row;
-        const long long blocks = (packs + kThreads * kLookupPacks - 1) / (kThreads * kLookupPacks);
-        if (blocks > kMaxBlocks) {
-            return invalid("more output than one launch can write");
-        }
-        clearRowsKernel<Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            static_cast<Out*>(args.table_gradient), args.table_gradient_stride, packs, packs_per_row);
-        ZCGVS_LAUNCH_CHECK("embedding gradient");
+        clear.out = static_cast<Out*>(args.table_gradient);
+        clear.stride = args.table_gradient_stride;
+        clear.packs_per_row = d.dim / kPack;
+        clear.packs = static_cast<long long>(d.vocab) * clear.packs_per_row;
     }
     if (args.count == 0) {
+        if (clear.out != nullptr) {
+            clearRowsKernel<Out, kPack><<<ClearRows<Out, kPack>::kBlocks, kThreads, 0, stream>>>(clear);
+            ZCGVS_LAUNCH_CHECK("embedding gradient");
+        }
         return ZCGVS_OK;
     }
+    const int sorted = args.accumulate ? sortTokens(d, s, workspace, &args.keys, &args.rows, NoSideWork{}, stream)
+                                       : sortTokens(d, s, workspace, &args.keys, &args.rows, clear, stream);
+    if (sorted != ZCGVS_OK) {
+        return sorted;
+    }
     const int chunks = static_cast<int>((static_cast<long long>(args.count) + s.chunk - 1) / s.chunk);
-    const unsigned columns = static_cast<unsigned>((d.dim + kThreads * kPack - 1) / (kThreads * kPack));
-    gradientChunkKernel<In, Out, kPack><<<dim3(static_cast<unsigned>(chunks), columns), kThreads, 0, stream>>>(args);
+    const int slices = (d.dim / kPack + kWave - 1) / kWave;
+    const long long items = static_cast<long long>(chunks) * slices;
+    const long long blocks = (items + kWavesPerBlock - 1) / kWavesPerBlock;
+    if (blocks > kMaxBlocks) {
+        return invalid("more tokens than one launch can take");
+    }
+    gradientChunkKernel<In, Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(args, items, slices);
     ZCGVS_LAUNCH_CHECK("embedding gradient");
     if (chunks > 1) {
-        const unsigned slices = static_cast<unsigned>((d.dim + kWave - 1) / kWave);
-        gradientJoinKernel<Out><<<dim3(static_cast<unsigned>(chunks - 1), slices), kThreads, 0, stream>>>(args);
+        gradientJoinKernel<Out, kPack><<<dim3(static_cast<unsigned>(chunks - 1), static_cast<unsigned>(slices)),
+                                         kJoinThreads, 0, stream>>>(args);
         ZCGVS_LAUNCH_CHECK("embedding gradient");
     }
     return ZCGVS_OK;
@@ -640,10 +712,6 @@ int zcgvs_embedding_gradient(const zcgvs_embedding_desc* desc, const void* d_out
     char* workspace = static_cast<char*>(d_workspace);
     GradientArgs args{};
     if (!no_tokens) {
-        const int sorted = sortTokens(d, space, workspace, &args.keys, &args.rows, toStream(stream));
-        if (sorted != ZCGVS_OK) {
-            return sorted;
-        }
         args.partials = reinterpret_cast<float*>(workspace + space.partials);
     }
     args.count = no_tokens ? 0 : static_cast<int>(d.token_count);
@@ -666,8 +734,8 @@ int zcgvs_embedding_gradient(const zcgvs_embedding_desc* desc, const void* d_out
         return withElement(table_gradient_dtype, [&](auto element) {
             using Out = decltype(element);
             if constexpr (std::is_same_v<Out, In> || std::is_same_v<Out, float>) {
-                return pack == 4 ? gradientTyped<In, Out, 4>(d, space, args, toStream(stream))
-                                 : gradientTyped<In, Out, 1>(d, space, args, toStream(stream));
+                return pack == 4 ? gradientTyped<In, Out, 4>(d, space, args, workspace, toStream(stream))
+                                 : gradientTyped<In, Out, 1>(d, space, args, workspace, toStream(stream));
             } else {
                 return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above
             }

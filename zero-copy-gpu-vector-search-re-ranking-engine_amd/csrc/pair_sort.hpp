@@ -21,10 +21,9 @@ namespace {
 
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
-constexpr int kSortThreads = 256;
+constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr int kSortItems = 1024;
-constexpr int kSortRounds = kSortItems / kSortThreads;
+constexpr int kSortItems = kSortThreads;  // an item a thread
 constexpr int kMaxTiles = 256;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallWaves = kSmallThreads / kWave;
@@ -98,11 +97,23 @@ __device__ __forceinline__ unsigned digitRank(unsigned digit, int bits, bool ok,
     return before + static_cast<unsigned>(below);
 }
 
+// What a sort's launches do beside it: sorting waits on latency and leaves the memory idle. Blocks past the
+// sort's own call run(block, blocks) with what is theirs of launch `launch` out of `launches`.
+struct NoSideWork {
+    static constexpr int kBlocks = 0;
+    __device__ void run(int, int, int, int) const {}
+};
+
 // ---- one workgroup ------------------------------------------------------------------------------
 
+template <class Side>
 __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(SortInput in, int bits, int passes,
                                                                  int* __restrict__ keys_out,
-                                                                 int* __restrict__ rows_out) {
+                                                                 int* __restrict__ rows_out, Side side) {
+    if (blockIdx.x > 0) {
+        side.run(static_cast<int>(blockIdx.x) - 1, static_cast<int>(gridDim.x) - 1, 0, 1);
+        return;
+    }
     __shared__ int keys[2][kSmallItems];
     __shared__ std::uint16_t places[2][kSmallItems];
     __shared__ unsigned seen[kSmallWaves][kDigits];
@@ -184,10 +195,18 @@ struct SortPass {
     int tiles;
     int shift;
     int bits;
+    int launch;    // of this pass's count; its placement is the next one
+    int launches;
 };
 
-__global__ __launch_bounds__(kSortThreads) void sortCountKernel(SortPass pass) {
+template <class Side>
+__global__ __launch_bounds__(kSortThreads) void sortCountKernel(SortPass pass, Side side) {
     __shared__ unsigned histogram[kDigits];
+    if (static_cast<int>(blockIdx.x) >= pass.tiles) {
+        side.run(static_cast<int>(blockIdx.x) - pass.tiles, static_cast<int>(gridDim.x) - pass.tiles, pass.launch,
+                 pass.launches);
+        return;
+    }
     for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
         histogram[d] = 0;
     }
@@ -204,19 +223,27 @@ __global__ __launch_bounds__(kSortThreads) void sortCountKernel(SortPass pass) {
     }
 }
 
-__global__ __launch_bounds__(kSortThreads) void sortPlaceKernel(SortPass pass) {
+template <class Side>
+__global__ __launch_bounds__(kSortThreads) void sortPlaceKernel(SortPass pass, Side side) {
     __shared__ unsigned start[kDigits];
     __shared__ unsigned seen[kSortWaves][kDigits];
     __shared__ unsigned wave_sums[kSortWaves];
-    const int lane = threadIdx.x & (kWave - 1);
+    if (static_cast<int>(blockIdx.x) >= pass.tiles) {
+        side.run(static_cast<int>(blockIdx.x) - pass.tiles, static_cast<int>(gridDim.x) - pass.tiles, pass.launch + 1,
+                 pass.launches);
+        return;
+    }
     const int wave = threadIdx.x / kWave;
-    // digits of smaller value in all tiles, then the same digit in the tiles before this one; thread t
-    // holds the neighbouring digits 2 t and 2 t + 1
-    static_assert(kDigits == 2 * kSortThreads, "two digits a thread");
+    // digits of smaller value in all tiles, then the same digit in the tiles before this one: thread t adds
+    // up digits 2 t' and 2 t' + 1 (t' = t % 256) over every fourth tile
+    constexpr int kGroups = kSortThreads / (kDigits / 2);
+    static_assert(kGroups * 2 * kDigits <= kSortWaves * kDigits, "the groups' sums fit where `seen` stands");
+    const int pair = static_cast<int>(threadIdx.x) % (kDigits / 2);
+    const int group = static_cast<int>(threadIdx.x) / (kDigits / 2);
     unsigned total[2] = {0, 0}, before[2] = {0, 0};
-    const uint2* counts_of = reinterpret_cast<const uint2*>(pass.tile_counts) + threadIdx.x;
+    const uint2* counts_of = reinterpret_cast<const uint2*>(pass.tile_counts) + pair;
 #pragma unroll 8
-    for (int t = 0; t < pass.tiles; ++t) {
+    for (int t = group; t < pass.tiles; t += kGroups) {
         const uint2 c = counts_of[static_cast<std::size_t>(t) * (kDigits / 2)];
         total[0] += c.x;
         total[1] += c.y;
@@ -225,49 +252,54 @@ __global__ __launch_bounds__(kSortThreads) void sortPlaceKernel(SortPass pass) {
             before[1] += c.y;
         }
     }
-    const unsigned base = blockPrefix(total[0] + total[1], wave_sums);
-    start[2 * threadIdx.x] = base + before[0];
-    start[2 * threadIdx.x + 1] = base + total[0] + before[1];
+    unsigned* sums = &seen[0][0];  // [groups][2][digits]
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        sums[(group * 2 + 0) * kDigits + 2 * pair + e] = total[e];
+        sums[(group * 2 + 1) * kDigits + 2 * pair + e] = before[e];
+    }
+    __syncthreads();
+    unsigned all = 0, earlier = 0;
+    if (threadIdx.x < kDigits) {
+        for (int g = 0; g < kGroups; ++g) {
+            all += sums[(g * 2 + 0) * kDigits + threadIdx.x];
+            earlier += sums[(g * 2 + 1) * kDigits + threadIdx.x];
+        }
+    }
+    const unsigned base = blockPrefix(all, wave_sums);
+    if (threadIdx.x < kDigits) {
+        start[threadIdx.x] = base + earlier;
+    }
     const int begin = static_cast<int>(blockIdx.x) * pass.tile_items;
     const int end = min(begin + pass.tile_items, pass.in.count);
     const unsigned mask = (1u << pass.bits) - 1u;
     for (int first = begin; first < end; first += kSortItems) {
+        __syncthreads();
         for (int d = threadIdx.x; d < kDigits * kSortWaves; d += kSortThreads) {
             (&seen[0][0])[d] = 0;
         }
         __syncthreads();
-        // a wavefront owns kSortRounds * 64 consecutive items
-        int key[kSortRounds];
-        unsigned rank[kSortRounds];
-#pragma unroll
-        for (int round = 0; round < kSortRounds; ++round) {
-            const int i = first + (wave * kSortRounds + round) * kWave + lane;
-            const bool ok = i < end;
-            key[round] = ok ? sortKey(pass.in, i) : 0;
-            rank[round] = digitRank((static_cast<unsigned>(key[round]) >> pass.shift) & mask, pass.bits, ok, seen[wave]);
-        }
+        const int i = first + static_cast<int>(threadIdx.x);
+        const bool ok = i < end;
+        const int key = ok ? sortKey(pass.in, i) : 0;
+        const unsigned digit = (static_cast<unsigned>(key) >> pass.shift) & mask;
+        const unsigned rank = digitRank(digit, pass.bits, ok, seen[wave]);
         __syncthreads();
-        for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
-            unsigned at = start[d];
+        if (threadIdx.x < kDigits) {
+            unsigned at = start[threadIdx.x];
             for (int w = 0; w < kSortWaves; ++w) {
-                const unsigned here = seen[w][d];
-                seen[w][d] = at;
+                const unsigned here = seen[w][threadIdx.x];
+                seen[w][threadIdx.x] = at;
                 at += here;
             }
-            start[d] = at;
+            start[threadIdx.x] = at;
         }
         __syncthreads();
-#pragma unroll
-        for (int round = 0; round < kSortRounds; ++round) {
-            const int i = first + (wave * kSortRounds + round) * kWave + lane;
-            if (i < end) {
-                const unsigned digit = (static_cast<unsigned>(key[round]) >> pass.shift) & mask;
-                const unsigned at = seen[wave][digit] + rank[round];
-                pass.keys_out[at] = key[round];
-                pass.rows_out[at] = pass.in.rows == nullptr ? i : pass.in.rows[i];
-            }
+        if (ok) {
+            const unsigned at = seen[wave][digit] + rank;
+            pass.keys_out[at] = key;
+            pass.rows_out[at] = pass.in.rows == nullptr ? i : pass.in.rows[i];
         }
-        __syncthreads();
     }
 }
 
@@ -281,7 +313,8 @@ inline std::size_t pairSortBytes(std::size_t count) {
 }
 
 // Sorts count >= 1 pairs (at most 2^29); *keys and *rows are where they then stand, in `scratch`.
-inline int sortPairs(SortInput in, char* scratch, const int** keys, const int** rows, hipStream_t stream) {
+template <class Side>
+int sortPairs(SortInput in, char* scratch, const int** keys, const int** rows, const Side& side, hipStream_t stream) {
     const std::size_t n = static_cast<std::size_t>(in.count);
     const std::size_t one = sortAligned(n * 4);
     int* key_buffer[2] = {reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + one)};
@@ -292,7 +325,8 @@ inline int sortPairs(SortInput in, char* scratch, const int** keys, const int** 
     }
     const int passes = (bits + kDigitBits - 1) / kDigitBits;
     if (in.count <= kSmallItems) {
-        sortSmallKernel<<<1, kSmallThreads, 0, stream>>>(in, bits, passes, key_buffer[0], row_buffer[0]);
+        sortSmallKernel<Side><<<1 + Side::kBlocks, kSmallThreads, 0, stream>>>(in, bits, passes, key_buffer[0],
+                                                                              row_buffer[0], side);
         ZCGVS_LAUNCH_CHECK("sort");
         *keys = key_buffer[0];
         *rows = row_buffer[0];
@@ -310,9 +344,12 @@ inline int sortPairs(SortInput in, char* scratch, const int** keys, const int** 
         pass.bits = std::min(per_pass, bits - pass.shift);
         pass.keys_out = key_buffer[p & 1];
         pass.rows_out = row_buffer[p & 1];
-        sortCountKernel<<<static_cast<unsigned>(pass.tiles), kSortThreads, 0, stream>>>(pass);
+        pass.launch = 2 * p;
+        pass.launches = 2 * passes;
+        const unsigned blocks = static_cast<unsigned>(pass.tiles + Side::kBlocks);
+        sortCountKernel<Side><<<blocks, kSortThreads, 0, stream>>>(pass, side);
         ZCGVS_LAUNCH_CHECK("sort");
-        sortPlaceKernel<<<static_cast<unsigned>(pass.tiles), kSortThreads, 0, stream>>>(pass);
+        sortPlaceKernel<Side><<<blocks, kSortThreads, 0, stream>>>(pass, side);
         ZCGVS_LAUNCH_CHECK("sort");
         pass.in.keys = pass.keys_out;
         pass.in.rows = pass.rows_out;
