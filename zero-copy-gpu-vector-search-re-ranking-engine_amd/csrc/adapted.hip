@@ -4,8 +4,8 @@
 //
 // The rows are sorted by adapter, so that rows of one adapter are next to each other in any batch, and
 // x and out are addressed through the order. `low` = scale_a x[r] down_a^T is formed first, one group of
-// up to 16 rows of one adapter at a time; the projection's kernel then starts each tile's sums with
-// low up_a^T and adds x weight^T on top: one read of x and one write of out for both.
+// up to 16 rows of one adapter at a time; the projection's kernel then adds low up_a^T to each tile's
+// sums: out is written once for both.
 //
 // low between the two products. The products are the 16-bit matrix instructions', so low is handed over
 // in parts of the operands' type, high + rest (+ rest of that), as many as keep a float32 output's digits:
@@ -86,12 +86,23 @@ __device__ __forceinline__ typename Fragment<T>::type loadChunk(const T* from, i
     return v;
 }
 
+// The same where the row has `stored` values from `from` on, of which the first `valid` are wanted.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::type loadMasked(const T* from, int stored, int valid) {
+    typename Fragment<T>::type v = loadChunk(from, stored);
+#pragma unroll
+    for (int e = 0; e < kChunk<T>; ++e) {
+        v[e] = e < valid ? v[e] : static_cast<T>(0.0f);
+    }
+    return v;
+}
+
 // ---- low = scale x down^T -----------------------------------------------------------------------
 
-// A workgroup looks at kLowPositions sorted positions; each that begins a group (the first of its
-// adapter or of a block of 16) makes it form the group's rows of low. The four wavefronts take a quarter
-// of the steps over dim each and their sums are joined through LDS.
-constexpr int kLowThreads = 256;
+// A workgroup takes the groups that begin among `positions` sorted positions (1, or a block of 16; a group is
+// the rows of one adapter within a block). Its eight wavefronts take an eighth of the steps over dim each and
+// their sums are joined through LDS.
+constexpr int kLowThreads = 512;
 constexpr int kLowWaves = kLowThreads / kWave;
 
 template <typename T, int kRankBlocks>
@@ -107,23 +118,26 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
     constexpr int kStepK = 4 * kChunk<T>;
     const int steps = (args.dim + kStepK - 1) / kStepK;
     const int share = (steps + kLowWaves - 1) / kLowWaves;
-    const int first_position = static_cast<int>(blockIdx.x) * positions;
-    const int past_position = min(first_position + positions, args.rows);
-    for (int p = first_position; p < past_position; ++p) {
-        const int adapter = args.adapters[p];
-        if (adapter >= args.adapter_count) {
-            return;  // rows without an adapter stand at the end
-        }
-        if (p % 16 != 0 && args.adapters[p - 1] == adapter) {
-            continue;
-        }
-        const int most = min(16 - p % 16, args.rows - p);
-        int length = 1;
-        while (length < most && args.adapters[p + length] == adapter) {
-            ++length;
-        }
+    const int first = static_cast<int>(blockIdx.x) * positions;
+    const int block = first / 16 * 16;
+    const int in_block = min(16, args.rows - block);
+    // the block's adapters, a lane each
+    const int at = block + min(r16, in_block - 1);
+    const int my_adapter = args.adapters[at];
+    const int my_row = args.order[at];
+    const int adapter_before = __shfl_up(my_adapter, 1, kWave);
+    const unsigned begins = static_cast<unsigned>(
+        __ballot(lane < in_block && my_adapter < args.adapter_count && (lane == 0 || my_adapter != adapter_before)));
+    unsigned left = positions == 1 ? begins & (1u << (first - block)) : begins;
+    while (left != 0) {
+        const int start = __builtin_ctz(left);
+        left &= left - 1;
+        const int adapter = __builtin_amdgcn_readlane(my_adapter, start);
+        const int length = __popcll(__ballot(lane < in_block && my_adapter == adapter));
+        const int p = block + start;
         const int rank = rankOf(args, adapter);
-        const T* x = static_cast<const T*>(args.x) + args.order[p + min(r16, length - 1)] * args.x_stride;
+        const T* x = static_cast<const T*>(args.x) +
+                     __shfl(my_row, start + min(r16, length - 1), kWave) * args.x_stride;
         const T* down = static_cast<const T*>(args.down) +
                         static_cast<std::int64_t>(adapter) * args.max_rank * args.dim;
         f32x4 sums[kRankBlocks];
@@ -172,8 +186,8 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
             }
         }
         __syncthreads();
-        // 16 threads a row
-        const int row = static_cast<int>(threadIdx.x) / 16;
+        // 16 threads a row; the others look on
+        const int row = static_cast<int>(threadIdx.x) / 16 % 16;
         const int column = static_cast<int>(threadIdx.x) % 16;
         const float scale = args.scales == nullptr ? 1.0f : args.scales[adapter];
         float value[kRankBlocks];
@@ -190,14 +204,14 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
             peak = fmaxf(peak, fabsf(value[j]));
         }
         if constexpr (sizeof(T) == 2) {
-            row_peak[row][column] = peak;
+            row_peak[row][column] = peak;  // the same from both halves of the workgroup
             __syncthreads();
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
                 peak = fmaxf(peak, row_peak[row][c]);
             }
         }
-        if (row < length) {
+        if (row < length && threadIdx.x < 256) {
             const std::int64_t at = p + row;
             if constexpr (sizeof(T) == 2) {
                 int exponent = 0;
@@ -253,56 +267,92 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
 
 // ---- the projection -----------------------------------------------------------------------------
 
-// Starts a wavefront's sums with low up^T, in one of two ways.
-// By adapter: one adapter of the wavefront's rows after the other, for each the matrix products of all its
-// rows with the adapter's up, kept in the rows that are the adapter's. An adapter costs about 1.2 us, the
-// latency of its rank and of its up.
-// By row: every lane forms its own results, 4 columns of a row, from its row's adapter. That costs a fused
-// multiply-add for each rank and result (64 x 32 results of rank 32 about 3 us), whatever the adapters, and
-// is taken where the wavefront's rows have many of them.
+// Adds low up^T to a tile's sums, in one of two ways.
+// By adapter: one adapter of the tile's rows after the other. Its rows of low (zeros for the other rows) and
+// its columns of up go through LDS like a stage of the products over dim, and the result is kept in the rows
+// that are the adapter's. An adapter costs about 1.6 us for every 64 values of low's parts (float32: 32).
+// By row: every lane forms its own results, 4 columns of a row, from its row's adapter: a fused
+// multiply-add for each rank and result (64 x 32 results of rank 32 about 3 us), whatever the adapters; taken
+// where the tile's rows have many.
+// Every thread of the workgroup calls it, behind the products over dim.
+
+// A tile's rows, 64 to a register: their adapters (adapter_count: none), ranks and low's scales. Read before
+// the products over dim, behind which the latency is gone.
+template <int kTileRows>
+struct TileAdapters {
+    static constexpr int kSets = kTileRows / kWave;
+    int adapter[kSets];
+    int rank[kSets];
+    float scale[kSets];
+    int changes;  // rows whose adapter is not that of the row before
+
+    __device__ __forceinline__ void read(const AdaptedArgs& args, int m0) {
+        const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+        int before[kSets];
+#pragma unroll
+        for (int i = 0; i < kSets; ++i) {
+            const int p = min(m0 + i * kWave + lane, args.rows - 1);
+            adapter[i] = args.adapters[p];
+            before[i] = args.adapters[max(p - 1, 0)];
+            scale[i] = args.low_scale[p];
+        }
+        changes = 0;
+#pragma unroll
+        for (int i = 0; i < kSets; ++i) {
+            adapter[i] = m0 + i * kWave + lane < args.rows ? adapter[i] : args.adapter_count;
+            const bool has = adapter[i] < args.adapter_count;
+            rank[i] = has ? rankOf(args, adapter[i]) : 0;
+            scale[i] = has ? scale[i] : 0.0f;
+            changes += __popcll(__ballot(has && adapter[i] != before[i]));
+        }
+    }
+    // Of the tile's row `row`, which may differ from lane to lane.
+    template <typename V>
+    static __device__ __forceinline__ V at(const V (&values)[kSets], int row) {
+        V value = __shfl(values[0], row % kWave, kWave);
+#pragma unroll
+        for (int i = 1; i < kSets; ++i) {
+            const V other = __shfl(values[i], row % kWave, kWave);
+            value = row / kWave == i ? other : value;
+        }
+        return value;
+    }
+};
+
 template <class Tile, typename Out>
-__device__ __forceinline__ void addAdapters(const AdaptedArgs& args, int m0, int n0, typename Tile::Sums& sums) {
+__device__ __forceinline__ void addAdapters(const AdaptedArgs& args, const TileAdapters<Tile::kM>& rows,
+                                            std::uint8_t* lds, int m0, int n0, typename Tile::Sums& sums) {
     using T = typename Tile::T;
-    constexpr int kStepR = 4 * kChunk<T>;
     constexpr int kHere = kParts<T, Out>;
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int r16 = lane & 15;
     const int h = lane >> 4;
-    int adapter[Tile::kBlocksM];
-    float scale[Tile::kBlocksM];
-    int first = args.adapter_count;  // the smallest adapter of the wavefront's rows
-    int changes = 0;                 // rows whose adapter is not that of the row before
-#pragma unroll
-    for (int i = 0; i < Tile::kBlocksM; ++i) {
-        const int p = m0 + i * 16 + r16;
-        adapter[i] = p < args.rows ? args.adapters[p] : args.adapter_count;
-        const int before = p > 0 && p < args.rows ? args.adapters[p - 1] : adapter[i];
-        scale[i] = adapter[i] < args.adapter_count ? args.low_scale[p] : 0.0f;
-        changes += __popcll(__ballot(adapter[i] < args.adapter_count && adapter[i] != before)) / 4;
-        first = min(first, adapter[i]);
+    int left = __builtin_amdgcn_readfirstlane(rows.adapter[0]);  // sorted: the first row's is the smallest
+    if (left >= args.adapter_count) {
+        return;
     }
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        first = min(first, __shfl_xor(first, d, kWave));
-    }
-    int left = __builtin_amdgcn_readfirstlane(first);
-    if (changes > 2 + args.max_rank / 8) {
+    const int wave_row = Tile::waveM() * Tile::kBlocksM * 16 + r16;
+    if (rows.changes > 2 + args.max_rank / 8) {
+        const int wave_n0 = n0 + Tile::waveN() * Tile::kBlocksN * 16 + 4 * h;
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
-            const int p = min(m0 + i * 16 + r16, args.rows - 1);
-            const bool has = adapter[i] < args.adapter_count;
-            const int mine = has ? adapter[i] : 0;
-            const int rank = has ? rankOf(args, mine) : 0;
-            const T* low = static_cast<const T*>(args.low) + static_cast<std::int64_t>(p) * kHere * args.padded_rank;
-            const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(mine) * args.out_dim * args.max_rank;
+            const int row = wave_row + i * 16;
+            const int adapter = TileAdapters<Tile::kM>::at(rows.adapter, row);
+            const int rank = TileAdapters<Tile::kM>::at(rows.rank, row);
+            const float scale = TileAdapters<Tile::kM>::at(rows.scale, row);
+            // a row without an adapter has rank 0
+            const T* low = static_cast<const T*>(args.low) +
+                           static_cast<std::int64_t>(m0 + row) * kHere * args.padded_rank;
+            const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(adapter) * args.out_dim * args.max_rank;
+#pragma unroll 1
             for (int r = 0; r < rank; r += kChunk<T>) {
                 float values[kChunk<T>];
 #pragma unroll
-                for (int part = 0; part < kHere; ++part) {
-                    const auto v = *reinterpret_cast<const typename Fragment<T>::type*>(low + part * args.padded_rank + r);
+                for (int half = 0; half < kHere; ++half) {
+                    const auto v = *reinterpret_cast<const typename Fragment<T>::type*>(low + half * args.padded_rank + r);
 #pragma unroll
                     for (int e = 0; e < kChunk<T>; ++e) {
-                        values[e] = (part == 0 ? 0.0f : values[e]) + static_cast<float>(v[e]);
+                        values[e] = (half == 0 ? 0.0f : values[e]) + static_cast<float>(v[e]) * scale;
                     }
                 }
 #pragma unroll
@@ -310,8 +360,8 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, int m0, int
                     typename Fragment<T>::type b[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int n = min(n0 + j * 16 + 4 * h + e, args.out_dim - 1);
-                        b[e] = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + r, rank - r);
+                        const int n = min(wave_n0 + j * 16 + e, args.out_dim - 1);
+                        b[e] = loadMasked(up + static_cast<std::int64_t>(n) * args.max_rank + r, args.max_rank - r, rank - r);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -322,69 +372,85 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, int m0, int
                     }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                sums[i][j] *= scale[i];
-            }
         }
         return;
     }
+    using SideA = typename Tile::SideA;
+    using SideB = typename Tile::SideB;
+    const int low_values = kHere * args.padded_rank;
     while (left < args.adapter_count) {
-        const int rank = rankOf(args, left);
+        int rank = 0;
+        int next = args.adapter_count;
+#pragma unroll
+        for (int i = 0; i < TileAdapters<Tile::kM>::kSets; ++i) {
+            const unsigned long long mine = __ballot(rows.adapter[i] == left);
+            const unsigned long long later = __ballot(rows.adapter[i] > left);
+            rank = mine != 0 ? __builtin_amdgcn_readlane(rows.rank[i], __builtin_ctzll(mine)) : rank;
+            if (later != 0) {  // the first of them is the next
+                next = min(next, __builtin_amdgcn_readlane(rows.adapter[i], __builtin_ctzll(later)));
+            }
+        }
         const T* up = static_cast<const T*>(args.up) + static_cast<std::int64_t>(left) * args.out_dim * args.max_rank;
         typename Tile::Sums part;
         Tile::clear(part);
-        for (int r = 0; r < rank; r += kStepR) {
-            const int at = r + h * kChunk<T>;
-            typename Fragment<T>::type a[Tile::kBlocksM][kHere], b[Tile::kBlocksN];
+#pragma unroll 1
+        for (int k0 = 0; k0 < low_values; k0 += kStageK<T>) {
+            typename Fragment<T>::type a[SideA::kCopies], b[SideB::kCopies];
 #pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                const int n = min(n0 + j * 16 + r16, args.out_dim - 1);
-                b[j] = loadChunk(up + static_cast<std::int64_t>(n) * args.max_rank + at, rank - at);
-            }
-#pragma unroll
-            for (int i = 0; i < Tile::kBlocksM; ++i) {
-                const std::int64_t p = min(m0 + i * 16 + r16, args.rows - 1);
-#pragma unroll
-                for (int e = 0; e < kHere; ++e) {
-                    a[i][e] = *reinterpret_cast<const typename Fragment<T>::type*>(
-                        static_cast<const T*>(args.low) + (p * kHere + e) * args.padded_rank + at);
+            for (int i = 0; i < SideA::kCopies; ++i) {
+                int row, chunk;
+                SideA::placeOf(i, row, chunk);
+                const int k = k0 + chunk * kChunk<T>;
+                const bool mine = TileAdapters<Tile::kM>::at(rows.adapter, row) == left && k < low_values;
+                a[i] = typename Fragment<T>::type{};
+                if (mine) {
+                    a[i] = *reinterpret_cast<const typename Fragment<T>::type*>(
+                        static_cast<const T*>(args.low) + static_cast<std::int64_t>(m0 + row) * low_values + k);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < Tile::kBlocksM; ++i) {
-#pragma unroll
-                for (int e = 0; e < kHere; ++e) {
-#pragma unroll
-                    for (int j = 0; j < Tile::kBlocksN; ++j) {
-                        part[i][j] = multiplyAdd(b[j], a[i][e], part[i][j]);
-                    }
-                }
+            for (int i = 0; i < SideB::kCopies; ++i) {
+                int row, chunk;
+                SideB::placeOf(i, row, chunk);
+                const int n = min(n0 + row, args.out_dim - 1);
+                const int k = k0 + chunk * kChunk<T>;
+                const int r = k % args.padded_rank;  // every part meets the same columns of up
+                b[i] = loadMasked(up + static_cast<std::int64_t>(n) * args.max_rank + r,
+                                  k < low_values ? args.max_rank - r : 0, rank - r);
             }
+            __syncthreads();  // what stood in the LDS has been read
+#pragma unroll
+            for (int i = 0; i < SideA::kCopies; ++i) {
+                *reinterpret_cast<typename Fragment<T>::type*>(lds + (i * Tile::kThreads + static_cast<int>(threadIdx.x)) * 16) = a[i];
+            }
+#pragma unroll
+            for (int i = 0; i < SideB::kCopies; ++i) {
+                *reinterpret_cast<typename Fragment<T>::type*>(
+                    lds + SideA::kBytes + (i * Tile::kThreads + static_cast<int>(threadIdx.x)) * 16) = b[i];
+            }
+            __syncthreads();
+            Tile::multiplyStage(lds, part);
         }
-        int next = args.adapter_count;
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
-            const bool mine = adapter[i] == left;
+            const int row = wave_row + i * 16;
+            const bool mine = TileAdapters<Tile::kM>::at(rows.adapter, row) == left;
+            const float scale = TileAdapters<Tile::kM>::at(rows.scale, row);
 #pragma unroll
             for (int j = 0; j < Tile::kBlocksN; ++j) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sums[i][j][e] = mine ? part[i][j][e] * scale[i] : sums[i][j][e];
+                    sums[i][j][e] += mine ? part[i][j][e] * scale : 0.0f;
                 }
             }
-            next = adapter[i] > left ? min(next, adapter[i]) : next;
         }
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) {
-            next = min(next, __shfl_xor(next, d, kWave));
-        }
-        left = __builtin_amdgcn_readfirstlane(next);
+        left = next;
     }
 }
 
+// 128 registers, so that a CU holds two workgroups of the 128 x 128 tile.
 template <class Tile, typename Out>
-__global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args) {
+__global__ __launch_bounds__(Tile::kThreads, 4) void adaptedKernel(AdaptedArgs args) {
     using T = typename Tile::T;
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;
@@ -394,7 +460,6 @@ __global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args
     const T* x = static_cast<const T*>(args.x);
     const T* weight = static_cast<const T*>(args.weight);
     const auto row_at = [&](int p) { return args.order == nullptr ? p : args.order[p]; };
-    // the first stage is on its way while the adapters' part is formed
     typename Tile::Loads loads;
     loads.begin([&](int r) { return x + row_at(min(m0 + r, args.rows - 1)) * args.x_stride; }, args.x_stride, 0,
                 [&](int r) { return weight + min(n0 + r, args.out_dim - 1) * args.weight_stride; },
@@ -402,10 +467,14 @@ __global__ __launch_bounds__(Tile::kThreads) void adaptedKernel(AdaptedArgs args
     loads.start(lds);
     typename Tile::Sums sums;
     Tile::clear(sums);
+    TileAdapters<Tile::kM> rows;
     if (args.adapters != nullptr) {
-        addAdapters<Tile, Out>(args, m0 + Tile::waveM() * Tile::kBlocksM * 16, n0 + Tile::waveN() * Tile::kBlocksN * 16, sums);
+        rows.read(args, m0);
     }
     Tile::accumulate(lds, loads, args.dim, sums, [] {});
+    if (args.adapters != nullptr) {
+        addAdapters<Tile, Out>(args, rows, lds, m0, n0, sums);
+    }
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
 #pragma unroll
     for (int i = 0; i < Tile::kBlocksM; ++i) {
@@ -515,7 +584,7 @@ __global__ __launch_bounds__(kFewThreads) void adaptedFewKernel(AdaptedArgs args
         const T* up = static_cast<const T*>(args.up) +
                       (static_cast<std::int64_t>(adapter) * args.out_dim + n) * args.max_rank;
         for (int r = 0; r < rank; r += kChunk<T>) {
-            const auto b = loadChunk(up + r, rank - r);
+            const auto b = loadChunk(up + r, args.max_rank - r);
 #pragma unroll
             for (int e = 0; e < kChunk<T>; ++e) {
                 sum += r + e < rank ? low[row][r + e] * static_cast<float>(b[e]) : 0.0f;
@@ -600,12 +669,13 @@ AdaptedSpace adaptedSpace(const zcgvs_adapted_desc& d) {
 
 template <typename T>
 int launchLow(const AdaptedArgs& args, hipStream_t stream) {
-    // of many rows most begin no group
-    const int positions = args.rows <= 2048 ? 1 : 4;
-    const unsigned blocks = static_cast<unsigned>(divideUp(args.rows, positions));
-    if (blocks > (1u << 24) - 1u) {
+    // many rows of few adapters begin few groups: a workgroup a block of 16 then; else one a group
+    const int positions = args.rows <= 2048 ? 1 : 16;
+    const int blocks_needed = divideUp(args.rows, positions);
+    if (blocks_needed > (1 << 23) - 1) {
         return invalid("more rows than one launch can take");
     }
+    const unsigned blocks = static_cast<unsigned>(blocks_needed);
     const int rank_blocks = (args.max_rank + 15) / 16;
     if (rank_blocks <= 1) {
         lowKernel<T, 1><<<blocks, kLowThreads, 0, stream>>>(args, positions);

@@ -58,6 +58,19 @@ __device__ __forceinline__ void loadPack(const T* from, float (&to)[kCount]) {
     }
 }
 
+// sum += weight * the values of a pack as it was loaded.
+template <int kCount, typename V>
+__device__ __forceinline__ void addPack(const V& v, float weight, float (&sum)[kCount]) {
+    if constexpr (kCount == 1) {
+        sum[0] += weight * static_cast<float>(v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            sum[e] += weight * static_cast<float>(v[e]);
+        }
+    }
+}
+
 // Rounds to nearest even where T is narrower than float32.
 template <typename T, int kCount>
 __device__ __forceinline__ void storePack(const float (&from)[kCount], T* to) {
@@ -71,6 +84,21 @@ __device__ __forceinline__ void storePack(const float (&from)[kCount], T* to) {
         }
         *reinterpret_cast<typename Pack<T, kCount>::type*>(to) = v;
     }
+}
+
+// The same with the hint that nobody reads it soon.
+template <typename T, int kCount>
+__device__ __forceinline__ void storePackOnce(const float (&from)[kCount], T* to) {
+    typename Pack<T, kCount>::type v;
+    if constexpr (kCount == 1) {
+        v = static_cast<T>(from[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            v[e] = static_cast<T>(from[e]);
+        }
+    }
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, kCount>::type*>(to));
 }
 
 }  // namespace zcgvs_hip

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
         unsigned long long left = __ballot(counts(id, vocab, padding_id));
         count += __popcll(left);
         while (left != 0) {
-            float value[kBagAhead][kPack];
+            typename Pack<In, kPack>::type value[kBagAhead];
             int taken = 0;
 #pragma unroll
             for (int u = 0; u < kBagAhead; ++u) {
@@ -123,17 +123,14 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
                     const int next = __builtin_ctzll(left);
                     left &= left - 1;
                     const std::int64_t row = __builtin_amdgcn_readlane(id, next);
-                    loadPack(from + row * table_stride, value[u]);
+                    value[u] = *reinterpret_cast<const typename Pack<In, kPack>::type*>(from + row * table_stride);
                     ++taken;
                 }
             }
 #pragma unroll
             for (int u = 0; u < kBagAhead; ++u) {
                 if (u < taken) {
-#pragma unroll
-                    for (int e = 0; e < kPack; ++e) {
-                        sum[e] += value[u][e];
-                    }
+                    addPack(value[u], 1.0f, sum);
                 }
             }
         }
@@ -276,12 +273,13 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
     bool continued = key_before == current;  // the run so far began before this chunk
     float sum[kPack] = {};
     for (int j = 0; j < valid; j += kGradientAhead) {
-        float value[kGradientAhead][kPack];
+        typename Pack<In, kPack>::type value[kGradientAhead];
 #pragma unroll
         for (int u = 0; u < kGradientAhead; ++u) {
             if (j + u < valid) {
                 const std::int64_t row = __builtin_amdgcn_readlane(my_row, j + u);
-                loadPack(from + row * args.out_gradient_stride, value[u]);
+                value[u] = __builtin_nontemporal_load(
+                    reinterpret_cast<const typename Pack<In, kPack>::type*>(from + row * args.out_gradient_stride));
             }
         }
 #pragma unroll
@@ -304,10 +302,7 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
                     }
                 }
                 const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), j + u));
-#pragma unroll
-                for (int e = 0; e < kPack; ++e) {
-                    sum[e] += value[u][e] * weight;
-                }
+                addPack(value[u], weight, sum);
             }
         }
     }
@@ -323,71 +318,107 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
     }
 }
 
-// Joins a run that crosses chunks: the block of the chunk where it begins adds that chunk's last sum
-// and the first sums of the chunks it reaches, its wavefronts taking an equal share of those each.
+// Joins the runs that cross chunks: the sum of the chunk where a run begins and the first sums of the
+// chunks it reaches, over a slice of 64 packs. A wavefront looks at one chunk's end each and joins a run that
+// reaches few chunks by itself; the workgroup then takes the longer ones together, an equal share of the
+// chunks a wavefront.
 constexpr int kJoinThreads = 512;
 constexpr int kJoinWaves = kJoinThreads / kWave;
+constexpr int kJoinAlone = 16;  // chunks
 
 template <typename Out, int kPack>
 __global__ __launch_bounds__(kJoinThreads) void gradientJoinKernel(GradientArgs args) {
     __shared__ float sums[kJoinWaves][kWave * kPack];
-    const int chunk = blockIdx.x;
-    const int next = (chunk + 1) * args.chunk;  // the grid ends before the last chunk
-    const int key = args.keys[next - 1];
-    if (key != args.keys[next] || key >= args.vocab) {
-        return;
-    }
-    const int begin = chunk * args.chunk;
-    if (args.keys[begin] == key && begin > 0 && args.keys[begin - 1] == key) {
-        return;  // the run began in an earlier chunk
-    }
+    __shared__ int last_of[kJoinWaves];  // the last chunk of the run that begins in the wavefront's chunk
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int chunks = (args.count + args.chunk - 1) / args.chunk;
-    // the last chunk whose first id is the run's
-    int last = chunk + 1, past = chunks;
-    while (past - last > 1) {
-        const int middle = last + (past - last) / 2;
-        if (args.keys[middle * args.chunk] == key) {
-            last = middle;
-        } else {
-            past = middle;
+    const int column = (static_cast<int>(blockIdx.y) * kWave + lane) * kPack;
+    const bool has_column = column < args.dim;
+    const std::size_t stride = 2 * static_cast<std::size_t>(args.dim);
+    const float* partials = args.partials + (has_column ? column : 0);
+    const int first_chunk = static_cast<int>(blockIdx.x) * kJoinWaves;
+
+    int chunk = first_chunk + wave;
+    int last = chunk;  // no run to join
+    if (chunk + 1 < chunks) {
+        const int next = (chunk + 1) * args.chunk;
+        const int begin = chunk * args.chunk;
+        const int key = args.keys[next - 1];
+        const bool crosses = key == args.keys[next] && key < args.vocab;
+        const bool begins = begin == 0 || args.keys[begin] != key || args.keys[begin - 1] != key;
+        if (crosses && begins) {
+            // the last chunk whose first id is the run's
+            last = chunk + 1;
+            int past = chunks;
+            while (past - last > 1) {
+                const int middle = last + (past - last) / 2;
+                if (args.keys[middle * args.chunk] == key) {
+                    last = middle;
+                } else {
+                    past = middle;
+                }
+            }
         }
     }
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = threadIdx.x / kWave;
-    const int column = (static_cast<int>(blockIdx.y) * kWave + lane) * kPack;
-    const int reached = last - chunk;
-    const int share = (reached + kJoinWaves - 1) / kJoinWaves;
-    const int from = chunk + 1 + wave * share;
-    const int to = min(from + share, last + 1);
-    const std::size_t stride = 2 * static_cast<std::size_t>(args.dim);
-    float sum[kPack] = {};
-    if (column < args.dim) {
-        if (wave == 0) {
-            loadPack(args.partials + chunk * stride + args.dim + column, sum);
-        }
-#pragma unroll 8
-        for (int c = from; c < to; ++c) {
+    if (lane == 0) {
+        last_of[wave] = last;
+    }
+    if (last > chunk && last - chunk <= kJoinAlone) {
+        float sum[kPack];
+        loadPack(partials + chunk * stride + args.dim, sum);
+#pragma unroll 4
+        for (int c = chunk + 1; c <= last; ++c) {
             float more[kPack];
-            loadPack(args.partials + c * stride + column, more);
+            loadPack(partials + c * stride, more);
 #pragma unroll
             for (int e = 0; e < kPack; ++e) {
                 sum[e] += more[e];
             }
         }
-    }
-#pragma unroll
-    for (int e = 0; e < kPack; ++e) {
-        sums[wave][lane * kPack + e] = sum[e];
+        if (has_column) {
+            finishRow<Out, kPack>(args, args.keys[last * args.chunk], column, sum);
+        }
     }
     __syncthreads();
-    if (wave == 0 && column < args.dim) {
-        for (int w = 1; w < min(kJoinWaves, reached); ++w) {
+    for (int w = 0; w < kJoinWaves; ++w) {
+        chunk = first_chunk + w;
+        last = last_of[w];
+        const int reached = last - chunk;
+        if (reached <= kJoinAlone) {
+            continue;
+        }
+        const int share = (reached + kJoinWaves - 1) / kJoinWaves;
+        const int from = chunk + 1 + wave * share;
+        const int to = min(from + share, last + 1);
+        float sum[kPack] = {};
+        if (wave == 0) {
+            loadPack(partials + chunk * stride + args.dim, sum);
+        }
+#pragma unroll 8
+        for (int c = from; c < to; ++c) {
+            float more[kPack];
+            loadPack(partials + c * stride, more);
 #pragma unroll
             for (int e = 0; e < kPack; ++e) {
-                sum[e] += sums[w][lane * kPack + e];
+                sum[e] += more[e];
             }
         }
-        finishRow<Out, kPack>(args, key, column, sum);
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            sums[wave][lane * kPack + e] = sum[e];
+        }
+        __syncthreads();
+        if (wave == 0 && has_column) {
+            for (int v = 1; v < kJoinWaves; ++v) {
+#pragma unroll
+                for (int e = 0; e < kPack; ++e) {
+                    sum[e] += sums[v][lane * kPack + e];
+                }
+            }
+            finishRow<Out, kPack>(args, args.keys[last * args.chunk], column, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -415,7 +446,7 @@ struct ClearRows {
         const long long row_step = step / packs_per_row;
         const int pack_step = static_cast<int>(step - row_step * packs_per_row);
         for (; at < end; at += step) {
-            storePack(zeros, out + row * stride + static_cast<std::int64_t>(pack) * kPack);
+            storePackOnce(zeros, out + row * stride + static_cast<std::int64_t>(pack) * kPack);
             row += row_step;
             pack += pack_step;
             if (pack >= packs_per_row) {
@@ -611,7 +642,8 @@ int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, Gradien
     gradientChunkKernel<In, Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(args, items, slices);
     ZCGVS_LAUNCH_CHECK("embedding gradient");
     if (chunks > 1) {
-        gradientJoinKernel<Out, kPack><<<dim3(static_cast<unsigned>(chunks - 1), static_cast<unsigned>(slices)),
+        gradientJoinKernel<Out, kPack><<<dim3(static_cast<unsigned>((chunks - 1 + kJoinWaves - 1) / kJoinWaves),
+                                              static_cast<unsigned>(slices)),
                                          kJoinThreads, 0, stream>>>(args);
         ZCGVS_LAUNCH_CHECK("embedding gradient");
     }

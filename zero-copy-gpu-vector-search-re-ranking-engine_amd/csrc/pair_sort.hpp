@@ -122,40 +122,44 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(SortInput in, i
     const int wave = threadIdx.x / kWave;
     // a wavefront owns `rounds` * 64 consecutive items
     const int rounds = (in.count + kSmallThreads - 1) / kSmallThreads;
-    for (int i = threadIdx.x; i < in.count; i += kSmallThreads) {
-        keys[0][i] = sortKey(in, i);
-        places[0][i] = static_cast<std::uint16_t>(i);
-    }
     const int per_pass = (bits + passes - 1) / passes;
     for (int p = 0; p < passes; ++p) {
-        const int* from = keys[p & 1];
         const int shift = p * per_pass;
         const int here = min(per_pass, bits - shift);
-        const unsigned mask = (1u << here) - 1u;
-        for (int d = threadIdx.x; d < kDigits * kSmallWaves; d += kSmallThreads) {
-            (&seen[0][0])[d] = 0;
-        }
-        __syncthreads();
+        const int digits = 1 << here;
+        const unsigned mask = static_cast<unsigned>(digits) - 1u;
         int key[kSmallRounds];
         unsigned rank[kSmallRounds];
 #pragma unroll
         for (int round = 0; round < kSmallRounds; ++round) {
+            const int i = (wave * rounds + round) * kWave + lane;
+            key[round] = 0;
+            if (round < rounds && i < in.count) {
+                key[round] = p == 0 ? sortKey(in, i) : keys[p & 1][i];
+            }
+        }
+        for (int d = lane; d < digits; d += kWave) {
+            seen[wave][d] = 0;
+        }
+        waveFence();
+#pragma unroll
+        for (int round = 0; round < kSmallRounds; ++round) {
             if (round < rounds) {
-                const int i = (wave * rounds + round) * kWave + lane;
-                const bool ok = i < in.count;
-                key[round] = ok ? from[i] : 0;
+                const bool ok = (wave * rounds + round) * kWave + lane < in.count;
                 rank[round] = digitRank((static_cast<unsigned>(key[round]) >> shift) & mask, here, ok, seen[wave]);
             }
         }
         __syncthreads();
         unsigned total = 0;
-        if (threadIdx.x < kDigits) {
+        if (static_cast<int>(threadIdx.x) < digits) {
+#pragma unroll
             for (int w = 0; w < kSmallWaves; ++w) {
                 total += seen[w][threadIdx.x];
             }
         }
         unsigned at = blockPrefix(total, wave_sums);
-        if (threadIdx.x < kDigits) {
+        if (static_cast<int>(threadIdx.x) < digits) {
+#pragma unroll
             for (int w = 0; w < kSmallWaves; ++w) {
                 const unsigned count = seen[w][threadIdx.x];
                 seen[w][threadIdx.x] = at;
@@ -169,11 +173,11 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(SortInput in, i
             if (round < rounds && i < in.count) {
                 const unsigned digit = (static_cast<unsigned>(key[round]) >> shift) & mask;
                 const unsigned to = seen[wave][digit] + rank[round];
+                const int place = p == 0 ? i : places[p & 1][i];
                 if (p + 1 < passes) {
                     keys[(p & 1) ^ 1][to] = key[round];
-                    places[(p & 1) ^ 1][to] = places[p & 1][i];
+                    places[(p & 1) ^ 1][to] = static_cast<std::uint16_t>(place);
                 } else {
-                    const int place = places[p & 1][i];
                     keys_out[to] = key[round];
                     rows_out[to] = in.rows == nullptr ? place : in.rows[place];
                 }
