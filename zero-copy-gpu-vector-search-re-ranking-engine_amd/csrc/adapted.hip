@@ -375,8 +375,8 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, const TileA
         }
         return;
     }
-    using SideA = typename Tile::SideA;
-    using SideB = typename Tile::SideB;
+    using SideA = typename Tile::StageTile::SideA;
+    using SideB = typename Tile::StageTile::SideB;
     const int low_values = kHere * args.padded_rank;
     while (left < args.adapter_count) {
         int rank = 0;
@@ -429,7 +429,7 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, const TileA
                     lds + SideA::kBytes + (i * Tile::kThreads + static_cast<int>(threadIdx.x)) * 16) = b[i];
             }
             __syncthreads();
-            Tile::multiplyStage(lds, part);
+            Tile::StageTile::multiplyStage(lds, part);
         }
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
@@ -448,9 +448,9 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, const TileA
     }
 }
 
-// 128 registers, so that a CU holds two workgroups of the 128 x 128 tile.
+// 128 registers, so that a CU holds two workgroups of the 128 x 128 tile (float32's 64 x 64: three).
 template <class Tile, typename Out>
-__global__ __launch_bounds__(Tile::kThreads, 4) void adaptedKernel(AdaptedArgs args) {
+__global__ __launch_bounds__(Tile::kThreads, Tile::kThreads >= 512 ? 4 : 3) void adaptedKernel(AdaptedArgs args) {
     using T = typename Tile::T;
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;

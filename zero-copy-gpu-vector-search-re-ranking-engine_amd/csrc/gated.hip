@@ -496,7 +496,7 @@ int launchInputGradient(const zcgvs_gated_desc& d, InputGradientArgs args, hipSt
                         directRows(args.up, args.weight_stride, d.dim, d.dtype);
     const ProductPlan plan = inputPlan(d);
     args.splits = plan.splits;
-    args.split_k = plan.splits > 1 ? divideUp(divideUp(d.hidden, plan.splits / 2), kStageK<T>) * kStageK<T> : d.hidden;
+    args.split_k = plan.splits > 1 ? divideUp(divideUp(d.hidden, plan.splits / 2), kPlanStageK) * kPlanStageK : d.hidden;
     if (plan.splits > 1) {
         args.splits = 2 * divideUp(d.hidden, args.split_k);  // rounding to whole stages may leave fewer
     }
@@ -524,7 +524,7 @@ template <typename T>
 int launchWeightGradient(const zcgvs_gated_desc& d, WeightGradientArgs args, hipStream_t stream) {
     const bool direct = directRows(args.x, args.x_stride, d.dim, d.dtype);
     const ProductPlan plan = weightPlan(d);
-    args.split_k = divideUp(divideUp(d.rows, plan.splits), kStageK<T>) * kStageK<T>;
+    args.split_k = divideUp(divideUp(d.rows, plan.splits), kPlanStageK) * kPlanStageK;
     args.splits = divideUp(d.rows, args.split_k);
     const int launched = withTile<T, true, true, LargestTile::k256x256, false>(plan.shape, direct, [&](auto tile) {
         using Tile = decltype(tile);

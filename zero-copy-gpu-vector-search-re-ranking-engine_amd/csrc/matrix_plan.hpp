@@ -3,9 +3,11 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.hpp"
 #include "elements.hpp"
+#include "matrix_split.hpp"
 #include "matrix_tile.hpp"
 
 namespace zcgvs_hip {
@@ -33,12 +35,15 @@ struct ProductPlan {
     int splits;
 };
 
+// Values of k of a stage, of every type.
+constexpr int kPlanStageK = 64;
+
 // The plan of `count` products of m x n over k: the least time of the CU with the most tiles. A stage of a
 // tile takes alone_us, and more_us longer for every further tile that the CU holds beside it (as many as
-// `together`); fixed_us are the tile's first loads and its results. Measured: 128 stages of one 64 x 64 tile
-// a CU 58 us, of four 89 us; of one 128 x 128 tile 83 us, of two 111 us; 256 x 256 1.6 us a stage at any
-// length (1326 TFLOP/s over 8192). float32's matrix instructions take eight times as long and every shape
-// keeps them busy, so there a stage's time goes by its area.
+// `together`); fixed_us are the tile's first loads and its results. Measured, 16-bit: 128 stages of one
+// 64 x 64 tile a CU 58 us, of four 89 us; of one 128 x 128 tile 83 us, of two 111 us; 256 x 256 1.6 us a stage
+// at any length (1326 TFLOP/s over 8192). float32: of one 64 x 64 tile 190 us, of three 330 us; of one
+// 128 x 128 tile 343 us (198 TFLOP/s).
 // Splits write and read float32 sums of the whole product once each, at the rate of a copy; they come in
 // multiples of split_step, and only where a workspace can be had (split_step 0: one split).
 inline ProductPlan planProduct(std::int64_t m, std::int64_t n, std::int64_t k, int count, int dtype, int split_step,
@@ -46,21 +51,27 @@ inline ProductPlan planProduct(std::int64_t m, std::int64_t n, std::int64_t k, i
     struct Shape {
         TileShape shape;
         int m, n, together;
-        double alone_us, more_us, wide_us, fixed_us;
+        double alone_us, more_us, fixed_us;
     };
-    constexpr Shape kShapes[] = {
-        {TileShape::k256x256, 256, 256, 1, 1.60, 0.0, 7.0, 6.0},
-        {TileShape::k256x192, 256, 192, 1, 1.40, 0.0, 5.3, 4.5},
-        {TileShape::k128x128, 128, 128, 2, 0.65, 0.21, 1.75, 3.0},
-        {TileShape::k64x64, 64, 64, 4, 0.45, 0.083, 0.45, 2.0},
+    constexpr Shape kShapes16[] = {
+        {TileShape::k256x256, 256, 256, 1, 1.60, 0.0, 6.0},
+        {TileShape::k256x192, 256, 192, 1, 1.40, 0.0, 4.5},
+        {TileShape::k128x128, 128, 128, 2, 0.65, 0.21, 3.0},
+        {TileShape::k64x64, 64, 64, 4, 0.45, 0.083, 2.0},
+    };
+    constexpr Shape kShapes32[] = {
+        {TileShape::k128x128, 128, 128, 1, 2.70, 0.0, 3.0},
+        {TileShape::k64x64, 64, 64, 3, 1.50, 0.55, 3.0},
     };
     const bool wide = dtype == ZCGVS_DTYPE_F32;
-    const std::int64_t stage_k = kStageBytes / elementBytes(dtype);
-    const std::int64_t stages = (k + stage_k - 1) / stage_k;
+    const Shape* shapes = wide ? kShapes32 : kShapes16;
+    const int shape_count = wide ? 2 : 4;
+    const std::int64_t stages = (k + kPlanStageK - 1) / kPlanStageK;
     const std::int64_t units = deviceComputeUnits();
     ProductPlan best{TileShape::k64x64, 1};
     double best_us = 0.0;
-    for (const Shape& s : kShapes) {
+    for (int i = 0; i < shape_count; ++i) {
+        const Shape& s = shapes[i];
         if ((s.m > 128 && largest == LargestTile::k128x128) || (s.n > 192 && largest != LargestTile::k256x256)) {
             continue;
         }
@@ -74,14 +85,8 @@ inline ProductPlan planProduct(std::int64_t m, std::int64_t n, std::int64_t k, i
             const std::int64_t rounds = on_unit / s.together;
             const std::int64_t rest = on_unit % s.together;
             const double length = static_cast<double>((stages + splits - 1) / splits);
-            double us = 0.0;
-            if (wide) {
-                us = static_cast<double>(on_unit) * length * s.wide_us;
-            } else {
-                us = static_cast<double>(rounds) * length * (s.alone_us + (s.together - 1) * s.more_us);
-                us += rest > 0 ? length * (s.alone_us + static_cast<double>(rest - 1) * s.more_us) : 0.0;
-            }
-            us += static_cast<double>(rounds + (rest > 0 ? 1 : 0)) * s.fixed_us;
+            double us = static_cast<double>(rounds) * (length * (s.alone_us + (s.together - 1) * s.more_us) + s.fixed_us);
+            us += rest > 0 ? length * (s.alone_us + static_cast<double>(rest - 1) * s.more_us) + s.fixed_us : 0.0;
             if (splits > 1) {
                 us += 4.0 + 8.0 * static_cast<double>(count) * static_cast<double>(m) * static_cast<double>(n) * splits / 4.5e6;
             }
@@ -101,26 +106,31 @@ inline int persistentBlocks(TileShape shape) {
                                                                           : static_cast<int>(kMaxBlocks) / 8 * 8;
 }
 
-// Calls body(Tile{}) with a shape's tile; loads past the registers where the rows allow. kPaired: every
+// Calls body(Tile{}) with a shape's tile; loads past the registers where the rows allow (16-bit). kPaired: every
 // wavefront has an even number of column blocks (256 x 192 by 8 x 2 wavefronts instead of 4 x 4).
 template <typename T, bool kTurnedA, bool kTurnedB, LargestTile kLargest, bool kPaired, typename Body>
 int withTile(TileShape shape, bool direct, Body&& body) {
-    if (!direct) {
-        return shape == TileShape::k64x64 ? body(MatrixTile<T, 64, 64, 2, 2, kTurnedA, kTurnedB, false>{})
-                                          : body(MatrixTile<T, 128, 128, 2, 4, kTurnedA, kTurnedB, false>{});
-    }
-    if constexpr (kLargest == LargestTile::k256x256) {
-        if (shape == TileShape::k256x256) {
-            return body(MatrixTile<T, 256, 256, 4, 4, kTurnedA, kTurnedB, true>{});
+    if constexpr (std::is_same_v<T, float>) {
+        return shape == TileShape::k64x64 ? body(SplitTile<64, 64, 2, 2, kTurnedA, kTurnedB>{})
+                                          : body(SplitTile<128, 128, 4, 4, kTurnedA, kTurnedB>{});
+    } else {
+        if (!direct) {
+            return shape == TileShape::k64x64 ? body(MatrixTile<T, 64, 64, 2, 2, kTurnedA, kTurnedB, false>{})
+                                              : body(MatrixTile<T, 128, 128, 2, 4, kTurnedA, kTurnedB, false>{});
         }
-    }
-    if constexpr (kLargest != LargestTile::k128x128) {
-        if (shape == TileShape::k256x192) {
-            return body(MatrixTile<T, 256, 192, kPaired ? 8 : 4, kPaired ? 2 : 4, kTurnedA, kTurnedB, true>{});
+        if constexpr (kLargest == LargestTile::k256x256) {
+            if (shape == TileShape::k256x256) {
+                return body(MatrixTile<T, 256, 256, 4, 4, kTurnedA, kTurnedB, true>{});
+            }
         }
+        if constexpr (kLargest != LargestTile::k128x128) {
+            if (shape == TileShape::k256x192) {
+                return body(MatrixTile<T, 256, 192, kPaired ? 8 : 4, kPaired ? 2 : 4, kTurnedA, kTurnedB, true>{});
+            }
+        }
+        return shape == TileShape::k64x64 ? body(MatrixTile<T, 64, 64, 2, 2, kTurnedA, kTurnedB, true>{})
+                                          : body(MatrixTile<T, 128, 128, 2, 4, kTurnedA, kTurnedB, true>{});
     }
-    return shape == TileShape::k64x64 ? body(MatrixTile<T, 64, 64, 2, 2, kTurnedA, kTurnedB, true>{})
-                                      : body(MatrixTile<T, 128, 128, 2, 4, kTurnedA, kTurnedB, true>{});
 }
 
 }  // namespace

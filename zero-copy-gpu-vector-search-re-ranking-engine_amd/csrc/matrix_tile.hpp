@@ -3,15 +3,15 @@
 // A workgroup forms a kM x kN tile of C[m, n] = sum_k A[m, k] B[n, k] in float32 accumulators. Each side
 // comes in one of two layouts: rows whose k are neighbours ("plain": the activations and weights of
 // a forward product), or k-rows whose m (or n) are neighbours ("turned": what the gradients contract).
-// A stage is 128 bytes of k a row (64 16-bit or 32 float32 values); two stages are in LDS, one being
-// read by the matrix cores while the next arrives.
+// A stage is 128 bytes of k a row (64 16-bit values); two stages are in LDS, one being read by the matrix
+// cores while the next arrives. float32 products are those of matrix_split.hpp, on planes of the same layouts;
+// of float32 itself this file holds what multiplies one plain stage.
 //
 // LDS layout. A plain side's row r takes 128 bytes; its 16-byte chunk c stands in slot
 // c ^ ((r >> 1) & 7), so that the 16 rows of one ds_read_b128 fall on 16 different 16-byte columns of
 // the 256 bytes that the 64 banks hold. A turned side's k-row takes its m (or n) in order, in granules
-// whose place is exchanged by the k-row's number (16-bit: 32-byte granules, read by
-// ds_read_b64_tr_b16, which hands lane i of 16 the column i of four k-rows; float32: 64-byte ones,
-// read a value at a time: their matrix instructions take sixteen times as long per value).
+// of 32 bytes whose place is exchanged by the k-row's number, read by ds_read_b64_tr_b16, which hands lane i
+// of 16 the column i of four k-rows.
 //
 // Matrix instructions. 16-bit: v_mfma_f32_16x16x32, float32: v_mfma_f32_16x16x4. The first operand
 // holds B's rows and the second A's, so that lane l of a 16 x 16 result has the four neighbouring columns
@@ -87,6 +87,7 @@ struct StageLoader {
     static constexpr int kCopies = (kWaveCopies + kWaves - 1) / kWaves;
     static constexpr bool kEven = kWaveCopies % kWaves == 0;
     static constexpr int kBytes = kRows * kStageBytes;
+    static_assert(sizeof(T) == 2 || !kTurned, "a turned side is 16-bit");
 
     static __device__ __forceinline__ bool hasCopy(int i) {
         return kEven || i + 1 < kCopies ||
@@ -151,20 +152,8 @@ struct StageLoader {
     }
 
     // Which chunk of k-row k stands in `slot` of its LDS row (an exchange, so also the reverse).
-    static __device__ __forceinline__ int sourceChunk(int k, int slot) {
-        if constexpr (sizeof(T) == 2) {
-            return slot ^ (2 * turnOf(k));
-        } else {
-            return slot ^ (4 * turnOf(k));
-        }
-    }
-    static __device__ __forceinline__ int turnOf(int k) {
-        if constexpr (sizeof(T) == 2) {
-            return ((k & 3) | ((k >> 1) & 4)) & (kRows / 16 - 1);
-        } else {
-            return (k >> 2) & 3;
-        }
-    }
+    static __device__ __forceinline__ int sourceChunk(int k, int slot) { return slot ^ (2 * turnOf(k)); }
+    static __device__ __forceinline__ int turnOf(int k) { return ((k & 3) | ((k >> 1) & 4)) & (kRows / 16 - 1); }
 
     // Starts the next stage's copies into `stage` (direct).
     __device__ __forceinline__ void issue(const std::uint8_t* stage) {
@@ -233,8 +222,9 @@ struct StageLoader {
             const int slot = (4 * t + h) ^ ((r16 >> 1) & 7);
             return *reinterpret_cast<const typename Fragment<T>::type*>(stage + (16 * block + r16) * kStageBytes +
                                                                         16 * slot);
-        } else if constexpr (sizeof(T) == 2) {
+        } else {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
             typedef __attribute__((address_space(3))) s16x4* LdsPointer;
             const int k = 32 * t + 8 * h + (r16 >> 2);
             const std::uint32_t offset =
@@ -243,17 +233,8 @@ struct StageLoader {
             const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(address));
             const s16x4 high =
                 __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(address + 4 * kRows * 2));
-            typedef short s16x8 __attribute__((ext_vector_type(8)));
             const s16x8 both = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
             return __builtin_bit_cast(typename Fragment<T>::type, both);
-        } else {
-            typename Fragment<T>::type v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int k = 16 * t + 4 * h + e;
-                v[e] = *reinterpret_cast<const float*>(stage + k * kRows * 4 + ((block ^ turnOf(k)) * 64) + r16 * 4);
-            }
-            return v;
         }
     }
 };
@@ -263,6 +244,7 @@ template <typename Element, int kTileM, int kTileN, int kSplitM, int kSplitN, bo
           bool kDirectLoads>
 struct MatrixTile {
     using T = Element;
+    using StageTile = MatrixTile;  // whose multiplyStage() takes one stage of T
     static constexpr int kM = kTileM;
     static constexpr int kN = kTileN;
     static constexpr int kWavesM = kSplitM;

@@ -24,7 +24,7 @@ constexpr int kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortItems = kSortThreads;  // an item a thread
-constexpr int kMaxTiles = 256;
+constexpr int kMaxTiles = 128;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallWaves = kSmallThreads / kWave;
 constexpr int kSmallItems = 8192;
