@@ -216,12 +216,10 @@ struct InputGradientArgs {
 };
 
 template <class Tile>
-__global__ __launch_bounds__(Tile::kThreads) void inputGradientKernel(InputGradientArgs args) {
+__device__ __forceinline__ void formInputGradient(const InputGradientArgs& args, std::uint8_t* lds, int tile, int split) {
     using T = typename Tile::T;
-    __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;
-    tileOf(static_cast<int>(blockIdx.x), args.tiles_m, args.tiles_n, tile_m, tile_n);
-    const int split = static_cast<int>(blockIdx.y);
+    tileOf(tile, args.tiles_m, args.tiles_n, tile_m, tile_n);
     const int m0 = tile_m * Tile::kM;
     const int n0 = tile_n * Tile::kN;
     const int half = args.splits / 2;
@@ -289,12 +287,11 @@ struct WeightGradientArgs {
 };
 
 template <class Tile>
-__global__ __launch_bounds__(Tile::kThreads) void weightGradientKernel(WeightGradientArgs args) {
+__device__ __forceinline__ void formWeightGradient(const WeightGradientArgs& args, std::uint8_t* lds, int tile,
+                                                   int split) {
     using T = typename Tile::T;
-    __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
     int tile_m, tile_n;
-    tileOf(static_cast<int>(blockIdx.x), 2 * args.tiles_m, args.tiles_n, tile_m, tile_n);
-    const int split = static_cast<int>(blockIdx.y);
+    tileOf(tile, 2 * args.tiles_m, args.tiles_n, tile_m, tile_n);
     const int k0 = split * args.split_k;
     const int k_total = min(args.split_k, args.rows - k0);
     const bool second = tile_m >= args.tiles_m;
@@ -327,6 +324,35 @@ __global__ __launch_bounds__(Tile::kThreads) void weightGradientKernel(WeightGra
                 }
             }
         }
+    }
+}
+
+template <class Tile>
+__global__ __launch_bounds__(Tile::kThreads) void inputGradientKernel(InputGradientArgs args) {
+    __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
+    formInputGradient<Tile>(args, lds, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y));
+}
+
+template <class Tile>
+__global__ __launch_bounds__(Tile::kThreads) void weightGradientKernel(WeightGradientArgs args) {
+    __shared__ __attribute__((aligned(256))) std::uint8_t lds[Tile::kLdsBytes];
+    formWeightGradient<Tile>(args, lds, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.y));
+}
+
+// Both in one launch, for products of few tiles: the first `input_blocks` blocks form the input's.
+template <class InputTile, class WeightTile>
+__global__ __launch_bounds__(InputTile::kThreads) void bothGradientsKernel(InputGradientArgs input,
+                                                                           WeightGradientArgs weight, int input_blocks) {
+    static_assert(InputTile::kThreads == WeightTile::kThreads, "one workgroup size");
+    __shared__ __attribute__((aligned(256))) std::uint8_t
+        lds[InputTile::kLdsBytes > WeightTile::kLdsBytes ? InputTile::kLdsBytes : WeightTile::kLdsBytes];
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < input_blocks) {
+        const int tiles = input.tiles_m * input.tiles_n;
+        formInputGradient<InputTile>(input, lds, block % tiles, block / tiles);
+    } else {
+        const int tiles = 2 * weight.tiles_m * weight.tiles_n;
+        formWeightGradient<WeightTile>(weight, lds, (block - input_blocks) % tiles, (block - input_blocks) / tiles);
     }
 }
 
@@ -464,13 +490,15 @@ ProductPlan weightPlan(const zcgvs_gated_desc& d) {
     return planProduct(d.hidden, d.dim, d.rows, 2, d.dtype, 1, LargestTile::k256x256);
 }
 
-// float32 partial sums of the two products, one after the other in the same place.
-std::size_t partialValues(const zcgvs_gated_desc& d) {
-    const ProductPlan input = inputPlan(d);
-    const ProductPlan weight = weightPlan(d);
-    const std::size_t for_input = input.splits > 1 ? static_cast<std::size_t>(input.splits) * static_cast<std::size_t>(d.rows) : 0;
-    const std::size_t for_weight = weight.splits > 1 ? static_cast<std::size_t>(weight.splits) * 2 * static_cast<std::size_t>(d.hidden) : 0;
-    return std::max(for_input, for_weight) * static_cast<std::size_t>(d.dim);
+// float32 partial sums of the two products: the input's, then the weights'.
+std::size_t inputPartials(const zcgvs_gated_desc& d) {
+    const ProductPlan plan = inputPlan(d);
+    return plan.splits > 1 ? static_cast<std::size_t>(plan.splits) * static_cast<std::size_t>(d.rows) * static_cast<std::size_t>(d.dim) / 4 * 4 + 4 : 0;
+}
+
+std::size_t weightPartials(const zcgvs_gated_desc& d) {
+    const ProductPlan plan = weightPlan(d);
+    return plan.splits > 1 ? static_cast<std::size_t>(plan.splits) * 2 * static_cast<std::size_t>(d.hidden) * static_cast<std::size_t>(d.dim) : 0;
 }
 
 template <typename T>
@@ -490,17 +518,25 @@ int launchJoin(const float* partials, int splits, std::int64_t rows, int columns
     return ZCGVS_OK;
 }
 
-template <typename T>
-int launchInputGradient(const zcgvs_gated_desc& d, InputGradientArgs args, hipStream_t stream) {
-    const bool direct = directRows(args.gate, args.weight_stride, d.dim, d.dtype) &&
-                        directRows(args.up, args.weight_stride, d.dim, d.dtype);
-    const ProductPlan plan = inputPlan(d);
-    args.splits = plan.splits;
-    args.split_k = plan.splits > 1 ? divideUp(divideUp(d.hidden, plan.splits / 2), kPlanStageK) * kPlanStageK : d.hidden;
+// The splits of a plan: whole stages each, which may leave fewer than planned.
+void splitInput(const zcgvs_gated_desc& d, const ProductPlan& plan, InputGradientArgs& args) {
+    args.splits = 1;
+    args.split_k = d.hidden;
     if (plan.splits > 1) {
-        args.splits = 2 * divideUp(d.hidden, args.split_k);  // rounding to whole stages may leave fewer
+        args.split_k = divideUp(divideUp(d.hidden, plan.splits / 2), kPlanStageK) * kPlanStageK;
+        args.splits = 2 * divideUp(d.hidden, args.split_k);
     }
-    const int launched = withTile<T, false, true, LargestTile::k256x192, false>(plan.shape, direct, [&](auto tile) {
+}
+
+void splitWeight(const zcgvs_gated_desc& d, const ProductPlan& plan, WeightGradientArgs& args) {
+    args.split_k = divideUp(divideUp(d.rows, plan.splits), kPlanStageK) * kPlanStageK;
+    args.splits = divideUp(d.rows, args.split_k);
+}
+
+template <typename T>
+int launchInputGradient(const zcgvs_gated_desc& d, const ProductPlan& plan, bool direct, InputGradientArgs args,
+                        hipStream_t stream) {
+    return withTile<T, false, true, LargestTile::k256x192, false>(plan.shape, direct, [&](auto tile) {
         using Tile = decltype(tile);
         args.tiles_m = divideUp(d.rows, Tile::kM);
         args.tiles_n = divideUp(d.dim, Tile::kN);
@@ -513,20 +549,12 @@ int launchInputGradient(const zcgvs_gated_desc& d, InputGradientArgs args, hipSt
         ZCGVS_LAUNCH_CHECK("gated gradient");
         return static_cast<int>(ZCGVS_OK);
     });
-    if (launched != ZCGVS_OK || args.splits == 1) {
-        return launched;
-    }
-    return launchJoin<T>(args.partials, args.splits, d.rows, d.dim, d.rows, args.out, nullptr, args.out_stride,
-                         args.out_packed, stream);
 }
 
 template <typename T>
-int launchWeightGradient(const zcgvs_gated_desc& d, WeightGradientArgs args, hipStream_t stream) {
-    const bool direct = directRows(args.x, args.x_stride, d.dim, d.dtype);
-    const ProductPlan plan = weightPlan(d);
-    args.split_k = divideUp(divideUp(d.rows, plan.splits), kPlanStageK) * kPlanStageK;
-    args.splits = divideUp(d.rows, args.split_k);
-    const int launched = withTile<T, true, true, LargestTile::k256x256, false>(plan.shape, direct, [&](auto tile) {
+int launchWeightGradient(const zcgvs_gated_desc& d, const ProductPlan& plan, bool direct, WeightGradientArgs args,
+                         hipStream_t stream) {
+    return withTile<T, true, true, LargestTile::k256x256, false>(plan.shape, direct, [&](auto tile) {
         using Tile = decltype(tile);
         args.tiles_m = divideUp(d.hidden, Tile::kM);
         args.tiles_n = divideUp(d.dim, Tile::kN);
@@ -539,11 +567,71 @@ int launchWeightGradient(const zcgvs_gated_desc& d, WeightGradientArgs args, hip
         ZCGVS_LAUNCH_CHECK("gated gradient");
         return static_cast<int>(ZCGVS_OK);
     });
-    if (launched != ZCGVS_OK || args.splits == 1) {
-        return launched;
+}
+
+// Both products where both take 64 x 64 tiles, which leave the GPU idle between launches (500 rows of 384,
+// hidden 1024: 19.4 us instead of 22.8).
+template <class InputTile, class WeightTile>
+int launchBothGradients(const zcgvs_gated_desc& d, InputGradientArgs input, WeightGradientArgs weight,
+                        hipStream_t stream) {
+    input.tiles_m = divideUp(d.rows, InputTile::kM);
+    input.tiles_n = divideUp(d.dim, InputTile::kN);
+    weight.tiles_m = divideUp(d.hidden, WeightTile::kM);
+    weight.tiles_n = divideUp(d.dim, WeightTile::kN);
+    const long long input_blocks = static_cast<long long>(input.tiles_m) * input.tiles_n * input.splits;
+    const long long weight_blocks = 2ll * weight.tiles_m * weight.tiles_n * weight.splits;
+    if (input_blocks + weight_blocks > kMaxBlocks) {
+        return invalid("more output than one launch can write");
     }
-    return launchJoin<T>(args.partials, args.splits, 2 * static_cast<std::int64_t>(d.hidden), d.dim, d.hidden,
-                         args.gate_out, args.up_out, args.out_stride, args.out_packed, stream);
+    bothGradientsKernel<InputTile, WeightTile><<<static_cast<unsigned>(input_blocks + weight_blocks),
+                                                 InputTile::kThreads, 0, stream>>>(input, weight,
+                                                                                   static_cast<int>(input_blocks));
+    ZCGVS_LAUNCH_CHECK("gated gradient");
+    return ZCGVS_OK;
+}
+
+// The products with dg and du, and the sums over their splits. An output that is null is not wanted.
+template <typename T>
+int launchGradients(const zcgvs_gated_desc& d, InputGradientArgs input, WeightGradientArgs weight, hipStream_t stream) {
+    const ProductPlan input_plan = inputPlan(d);
+    const ProductPlan weight_plan = weightPlan(d);
+    splitInput(d, input_plan, input);
+    splitWeight(d, weight_plan, weight);
+    const bool wants_input = input.out != nullptr;
+    const bool wants_weight = weight.gate_out != nullptr;
+    const bool direct_input = directRows(input.gate, input.weight_stride, d.dim, d.dtype) &&
+                              directRows(input.up, input.weight_stride, d.dim, d.dtype);
+    const bool direct_weight = directRows(weight.x, weight.x_stride, d.dim, d.dtype);
+    int status = ZCGVS_OK;
+    if (wants_input && wants_weight && direct_input == direct_weight && input_plan.shape == TileShape::k64x64 &&
+        weight_plan.shape == TileShape::k64x64) {
+        if constexpr (std::is_same_v<T, float>) {
+            status = launchBothGradients<SplitTile<64, 64, 2, 2, false, true>, SplitTile<64, 64, 2, 2, true, true>>(
+                d, input, weight, stream);
+        } else if (direct_input) {
+            status = launchBothGradients<MatrixTile<T, 64, 64, 2, 2, false, true, true>,
+                                         MatrixTile<T, 64, 64, 2, 2, true, true, true>>(d, input, weight, stream);
+        } else {
+            status = launchBothGradients<MatrixTile<T, 64, 64, 2, 2, false, true, false>,
+                                         MatrixTile<T, 64, 64, 2, 2, true, true, false>>(d, input, weight, stream);
+        }
+    } else {
+        if (wants_input) {
+            status = launchInputGradient<T>(d, input_plan, direct_input, input, stream);
+        }
+        if (status == ZCGVS_OK && wants_weight) {
+            status = launchWeightGradient<T>(d, weight_plan, direct_weight, weight, stream);
+        }
+    }
+    if (status == ZCGVS_OK && wants_input && input.splits > 1) {
+        status = launchJoin<T>(input.partials, input.splits, d.rows, d.dim, d.rows, input.out, nullptr,
+                               input.out_stride, input.out_packed, stream);
+    }
+    if (status == ZCGVS_OK && wants_weight && weight.splits > 1) {
+        status = launchJoin<T>(weight.partials, weight.splits, 2 * static_cast<std::int64_t>(d.hidden), d.dim, d.hidden,
+                               weight.gate_out, weight.up_out, weight.out_stride, weight.out_packed, stream);
+    }
+    return status;
 }
 
 // Zeros for the weight gradients of a batch without rows.
@@ -594,7 +682,7 @@ std::size_t zcgvs_gated_gradient_workspace_bytes(const zcgvs_gated_desc* desc) {
         return 0;
     }
     clearError();
-    return desc->rows == 0 ? 256 : partialsOffset(*desc) + partialValues(*desc) * sizeof(float);
+    return desc->rows == 0 ? 256 : partialsOffset(*desc) + (inputPartials(*desc) + weightPartials(*desc)) * sizeof(float);
 }
 
 int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradient, std::int64_t out_gradient_stride,
@@ -654,45 +742,42 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
         form.out_gradient = d_out_gradient;
         form.out_gradient_stride = from_stride;
         form.gradient_packed = alignedRows(d_out_gradient, from_stride, d.dtype, 4 * elementBytes(d.dtype));
-        float* partials = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + partialsOffset(d));
         form.du_offset = d.rows * form.out_stride;
-        int done = launchGated<T, true>(d, form, toStream(stream));
-        if (done == ZCGVS_OK && d_x_gradient != nullptr) {
-            InputGradientArgs args{};
-            args.dg = d_workspace;
-            args.d_stride = form.out_stride;
-            args.du_offset = form.du_offset;
-            args.gate = d.gate;
-            args.up = d.up;
-            args.weight_stride = rowStride(d.weight_stride, d.dim);
-            args.rows = static_cast<int>(d.rows);
-            args.dim = d.dim;
-            args.hidden = d.hidden;
-            args.partials = partials;
-            args.out = d_x_gradient;
-            args.out_stride = x_out_stride;
-            args.out_packed = alignedRows(d_x_gradient, x_out_stride, d.dtype, 4 * elementBytes(d.dtype));
-            done = launchInputGradient<T>(d, args, toStream(stream));
+        const int formed = launchGated<T, true>(d, form, toStream(stream));
+        if (formed != ZCGVS_OK) {
+            return formed;
         }
-        if (done == ZCGVS_OK && d_gate_gradient != nullptr) {
-            WeightGradientArgs args{};
-            args.dg = d_workspace;
-            args.d_stride = form.out_stride;
-            args.du_offset = form.du_offset;
-            args.x = d.x;
-            args.x_stride = rowStride(d.x_stride, d.dim);
-            args.rows = static_cast<int>(d.rows);
-            args.dim = d.dim;
-            args.hidden = d.hidden;
-            args.partials = partials;
-            args.gate_out = d_gate_gradient;
-            args.up_out = d_up_gradient;
-            args.out_stride = weight_out_stride;
-            args.out_packed = alignedRows(d_gate_gradient, weight_out_stride, d.dtype, 4 * elementBytes(d.dtype)) &&
-                              alignedRows(d_up_gradient, weight_out_stride, d.dtype, 4 * elementBytes(d.dtype));
-            done = launchWeightGradient<T>(d, args, toStream(stream));
-        }
-        return done;
+        float* partials = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + partialsOffset(d));
+        InputGradientArgs input{};
+        input.dg = d_workspace;
+        input.d_stride = form.out_stride;
+        input.du_offset = form.du_offset;
+        input.gate = d.gate;
+        input.up = d.up;
+        input.weight_stride = rowStride(d.weight_stride, d.dim);
+        input.rows = static_cast<int>(d.rows);
+        input.dim = d.dim;
+        input.hidden = d.hidden;
+        input.partials = partials;
+        input.out = d_x_gradient;
+        input.out_stride = x_out_stride;
+        input.out_packed = alignedRows(d_x_gradient, x_out_stride, d.dtype, 4 * elementBytes(d.dtype));
+        WeightGradientArgs weight{};
+        weight.dg = d_workspace;
+        weight.d_stride = form.out_stride;
+        weight.du_offset = form.du_offset;
+        weight.x = d.x;
+        weight.x_stride = rowStride(d.x_stride, d.dim);
+        weight.rows = input.rows;
+        weight.dim = d.dim;
+        weight.hidden = d.hidden;
+        weight.partials = partials + inputPartials(d);
+        weight.gate_out = d_gate_gradient;
+        weight.up_out = d_up_gradient;
+        weight.out_stride = weight_out_stride;
+        weight.out_packed = alignedRows(d_gate_gradient, weight_out_stride, d.dtype, 4 * elementBytes(d.dtype)) &&
+                            alignedRows(d_up_gradient, weight_out_stride, d.dtype, 4 * elementBytes(d.dtype));
+        return launchGradients<T>(d, input, weight, toStream(stream));
     });
     return launched == ZCGVS_OK ? clearError() : launched;
 }
