@@ -66,7 +66,6 @@ struct AdaptedArgs {
     int tiles_n;
     void* out;
     std::int64_t out_stride;
-    bool out_packed;
 };
 
 __device__ __forceinline__ int rankOf(const AdaptedArgs& args, int adapter) {
@@ -491,7 +490,7 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kThreads >= 512 ? 4 : 3) void
         for (int j = 0; j < Tile::kBlocksN; ++j) {
             const int n = n0 + (Tile::waveN() * Tile::kBlocksN + j) * 16 + 4 * (lane >> 4);
             if (n < args.out_dim) {
-                storeFour(sums[i][j], out + n, args.out_dim - n, args.out_packed);
+                storeFour(sums[i][j], out + n, args.out_dim - n);
             }
         }
     }
@@ -776,7 +775,6 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
     args.out_dim = d.out_dim;
     args.out = d_out;
     args.out_stride = stride;
-    args.out_packed = alignedRows(d_out, stride, out_dtype, 4 * elementBytes(out_dtype));
     const bool few = d.rows <= kFewRows;
     if (hasAdapters(d)) {
         char* workspace = static_cast<char*>(d_workspace);

@@ -35,22 +35,33 @@ inline bool alignedRows(const void* base, std::int64_t stride, int dtype, int by
            stride * elementBytes(dtype) % bytes == 0;
 }
 
-// kCount neighbouring elements as one load or store of the vector's natural size.
+// kCount neighbouring elements as one load or store. `stored` may stand at any element: the hardware takes
+// vector accesses at any alignment.
 template <typename T, int kCount>
 struct Pack {
     typedef T type __attribute__((ext_vector_type(kCount)));
+    typedef T stored __attribute__((ext_vector_type(kCount), aligned(sizeof(T))));
 };
 template <typename T>
 struct Pack<T, 1> {
     typedef T type;
+    typedef T stored;
 };
+
+// The first column of a row's pack `pack`: the last pack of a row that is no whole number of them begins
+// early and overlaps the one before.
+template <int kCount>
+__host__ __device__ __forceinline__ int packColumn(int pack, int columns) {
+    const int column = pack * kCount;
+    return column < columns - kCount ? column : columns - kCount;
+}
 
 template <typename T, int kCount>
 __device__ __forceinline__ void loadPack(const T* from, float (&to)[kCount]) {
     if constexpr (kCount == 1) {
         to[0] = static_cast<float>(*from);
     } else {
-        const auto v = *reinterpret_cast<const typename Pack<T, kCount>::type*>(from);
+        const auto v = *reinterpret_cast<const typename Pack<T, kCount>::stored*>(from);
 #pragma unroll
         for (int e = 0; e < kCount; ++e) {
             to[e] = static_cast<float>(v[e]);
@@ -82,14 +93,14 @@ __device__ __forceinline__ void storePack(const float (&from)[kCount], T* to) {
         for (int e = 0; e < kCount; ++e) {
             v[e] = static_cast<T>(from[e]);
         }
-        *reinterpret_cast<typename Pack<T, kCount>::type*>(to) = v;
+        *reinterpret_cast<typename Pack<T, kCount>::stored*>(to) = v;
     }
 }
 
 // The same with the hint that nobody reads it soon.
 template <typename T, int kCount>
 __device__ __forceinline__ void storePackOnce(const float (&from)[kCount], T* to) {
-    typename Pack<T, kCount>::type v;
+    typename Pack<T, kCount>::stored v;
     if constexpr (kCount == 1) {
         v = static_cast<T>(from[0]);
     } else {
@@ -98,7 +109,7 @@ __device__ __forceinline__ void storePackOnce(const float (&from)[kCount], T* to
             v[e] = static_cast<T>(from[e]);
         }
     }
-    __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, kCount>::type*>(to));
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Pack<T, kCount>::stored*>(to));
 }
 
 }  // namespace zcgvs_hip

@@ -41,9 +41,10 @@ constexpr int kLookupPacks = 4;
 
 template <typename In, typename Out, int kPack>
 __global__ __launch_bounds__(kThreads) void lookupKernel(const In* __restrict__ table, std::int64_t table_stride,
-                                                         int vocab, int packs_per_row, const int* __restrict__ ids,
+                                                         int vocab, int dim, const int* __restrict__ ids,
                                                          long long packs, int padding_id, float scale,
                                                          Out* __restrict__ out, std::int64_t out_stride) {
+    const int packs_per_row = (dim + kPack - 1) / kPack;
     const long long first = static_cast<long long>(blockIdx.x) * (kThreads * kLookupPacks);
     const long long first_row = first / packs_per_row;
     const unsigned first_pack = static_cast<unsigned>(first - first_row * packs_per_row);
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(kThreads) void lookupKernel(const In* __restrict__ 
             const unsigned pack = at - row * static_cast<unsigned>(packs_per_row);
             const int id = ids[first_row + row];
             if (counts(id, vocab, padding_id)) {
-                loadPack(table + id * table_stride + static_cast<std::int64_t>(pack) * kPack, value[u]);
+                loadPack(table + id * table_stride + packColumn<kPack>(static_cast<int>(pack), dim), value[u]);
             }
         }
     }
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(kThreads) void lookupKernel(const In* __restrict__ 
             for (int e = 0; e < kPack; ++e) {
                 value[u][e] *= scale;
             }
-            storePack(value[u], out + (first_row + row) * out_stride + static_cast<std::int64_t>(pack) * kPack);
+            storePack(value[u], out + (first_row + row) * out_stride + packColumn<kPack>(static_cast<int>(pack), dim));
         }
     }
 }
@@ -92,7 +93,7 @@ constexpr int kBagAhead = 16;
 
 template <typename In, typename Out, int kPack, int kShares>
 __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ table, std::int64_t table_stride,
-                                                      int vocab, int packs_per_row, const int* __restrict__ ids,
+                                                      int vocab, int dim, const int* __restrict__ ids,
                                                       long long token_count,
                                                       const std::int64_t* __restrict__ bag_offsets, long long items,
                                                       int slices, bool mean, int padding_id, float scale,
@@ -107,10 +108,11 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
     const bool has_item = item < items;
     const long long bag = has_item ? item / slices : 0;
     const int pack = static_cast<int>(item - bag * slices) * kWave + lane;
-    const bool has_pack = has_item && pack < packs_per_row;
+    const bool has_pack = has_item && pack < (dim + kPack - 1) / kPack;
+    const int column = has_pack ? packColumn<kPack>(pack, dim) : 0;
     const long long begin = min(max(static_cast<long long>(bag_offsets[bag]), 0ll), token_count);
     const long long end = has_item ? min(static_cast<long long>(bag_offsets[bag + 1]), token_count) : begin;
-    const In* from = table + static_cast<std::int64_t>(has_pack ? pack : 0) * kPack;
+    const In* from = table + column;
 
     float sum[kPack] = {};
     int count = 0;
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
         unsigned long long left = __ballot(counts(id, vocab, padding_id));
         count += __popcll(left);
         while (left != 0) {
-            typename Pack<In, kPack>::type value[kBagAhead];
+            typename Pack<In, kPack>::stored value[kBagAhead];
             int taken = 0;
 #pragma unroll
             for (int u = 0; u < kBagAhead; ++u) {
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
                     const int next = __builtin_ctzll(left);
                     left &= left - 1;
                     const std::int64_t row = __builtin_amdgcn_readlane(id, next);
-                    value[u] = *reinterpret_cast<const typename Pack<In, kPack>::type*>(from + row * table_stride);
+                    value[u] = *reinterpret_cast<const typename Pack<In, kPack>::stored*>(from + row * table_stride);
                     ++taken;
                 }
             }
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void bagKernel(const In* __restrict__ tab
         for (int e = 0; e < kPack; ++e) {
             sum[e] *= weight;
         }
-        storePack(sum, out + bag * out_stride + static_cast<std::int64_t>(pack) * kPack);
+        storePack(sum, out + bag * out_stride + column);
     }
 }
 
@@ -227,18 +229,34 @@ struct GradientArgs {
     float* partials;  // [chunks, 2, dim]: sums of a chunk's first and last run where they cross chunks
 };
 
+// Writes pack `pack` of row `key`, or adds it to what is there: there only the columns that are not the pack
+// before's too.
 template <typename Out, int kPack>
-__device__ __forceinline__ void finishRow(const GradientArgs& args, int key, int column, float (&sum)[kPack]) {
+__device__ __forceinline__ void finishRow(const GradientArgs& args, int key, int pack, float (&sum)[kPack]) {
+    const int column = packColumn<kPack>(pack, args.dim);
     Out* to = static_cast<Out*>(args.table_gradient) + key * args.table_gradient_stride + column;
-    float old[kPack] = {};
-    if (args.accumulate) {
-        loadPack(static_cast<const Out*>(to), old);
-    }
 #pragma unroll
     for (int e = 0; e < kPack; ++e) {
-        sum[e] = sum[e] * args.scale + old[e];
+        sum[e] *= args.scale;
     }
-    storePack(sum, to);
+    if (!args.accumulate) {
+        storePack(sum, to);
+    } else if (column == pack * kPack) {
+        float old[kPack];
+        loadPack(static_cast<const Out*>(to), old);
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            sum[e] += old[e];
+        }
+        storePack(sum, to);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            if (column + e >= pack * kPack) {
+                to[e] = static_cast<Out>(static_cast<float>(to[e]) + sum[e]);
+            }
+        }
+    }
 }
 
 // A wavefront sums one chunk's rows over 64 packs of columns: it reads the chunk's ids and rows at once, a
@@ -255,8 +273,9 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
         return;
     }
     const int chunk = static_cast<int>(item / slices);
-    const int column = (static_cast<int>(item - static_cast<long long>(chunk) * slices) * kWave + lane) * kPack;
-    const bool has_column = column < args.dim;
+    const int pack = static_cast<int>(item - static_cast<long long>(chunk) * slices) * kWave + lane;
+    const bool has_column = pack < (args.dim + kPack - 1) / kPack;
+    const int column = has_column ? packColumn<kPack>(pack, args.dim) : 0;
     const int begin = chunk * args.chunk;
     const int length = min(args.chunk, args.count - begin);
     const int at = begin + min(lane, length - 1);
@@ -273,19 +292,19 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
     }
     const int key_before = begin > 0 ? args.keys[begin - 1] : -1;
     const int key_after = begin + length < args.count ? args.keys[begin + length] : args.vocab;
-    const In* from = static_cast<const In*>(args.out_gradient) + (has_column ? column : 0);
+    const In* from = static_cast<const In*>(args.out_gradient) + column;
     float* partials = args.partials + static_cast<std::size_t>(chunk) * 2 * args.dim + column;
     int current = __builtin_amdgcn_readlane(my_key, 0);
     bool continued = key_before == current;  // the run so far began before this chunk
     float sum[kPack] = {};
     for (int j = 0; j < valid; j += kGradientAhead) {
-        typename Pack<In, kPack>::type value[kGradientAhead];
+        typename Pack<In, kPack>::stored value[kGradientAhead];
 #pragma unroll
         for (int u = 0; u < kGradientAhead; ++u) {
             if (j + u < valid) {
                 const std::int64_t row = __builtin_amdgcn_readlane(my_row, j + u);
                 value[u] = __builtin_nontemporal_load(
-                    reinterpret_cast<const typename Pack<In, kPack>::type*>(from + row * args.out_gradient_stride));
+                    reinterpret_cast<const typename Pack<In, kPack>::stored*>(from + row * args.out_gradient_stride));
             }
         }
 #pragma unroll
@@ -297,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
                         if (continued) {
                             storePack(sum, partials);
                         } else {
-                            finishRow<Out, kPack>(args, current, column, sum);
+                            finishRow<Out, kPack>(args, current, pack, sum);
                         }
                     }
                     continued = false;
@@ -320,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void gradientChunkKernel(GradientArgs arg
     } else if (valid == length && key_after == current) {
         storePack(sum, partials + args.dim);
     } else {
-        finishRow<Out, kPack>(args, current, column, sum);
+        finishRow<Out, kPack>(args, current, pack, sum);
     }
 }
 
@@ -339,10 +358,10 @@ __global__ __launch_bounds__(kJoinThreads) void gradientJoinKernel(GradientArgs 
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int chunks = (args.count + args.chunk - 1) / args.chunk;
-    const int column = (static_cast<int>(blockIdx.y) * kWave + lane) * kPack;
-    const bool has_column = column < args.dim;
+    const int pack = static_cast<int>(blockIdx.y) * kWave + lane;
+    const bool has_column = pack < (args.dim + kPack - 1) / kPack;
     const std::size_t stride = 2 * static_cast<std::size_t>(args.dim);
-    const float* partials = args.partials + (has_column ? column : 0);
+    const float* partials = args.partials + (has_column ? packColumn<kPack>(pack, args.dim) : 0);
     const int first_chunk = static_cast<int>(blockIdx.x) * kJoinWaves;
 
     int chunk = first_chunk + wave;
@@ -383,7 +402,7 @@ __global__ __launch_bounds__(kJoinThreads) void gradientJoinKernel(GradientArgs 
             }
         }
         if (has_column) {
-            finishRow<Out, kPack>(args, args.keys[last * args.chunk], column, sum);
+            finishRow<Out, kPack>(args, args.keys[last * args.chunk], pack, sum);
         }
     }
     __syncthreads();
@@ -422,7 +441,7 @@ __global__ __launch_bounds__(kJoinThreads) void gradientJoinKernel(GradientArgs 
                     sum[e] += sums[v][lane * kPack + e];
                 }
             }
-            finishRow<Out, kPack>(args, args.keys[last * args.chunk], column, sum);
+            finishRow<Out, kPack>(args, args.keys[last * args.chunk], pack, sum);
         }
         __syncthreads();
     }
@@ -436,12 +455,13 @@ struct ClearRows {
     Out* out;  // null: nothing to clear
     std::int64_t stride;
     long long packs;
-    int packs_per_row;
+    int dim;
 
     __device__ void run(int block, int blocks, int launch, int launches) const {
         if (out == nullptr) {
             return;
         }
+        const int packs_per_row = (dim + kPack - 1) / kPack;
         const long long begin = packs * launch / launches;
         const long long end = packs * (launch + 1) / launches;
         const float zeros[kPack] = {};
@@ -452,7 +472,7 @@ struct ClearRows {
         const long long row_step = step / packs_per_row;
         const int pack_step = static_cast<int>(step - row_step * packs_per_row);
         for (; at < end; at += step) {
-            storePackOnce(zeros, out + row * stride + static_cast<std::int64_t>(pack) * kPack);
+            storePackOnce(zeros, out + row * stride + packColumn<kPack>(pack, dim));
             row += row_step;
             pack += pack_step;
             if (pack >= packs_per_row) {
@@ -506,20 +526,11 @@ int checkEmbedding(const zcgvs_embedding_desc* desc) {
     return ZCGVS_OK;
 }
 
-// The widest pack (16 bytes of the wider type at most) that both sides' rows allow: 4 or 1 elements.
-int packElements(int dim, const void* a, std::int64_t a_stride, int a_dtype, const void* b, std::int64_t b_stride,
-                 int b_dtype) {
-    return dim % 4 == 0 && alignedRows(a, a_stride, a_dtype, 4 * elementBytes(a_dtype)) &&
-                   alignedRows(b, b_stride, b_dtype, 4 * elementBytes(b_dtype))
-               ? 4
-               : 1;
-}
-
 template <typename In, typename Out, int kPack>
 int lookupTyped(const zcgvs_embedding_desc& d, Out* out, std::int64_t out_stride, hipStream_t stream) {
     const In* table = static_cast<const In*>(d.table);
     const std::int64_t table_stride = rowStride(d.table_stride, d.dim);
-    const int packs_per_row = d.dim / kPack;
+    const int packs_per_row = (d.dim + kPack - 1) / kPack;
     if (d.bag_offsets == nullptr) {
         const long long packs = static_cast<long long>(d.token_count) * packs_per_row;
         const long long blocks = (packs + kThreads * kLookupPacks - 1) / (kThreads * kLookupPacks);
@@ -527,7 +538,7 @@ int lookupTyped(const zcgvs_embedding_desc& d, Out* out, std::int64_t out_stride
             return invalid("more output than one launch can write");
         }
         lookupKernel<In, Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            table, table_stride, d.vocab, packs_per_row, d.ids, packs, d.padding_id, d.scale, out, out_stride);
+            table, table_stride, d.vocab, d.dim, d.ids, packs, d.padding_id, d.scale, out, out_stride);
     } else {
         const int slices = (packs_per_row + kWave - 1) / kWave;
         // a wavefront a bag where that keeps the GPU's memory busy, else four
@@ -538,7 +549,7 @@ int lookupTyped(const zcgvs_embedding_desc& d, Out* out, std::int64_t out_stride
             const long long items = std::min<std::int64_t>(most, d.bag_count - bag) * slices;
             const unsigned blocks = static_cast<unsigned>((items + items_per_block - 1) / items_per_block);
             const auto kernel = alone ? bagKernel<In, Out, kPack, 1> : bagKernel<In, Out, kPack, kWavesPerBlock>;
-            kernel<<<blocks, kThreads, 0, stream>>>(table, table_stride, d.vocab, packs_per_row, d.ids, d.token_count,
+            kernel<<<blocks, kThreads, 0, stream>>>(table, table_stride, d.vocab, d.dim, d.ids, d.token_count,
                                                     d.bag_offsets + bag, items, slices,
                                                     d.reduce == ZCGVS_EMBEDDING_MEAN, d.padding_id, d.scale,
                                                     out + bag * out_stride, out_stride);
@@ -623,8 +634,8 @@ int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, Gradien
     if (!args.accumulate) {
         clear.out = static_cast<Out*>(args.table_gradient);
         clear.stride = args.table_gradient_stride;
-        clear.packs_per_row = d.dim / kPack;
-        clear.packs = static_cast<long long>(d.vocab) * clear.packs_per_row;
+        clear.dim = d.dim;
+        clear.packs = static_cast<long long>(d.vocab) * ((d.dim + kPack - 1) / kPack);
     }
     if (args.count == 0) {
         if (clear.out != nullptr) {
@@ -639,7 +650,7 @@ int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, Gradien
         return sorted;
     }
     const int chunks = static_cast<int>((static_cast<long long>(args.count) + s.chunk - 1) / s.chunk);
-    const int slices = (d.dim / kPack + kWave - 1) / kWave;
+    const int slices = ((d.dim + kPack - 1) / kPack + kWave - 1) / kWave;
     const long long items = static_cast<long long>(chunks) * slices;
     const long long blocks = (items + kWavesPerBlock - 1) / kWavesPerBlock;
     if (blocks > kMaxBlocks) {
@@ -689,13 +700,12 @@ int zcgvs_embedding_lookup(const zcgvs_embedding_desc* desc, void* d_out, std::i
     if (d.table == nullptr || d_out == nullptr) {
         return invalid("null device pointer");
     }
-    const int pack = packElements(d.dim, d.table, table_stride, d.dtype, d_out, stride, out_dtype);
     const int launched = withElement(d.dtype, [&](auto in) {
         using In = decltype(in);
         return withElement(out_dtype, [&](auto element) {
             using Out = decltype(element);
             if constexpr (std::is_same_v<Out, In> || std::is_same_v<Out, float>) {
-                return pack == 4 ? lookupTyped<In, Out, 4>(d, static_cast<Out*>(d_out), stride, toStream(stream))
+                return d.dim >= 4 ? lookupTyped<In, Out, 4>(d, static_cast<Out*>(d_out), stride, toStream(stream))
                                  : lookupTyped<In, Out, 1>(d, static_cast<Out*>(d_out), stride, toStream(stream));
             } else {
                 return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above
@@ -765,14 +775,12 @@ int zcgvs_embedding_gradient(const zcgvs_embedding_desc* desc, const void* d_out
     args.table_gradient = d_table_gradient;
     args.table_gradient_stride = to_stride;
     args.accumulate = accumulate != 0;
-    const int pack = packElements(d.dim, d_out_gradient, from_stride, gradient_dtype, d_table_gradient, to_stride,
-                                  table_gradient_dtype);
     const int launched = withElement(gradient_dtype, [&](auto in) {
         using In = decltype(in);
         return withElement(table_gradient_dtype, [&](auto element) {
             using Out = decltype(element);
             if constexpr (std::is_same_v<Out, In> || std::is_same_v<Out, float>) {
-                return pack == 4 ? gradientTyped<In, Out, 4>(d, space, args, workspace, toStream(stream))
+                return d.dim >= 4 ? gradientTyped<In, Out, 4>(d, space, args, workspace, toStream(stream))
                                  : gradientTyped<In, Out, 1>(d, space, args, workspace, toStream(stream));
             } else {
                 return static_cast<int>(ZCGVS_ERR_INVALID_ARGUMENT);  // refused above

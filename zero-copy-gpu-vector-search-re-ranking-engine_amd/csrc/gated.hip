@@ -76,12 +76,10 @@ struct GatedArgs {
     int tiles_n;
     void* out;
     std::int64_t out_stride;
-    bool out_packed;  // stores of four results are aligned
     // gradient only: `out` is dg and du is out + du_offset, both [rows, out_stride] with the columns
     // past hidden written as zeros
     const void* out_gradient;
     std::int64_t out_gradient_stride;
-    bool gradient_packed;
     std::int64_t du_offset;
 };
 
@@ -145,8 +143,7 @@ __global__ __launch_bounds__(Tile::kThreads) void gatedKernel(GatedArgs args) {
                     const int m = m0 + i * 16;
                     const int n = n0 + j * 16;
                     if (m < args.rows && n < args.hidden) {
-                        storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.hidden - n,
-                                  args.out_packed);
+                        storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.hidden - n);
                     }
                 }
             }
@@ -161,7 +158,7 @@ __global__ __launch_bounds__(Tile::kThreads) void gatedKernel(GatedArgs args) {
                     from[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                     if (m < args.rows && n < args.hidden) {
                         from[j] = loadFour(static_cast<const T*>(args.out_gradient) + m * args.out_gradient_stride + n,
-                                           args.hidden - n, args.gradient_packed);
+                                           args.hidden - n);
                     }
                 }
 #pragma unroll
@@ -187,8 +184,8 @@ __global__ __launch_bounds__(Tile::kThreads) void gatedKernel(GatedArgs args) {
                     const int n = n0 + j * 16;
                     if (m < args.rows && n < args.out_stride) {
                         T* to = static_cast<T*>(args.out) + m * args.out_stride + n;
-                        storeFour(sums[i][j], to, 4, true);
-                        storeFour(sums[i][j + kPairs], to + args.du_offset, 4, true);
+                        storeFour(sums[i][j], to, 4);
+                        storeFour(sums[i][j + kPairs], to + args.du_offset, 4);
                     }
                 }
             }
@@ -217,7 +214,6 @@ struct InputGradientArgs {
     float* partials;  // [splits, rows, dim]
     void* out;
     std::int64_t out_stride;
-    bool out_packed;
 };
 
 template <class Tile>
@@ -260,10 +256,9 @@ __device__ __forceinline__ void formInputGradient(const InputGradientArgs& args,
             if (m < args.rows && n < args.dim) {
                 if (args.splits > 1) {
                     float* to = args.partials + (static_cast<std::int64_t>(split) * args.rows + m) * args.dim + n;
-                    storeFour(sums[i][j], to, args.dim - n, args.dim % 4 == 0);
+                    storeFour(sums[i][j], to, args.dim - n);
                 } else {
-                    storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.dim - n,
-                              args.out_packed);
+                    storeFour(sums[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, args.dim - n);
                 }
             }
         }
@@ -288,7 +283,6 @@ struct WeightGradientArgs {
     void* gate_out;
     void* up_out;
     std::int64_t out_stride;
-    bool out_packed;
 };
 
 template <class Tile>
@@ -323,9 +317,9 @@ __device__ __forceinline__ void formWeightGradient(const WeightGradientArgs& arg
             if (m < args.hidden && n < args.dim) {
                 if (args.splits > 1) {
                     const std::int64_t row = (2 * static_cast<std::int64_t>(split) + (second ? 1 : 0)) * args.hidden + m;
-                    storeFour(sums[i][j], args.partials + row * args.dim + n, args.dim - n, args.dim % 4 == 0);
+                    storeFour(sums[i][j], args.partials + row * args.dim + n, args.dim - n);
                 } else {
-                    storeFour(sums[i][j], out + m * args.out_stride + n, args.dim - n, args.out_packed);
+                    storeFour(sums[i][j], out + m * args.out_stride + n, args.dim - n);
                 }
             }
         }
@@ -369,24 +363,25 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(const float* __restri
                                                            long long rows, int columns, long long rows_first,
                                                            T* __restrict__ first, T* __restrict__ second,
                                                            std::int64_t stride) {
-    const long long packs = rows * (columns / kPack);
-    const int packs_per_row = columns / kPack;
+    const int packs_per_row = (columns + kPack - 1) / kPack;
+    const long long packs = rows * packs_per_row;
     const long long split_values = rows * columns;
     for (long long p = static_cast<long long>(blockIdx.x) * kJoinThreads + threadIdx.x; p < packs;
          p += static_cast<long long>(gridDim.x) * kJoinThreads) {
+        const long long row = p / packs_per_row;
+        const int column = packColumn<kPack>(static_cast<int>(p - row * packs_per_row), columns);
+        const float* from = partials + row * columns + column;
         float sum[kPack];
-        loadPack(partials + p * kPack, sum);
+        loadPack(from, sum);
 #pragma unroll 4
         for (int s = 1; s < splits; ++s) {
             float more[kPack];
-            loadPack(partials + s * split_values + p * kPack, more);
+            loadPack(from + s * split_values, more);
 #pragma unroll
             for (int e = 0; e < kPack; ++e) {
                 sum[e] += more[e];
             }
         }
-        const long long row = p / packs_per_row;
-        const int column = static_cast<int>(p - row * packs_per_row) * kPack;
         T* to = row < rows_first ? first + row * stride : second + (row - rows_first) * stride;
         storePack(sum, to + column);
     }
@@ -508,9 +503,9 @@ std::size_t weightPartials(const zcgvs_gated_desc& d) {
 
 template <typename T>
 int launchJoin(const float* partials, int splits, std::int64_t rows, int columns, std::int64_t rows_first, void* first,
-               void* second, std::int64_t stride, bool packed, hipStream_t stream) {
-    const bool four = packed && columns % 4 == 0;
-    const long long packs = static_cast<long long>(rows) * (columns / (four ? 4 : 1));
+               void* second, std::int64_t stride, hipStream_t stream) {
+    const bool four = columns >= 4;
+    const long long packs = static_cast<long long>(rows) * (four ? (columns + 3) / 4 : columns);
     const unsigned blocks = static_cast<unsigned>(std::min(8192ll, (packs + kJoinThreads - 1) / kJoinThreads));
     if (four) {
         joinKernel<T, 4><<<blocks, kJoinThreads, 0, stream>>>(partials, splits, rows, columns, rows_first,
@@ -630,11 +625,11 @@ int launchGradients(const zcgvs_gated_desc& d, InputGradientArgs input, WeightGr
     }
     if (status == ZCGVS_OK && wants_input && input.splits > 1) {
         status = launchJoin<T>(input.partials, input.splits, d.rows, d.dim, d.rows, input.out, nullptr,
-                               input.out_stride, input.out_packed, stream);
+                               input.out_stride, stream);
     }
     if (status == ZCGVS_OK && wants_weight && weight.splits > 1) {
         status = launchJoin<T>(weight.partials, weight.splits, 2 * static_cast<std::int64_t>(d.hidden), d.dim, d.hidden,
-                               weight.gate_out, weight.up_out, weight.out_stride, weight.out_packed, stream);
+                               weight.gate_out, weight.up_out, weight.out_stride, stream);
     }
     return status;
 }
@@ -675,7 +670,6 @@ int zcgvs_gated_projection(const zcgvs_gated_desc* desc, void* d_out, std::int64
     GatedArgs args{};
     args.out = d_out;
     args.out_stride = rowStride(out_stride, d.hidden);
-    args.out_packed = alignedRows(d_out, args.out_stride, d.dtype, 4 * elementBytes(d.dtype));
     const int launched = withElement(d.dtype, [&](auto element) {
         return launchGated<decltype(element), false>(d, args, toStream(stream));
     });
@@ -743,10 +737,8 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
         GatedArgs form{};
         form.out = d_workspace;
         form.out_stride = gradientStride(d);
-        form.out_packed = true;
         form.out_gradient = d_out_gradient;
         form.out_gradient_stride = from_stride;
-        form.gradient_packed = alignedRows(d_out_gradient, from_stride, d.dtype, 4 * elementBytes(d.dtype));
         form.du_offset = d.rows * form.out_stride;
         const int formed = launchGated<T, true>(d, form, toStream(stream));
         if (formed != ZCGVS_OK) {
@@ -766,7 +758,6 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
         input.partials = partials;
         input.out = d_x_gradient;
         input.out_stride = x_out_stride;
-        input.out_packed = alignedRows(d_x_gradient, x_out_stride, d.dtype, 4 * elementBytes(d.dtype));
         WeightGradientArgs weight{};
         weight.dg = d_workspace;
         weight.d_stride = form.out_stride;
@@ -780,8 +771,6 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
         weight.gate_out = d_gate_gradient;
         weight.up_out = d_up_gradient;
         weight.out_stride = weight_out_stride;
-        weight.out_packed = alignedRows(d_gate_gradient, weight_out_stride, d.dtype, 4 * elementBytes(d.dtype)) &&
-                            alignedRows(d_up_gradient, weight_out_stride, d.dtype, 4 * elementBytes(d.dtype));
         return launchGradients<T>(d, input, weight, toStream(stream));
     });
     return launched == ZCGVS_OK ? clearError() : launched;

@@ -62,15 +62,19 @@ struct SplitLoader {
         k_left = k_total;
     }
     __device__ __forceinline__ void fetch() {
+        if (k_left >= kStage && (!kTurned || columns_left >= kRows)) {
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            int row, chunk;
-            Plane::placeOf(i, row, chunk);
-            const int valid = kTurned ? (row < k_left ? columns_left - chunk * kValues : 0) : k_left - chunk * kValues;
-            if (valid >= kValues) {
+            for (int i = 0; i < kCopies; ++i) {
                 __builtin_memcpy(&held[i][0], src[i], 16);
                 __builtin_memcpy(&held[i][4], src[i] + 4, 16);
-            } else {
+                src[i] += step;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                int row, chunk;
+                Plane::placeOf(i, row, chunk);
+                const int valid = kTurned ? (row < k_left ? columns_left - chunk * kValues : 0) : k_left - chunk * kValues;
 #pragma unroll
                 for (int e = 0; e < kValues; ++e) {
                     held[i][e] = 0.0f;
@@ -78,8 +82,8 @@ struct SplitLoader {
                         held[i][e] = src[i][e];
                     }
                 }
+                src[i] += k_left >= kStage ? step : 0;
             }
-            src[i] += k_left >= kStage ? step : 0;
         }
         k_left -= kStage;
     }

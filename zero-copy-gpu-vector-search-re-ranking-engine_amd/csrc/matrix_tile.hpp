@@ -181,26 +181,36 @@ struct StageLoader {
 
     // Reads the next stage into registers, and later writes it to `stage` (not direct).
     __device__ __forceinline__ void fetch() {
+        if (k_left >= kStageK<T> && (!kTurned || columns_left >= kRows)) {
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            int row, chunk;
-            placeOf(i, row, chunk);
-            int valid = kTurned ? (row < k_left ? columns_left - chunk * kChunk<T> : 0) : k_left - chunk * kChunk<T>;
-            valid = hasCopy(i) ? valid : 0;
-            if (valid >= kChunk<T>) {
-                __builtin_memcpy(&held[i], src[i], 16);
-            } else {
+            for (int i = 0; i < kCopies; ++i) {
+                if (hasCopy(i)) {
+                    __builtin_memcpy(&held[i], src[i], 16);
+                }
+                src[i] += step;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                int row, chunk;
+                placeOf(i, row, chunk);
+                int valid = kTurned ? (row < k_left ? columns_left - chunk * kChunk<T> : 0) : k_left - chunk * kChunk<T>;
+                valid = hasCopy(i) ? valid : 0;
                 typename Fragment<T>::type v = {};
                 const T* from = reinterpret_cast<const T*>(src[i]);
+                if (valid >= kChunk<T>) {
+                    __builtin_memcpy(&v, from, 16);
+                } else {
 #pragma unroll
-                for (int e = 0; e < kChunk<T>; ++e) {
-                    if (e < valid) {
-                        v[e] = from[e];
+                    for (int e = 0; e < kChunk<T>; ++e) {
+                        if (e < valid) {
+                            v[e] = from[e];
+                        }
                     }
                 }
                 held[i] = __builtin_bit_cast(u32x4, v);
+                src[i] += k_left >= kStageK<T> ? step : 0;
             }
-            src[i] += k_left >= kStageK<T> ? step : 0;
         }
         k_left -= kStageK<T>;
     }
@@ -417,9 +427,9 @@ __device__ __forceinline__ void tileOf(int index, int tiles_m, int tiles_n, int&
 
 // Reads four neighbouring values of one row of which `left` exist; the others are zeros.
 template <typename T>
-__device__ __forceinline__ f32x4 loadFour(const T* from, int left, bool packed) {
+__device__ __forceinline__ f32x4 loadFour(const T* from, int left) {
     f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (packed && left >= 4) {
+    if (left >= 4) {
         float v[4];
         loadPack(from, v);
         value = f32x4{v[0], v[1], v[2], v[3]};
@@ -434,11 +444,10 @@ __device__ __forceinline__ f32x4 loadFour(const T* from, int left, bool packed) 
     return value;
 }
 
-// Stores four neighbouring results of one row; `left` of them exist. `packed`: rows and their first
-// element allow stores of four.
+// Stores four neighbouring results of one row; `left` of them exist.
 template <typename Out>
-__device__ __forceinline__ void storeFour(const f32x4& value, Out* to, int left, bool packed) {
-    if (packed && left >= 4) {
+__device__ __forceinline__ void storeFour(const f32x4& value, Out* to, int left) {
+    if (left >= 4) {
         const float v[4] = {value[0], value[1], value[2], value[3]};
         storePack(v, to);
     } else {
