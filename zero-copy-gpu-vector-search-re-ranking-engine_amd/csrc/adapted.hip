@@ -15,7 +15,7 @@
 //
 // Measured: 8192 rows 1024 -> 1024, 32 adapters of rank 32 in runs of 250, bfloat16: 59 us, of which the sort 11,
 // low 12.5, the projection 23 (a library product 25) and the adapters' part 13; 300 mixed rows of 200 adapters
-// 20.8 us, three launches' latency; 8 rows 10.3 us in one launch.
+// 14.0 us, 8 rows of 64 9.7 us, in two launches.
 //
 // Rows are kept apart: a row's sums take the products with its own adapter only, chosen and not
 // multiplied by zero, so infinities and NaN in one adapter stay in its rows.
@@ -498,13 +498,18 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kThreads >= 512 ? 4 : 3) void
 
 // ---- few rows -----------------------------------------------------------------------------------
 
-// Up to 16 rows in one launch: a workgroup forms 16 columns of all of them. Its wavefronts first form low, a
-// row each (every workgroup does: low is small, and another launch would cost more), then an eighth of the
-// products over dim each; 256 threads add those up, and their result's share of low up^T to it. All of low
-// stays in float32.
+// Few rows, in their own order: a workgroup forms 16 columns of 16 rows. Its 16 wavefronts form a sixteenth of
+// the products over dim each; 256 threads add those up and their result's share of low up^T. low is formed
+// either by every workgroup for itself (as many wavefronts to a row as there are for each, every one over its part
+// of dim), which saves a launch while the rows of down that it reads are few, or by a launch before. All of
+// low stays in float32. Measured, float16, rank 16, mixed adapters, against the sorted rows' three launches: 1 row
+// of 768 -> 768 6.8 us (two launches 9.9), 8 rows 9.9 (one launch 12.2); 300 rows of 384 -> 384 9.6 against 18.1,
+// 1000 rows 16.1 against 23.1; 300 rows of 1024 -> 1024 20.8 against 24.9, 500 rows 28.6 against 25.4.
 constexpr int kFewRows = 16;
-constexpr int kFewThreads = 512;
+constexpr int kFewThreads = 1024;
 constexpr int kFewWaves = kFewThreads / kWave;
+constexpr std::int64_t kFewProducts = 400'000'000;  // rows * dim * out_dim up to which it is taken
+constexpr std::int64_t kFewDownBytes = 50 * 1024;   // of down that a workgroup reads
 
 // Products of 16 rows of `a_row` and 16 rows of `b_row` (a lane has its row l % 16 of each) over the steps
 // [step, past).
@@ -535,41 +540,89 @@ __device__ __forceinline__ f32x4 multiplyRows(const T* a_row, const T* b_row, in
     return sum;
 }
 
-template <typename T, typename Out>
+// low of one row and 16 ranks: args.low is float32 [rows, max_rank] here.
+constexpr int kLowFewThreads = 256;
+constexpr int kLowFewWaves = kLowFewThreads / kWave;
+
+template <typename T>
+__global__ __launch_bounds__(kLowFewThreads) void lowFewKernel(AdaptedArgs args, const int* adapter_ids) {
+    __shared__ float joined[kLowFewWaves][16];
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int row = static_cast<int>(blockIdx.x);
+    const int r = static_cast<int>(blockIdx.y) * 16;
+    const int adapter = adapter_ids[row];
+    if (!counts(adapter, args.adapter_count, -1)) {
+        return;
+    }
+    const int rank = rankOf(args, adapter);
+    if (r >= rank) {
+        return;
+    }
+    const int steps = (args.dim + 4 * kChunk<T> - 1) / (4 * kChunk<T>);
+    const int share = (steps + kLowFewWaves - 1) / kLowFewWaves;
+    const T* down = static_cast<const T*>(args.down) +
+                    (static_cast<std::int64_t>(adapter) * args.max_rank + min(r + (lane & 15), rank - 1)) * args.dim;
+    const f32x4 sum = multiplyRows(static_cast<const T*>(args.x) + row * args.x_stride, down, wave * share,
+                                   min((wave + 1) * share, steps), args.dim);
+    if ((lane & 15) == 0) {  // every column holds the row
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            joined[wave][4 * (lane >> 4) + e] = sum[e];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 16 && r + static_cast<int>(threadIdx.x) < rank) {
+        float whole = 0.0f;
+        for (int w = 0; w < kLowFewWaves; ++w) {
+            whole += joined[w][threadIdx.x];
+        }
+        const float scale = args.scales == nullptr ? 1.0f : args.scales[adapter];
+        static_cast<float*>(args.low)[static_cast<std::int64_t>(row) * args.max_rank + r + threadIdx.x] = whole * scale;
+    }
+}
+
+// kFormLow: low is formed here; otherwise it stands in args.low.
+template <typename T, typename Out, bool kFormLow>
 __global__ __launch_bounds__(kFewThreads) void adaptedFewKernel(AdaptedArgs args, const int* adapter_ids) {
-    __shared__ float low[kFewRows][kMaxRank + 4];
+    __shared__ float low[kFormLow ? kFewWaves : 1][kMaxRank + 4];
     __shared__ float parts[kFewWaves][16][17];
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int r16 = lane & 15;
     const int h = lane >> 4;
     const int n0 = static_cast<int>(blockIdx.x) * 16;
+    const int m0 = static_cast<int>(blockIdx.y) * kFewRows;
+    const int rows = min(kFewRows, args.rows - m0);
     const int steps = (args.dim + 4 * kChunk<T> - 1) / (4 * kChunk<T>);
+    const T* x_row = static_cast<const T*>(args.x) + (m0 + min(r16, rows - 1)) * args.x_stride;
+    // wavefronts to a row of low: the largest power of two that serves all rows
+    int helpers = kFewWaves;
+    while (helpers * rows > kFewWaves) {
+        helpers /= 2;
+    }
+    const int my_row = wave / helpers;
+    const int my_adapter = kFormLow && adapter_ids != nullptr && my_row < rows ? adapter_ids[m0 + my_row] : -1;
     const int share = (steps + kFewWaves - 1) / kFewWaves;
-    const T* x_row = static_cast<const T*>(args.x) + min(r16, args.rows - 1) * args.x_stride;
     const T* weight_row = static_cast<const T*>(args.weight) + min(n0 + r16, args.out_dim - 1) * args.weight_stride;
     const f32x4 product = multiplyRows(x_row, weight_row, wave * share, min((wave + 1) * share, steps), args.dim);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         parts[wave][r16][4 * h + e] = product[e];
     }
-    if (adapter_ids != nullptr) {
-        for (int row = wave; row < args.rows; row += kFewWaves) {
-            const int adapter = adapter_ids[row];
-            if (!counts(adapter, args.adapter_count, -1)) {
-                continue;
-            }
-            const int rank = rankOf(args, adapter);
-            const float scale = args.scales == nullptr ? 1.0f : args.scales[adapter];
-            const T* down = static_cast<const T*>(args.down) + static_cast<std::int64_t>(adapter) * args.max_rank * args.dim;
-            for (int r = 0; r < rank; r += 16) {
-                const f32x4 sum = multiplyRows(x_row, down + static_cast<std::int64_t>(min(r + r16, rank - 1)) * args.dim, 0,
-                                               steps, args.dim);
-                if (r16 == row) {
+    if (kFormLow && counts(my_adapter, args.adapter_count, -1)) {
+        const int rank = rankOf(args, my_adapter);
+        const float scale = args.scales == nullptr ? 1.0f : args.scales[my_adapter];
+        const T* down = static_cast<const T*>(args.down) + static_cast<std::int64_t>(my_adapter) * args.max_rank * args.dim;
+        const int low_share = (steps + helpers - 1) / helpers;
+        const int first = wave % helpers * low_share;
+        for (int r = 0; r < rank; r += 16) {
+            const f32x4 sum = multiplyRows(x_row, down + static_cast<std::int64_t>(min(r + r16, rank - 1)) * args.dim, first,
+                                           min(first + low_share, steps), args.dim);
+            if (r16 == my_row) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        low[row][r + 4 * h + e] = sum[e] * scale;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    low[wave][r + 4 * h + e] = sum[e] * scale;
                 }
             }
         }
@@ -577,11 +630,11 @@ __global__ __launch_bounds__(kFewThreads) void adaptedFewKernel(AdaptedArgs args
     __syncthreads();
     const int row = static_cast<int>(threadIdx.x) / 16;
     const int n = n0 + static_cast<int>(threadIdx.x) % 16;
-    if (row >= args.rows || n >= args.out_dim) {
+    if (row >= rows || n >= args.out_dim) {
         return;
     }
     float sum = 0.0f;
-    const int adapter = adapter_ids == nullptr ? -1 : adapter_ids[row];
+    const int adapter = adapter_ids == nullptr ? -1 : adapter_ids[m0 + row];
     if (counts(adapter, args.adapter_count, -1)) {
         const int rank = rankOf(args, adapter);
         const T* up = static_cast<const T*>(args.up) +
@@ -590,7 +643,17 @@ __global__ __launch_bounds__(kFewThreads) void adaptedFewKernel(AdaptedArgs args
             const auto b = loadChunk(up + r, args.max_rank - r);
 #pragma unroll
             for (int e = 0; e < kChunk<T>; ++e) {
-                sum += r + e < rank ? low[row][r + e] * static_cast<float>(b[e]) : 0.0f;
+                if (r + e < rank) {
+                    float whole = 0.0f;
+                    if constexpr (kFormLow) {
+                        for (int w = 0; w < helpers; ++w) {
+                            whole += low[row * helpers + w][r + e];
+                        }
+                    } else {
+                        whole = static_cast<const float*>(args.low)[static_cast<std::int64_t>(m0 + row) * args.max_rank + r + e];
+                    }
+                    sum += whole * static_cast<float>(b[e]);
+                }
             }
         }
     }
@@ -598,7 +661,7 @@ __global__ __launch_bounds__(kFewThreads) void adaptedFewKernel(AdaptedArgs args
     for (int w = 0; w < kFewWaves; ++w) {
         sum += parts[w][row][static_cast<int>(threadIdx.x) % 16];
     }
-    static_cast<Out*>(args.out)[row * args.out_stride + n] = static_cast<Out>(sum);
+    static_cast<Out*>(args.out)[(m0 + row) * args.out_stride + n] = static_cast<Out>(sum);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -775,7 +838,10 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
     args.out_dim = d.out_dim;
     args.out = d_out;
     args.out_stride = stride;
-    const bool few = d.rows <= kFewRows;
+    const bool few = d.rows <= kFewRows ||
+                     (hasAdapters(d) && d.rows <= 4096 && d.rows * d.dim * d.out_dim <= kFewProducts);
+    const bool low_by_all =
+        !hasAdapters(d) || (d.max_rank <= 16 && d.rows * d.max_rank * d.dim * elementBytes(d.dtype) <= kFewDownBytes);
     if (hasAdapters(d)) {
         char* workspace = static_cast<char*>(d_workspace);
         args.down = d.down;
@@ -809,8 +875,17 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, std::i
             using Out = decltype(element);
             if constexpr (std::is_same_v<Out, T> || std::is_same_v<Out, float>) {
                 if (few) {
-                    adaptedFewKernel<T, Out><<<static_cast<unsigned>(divideUp(d.out_dim, 16)), kFewThreads, 0,
-                                               toStream(stream)>>>(args, hasAdapters(d) ? d.adapter_ids : nullptr);
+                    const dim3 grid(static_cast<unsigned>(divideUp(d.out_dim, 16)),
+                                    static_cast<unsigned>(divideUp(d.rows, kFewRows)));
+                    const int* ids = hasAdapters(d) ? d.adapter_ids : nullptr;
+                    if (low_by_all) {
+                        adaptedFewKernel<T, Out, true><<<grid, kFewThreads, 0, toStream(stream)>>>(args, ids);
+                    } else {
+                        lowFewKernel<T><<<dim3(static_cast<unsigned>(d.rows), static_cast<unsigned>(divideUp(d.max_rank, 16))),
+                                          kLowFewThreads, 0, toStream(stream)>>>(args, ids);
+                        ZCGVS_LAUNCH_CHECK("adapted projection");
+                        adaptedFewKernel<T, Out, false><<<grid, kFewThreads, 0, toStream(stream)>>>(args, ids);
+                    }
                     ZCGVS_LAUNCH_CHECK("adapted projection");
                     return static_cast<int>(ZCGVS_OK);
                 }
