@@ -145,6 +145,22 @@ def test_gradient(gpu, case, accumulate):
     assert np.all(np.abs(result - expected) <= tolerance)
 
 
+FEW_CASES = [
+    ("f32", "f32", 40, 5, 2, 2, True, -1, 0, 0, 1.0),
+    ("f16", "f32", 300, 130, 60, 7, True, 5, 2, 0, 2.0),
+    ("bf16", "bf16", 2, 1028, 511, 0, False, -1, 0, 0, 1.0),
+    ("f32", "f32", 7, 384, 512, 40, True, 0, 3, 1, 1.0),
+    ("bf16", "f32", 30_000, 260, 512, 1, False, 0, 0, 0, 0.5),
+]
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("case", FEW_CASES, ids=str)
+def test_gradient_of_few_tokens(gpu, case, accumulate):
+    """Up to 512 tokens are not sorted: bags, one id at nearly all positions, several slices of columns."""
+    test_gradient(gpu, case, accumulate)
+
+
 def test_gradient_is_the_difference_of_the_lookup(gpu):
     """A step in one table entry changes the weighted sum of the outputs by the gradient's entry."""
     capi = gpu

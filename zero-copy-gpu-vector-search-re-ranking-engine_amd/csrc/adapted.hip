@@ -2,8 +2,8 @@
 //
 //     out[r] = x[r] weight^T + scale_a (x[r] down_a^T) up_a^T,   a = adapter_ids[r]
 //
-// The rows are sorted by adapter, so that rows of one adapter are next to each other in any batch, and
-// x and out are addressed through the order. `low` = scale_a x[r] down_a^T is formed first, one group of
+// The rows of a large batch are sorted by adapter, so that rows of one adapter are next to each other, and
+// x and out are addressed through the order; few rows keep theirs. `low` = scale_a x[r] down_a^T is formed first, one group of
 // up to 16 rows of one adapter at a time; the projection's kernel then adds low up_a^T to each tile's
 // sums: out is written once for both.
 //
