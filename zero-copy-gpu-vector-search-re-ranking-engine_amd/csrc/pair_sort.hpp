@@ -42,10 +42,11 @@ struct SortInput {
 
 __device__ __forceinline__ bool counts(int id, int end, int skipped) { return id >= 0 && id < end && id != skipped; }
 
-__device__ __forceinline__ int sortKey(const SortInput& in, int i) {
-    const int key = in.keys[i];
+__device__ __forceinline__ int checkedKey(const SortInput& in, int key) {
     return !in.raw || counts(key, in.key_end, in.skipped) ? key : in.key_end;
 }
+
+__device__ __forceinline__ int sortKey(const SortInput& in, int i) { return checkedKey(in, in.keys[i]); }
 
 // Orders a wavefront's LDS accesses before and after it.
 __device__ __forceinline__ void waveFence() {
@@ -130,12 +131,20 @@ __global__ __launch_bounds__(kSmallThreads) void sortSmallKernel(SortInput in, i
         const unsigned mask = static_cast<unsigned>(digits) - 1u;
         int key[kSmallRounds];
         unsigned rank[kSmallRounds];
+        // all loads before the first use: one latency, not one a round
+        if (p == 0) {
 #pragma unroll
-        for (int round = 0; round < kSmallRounds; ++round) {
-            const int i = (wave * rounds + round) * kWave + lane;
-            key[round] = 0;
-            if (round < rounds && i < in.count) {
-                key[round] = p == 0 ? sortKey(in, i) : keys[p & 1][i];
+            for (int round = 0; round < kSmallRounds; ++round) {
+                key[round] = in.keys[min((wave * rounds + round) * kWave + lane, in.count - 1)];
+            }
+#pragma unroll
+            for (int round = 0; round < kSmallRounds; ++round) {
+                key[round] = checkedKey(in, key[round]);
+            }
+        } else {
+#pragma unroll
+            for (int round = 0; round < kSmallRounds; ++round) {
+                key[round] = keys[p & 1][min((wave * rounds + round) * kWave + lane, in.count - 1)];
             }
         }
         for (int d = lane; d < digits; d += kWave) {
