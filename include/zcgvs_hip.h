@@ -474,8 +474,8 @@ int zcgvs_embedding_lookup(const zcgvs_embedding_desc* desc, void* d_out, int64_
 
 /* The gradient of zcgvs_embedding_lookup with respect to the table, from the gradient of its output
  * rows (d_out_gradient, of `gradient_dtype`): d_table_gradient[v] = scale * the sum of the output
- * gradients of v's tokens (with ZCGVS_EMBEDDING_MEAN each over its bag's counting tokens). The tokens
- * are sorted by id, stably, and each row's terms are added in a fixed grouping of that order.
+ * gradients of v's tokens (with ZCGVS_EMBEDDING_MEAN each over its bag's counting tokens). Each
+ * row's terms are added in a fixed grouping of the tokens' order.
  * accumulate == 0: every row of d_table_gradient [vocab, dim] is written, those of tokens that do not
  * occur with zeros. accumulate != 0: the sums are added to d_table_gradient and only rows of tokens
  * that occur are touched. table_gradient_dtype is gradient_dtype or ZCGVS_DTYPE_F32. */
