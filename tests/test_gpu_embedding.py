@@ -151,6 +151,8 @@ FEW_CASES = [
     ("bf16", "bf16", 2, 1028, 511, 0, False, -1, 0, 0, 1.0),
     ("f32", "f32", 7, 384, 512, 40, True, 0, 3, 1, 1.0),
     ("bf16", "f32", 30_000, 260, 512, 1, False, 0, 0, 0, 0.5),
+    ("f32", "f32", 2_200_001, 4, 100, 0, False, -1, 0, 0, 1.0),
+    ("f16", "f16", 5000, 2051, 9, 0, False, 0, 3, 0, 1.0),
 ]
 
 
@@ -224,6 +226,21 @@ def test_no_tokens(gpu):
     capi.embedding_gradient(desc, None, capi.F32, grad, capi.F32, None, 0, accumulate=True)
     capi.synchronize()
     assert np.all(out.to_host() == 0.0) and np.all(grad.to_host() == 1.0)
+    capi.embedding_gradient(desc, None, capi.F32, grad, capi.F32, None, 0)
+    capi.synchronize()
+    assert np.all(grad.to_host() == 0.0)
+
+
+def test_tokens_of_no_bag(gpu):
+    """Without bags no token counts, and every row of the gradient is zeros."""
+    capi = gpu
+    ids = capi.DeviceArray.from_host(np.arange(4, dtype=np.int32))
+    offsets = capi.DeviceArray.from_host(np.zeros(1, np.int64))
+    grad = capi.DeviceArray.from_host(np.ones((5, 6), np.float32))
+    desc = capi.embedding_desc(None, 5, 6, capi.F32, ids, 4, bag_offsets=offsets, bag_count=0)
+    capi.embedding_gradient(desc, None, capi.F32, grad, capi.F32, None, 0, accumulate=True)
+    capi.synchronize()
+    assert np.all(grad.to_host() == 1.0)
     capi.embedding_gradient(desc, None, capi.F32, grad, capi.F32, None, 0)
     capi.synchronize()
     assert np.all(grad.to_host() == 0.0)

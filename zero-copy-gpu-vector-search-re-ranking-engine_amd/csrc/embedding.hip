@@ -260,87 +260,6 @@ __device__ __forceinline__ void finishRow(const GradientArgs& args, int key, int
     }
 }
 
-// Few tokens need no sort: a workgroup looks whether its token is the first of its id and sums the id's
-// tokens then, over a slice of 64 packs. Every wavefront takes a quarter of the positions from the token's on, in
-// their order; the quarters are joined in theirs. A launch instead of the sort's and its followers': 500
-// tokens of 384 columns take 13.0 us with the clearing of 30,000 rows, sorted 18.0 us, and 10.2 us against 15.9 us
-// at 2,000 rows. The time grows with the tokens of one id: 500 of the same take 13.5 us against 13.4 us,
-// 1,000 24 us against 13.5 us, so more are sorted.
-constexpr int kFewAhead = 16;
-constexpr std::int64_t kFewTokens = 512;
-
-template <typename In, typename Out, int kPack>
-__global__ __launch_bounds__(kThreads) void gradientFewKernel(GradientArgs args, SortInput in, int slices) {
-    __shared__ float sums[kWavesPerBlock][kWave * kPack];
-    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
-    const int token = static_cast<int>(blockIdx.x) / slices;
-    const int pack = (static_cast<int>(blockIdx.x) - token * slices) * kWave + lane;
-    const int key = sortKey(in, token);
-    if (key >= in.key_end) {
-        return;
-    }
-    bool earlier = false;
-    for (int i = static_cast<int>(threadIdx.x); i < token; i += kThreads) {
-        earlier |= sortKey(in, i) == key;
-    }
-    if (__syncthreads_or(earlier ? 1 : 0) != 0) {
-        return;
-    }
-    const bool has_column = pack < (args.dim + kPack - 1) / kPack;
-    const In* from = static_cast<const In*>(args.out_gradient) + (has_column ? packColumn<kPack>(pack, args.dim) : 0);
-    const int share = (in.count - token + kThreads - 1) / kThreads * kWave;
-    const int end = min(token + (wave + 1) * share, in.count);
-    float sum[kPack] = {};
-    for (int base = token + wave * share; base < end; base += kWave) {
-        const int position = min(base + lane, in.count - 1);
-        const int my_row = in.rows == nullptr ? position : in.rows[position];
-        const bool mine = base + lane < end && sortKey(in, position) == key;
-        float my_weight = 1.0f;
-        if (args.bag_counts != nullptr && mine) {
-            my_weight = 1.0f / static_cast<float>(args.bag_counts[my_row]);
-        }
-        unsigned long long left = __ballot(mine);
-        while (left != 0) {
-            typename Pack<In, kPack>::stored value[kFewAhead];
-            int at[kFewAhead];
-            int taken = 0;
-#pragma unroll
-            for (int u = 0; u < kFewAhead; ++u) {
-                if (left != 0) {
-                    at[u] = __builtin_ctzll(left);
-                    left &= left - 1;
-                    const std::int64_t row = __builtin_amdgcn_readlane(my_row, at[u]);
-                    value[u] = *reinterpret_cast<const typename Pack<In, kPack>::stored*>(
-                        from + row * args.out_gradient_stride);
-                    ++taken;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kFewAhead; ++u) {
-                if (u < taken) {
-                    const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), at[u]));
-                    addPack(value[u], weight, sum);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < kPack; ++e) {
-        sums[wave][lane * kPack + e] = sum[e];
-    }
-    __syncthreads();
-    if (wave == 0 && has_column) {
-        for (int w = 1; w < kWavesPerBlock; ++w) {
-#pragma unroll
-            for (int e = 0; e < kPack; ++e) {
-                sum[e] += sums[w][lane * kPack + e];
-            }
-        }
-        finishRow<Out, kPack>(args, key, pack, sum);
-    }
-}
-
 // A wavefront sums one chunk's rows over 64 packs of columns: it reads the chunk's ids and rows at once, a
 // lane each (a chunk is at most 64 positions), and hands them on as scalars; kGradientAhead rows are in
 // flight.
@@ -565,12 +484,137 @@ struct ClearRows {
     }
 };
 
-// The same without a sort, for few tokens.
-constexpr int kClearBlocks = 2048;
+// Few tokens need no sort: a workgroup looks whether its token is the first of its id and sums the id's
+// tokens then, over a slice of 64 packs. Every wavefront takes a quarter of the positions from the token's on, in
+// their order; the quarters are joined in theirs. One launch instead of three: 500
+// tokens of 384 columns take 9.9 us with the clearing of 30,000 rows, sorted 18.0 us, and 7.5 us against 15.9 us at
+// 2,000 rows. The time grows with the tokens of one id, as its workgroup's loads do: 500 of the same take 11.7 us
+// against 13.4 us, 1,000 about 24 us against 13.5 us, so more are sorted.
+// Blocks past those of the sums clear the rows that no token names, a range of rows at a time, whose named ones
+// they mark first: one launch for both, 2 to 3 us less than two (500 tokens and 30,000 rows of 384 columns
+// 13.4 -> 9.9 us).
+constexpr int kFewAhead = 16;
+constexpr std::int64_t kFewTokens = 512;
+constexpr int kFewClearBlocks = 2048;
+constexpr int kFewClearRows = 1024;  // of a range
 
 template <typename Out, int kPack>
-__global__ __launch_bounds__(kThreads) void clearRowsKernel(ClearRows<Out, kPack> clear) {
-    clear.run(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), 0, 1);
+__device__ __forceinline__ void clearUnnamed(const ClearRows<Out, kPack>& clear, const SortInput& in, int block) {
+    __shared__ unsigned named[kFewClearRows / 32];
+    const int packs_per_row = (clear.dim + kPack - 1) / kPack;
+    const int range_rows = min(kFewClearRows, (in.key_end - 1) / kFewClearBlocks + 1);
+    const int ranges = (in.key_end - 1) / range_rows + 1;
+    const float zeros[kPack] = {};
+    for (int range = block; range < ranges; range += kFewClearBlocks) {
+        const int first = range * range_rows;
+        const int rows = min(range_rows, in.key_end - first);
+        if (threadIdx.x < kFewClearRows / 32) {
+            named[threadIdx.x] = 0;
+        }
+        __syncthreads();
+        for (int i = static_cast<int>(threadIdx.x); i < in.count; i += kThreads) {
+            const int row = sortKey(in, i) - first;
+            if (row >= 0 && row < rows) {
+                atomicOr(&named[row / 32], 1u << (row % 32));
+            }
+        }
+        __syncthreads();
+        int row = static_cast<int>(threadIdx.x) / packs_per_row;
+        int pack = static_cast<int>(threadIdx.x) - row * packs_per_row;
+        const int row_step = kThreads / packs_per_row;
+        const int pack_step = kThreads - row_step * packs_per_row;
+        while (row < rows) {
+            if (((named[row / 32] >> (row % 32)) & 1u) == 0) {
+                storePackOnce(zeros, clear.out + static_cast<std::int64_t>(first + row) * clear.stride +
+                                         packColumn<kPack>(pack, clear.dim));
+            }
+            row += row_step;
+            pack += pack_step;
+            if (pack >= packs_per_row) {
+                pack -= packs_per_row;
+                ++row;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename In, typename Out, int kPack>
+__global__ __launch_bounds__(kThreads) void gradientFewKernel(GradientArgs args, SortInput in, int slices,
+                                                            ClearRows<Out, kPack> clear) {
+    const int sum_blocks = in.count * slices;
+    if (static_cast<int>(blockIdx.x) >= sum_blocks) {
+        clearUnnamed<Out, kPack>(clear, in, static_cast<int>(blockIdx.x) - sum_blocks);
+        return;
+    }
+    __shared__ float sums[kWavesPerBlock][kWave * kPack];
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int token = static_cast<int>(blockIdx.x) / slices;
+    const int pack = (static_cast<int>(blockIdx.x) - token * slices) * kWave + lane;
+    const int key = sortKey(in, token);
+    if (key >= in.key_end) {
+        return;
+    }
+    bool earlier = false;
+    for (int i = static_cast<int>(threadIdx.x); i < token; i += kThreads) {
+        earlier |= sortKey(in, i) == key;
+    }
+    if (__syncthreads_or(earlier ? 1 : 0) != 0) {
+        return;
+    }
+    const bool has_column = pack < (args.dim + kPack - 1) / kPack;
+    const In* from = static_cast<const In*>(args.out_gradient) + (has_column ? packColumn<kPack>(pack, args.dim) : 0);
+    const int share = (in.count - token + kThreads - 1) / kThreads * kWave;
+    const int end = min(token + (wave + 1) * share, in.count);
+    float sum[kPack] = {};
+    for (int base = token + wave * share; base < end; base += kWave) {
+        const int position = min(base + lane, in.count - 1);
+        const int my_row = in.rows == nullptr ? position : in.rows[position];
+        const bool mine = base + lane < end && sortKey(in, position) == key;
+        float my_weight = 1.0f;
+        if (args.bag_counts != nullptr && mine) {
+            my_weight = 1.0f / static_cast<float>(args.bag_counts[my_row]);
+        }
+        unsigned long long left = __ballot(mine);
+        while (left != 0) {
+            typename Pack<In, kPack>::stored value[kFewAhead];
+            int at[kFewAhead];
+            int taken = 0;
+#pragma unroll
+            for (int u = 0; u < kFewAhead; ++u) {
+                if (left != 0) {
+                    at[u] = __builtin_ctzll(left);
+                    left &= left - 1;
+                    const std::int64_t row = __builtin_amdgcn_readlane(my_row, at[u]);
+                    value[u] = *reinterpret_cast<const typename Pack<In, kPack>::stored*>(
+                        from + row * args.out_gradient_stride);
+                    ++taken;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kFewAhead; ++u) {
+                if (u < taken) {
+                    const float weight = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_weight), at[u]));
+                    addPack(value[u], weight, sum);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kPack; ++e) {
+        sums[wave][lane * kPack + e] = sum[e];
+    }
+    __syncthreads();
+    if (wave == 0 && has_column) {
+        for (int w = 1; w < kWavesPerBlock; ++w) {
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                sum[e] += sums[w][lane * kPack + e];
+            }
+        }
+        finishRow<Out, kPack>(args, key, pack, sum);
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -720,25 +764,20 @@ int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, Gradien
         clear.dim = d.dim;
         clear.packs = static_cast<long long>(d.vocab) * ((d.dim + kPack - 1) / kPack);
     }
-    if (args.count <= kFewTokens && clear.out != nullptr) {
-        clearRowsKernel<Out, kPack><<<kClearBlocks, kThreads, 0, stream>>>(clear);
-        ZCGVS_LAUNCH_CHECK("embedding gradient");
-    }
-    if (args.count == 0) {
-        return ZCGVS_OK;
-    }
     SortInput input{};
-    const int paired = tokenPairs(d, s, workspace, input, stream);
-    if (paired != ZCGVS_OK) {
-        return paired;
-    }
-    if (args.count <= kFewTokens) {
-        const int slices = ((d.dim + kPack - 1) / kPack + kWave - 1) / kWave;
-        const long long blocks = static_cast<long long>(args.count) * slices;
-        if (blocks > kMaxBlocks) {
-            return invalid("more columns than one launch can take");
+    input.key_end = d.vocab;
+    if (args.count > 0) {
+        const int paired = tokenPairs(d, s, workspace, input, stream);
+        if (paired != ZCGVS_OK) {
+            return paired;
         }
-        gradientFewKernel<In, Out, kPack><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(args, input, slices);
+    }
+    const int slices = ((d.dim + kPack - 1) / kPack + kWave - 1) / kWave;
+    const long long few_blocks =
+        static_cast<long long>(args.count) * slices + (args.accumulate ? 0 : kFewClearBlocks);
+    if (args.count == 0 || (args.count <= kFewTokens && few_blocks <= kMaxBlocks)) {
+        gradientFewKernel<In, Out, kPack>
+            <<<static_cast<unsigned>(few_blocks), kThreads, 0, stream>>>(args, input, slices, clear);
         ZCGVS_LAUNCH_CHECK("embedding gradient");
         return ZCGVS_OK;
     }
@@ -749,7 +788,6 @@ int gradientTyped(const zcgvs_embedding_desc& d, const GradientSpace& s, Gradien
         return sorted;
     }
     const int chunks = static_cast<int>((static_cast<long long>(args.count) + s.chunk - 1) / s.chunk);
-    const int slices = ((d.dim + kPack - 1) / kPack + kWave - 1) / kWave;
     const long long items = static_cast<long long>(chunks) * slices;
     const long long blocks = (items + kWavesPerBlock - 1) / kWavesPerBlock;
     if (blocks > kMaxBlocks) {
