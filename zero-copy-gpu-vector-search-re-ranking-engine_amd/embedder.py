@@ -11,6 +11,9 @@ travels to the host between the token ids and the hits:
     queries = model.embed(ids, offsets, adapter_ids)
     desc = capi.search_desc(corpus, queries, len(offsets) - 1, k, capi.DOT)
 
+With `stream`, a call's copies and kernels run on that stream (the caller waits for it before another stream reads
+what the call returns); calls may follow each other without a wait, also on changing streams.
+
 The reference's QueryEmbedder (include/zcgvs/embed/query_embedder.hpp:8-15) returns one text's vector on
 the host instead. `gradient` gives what training the table and the gated block needs.
 """
@@ -49,6 +52,15 @@ class DeviceEmbedder:
                     values = adapters[name] if kind is None else np.asarray(adapters[name], kind)
                     self._adapters[name] = capi.DeviceArray.from_host(values)
         self._buffers = {}
+        self._stream = None  # of the last call
+        self._host = []      # arrays whose copies may be on their way
+
+    def _enter(self, stream):
+        """A call's copies and kernels go to its stream, in order behind those of the calls before it on that
+        stream. The buffers are shared by all calls, so one on another stream waits for the last one's."""
+        if getattr(stream, "handle", stream) != getattr(self._stream, "handle", self._stream):
+            capi.synchronize()
+        self._stream = stream  # kept: a destroyed stream's handle could come back as another stream's
 
     def _buffer(self, name, shape, kind):
         """A work buffer that grows and is kept; `shape` of it is used."""
@@ -65,36 +77,49 @@ class DeviceEmbedder:
                                    scale=self.scale)
 
     def _upload(self, name, values, kind):
+        """Starts the copy of a host array on the call's stream; _settle() waits for it."""
         values = np.ascontiguousarray(values, dtype=kind)
         buffer = self._buffer(name, values.shape, kind)
         if values.nbytes:
-            capi.call("zcgvs_memcpy_h2d", buffer.ptr, values.ctypes.data, values.nbytes, None)
-            capi.synchronize()
+            self._host.append(values)
+            capi.call("zcgvs_memcpy_h2d", buffer.ptr, values.ctypes.data, values.nbytes,
+                      getattr(self._stream, "handle", self._stream))
         return buffer
 
-    def _forward(self, ids, offsets, stream):
+    def _settle(self):
+        """Waits for the call's stream alone."""
+        capi.call("zcgvs_stream_synchronize", getattr(self._stream, "handle", self._stream))
+        self._host.clear()
+
+    def _forward(self, ids, offsets, stream, **more):
+        """The lookup and the gated block; `more`: further host arrays of the call, name=(values, type), copied
+        beside the ids."""
         texts, tokens = len(offsets) - 1, len(ids)
+        self._enter(stream)
         d_ids, d_offsets = self._upload("ids", ids, np.int32), self._upload("offsets", offsets, np.int64)
+        uploaded = {name: self._upload(name, *values) for name, values in more.items()}
+        self._settle()
         lookup = self._lookup_desc(d_ids, d_offsets, texts, tokens)
         rows = self._buffer("rows", (texts, self.dim), self._element)
         hidden = self._buffer("hidden", (texts, self.hidden), self._element)
         capi.embedding_lookup(lookup, rows, self.dtype, stream=stream)
         gated = capi.gated_desc(rows, texts, self.dim, self.gate, self.up, self.hidden, self.dtype, self.activation)
         capi.gated_projection(gated, hidden, stream=stream)
-        return lookup, gated, hidden
+        return lookup, gated, hidden, uploaded
 
     def embed(self, ids, offsets, adapter_ids=None, stream=None) -> capi.DeviceArray:
         """Queries of the texts ids[offsets[t]:offsets[t + 1]], each through adapter adapter_ids[t] (-1: none).
         The array belongs to the model and holds until the next call."""
         texts = len(offsets) - 1
-        _, _, hidden = self._forward(ids, offsets, stream)
-        extra = {}
+        more = {}
         if adapter_ids is not None:
             if not self._adapters:
                 raise ValueError("zcgvs embedder: the model has no adapters")
             if len(adapter_ids) != texts:
                 raise ValueError("zcgvs embedder: one adapter id per text")
-            extra = dict(self._adapters, adapter_ids=self._upload("adapter_ids", adapter_ids, np.int32))
+            more = dict(adapter_ids=(adapter_ids, np.int32))
+        _, _, hidden, uploaded = self._forward(ids, offsets, stream, **more)
+        extra = dict(self._adapters, **uploaded) if uploaded else {}
         desc = capi.adapted_desc(hidden, texts, self.hidden, self.projection, self.width, self.dtype, **extra)
         size = capi.adapted_projection_workspace_bytes(desc)
         workspace = self._buffer("workspace", (size,), np.uint8)
@@ -104,20 +129,19 @@ class DeviceEmbedder:
 
     def hidden_rows(self, ids, offsets, stream=None) -> np.ndarray:
         """The hidden rows on the host, as stored (for training, where a loss is formed from them)."""
-        _, _, hidden = self._forward(ids, offsets, stream)
+        _, _, hidden, _ = self._forward(ids, offsets, stream)
         out = np.empty((len(offsets) - 1, self.hidden), dtype=self._element)
-        capi.synchronize()
         if out.nbytes:
-            capi.call("zcgvs_memcpy_d2h", out.ctypes.data, hidden.ptr, out.nbytes, None)
-        capi.synchronize()
+            capi.call("zcgvs_memcpy_d2h", out.ctypes.data, hidden.ptr, out.nbytes, getattr(stream, "handle", stream))
+        self._settle()
         return out
 
     def gradient(self, ids, offsets, hidden_gradient, stream=None) -> dict:
         """The gradients of the table (float32) and of gate and up (their type), as device arrays, from the
         gradient of the hidden rows (host, of the model's type)."""
         texts, tokens = len(offsets) - 1, len(ids)
-        lookup, gated, _ = self._forward(ids, offsets, stream)
-        d_hidden = self._upload("hidden_gradient", hidden_gradient, self._element)
+        lookup, gated, _, uploaded = self._forward(ids, offsets, stream, hidden_gradient=(hidden_gradient, self._element))
+        d_hidden = uploaded["hidden_gradient"]
         rows = self._buffer("rows_gradient", (texts, self.dim), self._element)
         gate, up = (capi.DeviceArray((self.hidden, self.dim), self._element) for _ in range(2))
         size = capi.gated_gradient_workspace_bytes(gated)
