@@ -87,3 +87,98 @@ def test_calls_on_one_stream_leave_other_streams_alone(capi, recorded):
     for call in _calls(model, stream):
         call()
     assert recorded.device_waits == before
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(table=np.ones((50, 8), np.float16)), "table must hold float32"),
+    (dict(gate=np.ones((12, 8), np.float64)), "gate must hold float32"),
+    (dict(projection=np.ones((10, 12), np.uint16)), "projection must hold float32"),
+    (dict(table=np.ones(50, np.float32)), "table has shape"),
+    (dict(gate=np.ones((12, 9), np.float32)), "gate has shape"),
+    (dict(up=np.ones((11, 8), np.float32)), "up has shape"),
+    (dict(projection=np.ones((10, 8), np.float32)), "projection has shape"),
+])
+def test_weights_that_do_not_fit(capi, recorded, change, match):
+    from zcgvs_amd.embedder import DeviceEmbedder
+    with pytest.raises(ValueError, match=match):
+        DeviceEmbedder(*dict(_weights(), **change).values(), dtype=capi.F32)
+    assert not recorded.made  # refused before anything is allocated
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(down=None), "need down and up"),
+    (dict(up=None), "need down and up"),
+    (dict(down=np.ones((3, 4, 12), np.float16)), "down must hold float32"),
+    (dict(up=np.ones((3, 10, 4), np.float64)), "up must hold float32"),
+    (dict(up=np.ones((2, 10, 4), np.float32)), "up has shape"),
+    (dict(down=np.ones((3, 4, 8), np.float32)), "down has shape"),
+    (dict(ranks=[4, 4]), "one of ranks"),
+    (dict(ranks=[4.0, 4.0, 4.0]), "whole numbers"),
+    (dict(scales=[1.0]), "one of scales"),
+])
+def test_adapters_that_do_not_fit(capi, recorded, change, match):
+    from zcgvs_amd.embedder import DeviceEmbedder
+    adapters = dict(down=np.ones((3, 4, 12), np.float32), up=np.ones((3, 10, 4), np.float32))
+    with pytest.raises(ValueError, match=match):
+        DeviceEmbedder(*_weights().values(), dtype=capi.F32, adapters=dict(adapters, **change))
+    assert not recorded.made
+
+
+def test_types_that_are_none(capi, recorded):
+    from zcgvs_amd.embedder import DeviceEmbedder
+    for dtype in (capi.I8, capi.BINARY, 9):
+        with pytest.raises(ValueError, match="F32, F16 or BF16"):
+            DeviceEmbedder(*_weights().values(), dtype=dtype)
+    with pytest.raises(ValueError, match="table must hold uint16"):
+        DeviceEmbedder(*_weights().values(), dtype=capi.BF16)
+
+
+@pytest.mark.parametrize("ids,offsets,match", [
+    (IDS, [0, 2, 7], "offsets must ascend"),
+    (IDS, [0, 3, 2], "offsets must ascend"),
+    (IDS, [-1, 3], "offsets must ascend"),
+    (IDS, [], "offsets must ascend"),
+    (IDS, [0.0, 6.0], "whole numbers"),
+    (IDS.astype(np.float32), OFFSETS, "whole numbers"),
+    (IDS.reshape(2, 3), OFFSETS, "whole numbers"),
+    ([0, 2 ** 32, 1, 1, 1, 1], OFFSETS, "must fit int32"),
+])
+def test_ids_and_offsets_that_do_not_fit(capi, recorded, ids, offsets, match):
+    model = _model(capi)
+    made = len(recorded.made)
+    for call in (model.embed, model.hidden_rows, lambda i, o: model.gradient(i, o, GRADIENT)):
+        with pytest.raises(ValueError, match=match):
+            call(ids, offsets)
+    assert len(recorded.made) == made
+
+
+def test_adapter_ids_that_do_not_fit(capi, recorded):
+    model = _model(capi)
+    for ids, match in (([1], "one adapter id per text"), ([0.5, 1.0], "whole numbers"), ([0, 2 ** 31], "must fit int32")):
+        with pytest.raises(ValueError, match=match):
+            model.embed(IDS, OFFSETS, ids)
+    with pytest.raises(ValueError, match="no adapters"):
+        _model(capi, adapters=False).embed(IDS, OFFSETS, [0, 0])
+
+
+@pytest.mark.parametrize("gradient,match", [
+    (np.ones((1, 12), np.float32), "hidden_gradient has shape"),
+    (np.ones((2, 11), np.float32), "hidden_gradient has shape"),
+    (np.ones(24, np.float32), "hidden_gradient has shape"),
+    (np.ones((2, 12), np.float64), "hidden_gradient must hold float32"),
+    (np.ones((2, 12), np.uint16), "hidden_gradient must hold float32"),
+])
+def test_gradients_that_do_not_fit(capi, recorded, gradient, match):
+    model = _model(capi)
+    made = len(recorded.made)
+    with pytest.raises(ValueError, match=match):
+        model.gradient(IDS, OFFSETS, gradient)
+    assert len(recorded.made) == made
+
+
+def test_empty_lists(capi, recorded):
+    model = _model(capi)
+    model.embed([], [0])
+    model.embed([], [0, 0], [0])
+    model.gradient([], [0, 0], GRADIENT[:1])
+    assert model.hidden_rows([], [0]).shape == (0, 12)

@@ -24,33 +24,72 @@ import numpy as np
 
 from . import capi
 
+_STORAGE = {capi.F32: np.dtype(np.float32), capi.F16: np.dtype(np.float16), capi.BF16: np.dtype(np.uint16)}
+
+
+def _refuse(message):
+    raise ValueError(f"zcgvs embedder: {message}")
+
+
+def _matrix(name, values, shape, element):
+    """A host array whose address goes to the kernels: its shape (None: any length) and type have to be right."""
+    values = np.asarray(values)
+    if values.dtype != element:
+        _refuse(f"{name} must hold {element}, not {values.dtype}")
+    if values.ndim != len(shape) or any(want is not None and have != want for have, want in zip(values.shape, shape)):
+        _refuse(f"{name} has shape {values.shape}, not {shape}")
+    return values
+
+
+def _whole(name, values, kind):
+    """A list of whole numbers as an array of `kind`; none of them may change on the way."""
+    values = np.asarray(values)
+    if values.ndim != 1 or (values.size and values.dtype.kind not in "iu"):
+        _refuse(f"{name} must be a list of whole numbers")
+    limits = np.iinfo(kind)
+    if values.size and (values.min() < limits.min or values.max() > limits.max):
+        _refuse(f"{name} must fit {np.dtype(kind)}")
+    return values.astype(kind)
+
 
 class DeviceEmbedder:
     """Weights and work buffers of the model; host arrays in, device arrays out.
 
     table [vocab, dim], gate and up [hidden, dim] and projection [width, hidden] hold `dtype` (bfloat16 as
-    uint16 bit patterns). adapters: None, or a dict with down [n, rank, hidden], up [n, width, rank] and
+    uint16 bit patterns); arrays of other types, shapes or sizes are refused. adapters: None, or a dict with down [n, rank, hidden], up [n, width, rank] and
     optionally ranks [n] and scales [n]."""
 
     def __init__(self, table, gate, up, projection, *, dtype, scale=1.0, padding_id=-1, activation=capi.ACT_SILU,
                  adapters=None):
         self.dtype, self.scale, self.padding_id, self.activation = dtype, scale, padding_id, activation
+        if dtype not in _STORAGE:
+            _refuse("dtype must be F32, F16 or BF16")
+        self._element = element = _STORAGE[dtype]
+        table = _matrix("table", table, (None, None), element)
         self.vocab, self.dim = table.shape
-        self.hidden, self.width = gate.shape[0], projection.shape[0]
-        if gate.shape != up.shape or gate.shape[1] != self.dim or projection.shape[1] != self.hidden:
-            raise ValueError("zcgvs embedder: the weights' shapes do not match")
-        self._element = table.dtype
-        self.table, self.gate, self.up, self.projection = map(capi.DeviceArray.from_host, (table, gate, up, projection))
-        self._adapters = {}
+        gate = _matrix("gate", gate, (None, self.dim), element)
+        self.hidden = gate.shape[0]
+        up = _matrix("up", up, (self.hidden, self.dim), element)
+        projection = _matrix("projection", projection, (None, self.hidden), element)
+        self.width = projection.shape[0]
+        parts = {}
         if adapters is not None:
-            count, rank = adapters["down"].shape[:2]
-            if adapters["down"].shape[2] != self.hidden or adapters["up"].shape != (count, self.width, rank):
-                raise ValueError("zcgvs embedder: the adapters' shapes do not match")
-            self._adapters = dict(adapter_count=count, max_rank=rank)
-            for name, kind in (("down", None), ("up", None), ("ranks", np.int32), ("scales", np.float32)):
-                if adapters.get(name) is not None:
-                    values = adapters[name] if kind is None else np.asarray(adapters[name], kind)
-                    self._adapters[name] = capi.DeviceArray.from_host(values)
+            if adapters.get("down") is None or adapters.get("up") is None:
+                _refuse("adapters need down and up")
+            parts["down"] = _matrix("down", adapters["down"], (None, None, self.hidden), element)
+            count, rank = parts["down"].shape[:2]
+            parts["up"] = _matrix("the adapters' up", adapters["up"], (count, self.width, rank), element)
+            if adapters.get("ranks") is not None:
+                parts["ranks"] = _whole("ranks", adapters["ranks"], np.int32)
+            if adapters.get("scales") is not None:
+                parts["scales"] = np.asarray(adapters["scales"], np.float32)
+            for name in ("ranks", "scales"):
+                if name in parts and parts[name].shape != (count,):
+                    _refuse(f"one of {name} for each adapter")
+        self.table, self.gate, self.up, self.projection = map(capi.DeviceArray.from_host, (table, gate, up, projection))
+        self._adapters = {name: capi.DeviceArray.from_host(values) for name, values in parts.items()}
+        if parts:
+            self._adapters.update(adapter_count=count, max_rank=rank)
         self._buffers = {}
         self._stream = None  # of the last call
         self._host = []      # arrays whose copies may be on their way
@@ -91,6 +130,14 @@ class DeviceEmbedder:
         capi.call("zcgvs_stream_synchronize", getattr(self._stream, "handle", self._stream))
         self._host.clear()
 
+    @staticmethod
+    def _lists(ids, offsets):
+        """The checked ids and offsets: texts follow each other within the ids."""
+        ids, offsets = _whole("ids", ids, np.int32), _whole("offsets", offsets, np.int64)
+        if offsets.size == 0 or offsets[0] < 0 or offsets[-1] > ids.size or np.any(offsets[1:] < offsets[:-1]):
+            _refuse("offsets must ascend from 0 or more to at most the number of ids")
+        return ids, offsets
+
     def _forward(self, ids, offsets, stream, **more):
         """The lookup and the gated block; `more`: further host arrays of the call, name=(values, type), copied
         beside the ids."""
@@ -110,13 +157,15 @@ class DeviceEmbedder:
     def embed(self, ids, offsets, adapter_ids=None, stream=None) -> capi.DeviceArray:
         """Queries of the texts ids[offsets[t]:offsets[t + 1]], each through adapter adapter_ids[t] (-1: none).
         The array belongs to the model and holds until the next call."""
+        ids, offsets = self._lists(ids, offsets)
         texts = len(offsets) - 1
         more = {}
         if adapter_ids is not None:
             if not self._adapters:
-                raise ValueError("zcgvs embedder: the model has no adapters")
+                _refuse("the model has no adapters")
+            adapter_ids = _whole("adapter_ids", adapter_ids, np.int32)
             if len(adapter_ids) != texts:
-                raise ValueError("zcgvs embedder: one adapter id per text")
+                _refuse("one adapter id per text")
             more = dict(adapter_ids=(adapter_ids, np.int32))
         _, _, hidden, uploaded = self._forward(ids, offsets, stream, **more)
         extra = dict(self._adapters, **uploaded) if uploaded else {}
@@ -129,6 +178,7 @@ class DeviceEmbedder:
 
     def hidden_rows(self, ids, offsets, stream=None) -> np.ndarray:
         """The hidden rows on the host, as stored (for training, where a loss is formed from them)."""
+        ids, offsets = self._lists(ids, offsets)
         _, _, hidden, _ = self._forward(ids, offsets, stream)
         out = np.empty((len(offsets) - 1, self.hidden), dtype=self._element)
         if out.nbytes:
@@ -138,8 +188,10 @@ class DeviceEmbedder:
 
     def gradient(self, ids, offsets, hidden_gradient, stream=None) -> dict:
         """The gradients of the table (float32) and of gate and up (their type), as device arrays, from the
-        gradient of the hidden rows (host, of the model's type)."""
-        texts, tokens = len(offsets) - 1, len(ids)
+        gradient of the hidden rows (host [texts, hidden], of the model's type: no other is converted)."""
+        ids, offsets = self._lists(ids, offsets)
+        texts = len(offsets) - 1
+        hidden_gradient = _matrix("hidden_gradient", hidden_gradient, (texts, self.hidden), self._element)
         lookup, gated, _, uploaded = self._forward(ids, offsets, stream, hidden_gradient=(hidden_gradient, self._element))
         d_hidden = uploaded["hidden_gradient"]
         rows = self._buffer("rows_gradient", (texts, self.dim), self._element)
