@@ -182,3 +182,24 @@ def test_empty_lists(capi, recorded):
     model.embed([], [0, 0], [0])
     model.gradient([], [0, 0], GRADIENT[:1])
     assert model.hidden_rows([], [0]).shape == (0, 12)
+
+
+def test_queries_have_their_shape_and_type(capi, recorded):
+    """Also where the kept buffer is larger than this call's result."""
+    model = _model(capi)
+    for texts in (5, 2, 9, 0):
+        queries = model.embed(np.arange(texts), np.arange(texts + 1))
+        assert queries.shape == (texts, 10) and queries.dtype == np.float32 and queries.nbytes == texts * 40
+
+
+def test_views(capi, recorded):
+    whole = capi.DeviceArray((4, 6), np.uint8)
+    part = whole.view((2, 3), np.float32)
+    assert part.ptr == whole.ptr and part.shape == (2, 3) and part.nbytes == 24
+    with pytest.raises(ValueError, match="28 bytes of an allocation of 24"):
+        whole.view(7, np.float32)
+    address = whole.ptr
+    del whole
+    assert part.ptr == part.owner.ptr == address
+    part.free()
+    assert part.ptr == 0 and "zcgvs_free" not in recorded.made

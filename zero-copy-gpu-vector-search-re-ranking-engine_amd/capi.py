@@ -235,6 +235,10 @@ class DeviceArray:
         synchronize()
         return out
 
+    def view(self, shape, dtype) -> "DeviceArrayView":
+        """The allocation's first values as another shape and type."""
+        return DeviceArrayView(self, shape, dtype)
+
     def free(self) -> None:
         if self.ptr:
             call("zcgvs_free", self.ptr)
@@ -247,6 +251,24 @@ class DeviceArray:
                 self.ptr = 0
         except Exception:  # interpreter shutdown
             pass
+
+
+class DeviceArrayView(DeviceArray):
+    """Part of another DeviceArray's allocation, which it keeps alive and never frees."""
+
+    def __init__(self, owner: DeviceArray, shape, dtype):
+        self.shape = tuple(int(s) for s in (shape if isinstance(shape, (tuple, list)) else (shape,)))
+        self.dtype = np.dtype(dtype)
+        self.nbytes = int(np.prod(self.shape, dtype=np.int64)) * self.dtype.itemsize
+        if self.nbytes > owner.nbytes:
+            raise ValueError(f"a view of {self.nbytes} bytes of an allocation of {owner.nbytes}")
+        self.owner, self.ptr = owner, owner.ptr
+
+    def free(self) -> None:
+        self.owner, self.ptr = None, 0
+
+    def __del__(self):
+        pass
 
 
 def synchronize() -> None:

@@ -102,13 +102,13 @@ class DeviceEmbedder:
         self._stream = stream  # kept: a destroyed stream's handle could come back as another stream's
 
     def _buffer(self, name, shape, kind):
-        """A work buffer that grows and is kept; `shape` of it is used."""
+        """A work buffer that grows and is kept, as an array of `shape` and `kind`."""
         need = int(np.prod(shape, dtype=np.int64)) * np.dtype(kind).itemsize
         held = self._buffers.get(name)
         if held is None or held.nbytes < need:
             capi.synchronize()  # earlier calls may still use the smaller one
             held = self._buffers[name] = capi.DeviceArray(max(need, 1), np.uint8)
-        return held
+        return held.view(shape, kind)
 
     def _lookup_desc(self, ids, offsets, texts, tokens):
         return capi.embedding_desc(self.table, self.vocab, self.dim, self.dtype, ids, tokens, bag_offsets=offsets,
@@ -155,8 +155,8 @@ class DeviceEmbedder:
         return lookup, gated, hidden, uploaded
 
     def embed(self, ids, offsets, adapter_ids=None, stream=None) -> capi.DeviceArray:
-        """Queries of the texts ids[offsets[t]:offsets[t + 1]], each through adapter adapter_ids[t] (-1: none).
-        The array belongs to the model and holds until the next call."""
+        """Queries of the texts ids[offsets[t]:offsets[t + 1]], each through adapter adapter_ids[t] (-1: none):
+        float32 [texts, width]. The array belongs to the model and holds until the next call."""
         ids, offsets = self._lists(ids, offsets)
         texts = len(offsets) - 1
         more = {}
