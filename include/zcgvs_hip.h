@@ -433,7 +433,7 @@ int zcgvs_generate_normalized(float* d_out, int64_t rows, int dim, uint64_t seed
  *
  * Types: float32, float16 or bfloat16 operands (ZCGVS_DTYPE_F32 / F16 / BF16). Products and sums are
  * held in float32 whatever the type; results are rounded once, where they are written. Matrix products of
- * float32 operands are formed from exact parts of them, to within about 2^-23 of each product; an infinite
+ * float32 operands are formed from exact parts of them, to within 2^-23 of each product; an infinite
  * operand may give NaN there where the formula gives an infinity. Matrices are
  * row-major with a row stride in elements (at least the row's length). Rows may start at any address
  * that is aligned to their element; rows whose address and stride are multiples of 16 bytes take the

@@ -1,18 +1,20 @@
 // Tiled products of float32 operands on the bf16 matrix cores, in the interface of MatrixTile.
 //
-// A float32 value is the sum of three bf16 values, exactly: its upper 16 bits, the upper 16 bits of what
-// is left, and the rest (8 significant bits each). x y is formed as the six products of parts whose
-// size is at least 2^-16 of it; the other three are below 2^-23 of it, as much as a float32 sum rounds away.
+// A float32 value is the sum of three bf16 values, exactly: itself rounded to bf16, what is left rounded to
+// bf16, and the rest. Rounded to nearest, each part is at most 2^-8 of the one before and has either sign. x y is
+// formed as the six products of parts whose size is at least 2^-16 of it; the other three are together below
+// 2^-24 (1 + 2^-8) of it, half of what a float32 sum may round away, and no sign is preferred. (Parts cut off
+// instead have the value's sign, and the three products left out would reach 2^-21, all in one direction.)
 // Six v_mfma_f32_16x16x32_bf16 take 3/8 of the time of the eight v_mfma_f32_16x16x4_f32 that they stand for
 // (whose rate bounds a float32 product at 150 TFLOP/s).
 // A stage's products are summed by themselves and then added to the tile's sums: the matrix cores' additions
-// do not round to nearest, and 1536 of them in a row cost a sum over 8192 a relative 8e-6; like this it is
-// 4e-7 (float32 matrix instructions: 3e-6), at 2 to 8% of the time.
+// do not round to nearest, and cost a sum over 8192 a relative 1.5e-6 (2-norm) where all of them go to one sum;
+// like this it is 2.4e-7, at up to 4% of the time (float32 matrix instructions: 1.7e-6).
 // Operands are split once, between the registers that they are loaded into and LDS, where the three parts
 // are planes of the 16-bit layouts of matrix_tile.hpp; a stage is 64 values of k. The next stage is on its way
-// into registers while this one is multiplied. Loads take any alignment. Measured at 4096 x 8192 -> 4096:
-// 128 x 128 tiles 198 TFLOP/s, 64 x 64 155, float32 matrix instructions 126.
-// Infinite operands give NaN (the parts of an infinity are an infinity and NaN), and values below about
+// into registers while this one is multiplied. Loads take any alignment. Measured, gated products of 4096 rows,
+// 8192 -> 2048: 128 x 128 tiles 195 TFLOP/s, 64 x 64 149, float32 matrix instructions 127.
+// Infinite operands give NaN (which the last part of an infinity is), and values below about
 // 2^-110 lose bits.
 #pragma once
 
@@ -25,6 +27,7 @@
 namespace zcgvs_hip {
 
 constexpr int kSplitParts = 3;
+constexpr float kLargestPart = 3.38953139e38f;  // the largest finite bf16 value
 
 template <int kRows, bool kTurned, int kThreads>
 struct SplitLoader {
@@ -90,17 +93,23 @@ struct SplitLoader {
     __device__ __forceinline__ void put(std::uint8_t* stage) const {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
             u32x4 part[kSplitParts];
 #pragma unroll
             for (int e = 0; e < kValues; e += 2) {
                 float rest[2] = {held[i][e], held[i][e + 1]};
 #pragma unroll
                 for (int p = 0; p < kSplitParts; ++p) {
-                    const std::uint32_t low = __float_as_uint(rest[0]);
-                    const std::uint32_t high = __float_as_uint(rest[1]);
-                    part[p][e / 2] = __builtin_amdgcn_perm(high, low, 0x07060302u);  // both upper halves
-                    rest[0] -= __uint_as_float(low & 0xFFFF0000u);
-                    rest[1] -= __uint_as_float(high & 0xFFFF0000u);
+                    f32x2 from = {rest[0], rest[1]};
+                    if (p == 0) {  // a finite value's first part stays finite
+                        from = f32x2{__builtin_amdgcn_fmed3f(rest[0], -kLargestPart, kLargestPart),
+                                     __builtin_amdgcn_fmed3f(rest[1], -kLargestPart, kLargestPart)};
+                    }
+                    const std::uint32_t both = __builtin_bit_cast(std::uint32_t, __builtin_convertvector(from, bf16x2));
+                    part[p][e / 2] = both;
+                    rest[0] -= __uint_as_float(both << 16);
+                    rest[1] -= __uint_as_float(both & 0xFFFF0000u);
                 }
             }
 #pragma unroll
