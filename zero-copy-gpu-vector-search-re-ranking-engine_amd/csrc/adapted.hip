@@ -100,6 +100,20 @@ __device__ __forceinline__ typename Fragment<T>::type loadMasked(const T* from, 
     return v;
 }
 
+// Zeros in the place of infinities.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::type withoutInfinities(const typename Fragment<T>::type& v) {
+    static_assert(sizeof(T) == 2, "16-bit values");
+    typedef std::uint16_t Bits __attribute__((ext_vector_type(8)));
+    constexpr std::uint16_t kInfinity = std::is_same_v<T, __bf16> ? 0x7F80 : 0x7C00;
+    Bits bits = __builtin_bit_cast(Bits, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        bits[e] = (bits[e] & 0x7FFF) == kInfinity ? 0 : bits[e];
+    }
+    return __builtin_bit_cast(typename Fragment<T>::type, bits);
+}
+
 // ---- low = scale x down^T -----------------------------------------------------------------------
 
 // A workgroup takes the groups that begin among `positions` sorted positions (1, or a block of 16; a group is
@@ -420,6 +434,12 @@ __device__ __forceinline__ void addAdapters(const AdaptedArgs& args, const TileA
                 const int r = k % args.padded_rank;  // every part meets the same columns of up
                 b[i] = loadMasked(up + static_cast<std::int64_t>(n) * args.max_rank + r,
                                   k < low_values ? args.max_rank - r : 0, rank - r);
+                if constexpr (kHere > 1) {
+                    // an infinity times the first part is the result; a rest of 0 or of the other sign makes it NaN
+                    if (k >= args.padded_rank) {
+                        b[i] = withoutInfinities<T>(b[i]);
+                    }
+                }
             }
             __syncthreads();  // what stood in the LDS has been read
 #pragma unroll
