@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 TYPE = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 INF = float("inf")
 # rows, adapters, rows after each other with one adapter, rank
-PATHS = {"one launch": (9, 3, 1, 8), "few rows": (200, 3, 1, 16), "by adapter": (6000, 3, 300, 16), "by row": (6000, 40, 1, 8)}
+PATHS = {"one launch": (9, 3, 1, 8), "few rows": (200, 3, 1, 16), "by adapter": (6000, 3, 300, 16), "by row": (6000, 600, 1, 8)}
 # operands and output; rounding of the output; what is left out of x down^T between the products
 KINDS = {("f16", "f32"): (2.0 ** -24, 2.0 ** -22), ("bf16", "f32"): (2.0 ** -24, 2.0 ** -23),
          ("bf16", "bf16"): (2.0 ** -8, 2.0 ** -16), ("f16", "f16"): (2.0 ** -11, 2.0 ** -22)}
@@ -81,3 +81,18 @@ def test_infinite_up(gpu, kind, out, path):
         assert sure.any()
         assert torch.all(got[sure, column] == sign * torch.sign(low[sure, rank]) * INF)
     c.check(got, rest, *KINDS[kind, out])
+
+
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("kind,out", KINDS)
+def test_infinite_down(gpu, kind, out, path):
+    """An infinite value of x down^T makes its row infinite, whatever the size of the row's other values."""
+    c = Case(kind, path)
+    c.down[1] *= 2.0 ** 13  # x down^T up to 2^19, beyond float16's range
+    c.down[1, 3, 0] = INF  # x[:, 0] is 1 or -1
+    c.up[1, :, 3] = torch.where(c.up[1, :, 3] > 0, 1.0, -1.0).to(TYPE[kind])
+    got = c.run(gpu, out)
+    named = c.ids == 1
+    sign = torch.sign(c.x[named, 0].double())[:, None] * torch.sign(c.up[1, :, 3].double())[None, :]
+    assert torch.all(got[named] == sign * INF)
+    c.check(got, (~named)[:, None].expand_as(got), *KINDS[kind, out])

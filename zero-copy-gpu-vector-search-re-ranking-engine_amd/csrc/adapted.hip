@@ -218,7 +218,8 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
                 sum += joined[w][row][r];
             }
             value[j] = r < rank ? sum * scale : 0.0f;
-            peak = fmaxf(peak, fabsf(value[j]));
+            // of the finite ones: beside an infinity they still have to fit the parts
+            peak = fmaxf(peak, fabsf(value[j]) <= 3.402823466e+38f ? fabsf(value[j]) : 0.0f);
         }
         if constexpr (sizeof(T) == 2) {
             row_peak[row][column] = peak;  // the same from both halves of the workgroup
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(kLowThreads) void lowKernel(AdaptedArgs args, int p
             const std::int64_t at = p + row;
             if constexpr (sizeof(T) == 2) {
                 int exponent = 0;
-                if (peak > 0.0f && peak <= 3.402823466e+38f) {
+                if (peak > 0.0f) {
                     int e = 0;
                     frexpf(peak, &e);  // peak = m 2^e, m in [0.5, 1)
                     exponent = min(126, max(-126, 15 - e));
