@@ -96,3 +96,14 @@ def test_infinite_down(gpu, kind, out, path):
     sign = torch.sign(c.x[named, 0].double())[:, None] * torch.sign(c.up[1, :, 3].double())[None, :]
     assert torch.all(got[named] == sign * INF)
     c.check(got, (~named)[:, None].expand_as(got), *KINDS[kind, out])
+
+
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("kind,out", [k for k in KINDS if k[0] == "bf16"])
+@pytest.mark.parametrize("down_by,up_by", [(-40, 118), (115, -100), (60, 60)])
+def test_far_ends_of_bfloat16(gpu, kind, out, path, down_by, up_by):
+    """Values near float32's largest in up, or in x down^T, whose products are in its range."""
+    c = Case(kind, path)
+    c.down, c.up = c.down * 2.0 ** down_by, c.up * 2.0 ** up_by
+    got = c.run(gpu, out)
+    c.check(got, torch.ones_like(got, dtype=torch.bool), *KINDS[kind, out])
