@@ -59,7 +59,9 @@ __device__ __forceinline__ void activateBoth(float g, float& value, float& slope
     } else {
         const float y = logistic(1.59576912f * (g + 0.044715f * g * g * g));
         value = g * y;
-        slope = y + value * (1.0f - y) * (1.59576912f * (1.0f + 0.134145f * g * g));
+        // value * (1 - y) is 0 long before |g| is 100; the square must not make an infinity of it
+        const float square = fminf(g * g, 1.0e4f);
+        slope = y + value * (1.0f - y) * (1.59576912f * (1.0f + 0.134145f * square));
     }
 }
 
