@@ -55,3 +55,38 @@ def test_large_arguments(gpu, act):
     for value in (out, up):
         assert np.all(np.abs(value - g)[positive] <= 4 * 2.0 ** -23 * g[positive]) and np.all(np.abs(value[~positive]) < 1e-19)
     assert np.all(np.abs(slope[positive] - 1.0) <= 4 * 2.0 ** -23) and np.all(np.abs(slope[~positive]) < 1e-18)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_values_and_slopes(gpu, act):
+    """Errors by what the formulas round: with eps = 2^-24, the argument z of the logistic function (two or six
+    roundings and its constants, 3 eps |z| or 8 eps |z|, with those of g itself), its exponential and reciprocal (6 eps), a few
+    products; the error function's within 4 eps of 1 and its Gaussian's exponent."""
+    rng = np.random.default_rng(71)
+    g = np.concatenate([np.linspace(-12, 12, 4801), rng.standard_normal(4000), 2.0 ** rng.uniform(-20, 0, 500)]).astype(np.float32)
+    out, up, slope = run(gpu, act, g)
+    g = g.astype(np.float64)
+    value, exact_slope = activation(act, g)
+    eps, size = 2.0 ** -24, np.abs(g)
+    if act == "gelu":
+        # g (1 + erf): absolute in 1 + erf; products 8 eps of the value
+        value_error = size * (4 * eps + 3 * eps * size * np.exp(-0.5 * g * g)) + 8 * eps * np.abs(value)
+        slope_error = 4 * eps + (8 + 4 * g * g) * eps * size * np.exp(-0.5 * g * g) + 8 * eps
+    else:
+        z = size if act == "silu" else 1.5957691 * (size + 0.044715 * size ** 3)
+        dz = 1.0 if act == "silu" else 1.5957691 * (1 + 0.134145 * size ** 2)
+        with np.errstate(over="ignore", under="ignore"):
+            rest = 1.0 / (1.0 + np.exp(z))  # the smaller of y and 1 - y
+        # y moves by y (1 - y) times z's error; relative to y that is at most z's error
+        z_error = (4 if act == "silu" else 10) * eps * z
+        bent = np.minimum(1.0, np.where(g > 0, rest, 1.0)) * z_error + 6 * eps  # of y, relative
+        value_error = np.abs(value) * (bent + 6 * eps)
+        y = np.where(g > 0, 1.0 - rest, rest)
+        # y + g y (1 - y) dz: 1 - y is taken from 1, eps in y's own size there
+        slope_error = y * bent + size * dz * y * ((1 - y) * (2 * bent + 8 * eps) + y * bent + 2 * eps) + 8 * eps * np.abs(exact_slope)
+    floor = 2.0 ** -120
+    for got in (out, up):
+        # u is a product of 1, and one of g and of the result's
+        assert np.all(np.abs(got - value) <= value_error + 8 * eps * np.abs(value) + floor)
+    # gate_gradient contracts one row: another product of 1
+    assert np.all(np.abs(slope - exact_slope) <= slope_error + 8 * eps * np.abs(exact_slope) + floor)

@@ -28,9 +28,11 @@ namespace zcgvs_hip {
 
 namespace {
 
-// 1 / (1 + exp(-x)): exp2 and the reciprocal of the hardware, each within 1 ulp.
+// 1 / (1 + exp(-x)): exp2 and the reciprocal of the hardware, each within 1 ulp. The reciprocal gives zeros in the
+// place of results below 2^-126, so it is taken of 2^-32 of the sum.
 __device__ __forceinline__ float logistic(float x) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+    constexpr float kSmall = 0x1p-32f;
+    return kSmall * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(-1.44269504f * x), kSmall, kSmall));
 }
 
 // The activation's value and slope at g.
