@@ -456,7 +456,7 @@ typedef struct zcgvs_embedding_desc {
     const void* table;           /* [vocab, dim] rows of `dtype` (not read by the gradient)      */
     int64_t table_stride;        /* elements from row to row; 0: dim                             */
     int vocab;
-    int dim;
+    int dim;                     /* at most 2^23                                                 */
     int dtype;                   /* of the table                                                 */
     const int* ids;              /* [token_count]                                                */
     int64_t token_count;         /* at most 2^28                                                 */

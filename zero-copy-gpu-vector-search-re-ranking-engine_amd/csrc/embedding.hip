@@ -33,6 +33,7 @@ constexpr int kThreads = 256;
 constexpr int kWavesPerBlock = kThreads / kWave;
 constexpr std::int64_t kMaxTokens = 1 << 28;          // a launch a chunk of 64 has less than 2^32 threads
 constexpr long long kMaxBlocks = (1ll << 24) - 1;     // a launch has less than 2^32 threads
+constexpr int kMaxDim = 1 << 23;                      // slices of 256 columns in a grid's second dimension
 
 // ---- lookup, one output row per token ---------------------------------------------------------
 
@@ -632,6 +633,9 @@ int checkEmbedding(const zcgvs_embedding_desc* desc) {
     }
     if (desc->vocab <= 0 || desc->dim <= 0) {
         return invalid("vocab and dim must be positive");
+    }
+    if (desc->dim > kMaxDim) {
+        return invalid("dim must be at most 2^23");
     }
     if (desc->vocab == INT32_MAX) {
         return invalid("vocab must be below 2^31 - 1");
