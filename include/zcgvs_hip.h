@@ -526,8 +526,9 @@ int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradien
  * A row whose id lies outside [0, adapter_count) has no adapter, as have all rows where adapter_ids is
  * NULL. Of adapter a the first ranks[a] of max_rank rows of down[a] and columns of up[a] count; what
  * lies beyond is not used. Rows may come in any order; rows of one adapter next to each other (the
- * tokens of a request) cost least. A row's result does not depend on the other rows' adapters, also
- * where those hold infinities or NaN. */
+ * tokens of a request) cost least. Of the other rows and their adapters a row's result takes nothing, also
+ * where those hold infinities or NaN; but how many they are and how they mix chooses the kernel and the
+ * order of a row's sums, so in another batch it may be rounded otherwise. */
 typedef struct zcgvs_adapted_desc {
     const void* x;          /* [rows, dim]                                                  */
     int64_t x_stride;       /* 0: dim                                                       */
