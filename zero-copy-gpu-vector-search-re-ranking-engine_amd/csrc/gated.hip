@@ -456,8 +456,8 @@ int launchGated(const zcgvs_gated_desc& d, GatedArgs args, hipStream_t stream) {
         // the error function's terms do not fit the registers beside the sums of 256 x 256
         constexpr LargestTile kLargest = decltype(activation)::value == ZCGVS_ACT_GELU ? LargestTile::k256x192
                                                                                         : LargestTile::k256x256;
-        const ProductPlan plan =
-            planProduct(d.rows, 2 * static_cast<std::int64_t>(d.hidden), d.dim, 1, d.dtype, 0, kLargest);
+        const ProductPlan plan = planProduct(d.rows, 2 * static_cast<std::int64_t>(d.hidden), d.dim, 1, d.dtype, 0,
+                                             largestTile(kLargest, direct));
         return withTile<T, false, false, kLargest, true>(plan.shape, direct, [&](auto tile) {
             using Tile = decltype(tile);
             args.tiles_m = divideUp(d.rows, Tile::kM);
@@ -483,26 +483,29 @@ std::size_t partialsOffset(const zcgvs_gated_desc& d) {
     return (both * static_cast<std::size_t>(elementBytes(d.dtype)) + 255) / 256 * 256;
 }
 
-ProductPlan inputPlan(const zcgvs_gated_desc& d) {
+ProductPlan inputPlan(const zcgvs_gated_desc& d, bool direct) {
     // an even number of splits, each within one of the two products; 256 x 256 tiles of two products one
     // after the other do not fit the registers (measured 140 us for what 256 x 192 take 93)
     return planProduct(d.rows, d.dim, 2 * static_cast<std::int64_t>(d.hidden), 1, d.dtype, 2,
-                       LargestTile::k256x192);
+                       largestTile(LargestTile::k256x192, direct));
 }
 
-ProductPlan weightPlan(const zcgvs_gated_desc& d) {
-    return planProduct(d.hidden, d.dim, d.rows, 2, d.dtype, 1, LargestTile::k256x256);
+ProductPlan weightPlan(const zcgvs_gated_desc& d, bool direct) {
+    return planProduct(d.hidden, d.dim, d.rows, 2, d.dtype, 1, largestTile(LargestTile::k256x256, direct));
 }
 
-// float32 partial sums of the two products: the input's, then the weights'.
+// float32 partial sums of the two products: the input's, then the weights'. A call's workspace holds those of either
+// kind of rows, so that its size goes by the sizes and the type alone.
 std::size_t inputPartials(const zcgvs_gated_desc& d) {
-    const ProductPlan plan = inputPlan(d);
-    return plan.splits > 1 ? static_cast<std::size_t>(plan.splits) * static_cast<std::size_t>(d.rows) * static_cast<std::size_t>(d.dim) / 4 * 4 + 4 : 0;
+    const int splits = std::max(inputPlan(d, false).splits, inputPlan(d, true).splits);
+    const std::size_t values = static_cast<std::size_t>(d.rows) * static_cast<std::size_t>(d.dim);
+    return splits > 1 ? static_cast<std::size_t>(splits) * values / 4 * 4 + 4 : 0;
 }
 
 std::size_t weightPartials(const zcgvs_gated_desc& d) {
-    const ProductPlan plan = weightPlan(d);
-    return plan.splits > 1 ? static_cast<std::size_t>(plan.splits) * 2 * static_cast<std::size_t>(d.hidden) * static_cast<std::size_t>(d.dim) : 0;
+    const int splits = std::max(weightPlan(d, false).splits, weightPlan(d, true).splits);
+    const std::size_t values = 2 * static_cast<std::size_t>(d.hidden) * static_cast<std::size_t>(d.dim);
+    return splits > 1 ? static_cast<std::size_t>(splits) * values : 0;
 }
 
 template <typename T>
@@ -597,15 +600,15 @@ int launchBothGradients(const zcgvs_gated_desc& d, InputGradientArgs input, Weig
 // The products with dg and du, and the sums over their splits. An output that is null is not wanted.
 template <typename T>
 int launchGradients(const zcgvs_gated_desc& d, InputGradientArgs input, WeightGradientArgs weight, hipStream_t stream) {
-    const ProductPlan input_plan = inputPlan(d);
-    const ProductPlan weight_plan = weightPlan(d);
+    const bool direct_input = directRows(input.gate, input.weight_stride, d.dim, d.dtype) &&
+                              directRows(input.up, input.weight_stride, d.dim, d.dtype);
+    const bool direct_weight = directRows(weight.x, weight.x_stride, d.dim, d.dtype);
+    const ProductPlan input_plan = inputPlan(d, direct_input);
+    const ProductPlan weight_plan = weightPlan(d, direct_weight);
     splitInput(d, input_plan, input);
     splitWeight(d, weight_plan, weight);
     const bool wants_input = input.out != nullptr;
     const bool wants_weight = weight.gate_out != nullptr;
-    const bool direct_input = directRows(input.gate, input.weight_stride, d.dim, d.dtype) &&
-                              directRows(input.up, input.weight_stride, d.dim, d.dtype);
-    const bool direct_weight = directRows(weight.x, weight.x_stride, d.dim, d.dtype);
     int status = ZCGVS_OK;
     if (wants_input && wants_weight && direct_input == direct_weight && input_plan.shape == TileShape::k64x64 &&
         weight_plan.shape == TileShape::k64x64) {

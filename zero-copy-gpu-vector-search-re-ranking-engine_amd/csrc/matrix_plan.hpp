@@ -30,6 +30,11 @@ enum class TileShape { k256x256, k256x192, k128x128, k64x64 };
 // The largest tile a kernel is built with: those of 256 rows have 16 wavefronts of 128 registers.
 enum class LargestTile { k256x256, k256x192, k128x128 };
 
+// Rows that are no whole 16-byte chunks go through registers, for which the tiles of 256 rows have too few; they are
+// planned for the tiles they take. (Gradient of 16,384 rows 767 -> 2047 bfloat16 825 us, 870 us with the splits of the
+// larger tiles; rows of 768 and 2048 356 us. The stage times are those of whole chunks.)
+inline LargestTile largestTile(LargestTile largest, bool direct) { return direct ? largest : LargestTile::k128x128; }
+
 struct ProductPlan {
     TileShape shape;
     int splits;
