@@ -513,8 +513,9 @@ int zcgvs_gated_projection(const zcgvs_gated_desc* desc, void* d_out, int64_t ou
  *     x_gradient [rows, dim] = dg gate + du up,
  *     gate_gradient [hidden, dim] = dg^T x,   up_gradient [hidden, dim] = du^T x,
  * all of desc->dtype. dg and du are rounded to desc->dtype between the products, as tensors of a model
- * of that type are (float16: to an infinity beyond 65504, so scale the loss as for stored tensors). x_gradient may be NULL (not wanted), and so may gate_gradient and up_gradient, both
- * together. A stride of 0 is the row's length; gate_gradient and up_gradient share theirs. */
+ * of that type are (float16: to an infinity beyond 65504, so scale the loss as for stored tensors).
+ * x_gradient may be NULL (not wanted), and so may gate_gradient and up_gradient, both together. A stride
+ * of 0 is the row's length; gate_gradient and up_gradient share theirs. */
 size_t zcgvs_gated_gradient_workspace_bytes(const zcgvs_gated_desc* desc);
 int zcgvs_gated_gradient(const zcgvs_gated_desc* desc, const void* d_out_gradient,
                          int64_t out_gradient_stride, void* d_x_gradient, int64_t x_gradient_stride,
