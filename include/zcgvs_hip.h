@@ -556,6 +556,56 @@ int zcgvs_adapted_projection(const zcgvs_adapted_desc* desc, void* d_out, int64_
                              int out_dtype, void* d_workspace, size_t workspace_bytes,
                              zcgvs_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators of an encoder block: what stands between the token rows of zcgvs_embedding_lookup and
+ * the row that is pooled, beside zcgvs_gated_projection. No counterpart in the reference, whose
+ * QueryEmbedder runs a model outside its device code (include/zcgvs/embed/query_embedder.hpp:8-15).
+ * What the embedding-model operators above promise of types, sums, strides, alignment, streams,
+ * workspaces and equal bits on every call holds for these as well.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Root-mean-square norm of the sum of two rows (of one, where residual is NULL):
+ *     s = x + residual,   y = s / sqrt(mean(s^2) + eps) * (weight + weight_offset).
+ * s and y are formed in float32 of the operands as stored; the norm is that of the float32 sum, also where
+ * a rounded copy of the sum is written. eps > 0 keeps rows of zeros finite; a row whose squares pass
+ * float32's range gives zeros. */
+typedef struct zcgvs_norm_desc {
+    const void* x;          /* [rows, dim]                                                  */
+    int64_t x_stride;       /* 0: dim                                                       */
+    const void* residual;   /* [rows, dim], or NULL: none                                   */
+    int64_t residual_stride; /* 0: dim                                                      */
+    const void* weight;     /* [dim], or NULL: ones                                         */
+    int64_t rows;           /* at most 2^30                                                 */
+    int dim;                /* at most zcgvs_residual_norm_max_dim()                        */
+    int dtype;              /* of x, residual and weight                                    */
+    float weight_offset;    /* 1 for weights stored as their distance from one              */
+    float eps;              /* at least 0                                                   */
+} zcgvs_norm_desc;
+
+int zcgvs_residual_norm_max_dim(void); /* 16384 */
+/* d_out [rows, dim]: out_dtype is desc->dtype, ZCGVS_DTYPE_F32 or ZCGVS_DTYPE_I8. int8 rows are those of
+ * zcgvs_launch_quantize_rows_i8 over y: q = max|y| / 127 (1 for a row of zeros) goes to d_out_scales [rows],
+ * code = clamp(rint(y * (1/q)), -127, 127) to d_out: operands of zcgvs_linear, or rows of a
+ * ZCGVS_INT8_PER_VECTOR store. d_out_scales is not read or written otherwise. d_sum, NULL or [rows, dim] of
+ * desc->dtype, takes s, rounded once; it may be x or residual itself (with the same stride), and d_out may
+ * be x or residual where it has their type and stride and d_sum is another buffer. */
+int zcgvs_residual_norm(const zcgvs_norm_desc* desc, void* d_out, int64_t out_stride, int out_dtype,
+                        float* d_out_scales, void* d_sum, int64_t sum_stride, zcgvs_stream_t stream);
+
+/* The gradient of zcgvs_residual_norm (float output) from that of y and, where d_sum_gradient is not NULL,
+ * that of s. With u = s / sqrt(mean(s^2) + eps) and g = d_out_gradient * (weight + weight_offset):
+ *     x_gradient [rows, dim] = (g - u mean(g u)) / sqrt(mean(s^2) + eps) + d_sum_gradient,
+ *     weight_gradient [dim] = the sum over rows of d_out_gradient * u,
+ * all of desc->dtype. x_gradient is that of x and of residual alike. desc may give x and residual, or as x the
+ * sum that the forward call wrote. Either output may be NULL (not wanted); x_gradient may be d_out_gradient or
+ * d_sum_gradient itself (with the same stride). No rows: weight_gradient is zeros. */
+size_t zcgvs_residual_norm_gradient_workspace_bytes(const zcgvs_norm_desc* desc);
+int zcgvs_residual_norm_gradient(const zcgvs_norm_desc* desc, const void* d_out_gradient,
+                                 int64_t out_gradient_stride, const void* d_sum_gradient,
+                                 int64_t sum_gradient_stride, void* d_x_gradient, int64_t x_gradient_stride,
+                                 void* d_weight_gradient, void* d_workspace, size_t workspace_bytes,
+                                 zcgvs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

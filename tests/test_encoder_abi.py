@@ -1,0 +1,75 @@
+"""Refusals of the operators of an encoder block and what they answer without touching a GPU."""
+
+import pytest
+
+A = 1 << 20  # an address that nothing reads here
+NAN, INF = float("nan"), float("inf")
+
+
+def _norm(capi, **kw):
+    return capi.norm_desc(**dict(dict(x=A, rows=4, dim=8, dtype=capi.F32, weight=A, residual=A), **kw))
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(dtype=2), "float32, float16 or bfloat16"),
+    (dict(dtype=5), "float32, float16 or bfloat16"),
+    (dict(dim=0), "dim must lie"),
+    (dict(dim=16385), "dim must lie"),
+    (dict(rows=-1), "rows must lie"),
+    (dict(rows=2**30 + 1), "rows must lie"),
+    (dict(x_stride=7), "smaller than dim"),
+    (dict(residual_stride=7), "smaller than dim"),
+    (dict(x_stride=-8), "smaller than dim"),
+    (dict(eps=-1e-6), "eps must be finite"),
+    (dict(eps=NAN), "eps must be finite"),
+    (dict(eps=INF), "eps must be finite"),
+    (dict(weight_offset=INF), "weight_offset finite"),
+    (dict(x=None), "null device pointer"),
+])
+def test_norm_descriptor(capi, kw, match):
+    with pytest.raises(ValueError, match=match):
+        capi.residual_norm(_norm(capi, **kw), A, capi.F32)
+    with pytest.raises(ValueError, match=match):
+        capi.residual_norm_gradient_workspace_bytes(_norm(capi, **kw))
+    with pytest.raises(ValueError, match=match):
+        capi.residual_norm_gradient(_norm(capi, **kw), A, A, A, A, 1 << 30)
+
+
+def test_norm_operands(capi):
+    assert capi.library().zcgvs_residual_norm_max_dim() == 16384
+    with pytest.raises(ValueError, match="float32 or int8"):
+        capi.residual_norm(_norm(capi, dtype=capi.F16), A, capi.BF16)
+    with pytest.raises(ValueError, match="float32 or int8"):
+        capi.residual_norm(_norm(capi), A, capi.BINARY)
+    with pytest.raises(ValueError, match="smaller than dim"):
+        capi.residual_norm(_norm(capi), A, capi.F32, out_stride=7)
+    with pytest.raises(ValueError, match="smaller than dim"):
+        capi.residual_norm(_norm(capi), A, capi.F32, sum_out=A, sum_stride=7)
+    with pytest.raises(ValueError, match="null device pointer"):
+        capi.residual_norm(_norm(capi), None, capi.F32)
+    with pytest.raises(ValueError, match="null device pointer"):
+        capi.residual_norm(_norm(capi), A, capi.I8)  # codes without scales
+    with pytest.raises(ValueError, match="null device pointer"):
+        capi.residual_norm_gradient(_norm(capi), None, A, A, A, 1 << 30)
+    for name in ("out_gradient_stride", "sum_gradient_stride", "x_gradient_stride"):
+        with pytest.raises(ValueError, match="smaller than dim"):
+            capi.residual_norm_gradient(_norm(capi), A, A, A, A, 1 << 30, **{name: 7})
+    need = capi.residual_norm_gradient_workspace_bytes(_norm(capi))
+    with pytest.raises(ValueError, match="too small"):
+        capi.residual_norm_gradient(_norm(capi), A, A, A, A, need - 1)
+    with pytest.raises(ValueError, match="too small"):
+        capi.residual_norm_gradient(_norm(capi), A, A, A, None, need)
+    with pytest.raises(ValueError, match="16 bytes"):
+        capi.residual_norm_gradient(_norm(capi), A, A, A, A + 4, need)
+
+
+def test_null_descriptors(capi):
+    lib = capi.library()
+    assert lib.zcgvs_residual_norm(None, A, 0, capi.F32, None, None, 0, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.zcgvs_residual_norm_gradient_workspace_bytes(None) == 0 and "null descriptor" in capi.last_error()
+
+
+def test_empty_work_returns_ok(capi):
+    capi.residual_norm(_norm(capi, rows=0, x=None, residual=None), None, capi.F32)
+    capi.residual_norm_gradient(_norm(capi), None, None, None, None, 0)  # no gradient is wanted
+    capi.residual_norm_gradient(_norm(capi, rows=0, x=None), None, A, None, None, 0)

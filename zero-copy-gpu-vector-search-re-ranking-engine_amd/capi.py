@@ -77,6 +77,11 @@ class AdaptedDesc(ctypes.Structure):
                 ("max_rank", _i32), ("ranks", _vp), ("scales", _vp), ("adapter_ids", _vp)]
 
 
+class NormDesc(ctypes.Structure):
+    _fields_ = [("x", _vp), ("x_stride", _i64), ("residual", _vp), ("residual_stride", _i64), ("weight", _vp),
+                ("rows", _i64), ("dim", _i32), ("dtype", _i32), ("weight_offset", _f32), ("eps", _f32)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "zcgvs_last_error": (ctypes.c_char_p, []),
@@ -154,6 +159,10 @@ _SIGNATURES = {
     "zcgvs_adapted_max_rank": (_i32, []),
     "zcgvs_adapted_projection_workspace_bytes": (_sz, [ctypes.POINTER(AdaptedDesc)]),
     "zcgvs_adapted_projection": (_i32, [ctypes.POINTER(AdaptedDesc), _vp, _i64, _i32, _vp, _sz, _vp]),
+    "zcgvs_residual_norm_max_dim": (_i32, []),
+    "zcgvs_residual_norm": (_i32, [ctypes.POINTER(NormDesc), _vp, _i64, _i32, _vp, _vp, _i64, _vp]),
+    "zcgvs_residual_norm_gradient_workspace_bytes": (_sz, [ctypes.POINTER(NormDesc)]),
+    "zcgvs_residual_norm_gradient": (_i32, [ctypes.POINTER(NormDesc), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -638,3 +647,32 @@ def adapted_projection(desc: AdaptedDesc, out, out_dtype, workspace, workspace_b
     """x weight^T plus each row's own low-rank adapter."""
     call("zcgvs_adapted_projection", ctypes.byref(desc), ptr(out), out_stride, out_dtype, ptr(workspace),
          workspace_bytes, getattr(stream, "handle", stream))
+
+
+# ---- operators of an encoder block ---------------------------------------------------------
+
+def norm_desc(x, rows, dim, dtype, *, weight=None, weight_offset=0.0, residual=None, eps=1e-6, x_stride=0,
+              residual_stride=0) -> NormDesc:
+    return _keep_alive(NormDesc(ptr(x), x_stride, ptr(residual), residual_stride, ptr(weight), rows, dim, dtype,
+                                weight_offset, eps), x, residual, weight)
+
+
+def residual_norm(desc: NormDesc, out, out_dtype, *, out_scales=None, sum_out=None, out_stride=0, sum_stride=0,
+                  stream=None) -> None:
+    """The root-mean-square norm of x + residual (out_dtype I8: codes, with a scale a row in out_scales), and the
+    sum itself in sum_out."""
+    call("zcgvs_residual_norm", ctypes.byref(desc), ptr(out), out_stride, out_dtype, ptr(out_scales), ptr(sum_out),
+         sum_stride, getattr(stream, "handle", stream))
+
+
+def residual_norm_gradient_workspace_bytes(desc: NormDesc) -> int:
+    return _workspace_bytes("zcgvs_residual_norm_gradient_workspace_bytes", desc)
+
+
+def residual_norm_gradient(desc: NormDesc, out_gradient, x_gradient, weight_gradient, workspace, workspace_bytes, *,
+                           sum_gradient=None, out_gradient_stride=0, sum_gradient_stride=0, x_gradient_stride=0,
+                           stream=None) -> None:
+    """The gradients of residual_norm (either may be None)."""
+    call("zcgvs_residual_norm_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, ptr(sum_gradient),
+         sum_gradient_stride, ptr(x_gradient), x_gradient_stride, ptr(weight_gradient), ptr(workspace), workspace_bytes,
+         getattr(stream, "handle", stream))

@@ -117,6 +117,13 @@ __device__ __forceinline__ void writeHit(std::uint64_t key, int* index_out, floa
     }
 }
 
+// The int8 code of x: clamp(rint(x * inverse_scale), -127, 127), round half to even, like nearbyint in
+// tests/cpp/cpu_reference.hpp:51-62.
+__device__ __forceinline__ signed char quantizeCode(float x, float inverse_scale) {
+    const float scaled = rintf(x * inverse_scale);
+    return static_cast<signed char>(fminf(fmaxf(scaled, -127.0f), 127.0f));
+}
+
 template <typename T>
 __device__ __forceinline__ T waveXor(T value, int mask) {
     return __shfl_xor(value, mask, kWave);

@@ -94,18 +94,11 @@ __global__ __launch_bounds__(kConvertThreads) void convertF32ToF16Kernel(const f
     }
 }
 
-// q = clamp(rint(x * inverse_scale), -127, 127): round half to even, like nearbyint in
-// tests/cpp/cpu_reference.hpp:51-62.
-__device__ __forceinline__ signed char quantize(float x, float inverse_scale) {
-    const float scaled = rintf(x * inverse_scale);
-    return static_cast<signed char>(fminf(fmaxf(scaled, -127.0f), 127.0f));
-}
-
 template <bool kAligned>
 __global__ __launch_bounds__(kConvertThreads) void convertF32ToI8Kernel(const float* __restrict__ src,
                                                                         signed char* __restrict__ dst,
                                                                         std::size_t count, float inverse_scale) {
-    const auto convert = [inverse_scale](float x) { return quantize(x, inverse_scale); };
+    const auto convert = [inverse_scale](float x) { return quantizeCode(x, inverse_scale); };
     if constexpr (kAligned) {
         convertElements(src, dst, count, convert);
     } else {
@@ -209,7 +202,7 @@ __global__ __launch_bounds__(kConvertThreads) void quantizeRowsKernel(const floa
             i8x4 codes;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                codes[e] = quantize(x[i][e], inverse);
+                codes[e] = quantizeCode(x[i][e], inverse);
             }
             out[c] = codes;
         }
@@ -254,11 +247,11 @@ __global__ __launch_bounds__(kConvertThreads) void quantizeAnyRowsKernel(const f
     for (int i = 0; i < kKept; ++i) {
         const int j = i * kWave + lane;
         if (j < dim) {
-            out[j] = quantize(x[i], inverse);
+            out[j] = quantizeCode(x[i], inverse);
         }
     }
     for (int j = kKept * kWave + lane; j < dim; j += kWave) {
-        out[j] = quantize(values[j], inverse);
+        out[j] = quantizeCode(values[j], inverse);
     }
     if (lane == 0) {
         scales[row] = scale;

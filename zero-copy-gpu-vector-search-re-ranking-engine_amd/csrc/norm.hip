@@ -1,0 +1,591 @@
+// Root-mean-square norm of the sum of two rows, with int8 rows and scales as one of its outputs, and its gradient.
+//
+//     s = x + residual,  r = 1 / sqrt(mean(s^2) + eps),  y = s r (w + c)
+//     ds = r (g - u mean(g u)) + ds',  u = s r,  g = dy (w + c);   dw = sum over rows of dy u
+//
+// Memory bound: every operand is read once and every result written once. A row stays in the registers of one
+// wavefront (up to 2048 16-bit or 1024 float32 values) or of one workgroup between the sum of its squares and its
+// results, so nothing is read twice. The squares' sum, the mean and the rows are float32 throughout; s is rounded
+// where it is stored only.
+// The gradient's workgroups take every gridDim.x-th row and keep their part of dw in registers; each writes
+// one row of float32 sums, which a second launch adds in the order of the workgroups: the same bits on every call.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.hpp"
+#include "elements.hpp"
+#include "matrix_plan.hpp"
+
+namespace zcgvs_hip {
+
+namespace {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormWaves = kNormThreads / kWave;
+constexpr int kNormMaxDim = 16384;
+
+// Values of 16 bytes, which a thread takes at a time.
+template <typename T>
+constexpr int kNormPack = 16 / static_cast<int>(sizeof(T));
+
+// kCount values from `from` on, of which `left` exist; zeros past them.
+template <typename T, int kCount>
+__device__ __forceinline__ void loadSome(const T* from, int left, float (&to)[kCount]) {
+    if (left >= kCount) {
+        loadPack(from, to);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            to[e] = e < left ? static_cast<float>(from[e]) : 0.0f;
+        }
+    }
+}
+
+template <typename T, int kCount>
+__device__ __forceinline__ void storeSome(const float (&from)[kCount], int left, T* to) {
+    if (left >= kCount) {
+        storePack(from, to);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            if (e < left) {
+                to[e] = static_cast<T>(from[e]);
+            }
+        }
+    }
+}
+
+// The int8 codes of kCount values.
+template <int kCount>
+__device__ __forceinline__ void storeCodes(const float (&from)[kCount], float inverse, int left, std::int8_t* to) {
+    typename Pack<std::int8_t, kCount>::stored codes;
+#pragma unroll
+    for (int e = 0; e < kCount; ++e) {
+        codes[e] = quantizeCode(from[e], inverse);
+    }
+    if (left >= kCount) {
+        *reinterpret_cast<typename Pack<std::int8_t, kCount>::stored*>(to) = codes;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            if (e < left) {
+                to[e] = codes[e];
+            }
+        }
+    }
+}
+
+// op over a row's kThreads threads (a wavefront, or the whole workgroup through `shared`, which holds one value
+// a wavefront and is free again after the next call's barrier); every thread gets the result.
+template <int kThreads, typename Op>
+__device__ __forceinline__ float overRow(float value, float* shared, Op op) {
+#pragma unroll
+    for (int offset = kWave / 2; offset > 0; offset >>= 1) {
+        value = op(value, waveXor(value, offset));
+    }
+    if constexpr (kThreads > kWave) {
+        if ((threadIdx.x & (kWave - 1)) == 0) {
+            shared[threadIdx.x / kWave] = value;
+        }
+        __syncthreads();
+        value = shared[0];
+#pragma unroll
+        for (int w = 1; w < kThreads / kWave; ++w) {
+            value = op(value, shared[w]);
+        }
+    }
+    return value;
+}
+
+struct NormArgs {
+    const void* x;
+    std::int64_t x_stride;
+    const void* residual;
+    std::int64_t residual_stride;
+    const void* weight;
+    long long rows;
+    int dim;
+    float weight_offset;
+    float eps;
+    void* out;
+    std::int64_t out_stride;
+    float* out_scales;
+    void* sum;
+    std::int64_t sum_stride;
+};
+
+// 1 / sqrt(mean + eps) of a row whose squares add up to `squares`.
+__device__ __forceinline__ float rowFactor(float squares, int dim, float eps) {
+    return 1.0f / sqrtf(squares / static_cast<float>(dim) + eps);
+}
+
+// s of the calling thread's kVectors packs of one row.
+template <typename T, int kThreads, int kVectors>
+__device__ __forceinline__ void loadSum(const T* x, const T* residual, int dim, float (&s)[kVectors][kNormPack<T>]) {
+    constexpr int kPack = kNormPack<T>;
+    const int lane = static_cast<int>(threadIdx.x) % kThreads;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        const int c = (i * kThreads + lane) * kPack;
+        loadSome(x + c, dim - c, s[i]);
+    }
+    if (residual != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int c = (i * kThreads + lane) * kPack;
+            float more[kPack];
+            loadSome(residual + c, dim - c, more);
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                s[i][e] += more[e];
+            }
+        }
+    }
+}
+
+// kThreads threads a row, kVectors packs each.
+template <typename T, typename Out, int kThreads, int kVectors>
+__global__ __launch_bounds__(kNormThreads) void residualNormKernel(NormArgs args) {
+    constexpr int kPack = kNormPack<T>;
+    __shared__ float shared[2][kNormWaves];
+    const int lane = static_cast<int>(threadIdx.x) % kThreads;
+    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / kThreads) + threadIdx.x / kThreads;
+    if (row >= args.rows) {
+        return;  // (a whole row's threads, and the whole workgroup where they share memory)
+    }
+    float s[kVectors][kPack];
+    const T* x = static_cast<const T*>(args.x) + row * args.x_stride;
+    const T* residual = args.residual == nullptr ? nullptr : static_cast<const T*>(args.residual) + row * args.residual_stride;
+    loadSum<T, kThreads, kVectors>(x, residual, args.dim, s);
+    float squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            squares = fmaf(s[i][e], s[i][e], squares);
+        }
+    }
+    const auto add = [](float a, float b) { return a + b; };
+    const float factor = rowFactor(overRow<kThreads>(squares, shared[0], add), args.dim, args.eps);
+    if (args.sum != nullptr) {
+        T* sum = static_cast<T*>(args.sum) + row * args.sum_stride;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int c = (i * kThreads + lane) * kPack;
+            storeSome(s[i], args.dim - c, sum + c);
+        }
+    }
+    const T* weight = static_cast<const T*>(args.weight);
+    float peak = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        const int c = (i * kThreads + lane) * kPack;
+        float w[kPack];
+        if (weight != nullptr) {
+            loadSome(weight + c, args.dim - c, w);
+        }
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            s[i][e] *= factor * ((weight != nullptr ? w[e] : 1.0f) + args.weight_offset);
+            peak = fmaxf(peak, c + e < args.dim ? fabsf(s[i][e]) : 0.0f);
+        }
+    }
+    if constexpr (std::is_same_v<Out, std::int8_t>) {
+        peak = overRow<kThreads>(peak, shared[1], [](float a, float b) { return fmaxf(a, b); });
+        const float scale = peak > 0.0f ? peak / 127.0f : 1.0f;
+        const float inverse = 1.0f / scale;
+        std::int8_t* out = static_cast<std::int8_t*>(args.out) + row * args.out_stride;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int c = (i * kThreads + lane) * kPack;
+            storeCodes(s[i], inverse, args.dim - c, out + c);
+        }
+        if (lane == 0) {
+            args.out_scales[row] = scale;
+        }
+    } else {
+        Out* out = static_cast<Out*>(args.out) + row * args.out_stride;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int c = (i * kThreads + lane) * kPack;
+            storeSome(s[i], args.dim - c, out + c);
+        }
+    }
+}
+
+struct NormGradientArgs {
+    const void* out_gradient;
+    std::int64_t out_gradient_stride;
+    const void* sum_gradient;
+    std::int64_t sum_gradient_stride;
+    void* x_gradient;
+    std::int64_t x_gradient_stride;
+    float* partials;  // [workgroups, dim] of the weight's gradient, or null: not wanted
+};
+
+template <typename T, int kThreads, int kVectors>
+__global__ __launch_bounds__(kNormThreads) void residualNormGradientKernel(NormArgs args, NormGradientArgs more) {
+    constexpr int kPack = kNormPack<T>;
+    constexpr int kRows = kNormThreads / kThreads;
+    // sums over the row of two values a wavefront, two sets by turns; a workgroup of several rows joins its sums
+    // of the weight's gradient here
+    __shared__ float shared[kThreads > kWave ? 4 * kNormWaves : kThreads * kPack];
+    const int lane = static_cast<int>(threadIdx.x) % kThreads;
+    const int slot = static_cast<int>(threadIdx.x) / kThreads;
+    const T* weight = static_cast<const T*>(args.weight);
+    float w[kVectors][kPack], dw[kVectors][kPack];
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        const int c = (i * kThreads + lane) * kPack;
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            w[i][e] = 1.0f;
+            dw[i][e] = 0.0f;
+        }
+        if (weight != nullptr) {
+            loadSome(weight + c, args.dim - c, w[i]);
+        }
+#pragma unroll
+        for (int e = 0; e < kPack; ++e) {
+            w[i][e] += args.weight_offset;
+        }
+    }
+    int turn = 0;
+    for (long long row = static_cast<long long>(blockIdx.x) * kRows + slot; row < args.rows;
+         row += static_cast<long long>(gridDim.x) * kRows) {
+        float s[kVectors][kPack], d[kVectors][kPack];
+        const T* x = static_cast<const T*>(args.x) + row * args.x_stride;
+        const T* residual =
+            args.residual == nullptr ? nullptr : static_cast<const T*>(args.residual) + row * args.residual_stride;
+        const T* from = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride;
+        loadSum<T, kThreads, kVectors>(x, residual, args.dim, s);
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int c = (i * kThreads + lane) * kPack;
+            loadSome(from + c, args.dim - c, d[i]);
+        }
+        float squares = 0.0f, along = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                squares = fmaf(s[i][e], s[i][e], squares);
+                along = fmaf(d[i][e] * w[i][e], s[i][e], along);
+            }
+        }
+        const auto add = [](float a, float b) { return a + b; };
+        if constexpr (kThreads > kWave) {
+            // both sums with one barrier; the other set is the row's before, which every thread has read
+            float* set = shared + turn * 2 * kNormWaves;
+            turn ^= 1;
+            squares = overRow<kWave>(squares, nullptr, add);
+            along = overRow<kWave>(along, nullptr, add);
+            if ((threadIdx.x & (kWave - 1)) == 0) {
+                set[threadIdx.x / kWave] = squares;
+                set[kNormWaves + threadIdx.x / kWave] = along;
+            }
+            __syncthreads();
+            squares = set[0];
+            along = set[kNormWaves];
+#pragma unroll
+            for (int v = 1; v < kNormWaves; ++v) {
+                squares += set[v];
+                along += set[kNormWaves + v];
+            }
+        } else {
+            squares = overRow<kWave>(squares, nullptr, add);
+            along = overRow<kWave>(along, nullptr, add);
+        }
+        const float factor = rowFactor(squares, args.dim, args.eps);
+        const float mean = along * factor / static_cast<float>(args.dim);  // of g u
+        const T* through =
+            more.sum_gradient == nullptr ? nullptr : static_cast<const T*>(more.sum_gradient) + row * more.sum_gradient_stride;
+        T* to = static_cast<T*>(more.x_gradient) + row * more.x_gradient_stride;
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int c = (i * kThreads + lane) * kPack;
+            float result[kPack];
+            if (through != nullptr) {
+                loadSome(through + c, args.dim - c, result);
+            }
+#pragma unroll
+            for (int e = 0; e < kPack; ++e) {
+                const float u = s[i][e] * factor;
+                dw[i][e] = fmaf(d[i][e], u, dw[i][e]);
+                const float own = factor * (d[i][e] * w[i][e] - u * mean);
+                result[e] = through != nullptr ? result[e] + own : own;
+            }
+            if (more.x_gradient != nullptr) {
+                storeSome(result, args.dim - c, to + c);
+            }
+        }
+    }
+    if (more.partials == nullptr) {
+        return;
+    }
+    float* to = more.partials + static_cast<long long>(blockIdx.x) * args.dim;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        const int c = (i * kThreads + lane) * kPack;
+        if constexpr (kRows > 1) {
+            // the rows' threads add theirs one after the other
+            for (int turn_of = 0; turn_of < kRows; ++turn_of) {
+                __syncthreads();
+                if (slot == turn_of) {
+#pragma unroll
+                    for (int e = 0; e < kPack; ++e) {
+                        float* at = shared + e * kThreads + lane;
+                        dw[i][e] += turn_of > 0 ? *at : 0.0f;
+                        *at = dw[i][e];
+                    }
+                }
+            }
+        }
+        if (slot == kRows - 1) {
+            storeSome(dw[i], args.dim - c, to + c);
+        }
+    }
+}
+
+// out[c] = the sum over `count` rows of partials [count, dim], kJoinLanes threads a column in a fixed order.
+constexpr int kJoinColumns = 16;
+constexpr int kJoinLanes = kNormThreads / kJoinColumns;
+
+template <typename T>
+__global__ __launch_bounds__(kNormThreads) void joinColumnsKernel(const float* __restrict__ partials, int count, int dim,
+                                                                  T* __restrict__ out) {
+    __shared__ float shared[kJoinLanes][kJoinColumns];
+    const int column = static_cast<int>(threadIdx.x) % kJoinColumns;
+    const int part = static_cast<int>(threadIdx.x) / kJoinColumns;
+    const int c = static_cast<int>(blockIdx.x) * kJoinColumns + column;
+    float sum = 0.0f;
+    if (c < dim) {
+#pragma unroll 8
+        for (int r = part; r < count; r += kJoinLanes) {
+            sum += partials[static_cast<long long>(r) * dim + c];
+        }
+    }
+    shared[part][column] = sum;
+    __syncthreads();
+    if (part == 0 && c < dim) {
+#pragma unroll
+        for (int p = 1; p < kJoinLanes; ++p) {
+            sum += shared[p][column];
+        }
+        out[c] = static_cast<T>(sum);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+int invalid(const char* message) {
+    return setError(ZCGVS_ERR_INVALID_ARGUMENT, std::string("zcgvs residual norm: ") + message);
+}
+
+int checkNorm(const zcgvs_norm_desc* desc) {
+    if (desc == nullptr) {
+        return invalid("null descriptor");
+    }
+    const zcgvs_norm_desc& d = *desc;
+    if (!validElement(d.dtype)) {
+        return invalid("the operands must hold float32, float16 or bfloat16");
+    }
+    if (d.dim <= 0 || d.dim > kNormMaxDim) {
+        return invalid("dim must lie in [1, 16384]");
+    }
+    if (d.rows < 0 || d.rows > (1 << 30)) {
+        return invalid("rows must lie in [0, 2^30]");
+    }
+    if (rowStride(d.x_stride, d.dim) < d.dim || (d.residual != nullptr && rowStride(d.residual_stride, d.dim) < d.dim)) {
+        return invalid("a row stride is smaller than dim");
+    }
+    if (!(d.eps >= 0.0f) || !std::isfinite(d.eps) || !std::isfinite(d.weight_offset)) {
+        return invalid("eps must be finite and at least 0, weight_offset finite");
+    }
+    if (d.rows > 0 && d.x == nullptr) {
+        return invalid("null device pointer");
+    }
+    return ZCGVS_OK;
+}
+
+// Calls body(threads a row, packs a thread), both as integral constants: a wavefront a row where at most four packs
+// a thread hold it.
+template <typename T, typename Body>
+int withRowShape(int dim, Body&& body) {
+    const auto wave = std::integral_constant<int, kWave>{};
+    const auto group = std::integral_constant<int, kNormThreads>{};
+    const int packs = divideUp(dim, kNormPack<T>);
+    switch (divideUp(packs, kWave)) {
+        case 1: return body(wave, std::integral_constant<int, 1>{});
+        case 2: return body(wave, std::integral_constant<int, 2>{});
+        case 3: return body(wave, std::integral_constant<int, 3>{});
+        case 4: return body(wave, std::integral_constant<int, 4>{});
+        default: break;
+    }
+    const int each = divideUp(packs, kNormThreads);
+    if (each <= 2) {
+        return body(group, std::integral_constant<int, 2>{});
+    }
+    if (each <= 4) {
+        return body(group, std::integral_constant<int, 4>{});
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (each > 8) {
+            return body(group, std::integral_constant<int, 16>{});
+        }
+    }
+    return body(group, std::integral_constant<int, 8>{});
+}
+
+NormArgs normArgs(const zcgvs_norm_desc& d) {
+    NormArgs args{};
+    args.x = d.x;
+    args.x_stride = rowStride(d.x_stride, d.dim);
+    args.residual = d.residual;
+    args.residual_stride = rowStride(d.residual_stride, d.dim);
+    args.weight = d.weight;
+    args.rows = d.rows;
+    args.dim = d.dim;
+    args.weight_offset = d.weight_offset;
+    args.eps = d.eps;
+    return args;
+}
+
+// Workgroups of the gradient: four to a CU, for rows of a wavefront four at a time.
+int gradientBlocks(const zcgvs_norm_desc& d) {
+    const int pack = 16 / elementBytes(d.dtype);
+    const int rows_each = divideUp(divideUp(d.dim, pack), kWave) <= 4 ? kNormWaves : 1;
+    return static_cast<int>(std::min<long long>(4ll * deviceComputeUnits(), (d.rows + rows_each - 1) / rows_each));
+}
+
+}  // namespace
+
+}  // namespace zcgvs_hip
+
+using namespace zcgvs_hip;
+
+extern "C" {
+
+int zcgvs_residual_norm_max_dim(void) { return kNormMaxDim; }
+
+int zcgvs_residual_norm(const zcgvs_norm_desc* desc, void* d_out, std::int64_t out_stride, int out_dtype,
+                        float* d_out_scales, void* d_sum, std::int64_t sum_stride, zcgvs_stream_t stream) {
+    const int status = checkNorm(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_norm_desc& d = *desc;
+    const bool codes = out_dtype == ZCGVS_DTYPE_I8;
+    if (!codes && out_dtype != d.dtype && out_dtype != ZCGVS_DTYPE_F32) {
+        return invalid("the output must hold the operands' type, float32 or int8");
+    }
+    if (rowStride(out_stride, d.dim) < d.dim || (d_sum != nullptr && rowStride(sum_stride, d.dim) < d.dim)) {
+        return invalid("an output's row stride is smaller than dim");
+    }
+    if (d.rows == 0) {
+        return clearError();
+    }
+    if (d_out == nullptr || (codes && d_out_scales == nullptr)) {
+        return invalid("null device pointer");
+    }
+    NormArgs args = normArgs(d);
+    args.out = d_out;
+    args.out_stride = rowStride(out_stride, d.dim);
+    args.out_scales = d_out_scales;
+    args.sum = d_sum;
+    args.sum_stride = rowStride(sum_stride, d.dim);
+    const int launched = withElement(d.dtype, [&](auto element) {
+        using T = decltype(element);
+        return withRowShape<T>(d.dim, [&](auto threads, auto vectors) {
+            constexpr int kThreads = decltype(threads)::value;
+            constexpr int kVectors = decltype(vectors)::value;
+            // a wavefront's rows in workgroups of four, or of one where that leaves CUs without one
+            const int rows_each =
+                kThreads > kWave || d.rows <= kNormWaves * static_cast<std::int64_t>(deviceComputeUnits()) ? 1 : kNormWaves;
+            const unsigned blocks = static_cast<unsigned>((d.rows + rows_each - 1) / rows_each);
+            const unsigned block_threads = static_cast<unsigned>(rows_each * kThreads);
+            if (codes) {
+                residualNormKernel<T, std::int8_t, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+            } else if (out_dtype == d.dtype) {
+                residualNormKernel<T, T, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+            } else {
+                residualNormKernel<T, float, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+            }
+            ZCGVS_LAUNCH_CHECK("residual norm");
+            return static_cast<int>(ZCGVS_OK);
+        });
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+std::size_t zcgvs_residual_norm_gradient_workspace_bytes(const zcgvs_norm_desc* desc) {
+    if (checkNorm(desc) != ZCGVS_OK) {
+        return 0;
+    }
+    clearError();
+    return std::max<std::size_t>(256, static_cast<std::size_t>(gradientBlocks(*desc)) * desc->dim * sizeof(float));
+}
+
+int zcgvs_residual_norm_gradient(const zcgvs_norm_desc* desc, const void* d_out_gradient,
+                                 std::int64_t out_gradient_stride, const void* d_sum_gradient,
+                                 std::int64_t sum_gradient_stride, void* d_x_gradient, std::int64_t x_gradient_stride,
+                                 void* d_weight_gradient, void* d_workspace, std::size_t workspace_bytes,
+                                 zcgvs_stream_t stream) {
+    const int status = checkNorm(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_norm_desc& d = *desc;
+    if (rowStride(out_gradient_stride, d.dim) < d.dim || rowStride(sum_gradient_stride, d.dim) < d.dim ||
+        rowStride(x_gradient_stride, d.dim) < d.dim) {
+        return invalid("a gradient's row stride is smaller than dim");
+    }
+    if ((d_x_gradient == nullptr || d.rows == 0) && d_weight_gradient == nullptr) {
+        return clearError();
+    }
+    if (d.rows > 0 && d_out_gradient == nullptr) {
+        return invalid("null device pointer");
+    }
+    if (d_weight_gradient != nullptr && d.rows > 0) {
+        if (d_workspace == nullptr || workspace_bytes < zcgvs_residual_norm_gradient_workspace_bytes(desc)) {
+            return invalid("the workspace is too small");
+        }
+        if (!aligned16(d_workspace)) {
+            return invalid("the workspace must be aligned to 16 bytes");
+        }
+    }
+    NormGradientArgs more{};
+    more.out_gradient = d_out_gradient;
+    more.out_gradient_stride = rowStride(out_gradient_stride, d.dim);
+    more.sum_gradient = d_sum_gradient;
+    more.sum_gradient_stride = rowStride(sum_gradient_stride, d.dim);
+    more.x_gradient = d_x_gradient;
+    more.x_gradient_stride = rowStride(x_gradient_stride, d.dim);
+    more.partials = d_weight_gradient == nullptr ? nullptr : static_cast<float*>(d_workspace);
+    const int blocks = gradientBlocks(d);
+    const int launched = withElement(d.dtype, [&](auto element) {
+        using T = decltype(element);
+        if (d.rows > 0) {
+            const int formed = withRowShape<T>(d.dim, [&](auto threads, auto vectors) {
+                residualNormGradientKernel<T, decltype(threads)::value, decltype(vectors)::value>
+                    <<<static_cast<unsigned>(blocks), kNormThreads, 0, toStream(stream)>>>(normArgs(d), more);
+                ZCGVS_LAUNCH_CHECK("residual norm gradient");
+                return static_cast<int>(ZCGVS_OK);
+            });
+            if (formed != ZCGVS_OK) {
+                return formed;
+            }
+        }
+        if (d_weight_gradient != nullptr) {
+            joinColumnsKernel<T><<<static_cast<unsigned>(divideUp(d.dim, kJoinColumns)), kNormThreads, 0, toStream(stream)>>>(
+                more.partials, blocks, d.dim, static_cast<T*>(d_weight_gradient));
+            ZCGVS_LAUNCH_CHECK("residual norm gradient");
+        }
+        return static_cast<int>(ZCGVS_OK);
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+}  // extern "C"
