@@ -606,6 +606,47 @@ int zcgvs_residual_norm_gradient(const zcgvs_norm_desc* desc, const void* d_out_
                                  void* d_weight_gradient, void* d_workspace, size_t workspace_bytes,
                                  zcgvs_stream_t stream);
 
+/* A projection with its epilogue: out = act(x weight^T + bias) + residual, act one of enum
+ * zcgvs_activation or ZCGVS_ACT_NONE.
+ * int8 operands (dtype ZCGVS_DTYPE_I8, at most 131072 codes a row): x weight^T is the exact sum of the codes'
+ * products times x_scales[row] * weight_scales[column] (in this order). */
+enum { ZCGVS_ACT_NONE = 3 };
+
+typedef struct zcgvs_linear_desc {
+    const void* x;           /* [rows, dim]                                                  */
+    int64_t x_stride;        /* 0: dim                                                       */
+    const void* weight;      /* [out_dim, dim]                                               */
+    int64_t weight_stride;   /* 0: dim                                                       */
+    int64_t rows;            /* at most 2^30                                                 */
+    int dim;
+    int out_dim;
+    int dtype;               /* of x and weight: float32, float16, bfloat16 or int8          */
+    int activation;
+    int epilogue_dtype;      /* of bias and residual: dtype, or with int8 operands a float type */
+    const float* x_scales;      /* [rows] (int8)                                             */
+    const float* weight_scales; /* [out_dim] (int8)                                          */
+    const void* bias;        /* [out_dim], or NULL: none                                     */
+    const void* residual;    /* [rows, out_dim], or NULL: none                               */
+    int64_t residual_stride; /* 0: out_dim                                                   */
+} zcgvs_linear_desc;
+
+/* d_out [rows, out_dim]; out_dtype is epilogue_dtype or ZCGVS_DTYPE_F32; out_stride 0: out_dim. d_out may be
+ * the residual itself where it has its type and stride. */
+int zcgvs_linear(const zcgvs_linear_desc* desc, void* d_out, int64_t out_stride, int out_dtype,
+                 zcgvs_stream_t stream);
+
+/* The gradient of zcgvs_linear (float operands) from that of its output. With z = x weight^T + bias (computed
+ * again; not needed without an activation) and dz = d_out_gradient * act'(z):
+ *     x_gradient [rows, dim] = dz weight,   weight_gradient [out_dim, dim] = dz^T x,
+ *     bias_gradient [out_dim] = the sum of dz over rows,
+ * all of desc->dtype; that of the residual is d_out_gradient itself. dz is rounded to desc->dtype between the
+ * products where there is an activation. Any output may be NULL (not wanted). */
+size_t zcgvs_linear_gradient_workspace_bytes(const zcgvs_linear_desc* desc);
+int zcgvs_linear_gradient(const zcgvs_linear_desc* desc, const void* d_out_gradient, int64_t out_gradient_stride,
+                          void* d_x_gradient, int64_t x_gradient_stride, void* d_weight_gradient,
+                          int64_t weight_gradient_stride, void* d_bias_gradient, void* d_workspace,
+                          size_t workspace_bytes, zcgvs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

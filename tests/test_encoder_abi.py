@@ -63,8 +63,80 @@ def test_norm_operands(capi):
         capi.residual_norm_gradient(_norm(capi), A, A, A, A + 4, need)
 
 
+def _linear(capi, **kw):
+    return capi.linear_desc(**dict(dict(x=A, rows=4, dim=8, weight=A, out_dim=6, dtype=capi.F32, bias=A, residual=A), **kw))
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(dtype=3), "float16, bfloat16 or int8"),
+    (dict(dtype=-1), "float16, bfloat16 or int8"),
+    (dict(epilogue_dtype=1), "the operands' type"),
+    (dict(dtype=2), "the operands' type"),  # int8 codes with int8 biases
+    (dict(activation=4), "unknown activation"),
+    (dict(activation=-1), "unknown activation"),
+    (dict(dim=0), "must be positive"),
+    (dict(out_dim=-1), "must be positive"),
+    (dict(dim=2**24 + 1), "at most 2\\^24"),
+    (dict(out_dim=2**24 + 1), "at most 2\\^24"),
+    (dict(rows=-1), "rows must lie"),
+    (dict(rows=2**30 + 1), "rows must lie"),
+    (dict(x_stride=7), "smaller than dim"),
+    (dict(weight_stride=7), "smaller than dim"),
+    (dict(residual_stride=5), "smaller than out_dim"),
+    (dict(x=None), "null device pointer"),
+    (dict(weight=None), "null device pointer"),
+])
+def test_linear_descriptor(capi, kw, match):
+    with pytest.raises(ValueError, match=match):
+        capi.linear(_linear(capi, **kw), A, capi.F32)
+    with pytest.raises(ValueError, match=match):
+        capi.linear_gradient_workspace_bytes(_linear(capi, **kw))
+    with pytest.raises(ValueError, match=match):
+        capi.linear_gradient(_linear(capi, **kw), A, A, A, A, A, 1 << 30)
+
+
+def test_linear_int8(capi):
+    codes = dict(dtype=capi.I8, epilogue_dtype=capi.F16, x_scales=A, weight_scales=A)
+    with pytest.raises(ValueError, match="131072 codes"):
+        capi.linear(_linear(capi, **dict(codes, dim=131073)), A, capi.F16)
+    for name in ("x_scales", "weight_scales"):
+        with pytest.raises(ValueError, match="need the scales"):
+            capi.linear(_linear(capi, **dict(codes, **{name: None})), A, capi.F16)
+    with pytest.raises(ValueError, match="the bias's type or float32"):
+        capi.linear(_linear(capi, **codes), A, capi.BF16)
+    with pytest.raises(ValueError, match="the bias's type or float32"):
+        capi.linear(_linear(capi, **codes), A, capi.I8)
+    with pytest.raises(ValueError, match="takes float operands"):
+        capi.linear_gradient_workspace_bytes(_linear(capi, **codes))
+    with pytest.raises(ValueError, match="takes float operands"):
+        capi.linear_gradient(_linear(capi, **codes), A, A, A, A, A, 1 << 30)
+
+
+def test_linear_operands(capi):
+    with pytest.raises(ValueError, match="the bias's type or float32"):
+        capi.linear(_linear(capi, dtype=capi.F16), A, capi.BF16)
+    with pytest.raises(ValueError, match="smaller than out_dim"):
+        capi.linear(_linear(capi), A, capi.F32, out_stride=5)
+    with pytest.raises(ValueError, match="null device pointer"):
+        capi.linear(_linear(capi), None, capi.F32)
+    with pytest.raises(ValueError, match="null device pointer"):
+        capi.linear_gradient(_linear(capi), None, A, A, A, A, 1 << 30)
+    for name, short in (("out_gradient_stride", 5), ("x_gradient_stride", 7), ("weight_gradient_stride", 7)):
+        with pytest.raises(ValueError, match="smaller than its row"):
+            capi.linear_gradient(_linear(capi), A, A, A, A, A, 1 << 30, **{name: short})
+    need = capi.linear_gradient_workspace_bytes(_linear(capi))
+    with pytest.raises(ValueError, match="too small"):
+        capi.linear_gradient(_linear(capi), A, A, A, A, A, need - 1)
+    with pytest.raises(ValueError, match="too small"):
+        capi.linear_gradient(_linear(capi), A, A, A, A, None, need)
+    with pytest.raises(ValueError, match="16 bytes"):
+        capi.linear_gradient(_linear(capi), A, A, A, A, A + 8, need)
+
+
 def test_null_descriptors(capi):
     lib = capi.library()
+    assert lib.zcgvs_linear(None, A, 0, capi.F32, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.zcgvs_linear_gradient_workspace_bytes(None) == 0 and "null descriptor" in capi.last_error()
     assert lib.zcgvs_residual_norm(None, A, 0, capi.F32, None, None, 0, None) == capi.ERR_INVALID_ARGUMENT
     assert lib.zcgvs_residual_norm_gradient_workspace_bytes(None) == 0 and "null descriptor" in capi.last_error()
 
@@ -73,3 +145,6 @@ def test_empty_work_returns_ok(capi):
     capi.residual_norm(_norm(capi, rows=0, x=None, residual=None), None, capi.F32)
     capi.residual_norm_gradient(_norm(capi), None, None, None, None, 0)  # no gradient is wanted
     capi.residual_norm_gradient(_norm(capi, rows=0, x=None), None, A, None, None, 0)
+    capi.linear(_linear(capi, rows=0, x=None, weight=None), None, capi.F32)
+    capi.linear_gradient(_linear(capi), None, None, None, None, None, 0)  # no gradient is wanted
+    capi.linear_gradient(_linear(capi, rows=0, x=None, weight=None), None, A, None, None, None, 0)

@@ -21,7 +21,7 @@ COSINE, DOT, L2 = 0, 1, 2
 F32, F16, I8, BINARY = 0, 1, 2, 3
 BF16 = 4  # the embedding-model operators only
 EMBEDDING_SUM, EMBEDDING_MEAN = 0, 1
-ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_NONE = 0, 1, 2, 3  # ACT_NONE: linear only
 INT8_REFERENCE, INT8_PER_VECTOR = 0, 1
 SEARCH_MATERIALIZE = 1
 SEARCH_UNSORTED_POSTINGS = 2
@@ -80,6 +80,12 @@ class AdaptedDesc(ctypes.Structure):
 class NormDesc(ctypes.Structure):
     _fields_ = [("x", _vp), ("x_stride", _i64), ("residual", _vp), ("residual_stride", _i64), ("weight", _vp),
                 ("rows", _i64), ("dim", _i32), ("dtype", _i32), ("weight_offset", _f32), ("eps", _f32)]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [("x", _vp), ("x_stride", _i64), ("weight", _vp), ("weight_stride", _i64), ("rows", _i64), ("dim", _i32),
+                ("out_dim", _i32), ("dtype", _i32), ("activation", _i32), ("epilogue_dtype", _i32), ("x_scales", _vp),
+                ("weight_scales", _vp), ("bias", _vp), ("residual", _vp), ("residual_stride", _i64)]
 
 
 # name -> (restype, argtypes)
@@ -163,6 +169,9 @@ _SIGNATURES = {
     "zcgvs_residual_norm": (_i32, [ctypes.POINTER(NormDesc), _vp, _i64, _i32, _vp, _vp, _i64, _vp]),
     "zcgvs_residual_norm_gradient_workspace_bytes": (_sz, [ctypes.POINTER(NormDesc)]),
     "zcgvs_residual_norm_gradient": (_i32, [ctypes.POINTER(NormDesc), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "zcgvs_linear": (_i32, [ctypes.POINTER(LinearDesc), _vp, _i64, _i32, _vp]),
+    "zcgvs_linear_gradient_workspace_bytes": (_sz, [ctypes.POINTER(LinearDesc)]),
+    "zcgvs_linear_gradient": (_i32, [ctypes.POINTER(LinearDesc), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -676,3 +685,29 @@ def residual_norm_gradient(desc: NormDesc, out_gradient, x_gradient, weight_grad
     call("zcgvs_residual_norm_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, ptr(sum_gradient),
          sum_gradient_stride, ptr(x_gradient), x_gradient_stride, ptr(weight_gradient), ptr(workspace), workspace_bytes,
          getattr(stream, "handle", stream))
+
+
+def linear_desc(x, rows, dim, weight, out_dim, dtype, *, bias=None, activation=ACT_NONE, residual=None, epilogue_dtype=None,
+                x_scales=None, weight_scales=None, x_stride=0, weight_stride=0, residual_stride=0) -> LinearDesc:
+    """epilogue_dtype: of bias and residual; None for the operands' own (float) type."""
+    return _keep_alive(LinearDesc(ptr(x), x_stride, ptr(weight), weight_stride, rows, dim, out_dim, dtype, activation,
+                                  dtype if epilogue_dtype is None else epilogue_dtype, ptr(x_scales), ptr(weight_scales),
+                                  ptr(bias), ptr(residual), residual_stride),
+                       x, weight, x_scales, weight_scales, bias, residual)
+
+
+def linear(desc: LinearDesc, out, out_dtype, *, out_stride=0, stream=None) -> None:
+    """act(x weight^T + bias) + residual."""
+    call("zcgvs_linear", ctypes.byref(desc), ptr(out), out_stride, out_dtype, getattr(stream, "handle", stream))
+
+
+def linear_gradient_workspace_bytes(desc: LinearDesc) -> int:
+    return _workspace_bytes("zcgvs_linear_gradient_workspace_bytes", desc)
+
+
+def linear_gradient(desc: LinearDesc, out_gradient, x_gradient, weight_gradient, bias_gradient, workspace, workspace_bytes,
+                    *, out_gradient_stride=0, x_gradient_stride=0, weight_gradient_stride=0, stream=None) -> None:
+    """The gradients of linear (any may be None); the residual's is out_gradient itself."""
+    call("zcgvs_linear_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, ptr(x_gradient),
+         x_gradient_stride, ptr(weight_gradient), weight_gradient_stride, ptr(bias_gradient), ptr(workspace),
+         workspace_bytes, getattr(stream, "handle", stream))

@@ -14,7 +14,9 @@ inline bool validElement(int dtype) {
     return dtype == ZCGVS_DTYPE_F32 || dtype == ZCGVS_DTYPE_F16 || dtype == ZCGVS_DTYPE_BF16;
 }
 
-__host__ __device__ constexpr int elementBytes(int dtype) { return dtype == ZCGVS_DTYPE_F32 ? 4 : 2; }
+__host__ __device__ constexpr int elementBytes(int dtype) {
+    return dtype == ZCGVS_DTYPE_F32 ? 4 : dtype == ZCGVS_DTYPE_I8 ? 1 : 2;
+}
 
 // Calls body(T{}) with the C++ type of a valid element dtype.
 template <typename Body>

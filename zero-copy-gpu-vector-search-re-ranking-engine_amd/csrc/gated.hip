@@ -26,53 +26,16 @@
 
 #include <algorithm>
 
+#include "activation.hpp"
 #include "common.hpp"
 #include "elements.hpp"
+#include "matrix_join.hpp"
 #include "matrix_plan.hpp"
 #include "matrix_tile.hpp"
 
 namespace zcgvs_hip {
 
 namespace {
-
-// 1 / (1 + exp(-x)): exp2 and the reciprocal of the hardware, each within 1 ulp. The reciprocal gives zeros in the
-// place of results below 2^-126, so it is taken of 2^-32 of the sum.
-__device__ __forceinline__ float logistic(float x) {
-    constexpr float kSmall = 0x1p-32f;
-    return kSmall * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(-1.44269504f * x), kSmall, kSmall));
-}
-
-// The activation's value and slope at g.
-template <int kActivation>
-__device__ __forceinline__ float activate(float g) {
-    if constexpr (kActivation == ZCGVS_ACT_SILU) {
-        return g * logistic(g);
-    } else if constexpr (kActivation == ZCGVS_ACT_GELU) {
-        return 0.5f * g * (1.0f + erff(g * 0.70710678f));
-    } else {
-        // 0.5 (1 + tanh(z)) is the logistic function of 2 z
-        return g * logistic(1.59576912f * (g + 0.044715f * g * g * g));
-    }
-}
-
-template <int kActivation>
-__device__ __forceinline__ void activateBoth(float g, float& value, float& slope) {
-    if constexpr (kActivation == ZCGVS_ACT_SILU) {
-        const float y = logistic(g);
-        value = g * y;
-        slope = y + value * (1.0f - y);
-    } else if constexpr (kActivation == ZCGVS_ACT_GELU) {
-        const float y = 0.5f * (1.0f + erff(g * 0.70710678f));
-        value = g * y;
-        slope = y + g * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * g * g);
-    } else {
-        const float y = logistic(1.59576912f * (g + 0.044715f * g * g * g));
-        value = g * y;
-        // value * (1 - y) is 0 long before |g| is 100; the square must not make an infinity of it
-        const float square = fminf(g * g, 1.0e4f);
-        slope = y + value * (1.0f - y) * (1.59576912f * (1.0f + 0.134145f * square));
-    }
-}
 
 struct GatedArgs {
     const void* x;
@@ -366,38 +329,6 @@ __global__ __launch_bounds__(InputTile::kThreads) void bothGradientsKernel(Input
     }
 }
 
-// out = the sum of the splits' partials [splits, rows, columns]; rows from `rows_first` on go to `second`.
-constexpr int kJoinThreads = 256;
-
-template <typename T, int kPack>
-__global__ __launch_bounds__(kJoinThreads) void joinKernel(const float* __restrict__ partials, int splits,
-                                                           long long rows, int columns, long long rows_first,
-                                                           T* __restrict__ first, T* __restrict__ second,
-                                                           std::int64_t stride) {
-    const int packs_per_row = (columns + kPack - 1) / kPack;
-    const long long packs = rows * packs_per_row;
-    const long long split_values = rows * columns;
-    for (long long p = static_cast<long long>(blockIdx.x) * kJoinThreads + threadIdx.x; p < packs;
-         p += static_cast<long long>(gridDim.x) * kJoinThreads) {
-        const long long row = p / packs_per_row;
-        const int column = packColumn<kPack>(static_cast<int>(p - row * packs_per_row), columns);
-        const float* from = partials + row * columns + column;
-        float sum[kPack];
-        loadPack(from, sum);
-#pragma unroll 4
-        for (int s = 1; s < splits; ++s) {
-            float more[kPack];
-            loadPack(from + s * split_values, more);
-#pragma unroll
-            for (int e = 0; e < kPack; ++e) {
-                sum[e] += more[e];
-            }
-        }
-        T* to = row < rows_first ? first + row * stride : second + (row - rows_first) * stride;
-        storePack(sum, to + column);
-    }
-}
-
 // ---- host ---------------------------------------------------------------------------------------
 
 int invalid(const char* message) {
@@ -431,19 +362,6 @@ int checkGated(const zcgvs_gated_desc* desc) {
         return invalid("null device pointer");
     }
     return ZCGVS_OK;
-}
-
-// Calls body(std::integral_constant<int, activation>).
-template <typename Body>
-int withActivation(int activation, Body&& body) {
-    switch (activation) {
-        case ZCGVS_ACT_GELU:
-            return body(std::integral_constant<int, ZCGVS_ACT_GELU>{});
-        case ZCGVS_ACT_GELU_TANH:
-            return body(std::integral_constant<int, ZCGVS_ACT_GELU_TANH>{});
-        default:
-            return body(std::integral_constant<int, ZCGVS_ACT_SILU>{});
-    }
 }
 
 template <typename T, bool kGradient>
@@ -513,23 +431,6 @@ std::size_t weightPartials(const zcgvs_gated_desc& d) {
     const int splits = std::max(weightPlan(d, false).splits, weightPlan(d, true).splits);
     const std::size_t values = 2 * static_cast<std::size_t>(d.hidden) * static_cast<std::size_t>(d.dim);
     return splits > 1 ? static_cast<std::size_t>(splits) * values : 0;
-}
-
-template <typename T>
-int launchJoin(const float* partials, int splits, std::int64_t rows, int columns, std::int64_t rows_first, void* first,
-               void* second, std::int64_t stride, hipStream_t stream) {
-    const bool four = columns >= 4;
-    const long long packs = static_cast<long long>(rows) * (four ? (columns + 3) / 4 : columns);
-    const unsigned blocks = static_cast<unsigned>(std::min(8192ll, (packs + kJoinThreads - 1) / kJoinThreads));
-    if (four) {
-        joinKernel<T, 4><<<blocks, kJoinThreads, 0, stream>>>(partials, splits, rows, columns, rows_first,
-                                                              static_cast<T*>(first), static_cast<T*>(second), stride);
-    } else {
-        joinKernel<T, 1><<<blocks, kJoinThreads, 0, stream>>>(partials, splits, rows, columns, rows_first,
-                                                              static_cast<T*>(first), static_cast<T*>(second), stride);
-    }
-    ZCGVS_LAUNCH_CHECK("gated gradient");
-    return ZCGVS_OK;
 }
 
 // The splits of a plan: whole stages each, which may leave fewer than planned.

@@ -11,6 +11,14 @@
 #include "matrix_tile.hpp"
 
 namespace zcgvs_hip {
+
+enum class TileShape { k256x256, k256x192, k128x128, k64x64 };
+
+struct ProductPlan {
+    TileShape shape;
+    int splits;
+};
+
 namespace {
 
 // a launch has less than 2^32 threads, of up to 1024 a block
@@ -25,8 +33,6 @@ inline bool directRows(const void* base, std::int64_t stride, int length, int dt
     return alignedRows(base, stride, dtype, 16) && static_cast<std::int64_t>(length) * elementBytes(dtype) % 16 == 0;
 }
 
-enum class TileShape { k256x256, k256x192, k128x128, k64x64 };
-
 // The largest tile a kernel is built with: those of 256 rows have 16 wavefronts of 128 registers.
 enum class LargestTile { k256x256, k256x192, k128x128 };
 
@@ -34,11 +40,6 @@ enum class LargestTile { k256x256, k256x192, k128x128 };
 // planned for the tiles they take. (Gradient of 16,384 rows 767 -> 2047 bfloat16 825 us, 870 us with the splits of the
 // larger tiles; rows of 768 and 2048 356 us. The stage times are those of whole chunks.)
 inline LargestTile largestTile(LargestTile largest, bool direct) { return direct ? largest : LargestTile::k128x128; }
-
-struct ProductPlan {
-    TileShape shape;
-    int splits;
-};
 
 // Values of k of a stage, of every type.
 constexpr int kPlanStageK = 64;

@@ -1,6 +1,6 @@
 // Tiled matrix products on the matrix cores for the embedding-model operators.
 //
-// A workgroup forms a kM x kN tile of C[m, n] = sum_k A[m, k] B[n, k] in float32 accumulators. Each side
+// A workgroup forms a kM x kN tile of C[m, n] = sum_k A[m, k] B[n, k] in float32 accumulators (int8: int32). Each side
 // comes in one of two layouts: rows whose k are neighbours ("plain": the activations and weights of
 // a forward product), or k-rows whose m (or n) are neighbours ("turned": what the gradients contract).
 // A stage is 128 bytes of k a row (64 16-bit values); two stages are in LDS, one being read by the matrix
@@ -13,7 +13,7 @@
 // of 32 bytes whose place is exchanged by the k-row's number, read by ds_read_b64_tr_b16, which hands lane i
 // of 16 the column i of four k-rows.
 //
-// Matrix instructions. 16-bit: v_mfma_f32_16x16x32, float32: v_mfma_f32_16x16x4. The first operand
+// Matrix instructions. 16-bit: v_mfma_f32_16x16x32, float32: v_mfma_f32_16x16x4, int8: v_mfma_i32_16x16x64. The first operand
 // holds B's rows and the second A's, so that lane l of a 16 x 16 result has the four neighbouring columns
 // n = 4 (l / 16) + e of row m = l % 16 and can store them together. Lane group h = l / 16 holds the
 // 16 bytes of chunk 4 t + h in step t, on both sides: every k meets itself whatever the order.
@@ -34,6 +34,7 @@
 namespace zcgvs_hip {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStageBytes = 128;  // of k in a plain side's row
@@ -54,6 +55,9 @@ __device__ __forceinline__ f32x4 multiplyAdd(Fragment<_Float16>::type b, Fragmen
 }
 __device__ __forceinline__ f32x4 multiplyAdd(Fragment<__bf16>::type b, Fragment<__bf16>::type a, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
+}
+__device__ __forceinline__ i32x4 multiplyAdd(Fragment<std::int8_t>::type b, Fragment<std::int8_t>::type a, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, b), __builtin_bit_cast(i32x4, a), c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 multiplyAdd(Fragment<float>::type b, Fragment<float>::type a, f32x4 c) {
 #pragma unroll
@@ -268,7 +272,8 @@ struct MatrixTile {
     static constexpr int kStageLds = SideA::kBytes + SideB::kBytes;
     static constexpr int kLdsBytes = 2 * kStageLds;
 
-    using Sums = f32x4[kBlocksM][kBlocksN];
+    using Sum = std::conditional_t<std::is_same_v<T, std::int8_t>, i32x4, f32x4>;
+    using Sums = Sum[kBlocksM][kBlocksN];
 
     static __device__ __forceinline__ int waveId() {
         return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -281,7 +286,7 @@ struct MatrixTile {
         for (int i = 0; i < kBlocksM; ++i) {
 #pragma unroll
             for (int j = 0; j < kBlocksN; ++j) {
-                sums[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                sums[i][j] = Sum{};
             }
         }
     }

@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "column_sums.hpp"
 #include "common.hpp"
 #include "elements.hpp"
 #include "matrix_plan.hpp"
@@ -349,35 +350,6 @@ __global__ __launch_bounds__(kNormThreads) void residualNormGradientKernel(NormA
     }
 }
 
-// out[c] = the sum over `count` rows of partials [count, dim], kJoinLanes threads a column in a fixed order.
-constexpr int kJoinColumns = 16;
-constexpr int kJoinLanes = kNormThreads / kJoinColumns;
-
-template <typename T>
-__global__ __launch_bounds__(kNormThreads) void joinColumnsKernel(const float* __restrict__ partials, int count, int dim,
-                                                                  T* __restrict__ out) {
-    __shared__ float shared[kJoinLanes][kJoinColumns];
-    const int column = static_cast<int>(threadIdx.x) % kJoinColumns;
-    const int part = static_cast<int>(threadIdx.x) / kJoinColumns;
-    const int c = static_cast<int>(blockIdx.x) * kJoinColumns + column;
-    float sum = 0.0f;
-    if (c < dim) {
-#pragma unroll 8
-        for (int r = part; r < count; r += kJoinLanes) {
-            sum += partials[static_cast<long long>(r) * dim + c];
-        }
-    }
-    shared[part][column] = sum;
-    __syncthreads();
-    if (part == 0 && c < dim) {
-#pragma unroll
-        for (int p = 1; p < kJoinLanes; ++p) {
-            sum += shared[p][column];
-        }
-        out[c] = static_cast<T>(sum);
-    }
-}
-
 // ---- host ---------------------------------------------------------------------------------------
 
 int invalid(const char* message) {
@@ -579,9 +551,7 @@ int zcgvs_residual_norm_gradient(const zcgvs_norm_desc* desc, const void* d_out_
             }
         }
         if (d_weight_gradient != nullptr) {
-            joinColumnsKernel<T><<<static_cast<unsigned>(divideUp(d.dim, kJoinColumns)), kNormThreads, 0, toStream(stream)>>>(
-                more.partials, blocks, d.dim, static_cast<T*>(d_weight_gradient));
-            ZCGVS_LAUNCH_CHECK("residual norm gradient");
+            return launchJoinColumns<T>(more.partials, d.rows > 0 ? blocks : 0, d.dim, d_weight_gradient, toStream(stream));
         }
         return static_cast<int>(ZCGVS_OK);
     });
