@@ -121,17 +121,32 @@ bool directOperands(const zcgvs_linear_desc& d) {
            directRows(d.weight, rowStride(d.weight_stride, d.dim), d.dim, d.dtype);
 }
 
-// Rows up to which the wavefronts of a workgroup split k.
-constexpr int kThinRows = 64;
+// The time of the kernel for few rows: each of its workgroups takes 16 columns and 16 or 32 rows, and stage after stage of
+// 1024 bytes of k. A stage costs a CU c us for each of its workgroups, and the call 4 us. Measured, 16-bit 4096 -> 1024:
+// 64 rows 9.9 us (32 at a time 13.3, 64 x 64 tiles 32.7), 128 rows 17.4 (13.5, 32.8), 512 rows 58 (44, 33.2); 1024 -> 4096:
+// 64 rows 9.4 (7.9, 8.6), 256 rows 33 (26, 11.2); float32 4096 -> 1024, 64 rows 17.7 (24.1, 94), int8 8.8 (11.1, 15.3).
+double thinTime(const zcgvs_linear_desc& d, int row_blocks) {
+    const int values = kThinStageBytes / elementBytes(d.dtype);
+    const double each = d.dtype == ZCGVS_DTYPE_I8 ? (row_blocks == 1 ? 1.5 : 2.4) : (row_blocks == 1 ? 0.9 : 1.35);
+    const double groups = static_cast<double>(divideUp(d.out_dim, 16)) * divideUp(d.rows, 16 * row_blocks);
+    return 4.0 + divideUp(d.dim, values) * std::max(1.0, groups / deviceComputeUnits()) * each;
+}
 
 LinearPlan planLinear(const zcgvs_linear_desc& d, bool direct, bool gradient) {
-    // the error function's terms do not fit the registers beside the sums of 256 x 256
-    const LargestTile largest = d.activation == ZCGVS_ACT_GELU ? LargestTile::k256x192 : LargestTile::k256x256;
+    // What the results need beside the sums of 256 x 256 does not fit the registers of the forward kernel (8192 rows
+    // 1024 -> 4096 bfloat16 95 us, 87 with 256 x 192; int8 149 and 63), nor the error function's terms those of dz
+    // (16,384 rows 768 -> 2048, GELU by tanh: 228 us, 236 with 256 x 192).
+    const LargestTile largest = !gradient || d.activation == ZCGVS_ACT_GELU ? LargestTile::k256x192 : LargestTile::k256x256;
     // int8 stages hold twice the values and take the time of 16-bit ones
     const bool codes = d.dtype == ZCGVS_DTYPE_I8;
     const ProductPlan product = planProduct(d.rows, d.out_dim, codes ? (d.dim + 1) / 2 : d.dim, 1,
                                             codes ? static_cast<int>(ZCGVS_DTYPE_F16) : d.dtype, 0, largestTile(largest, direct));
-    return {product, !gradient && d.rows <= kThinRows, direct};
+    int thin = 0;
+    if (!gradient && d.rows <= kThinMostRows) {
+        const int row_blocks = thinTime(d, 1) <= thinTime(d, 2) ? 1 : 2;
+        thin = thinTime(d, row_blocks) < product.us ? row_blocks : 0;
+    }
+    return {product, thin, direct};
 }
 
 LinearArgs linearArgs(const zcgvs_linear_desc& d) {

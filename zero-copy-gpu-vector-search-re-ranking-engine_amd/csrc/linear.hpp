@@ -56,10 +56,13 @@ struct ProductArgs {
     std::int64_t out_stride;
 };
 
+constexpr int kThinStageBytes = 1024;  // of k that a workgroup of the kernel for few rows takes at a time
+constexpr int kThinMostRows = 4096;
+
 // How linear.hip runs a call.
 struct LinearPlan {
     ProductPlan product;
-    bool thin;    // few rows: the wavefronts of a workgroup split k
+    int thin;     // few rows: blocks of 16 of them that a workgroup takes, its wavefronts splitting k; 0: tiles
     bool direct;  // rows of whole aligned chunks
 };
 

@@ -7,7 +7,7 @@
 // tile's sums in registers, so each output is written once and nothing else is. The next tile's first stage is on
 // its way while a tile's results are formed.
 //
-// Few rows (linearThinKernel) are bound by latency and by reading W once: a workgroup takes 16 columns and up to 64
+// Few rows (linearThinKernel) are bound by latency and by reading W once: a workgroup takes 16 columns and 16 or 32
 // rows, its eight wavefronts every eighth 128 bytes of k, straight from memory into registers, and joins their sums
 // through LDS. No LDS stages, no splits over workgroups, one launch.
 #pragma once
@@ -43,6 +43,39 @@ __device__ __forceinline__ f32x4 loadEpilogue(const LinearArgs& args, const void
         return loadFour(static_cast<const T*>(base) + index, left);
     }
 }
+
+// The same as they are stored, until their values are wanted (int8 operands: the values).
+template <typename T>
+struct HeldFour {
+    static constexpr bool kValues = std::is_same_v<T, std::int8_t>;
+    using Stored = std::conditional_t<kValues, f32x4, typename Pack<T, 4>::type>;
+    Stored stored = {};
+
+    __device__ __forceinline__ void load(const LinearArgs& args, const void* base, std::int64_t index, int left) {
+        if constexpr (kValues) {
+            stored = loadEpilogue<T>(args, base, index, left);
+        } else {
+            const T* from = static_cast<const T*>(base) + index;
+            if (left >= 4) {
+                stored = *reinterpret_cast<const typename Pack<T, 4>::stored*>(from);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (e < left) {
+                        stored[e] = from[e];
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ f32x4 values() const {
+        if constexpr (kValues) {
+            return stored;
+        } else {
+            return __builtin_convertvector(stored, f32x4);
+        }
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void storeResult(const LinearArgs& args, const f32x4& value, std::int64_t index, int left) {
@@ -83,7 +116,6 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
     const T* weight = static_cast<const T*>(args.weight);
     const int total = args.tiles_m * args.tiles_n;
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-    constexpr f32x4 kZeros = {0.0f, 0.0f, 0.0f, 0.0f};
     typename Tile::Loads loads;
     auto begin = [&](int index) {
         int tile_m, tile_n;
@@ -108,44 +140,54 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
         tileOf(index, args.tiles_m, args.tiles_n, tile_m, tile_n);
         const int m0 = tile_m * Tile::kM + Tile::waveM() * Tile::kBlocksM * 16 + (lane & 15);
         const int n0 = tile_n * Tile::kN + Tile::waveN() * Tile::kBlocksN * 16 + 4 * (lane >> 4);
-        f32x4 bias[Tile::kBlocksN], scales[Tile::kBlocksN];
-#pragma unroll
-        for (int j = 0; j < Tile::kBlocksN; ++j) {
-            const int n = n0 + j * 16;
-            bias[j] = kZeros;
-            scales[j] = kZeros;
-            if (args.bias != nullptr && n < args.out_dim) {
-                bias[j] = loadEpilogue<T>(args, args.bias, n, args.out_dim - n);
-            }
-            if (std::is_same_v<T, std::int8_t> && n < args.out_dim) {
-                scales[j] = loadFour(args.weight_scales + n, args.out_dim - n);
-            }
-        }
-        f32x4 result[Tile::kBlocksM][Tile::kBlocksN];
+        // What a column block needs beside its sums is held as it is stored, that of the next one on its way where
+        // the registers allow. Results take the place of their sums; the barriers keep the compiler from taking
+        // several blocks at once, for which 256 x 256 tiles have no registers (up to 365 were spilled without them).
+        constexpr int kHeld = Tile::kBlocksM * Tile::kBlocksN >= 16 || std::is_same_v<T, std::int8_t> ? 1 : 2;
+        HeldFour<T> bias[kHeld], from[kHeld][Tile::kBlocksM];
+        f32x4 scales = {0.0f, 0.0f, 0.0f, 0.0f};
+        float x_scales[Tile::kBlocksM];
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i) {
-            const int m = m0 + i * 16;
-            float x_scale = 1.0f;
-            if constexpr (std::is_same_v<T, std::int8_t>) {
-                x_scale = args.x_scales[min(m, args.rows - 1)];
+            x_scales[i] = std::is_same_v<T, std::int8_t> ? args.x_scales[min(m0 + i * 16, args.rows - 1)] : 1.0f;
+        }
+        const void* base = kGradient ? args.out_gradient : args.residual;
+        const std::int64_t stride = kGradient ? args.out_gradient_stride : args.residual_stride;
+        auto hold = [&](int j) {
+            const int n = n0 + j * 16;
+            const int left = args.out_dim - n;
+            bias[j % kHeld] = HeldFour<T>{};
+            if (args.bias != nullptr && left > 0) {
+                bias[j % kHeld].load(args, args.bias, n, left);
             }
-            f32x4 from[Tile::kBlocksN];
+            if (std::is_same_v<T, std::int8_t> && left > 0) {
+                scales = loadFour(args.weight_scales + n, left);
+            }
 #pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                const int n = n0 + j * 16;
-                from[j] = kZeros;
-                if (m < args.rows && n < args.out_dim) {
-                    if constexpr (kGradient) {
-                        from[j] = loadFour(static_cast<const T*>(args.out_gradient) + m * args.out_gradient_stride + n,
-                                           args.out_dim - n);
-                    } else if (args.residual != nullptr) {
-                        from[j] = loadEpilogue<T>(args, args.residual, m * args.residual_stride + n, args.out_dim - n);
-                    }
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+                const int m = m0 + i * 16;
+                from[j % kHeld][i] = HeldFour<T>{};
+                if (base != nullptr && m < args.rows && left > 0) {
+                    from[j % kHeld][i].load(args, base, m * stride + n, left);
                 }
             }
+        };
+        if constexpr (kHeld > 1) {
+            hold(0);
+        }
 #pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                const f32x4 z = beforeActivation<T>(sums[i][j], x_scale, scales[j], bias[j]);
+        for (int j = 0; j < Tile::kBlocksN; ++j) {
+            if constexpr (kHeld == 1) {
+                hold(j);
+            } else if (j + 1 < Tile::kBlocksN) {
+                hold(j + 1);
+            }
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i) {
+                const int m = m0 + i * 16;
+                const f32x4 z = beforeActivation<T>(sums[i][j], x_scales[i], scales, bias[j % kHeld].values());
+                const f32x4 more = from[j % kHeld][i].values();
+                f32x4 result;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (kGradient) {
@@ -153,11 +195,13 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
                         activateBoth<kActivation>(z[e], value, slope);
                         // rows and columns past the ends are zeros whatever stands in for their operands
                         const bool inside = m < args.rows && n0 + j * 16 + e < args.out_dim;
-                        result[i][j][e] = inside ? from[j][e] * slope : 0.0f;
+                        result[e] = inside ? more[e] * slope : 0.0f;
                     } else {
-                        result[i][j][e] = activate<kActivation>(z[e]) + from[j][e];
+                        result[e] = activate<kActivation>(z[e]) + more[e];
                     }
                 }
+                sums[i][j] = __builtin_bit_cast(typename Tile::Sum, result);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         loads.land();
@@ -167,12 +211,13 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
 #pragma unroll
             for (int j = 0; j < Tile::kBlocksN; ++j) {
                 const int n = n0 + j * 16;
+                const f32x4 result = __builtin_bit_cast(f32x4, sums[i][j]);
                 if constexpr (kGradient) {
                     if (m < args.rows && n < args.out_stride) {
-                        storeFour(result[i][j], static_cast<T*>(args.out) + m * args.out_stride + n, 4);
+                        storeFour(result, static_cast<T*>(args.out) + m * args.out_stride + n, 4);
                     }
                 } else if (m < args.rows && n < args.out_dim) {
-                    storeResult<T>(args, result[i][j], m * args.out_stride + n, args.out_dim - n);
+                    storeResult<T>(args, result, m * args.out_stride + n, args.out_dim - n);
                 }
             }
         }
@@ -182,10 +227,10 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
                             (static_cast<std::int64_t>(tile_m) * Tile::kWavesM + Tile::waveM()) * args.out_dim;
 #pragma unroll
                 for (int j = 0; j < Tile::kBlocksN; ++j) {
-                    f32x4 sum = result[0][j];
+                    f32x4 sum = __builtin_bit_cast(f32x4, sums[0][j]);
 #pragma unroll
                     for (int i = 1; i < Tile::kBlocksM; ++i) {
-                        sum += result[i][j];
+                        sum += __builtin_bit_cast(f32x4, sums[i][j]);
                     }
 #pragma unroll
                     for (int offset = 1; offset < 16; offset *= 2) {
@@ -208,6 +253,7 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
 
 constexpr int kThinWaves = 8;
 constexpr int kThinThreads = kThinWaves * kWave;
+static_assert(kThinStageBytes == kThinWaves * kStageBytes, "a stage is 128 bytes of k for each wavefront");
 
 // A row's chunk of 16 bytes at value k, of which `left` values exist; zeros past them.
 template <typename T>
@@ -390,16 +436,11 @@ __global__ __launch_bounds__(InputTile::kThreads) void bothProductsKernel(Produc
 
 // ---- host ---------------------------------------------------------------------------------------
 
-// The tiles of a plan for the projection itself; the error function's terms do not fit the registers beside the sums of
-// 256 x 256, which linear.hip does not plan for it.
-template <typename T, typename Body>
-int withLinearTile(const LinearPlan& plan, Body&& body) {
-    return withTile<T, false, false, LargestTile::k256x256, false>(plan.product.shape, plan.direct, body);
-}
-
 template <typename T, bool kGradient>
 int launchTiles(const LinearPlan& plan, int activation, LinearArgs args, hipStream_t stream) {
-    return withLinearTile<T>(plan, [&](auto tile) {
+    // (the sizes that linear.hip plans for)
+    constexpr LargestTile kLargest = kGradient ? LargestTile::k256x256 : LargestTile::k256x192;
+    return withTile<T, false, false, kLargest, false>(plan.product.shape, plan.direct, [&](auto tile) {
         using Tile = decltype(tile);
         args.tiles_m = divideUp(args.rows, Tile::kM);
         args.tiles_n = divideUp(args.out_dim, Tile::kN);
@@ -429,7 +470,7 @@ int launchTiles(const LinearPlan& plan, int activation, LinearArgs args, hipStre
 }
 
 template <typename T>
-int launchThin(int activation, const LinearArgs& args, hipStream_t stream) {
+int launchThin(int row_blocks, int activation, const LinearArgs& args, hipStream_t stream) {
     const auto with = [&](auto blocks_m) {
         constexpr int kBlocksM = decltype(blocks_m)::value;
         const dim3 grid(static_cast<unsigned>(divideUp(args.out_dim, 16)),
@@ -442,10 +483,7 @@ int launchThin(int activation, const LinearArgs& args, hipStream_t stream) {
         return activation == ZCGVS_ACT_NONE ? launch(std::integral_constant<int, ZCGVS_ACT_NONE>{})
                                             : withActivation(activation, launch);
     };
-    if (args.rows <= 16) {
-        return with(std::integral_constant<int, 1>{});
-    }
-    return args.rows <= 32 ? with(std::integral_constant<int, 2>{}) : with(std::integral_constant<int, 4>{});
+    return row_blocks == 1 ? with(std::integral_constant<int, 1>{}) : with(std::integral_constant<int, 2>{});
 }
 
 template <typename T, bool kTurnedA>
@@ -493,7 +531,7 @@ int joinSplits(const ProductArgs& args, hipStream_t stream) {
 
 template <typename T>
 int launchLinear(const LinearPlan& plan, int activation, LinearArgs args, hipStream_t stream) {
-    return plan.thin ? launchThin<T>(activation, args, stream) : launchTiles<T, false>(plan, activation, args, stream);
+    return plan.thin > 0 ? launchThin<T>(plan.thin, activation, args, stream) : launchTiles<T, false>(plan, activation, args, stream);
 }
 
 template <typename T>

@@ -17,6 +17,7 @@ enum class TileShape { k256x256, k256x192, k128x128, k64x64 };
 struct ProductPlan {
     TileShape shape;
     int splits;
+    double us;  // the time it is planned for
 };
 
 namespace {
@@ -74,8 +75,7 @@ inline ProductPlan planProduct(std::int64_t m, std::int64_t n, std::int64_t k, i
     const int shape_count = wide ? 2 : 4;
     const std::int64_t stages = (k + kPlanStageK - 1) / kPlanStageK;
     const std::int64_t units = deviceComputeUnits();
-    ProductPlan best{TileShape::k64x64, 1};
-    double best_us = 0.0;
+    ProductPlan best{TileShape::k64x64, 1, 0.0};
     for (int i = 0; i < shape_count; ++i) {
         const Shape& s = shapes[i];
         if ((s.m > 128 && largest == LargestTile::k128x128) || (s.n > 192 && largest != LargestTile::k256x256)) {
@@ -96,9 +96,8 @@ inline ProductPlan planProduct(std::int64_t m, std::int64_t n, std::int64_t k, i
             if (splits > 1) {
                 us += 4.0 + 8.0 * static_cast<double>(count) * static_cast<double>(m) * static_cast<double>(n) * splits / 4.5e6;
             }
-            if (best_us == 0.0 || us < best_us) {
-                best_us = us;
-                best = {s.shape, splits};
+            if (best.us == 0.0 || us < best.us) {
+                best = {s.shape, splits, us};
             }
         }
     }

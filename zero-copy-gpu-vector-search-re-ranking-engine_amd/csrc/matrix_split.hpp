@@ -136,7 +136,8 @@ struct SplitTile {
     using SideA = SplitLoader<kM, kTurnedA, kThreads>;
     using SideB = SplitLoader<kN, kTurnedB, kThreads>;
     static constexpr int kLdsBytes = SideA::kBytes + SideB::kBytes;
-    using Sums = f32x4[kBlocksM][kBlocksN];
+    using Sum = f32x4;
+    using Sums = Sum[kBlocksM][kBlocksN];
 
     static __device__ __forceinline__ int waveM() { return StageTile::waveM(); }
     static __device__ __forceinline__ int waveN() { return StageTile::waveN(); }
