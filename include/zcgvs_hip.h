@@ -647,6 +647,64 @@ int zcgvs_linear_gradient(const zcgvs_linear_desc* desc, const void* d_out_gradi
                           int64_t weight_gradient_stride, void* d_bias_gradient, void* d_workspace,
                           size_t workspace_bytes, zcgvs_stream_t stream);
 
+/* Where the query rows of a text stand among its keys: from the first one on, or so that the last one
+ * stands at the last key. */
+enum zcgvs_attention_align { ZCGVS_ATTENTION_FIRST = 0, ZCGVS_ATTENTION_LAST = 1 };
+
+/* Attention within each text of a batch. Query row i of text t stands at position p = i (or
+ * p = key_count - query_count + i), key j of the text at position j; with head h of the query and key head
+ * h / (heads / kv_heads):
+ *     c = scale * q_i . k_j,  with cap > 0: c = cap * tanh(c / cap)
+ *     s_j = c - slopes[h] * |j - p| + distance_bias[h][clamp(j - p, -max_distance, max_distance) + max_distance]
+ *     out_i = sum_j softmax(s)_j v_j   over the keys that i sees.
+ * A query row sees the keys of its own text; with `causal` those at j <= p and, where prefix_lengths is
+ * given, those at j < prefix_lengths[t] as well. A row that sees no key gives zeros.
+ * The rows of text t are q_offsets[t] .. q_offsets[t + 1] - 1 (offsets ascend and lie in [0, q_rows]), or
+ * with q_offsets NULL t * (q_rows / texts) on (q_rows a multiple of texts): one query row a text, or a padded
+ * batch. Of these the first q_lengths[t] count (clamped to [0, the text's rows]; NULL: all); the rest are padding:
+ * their output rows are zeros, and so are the gradients of padding rows. Rows of no text (before the first
+ * offset, behind the last) are neither read nor written. Likewise for the keys.
+ * Padding rows, rows of no text and other texts may hold anything, infinities and NaN included. A key of the
+ * row's own text that only the causal mask hides must be finite, as must the queries that do not see a key
+ * for that key's gradient. */
+typedef struct zcgvs_attention_desc {
+    const void* q;             /* [q_rows, heads, head_dim]                                     */
+    int64_t q_stride;          /* elements from row to row; 0: heads * head_dim                 */
+    const void* k;             /* [k_rows, kv_heads, head_dim]                                  */
+    int64_t k_stride;          /* 0: kv_heads * head_dim                                        */
+    const void* v;             /* [k_rows, kv_heads, head_dim]                                  */
+    int64_t v_stride;          /* 0: kv_heads * head_dim                                        */
+    int64_t q_rows;            /* at most 2^28                                                  */
+    int64_t k_rows;            /* at most 2^28                                                  */
+    int64_t texts;             /* at most 2^24                                                  */
+    const int64_t* q_offsets;  /* [texts + 1], or NULL                                          */
+    const int64_t* k_offsets;  /* [texts + 1], or NULL                                          */
+    const int* q_lengths;      /* [texts], or NULL                                              */
+    const int* k_lengths;      /* [texts], or NULL                                              */
+    int heads;                 /* a multiple of kv_heads, at most 1024                          */
+    int kv_heads;
+    int head_dim;              /* at most zcgvs_attention_max_head_dim()                        */
+    int dtype;                 /* of q, k, v and distance_bias                                  */
+    int q_align;               /* enum zcgvs_attention_align                                    */
+    int causal;
+    const int* prefix_lengths; /* [texts] (causal), or NULL                                     */
+    float scale;               /* finite                                                        */
+    float cap;                 /* 0: none                                                       */
+    const float* slopes;       /* [heads], or NULL: none                                        */
+    const void* distance_bias; /* [heads, 2 * max_distance + 1], or NULL: none                  */
+    int max_distance;          /* at most zcgvs_attention_max_distance()                        */
+} zcgvs_attention_desc;
+
+int zcgvs_attention_max_head_dim(void); /* 128 */
+int zcgvs_attention_max_distance(void); /* 512 */
+/* d_out [q_rows, heads, head_dim] of desc->dtype (out_stride 0: heads * head_dim). d_lse, NULL or
+ * [q_rows, heads] float32, takes each row's logarithm of the sum of exponentials of s (minus infinity where
+ * it sees no key), which the gradient needs. With 16-bit operands the softmax's exponentials are rounded to
+ * that type for the product with v; their sum is that of the unrounded ones. */
+size_t zcgvs_attention_workspace_bytes(const zcgvs_attention_desc* desc);
+int zcgvs_attention(const zcgvs_attention_desc* desc, void* d_out, int64_t out_stride, float* d_lse,
+                    void* d_workspace, size_t workspace_bytes, zcgvs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

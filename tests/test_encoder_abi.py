@@ -133,8 +133,71 @@ def test_linear_operands(capi):
         capi.linear_gradient(_linear(capi), A, A, A, A, A + 8, need)
 
 
+def _attention(capi, **kw):
+    args = dict(q=A, k=A, v=A, texts=2, q_rows=6, k_rows=6, heads=4, head_dim=8, dtype=capi.F32, kv_heads=2)
+    return capi.attention_desc(**dict(args, **kw))
+
+
+ATTENTION_REFUSALS = [
+    (dict(dtype=2), "float32, float16 or bfloat16"),
+    (dict(heads=0), "multiple of kv_heads"),
+    (dict(heads=5), "multiple of kv_heads"),
+    (dict(heads=1026), "multiple of kv_heads"),
+    (dict(kv_heads=-1), "multiple of kv_heads"),
+    (dict(head_dim=0), "head_dim must lie"),
+    (dict(head_dim=129), "head_dim must lie"),
+    (dict(q_rows=-2), "must lie in \\[0, 2\\^28\\]"),
+    (dict(k_rows=2**28 + 2), "must lie in \\[0, 2\\^28\\]"),
+    (dict(texts=-1), "texts must lie"),
+    (dict(texts=2**24 + 1, q_offsets=A, k_offsets=A), "texts must lie"),
+    (dict(q_rows=7), "multiple of texts"),
+    (dict(k_rows=7), "multiple of texts"),
+    (dict(q_stride=31), "smaller than its heads"),
+    (dict(k_stride=15), "smaller than its heads"),
+    (dict(v_stride=15), "smaller than its heads"),
+    (dict(q_align=2), "unknown alignment"),
+    (dict(prefix_lengths=A), "need the causal mask"),
+    (dict(scale=NAN), "must be finite"),
+    (dict(scale=INF), "must be finite"),
+    (dict(cap=-1.0), "cap at least 0"),
+    (dict(cap=NAN), "must be finite"),
+    (dict(distance_bias=A, max_distance=-1), "max_distance must lie"),
+    (dict(distance_bias=A, max_distance=513), "max_distance must lie"),
+    (dict(q=None), "null device pointer"),
+    (dict(k=None), "null device pointer"),
+    (dict(v=None), "null device pointer"),
+]
+
+
+@pytest.mark.parametrize("kw,match", ATTENTION_REFUSALS)
+def test_attention_descriptor(capi, kw, match):
+    with pytest.raises(ValueError, match=match):
+        capi.attention_workspace_bytes(_attention(capi, **kw))
+    with pytest.raises(ValueError, match=match):
+        capi.attention(_attention(capi, **kw), A, A, 1 << 30)
+
+
+def test_attention_operands(capi):
+    assert capi.library().zcgvs_attention_max_head_dim() == 128
+    assert capi.library().zcgvs_attention_max_distance() == 512
+    with pytest.raises(ValueError, match="smaller than its heads"):
+        capi.attention(_attention(capi), A, A, 1 << 30, out_stride=31)
+    with pytest.raises(ValueError, match="null device pointer"):
+        capi.attention(_attention(capi), None, A, 1 << 30)
+    long = _attention(capi, q_rows=2, k_rows=100_000)  # split keys
+    need = capi.attention_workspace_bytes(long)
+    assert need > 256
+    with pytest.raises(ValueError, match="too small"):
+        capi.attention(long, A, A, need - 1)
+    with pytest.raises(ValueError, match="too small"):
+        capi.attention(long, A, None, need)
+    with pytest.raises(ValueError, match="16 bytes"):
+        capi.attention(long, A, A + 4, need)
+
+
 def test_null_descriptors(capi):
     lib = capi.library()
+    assert lib.zcgvs_attention(None, A, 0, None, A, 0, None) == capi.ERR_INVALID_ARGUMENT
     assert lib.zcgvs_linear(None, A, 0, capi.F32, None) == capi.ERR_INVALID_ARGUMENT
     assert lib.zcgvs_linear_gradient_workspace_bytes(None) == 0 and "null descriptor" in capi.last_error()
     assert lib.zcgvs_residual_norm(None, A, 0, capi.F32, None, None, 0, None) == capi.ERR_INVALID_ARGUMENT
@@ -148,3 +211,5 @@ def test_empty_work_returns_ok(capi):
     capi.linear(_linear(capi, rows=0, x=None, weight=None), None, capi.F32)
     capi.linear_gradient(_linear(capi), None, None, None, None, None, 0)  # no gradient is wanted
     capi.linear_gradient(_linear(capi, rows=0, x=None, weight=None), None, A, None, None, None, 0)
+    for kw in (dict(texts=0), dict(q_rows=0), dict(texts=0, q_rows=0, k_rows=0, q=None, k=None, v=None)):
+        capi.attention(_attention(capi, **kw), None, None, 0)

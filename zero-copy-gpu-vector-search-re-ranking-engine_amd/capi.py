@@ -22,6 +22,7 @@ F32, F16, I8, BINARY = 0, 1, 2, 3
 BF16 = 4  # the embedding-model operators only
 EMBEDDING_SUM, EMBEDDING_MEAN = 0, 1
 ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_NONE = 0, 1, 2, 3  # ACT_NONE: linear only
+ATTENTION_FIRST, ATTENTION_LAST = 0, 1
 INT8_REFERENCE, INT8_PER_VECTOR = 0, 1
 SEARCH_MATERIALIZE = 1
 SEARCH_UNSORTED_POSTINGS = 2
@@ -86,6 +87,14 @@ class LinearDesc(ctypes.Structure):
     _fields_ = [("x", _vp), ("x_stride", _i64), ("weight", _vp), ("weight_stride", _i64), ("rows", _i64), ("dim", _i32),
                 ("out_dim", _i32), ("dtype", _i32), ("activation", _i32), ("epilogue_dtype", _i32), ("x_scales", _vp),
                 ("weight_scales", _vp), ("bias", _vp), ("residual", _vp), ("residual_stride", _i64)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [("q", _vp), ("q_stride", _i64), ("k", _vp), ("k_stride", _i64), ("v", _vp), ("v_stride", _i64),
+                ("q_rows", _i64), ("k_rows", _i64), ("texts", _i64), ("q_offsets", _vp), ("k_offsets", _vp),
+                ("q_lengths", _vp), ("k_lengths", _vp), ("heads", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("dtype", _i32), ("q_align", _i32), ("causal", _i32), ("prefix_lengths", _vp), ("scale", _f32),
+                ("cap", _f32), ("slopes", _vp), ("distance_bias", _vp), ("max_distance", _i32)]
 
 
 # name -> (restype, argtypes)
@@ -171,6 +180,10 @@ _SIGNATURES = {
     "zcgvs_residual_norm_gradient": (_i32, [ctypes.POINTER(NormDesc), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
     "zcgvs_linear": (_i32, [ctypes.POINTER(LinearDesc), _vp, _i64, _i32, _vp]),
     "zcgvs_linear_gradient_workspace_bytes": (_sz, [ctypes.POINTER(LinearDesc)]),
+    "zcgvs_attention_max_head_dim": (_i32, []),
+    "zcgvs_attention_max_distance": (_i32, []),
+    "zcgvs_attention_workspace_bytes": (_sz, [ctypes.POINTER(AttentionDesc)]),
+    "zcgvs_attention": (_i32, [ctypes.POINTER(AttentionDesc), _vp, _i64, _vp, _vp, _sz, _vp]),
     "zcgvs_linear_gradient": (_i32, [ctypes.POINTER(LinearDesc), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
 }
 
@@ -711,3 +724,26 @@ def linear_gradient(desc: LinearDesc, out_gradient, x_gradient, weight_gradient,
     call("zcgvs_linear_gradient", ctypes.byref(desc), ptr(out_gradient), out_gradient_stride, ptr(x_gradient),
          x_gradient_stride, ptr(weight_gradient), weight_gradient_stride, ptr(bias_gradient), ptr(workspace),
          workspace_bytes, getattr(stream, "handle", stream))
+
+
+def attention_desc(q, k, v, texts, q_rows, k_rows, heads, head_dim, dtype, *, kv_heads=0, q_offsets=None, k_offsets=None,
+                   q_lengths=None, k_lengths=None, q_align=ATTENTION_FIRST, causal=False, prefix_lengths=None, scale=None,
+                   cap=0.0, slopes=None, distance_bias=None, max_distance=0, q_stride=0, k_stride=0,
+                   v_stride=0) -> AttentionDesc:
+    """kv_heads 0: as many as heads; scale None: 1 / sqrt(head_dim)."""
+    scale = max(head_dim, 1) ** -0.5 if scale is None else scale
+    return _keep_alive(AttentionDesc(ptr(q), q_stride, ptr(k), k_stride, ptr(v), v_stride, q_rows, k_rows, texts,
+                                     ptr(q_offsets), ptr(k_offsets), ptr(q_lengths), ptr(k_lengths), heads,
+                                     kv_heads or heads, head_dim, dtype, q_align, int(causal), ptr(prefix_lengths), scale,
+                                     cap, ptr(slopes), ptr(distance_bias), max_distance),
+                       q, k, v, q_offsets, k_offsets, q_lengths, k_lengths, prefix_lengths, slopes, distance_bias)
+
+
+def attention_workspace_bytes(desc: AttentionDesc) -> int:
+    return _workspace_bytes("zcgvs_attention_workspace_bytes", desc)
+
+
+def attention(desc: AttentionDesc, out, workspace, workspace_bytes, *, lse=None, out_stride=0, stream=None) -> None:
+    """Attention within each text; lse takes what attention_gradient needs of the softmax."""
+    call("zcgvs_attention", ctypes.byref(desc), ptr(out), out_stride, ptr(lse), ptr(workspace), workspace_bytes,
+         getattr(stream, "handle", stream))

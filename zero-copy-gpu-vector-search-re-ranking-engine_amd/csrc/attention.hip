@@ -1,0 +1,197 @@
+// Attention over packed texts: checks, plans and the launches' order. The kernels are in attention_kernel.hpp,
+// built for each operand type by a file of its own.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "attention.hpp"
+#include "common.hpp"
+#include "elements.hpp"
+#include "matrix_plan.hpp"
+
+namespace zcgvs_hip {
+
+int attentionInvalid(const char* message) {
+    return setError(ZCGVS_ERR_INVALID_ARGUMENT, std::string("zcgvs attention: ") + message);
+}
+
+namespace {
+
+constexpr int kNarrowTableFloats = 4096;  // of the heads' tables that the narrow shape holds in LDS
+
+int checkAttention(const zcgvs_attention_desc* desc) {
+    if (desc == nullptr) {
+        return attentionInvalid("null descriptor");
+    }
+    const zcgvs_attention_desc& d = *desc;
+    if (!validElement(d.dtype)) {
+        return attentionInvalid("the operands must hold float32, float16 or bfloat16");
+    }
+    if (d.heads <= 0 || d.heads > 1024 || d.kv_heads <= 0 || d.heads % d.kv_heads != 0) {
+        return attentionInvalid("heads must lie in [1, 1024] and be a multiple of kv_heads");
+    }
+    if (d.head_dim <= 0 || d.head_dim > kAttentionMaxDim) {
+        return attentionInvalid("head_dim must lie in [1, 128]");
+    }
+    if (d.q_rows < 0 || d.q_rows > (1 << 28) || d.k_rows < 0 || d.k_rows > (1 << 28)) {
+        return attentionInvalid("q_rows and k_rows must lie in [0, 2^28]");
+    }
+    if (d.texts < 0 || d.texts > (1 << 24)) {
+        return attentionInvalid("texts must lie in [0, 2^24]");
+    }
+    if (d.texts > 0 && ((d.q_offsets == nullptr && d.q_rows % d.texts != 0) || (d.k_offsets == nullptr && d.k_rows % d.texts != 0))) {
+        return attentionInvalid("rows without offsets must be a multiple of texts");
+    }
+    const int q_width = d.heads * d.head_dim;
+    const int k_width = d.kv_heads * d.head_dim;
+    if (rowStride(d.q_stride, q_width) < q_width || rowStride(d.k_stride, k_width) < k_width ||
+        rowStride(d.v_stride, k_width) < k_width) {
+        return attentionInvalid("a row stride is smaller than its heads");
+    }
+    if (d.q_align != ZCGVS_ATTENTION_FIRST && d.q_align != ZCGVS_ATTENTION_LAST) {
+        return attentionInvalid("unknown alignment of the queries");
+    }
+    if (d.prefix_lengths != nullptr && d.causal == 0) {
+        return attentionInvalid("prefix_lengths need the causal mask");
+    }
+    if (!std::isfinite(d.scale) || !std::isfinite(d.cap) || d.cap < 0.0f) {
+        return attentionInvalid("scale and cap must be finite, cap at least 0");
+    }
+    if (d.distance_bias != nullptr && (d.max_distance < 0 || d.max_distance > kAttentionMaxDistance)) {
+        return attentionInvalid("max_distance must lie in [0, 512]");
+    }
+    if (d.texts > 0 && d.q_rows > 0 && (d.q == nullptr || (d.k_rows > 0 && (d.k == nullptr || d.v == nullptr)))) {
+        return attentionInvalid("null device pointer");
+    }
+    return ZCGVS_OK;
+}
+
+bool noWork(const zcgvs_attention_desc& d) { return d.texts == 0 || d.q_rows == 0; }
+
+AttentionArgs attentionArgs(const zcgvs_attention_desc& d) {
+    AttentionArgs args{};
+    args.q = d.q;
+    args.k = d.k;
+    args.v = d.v;
+    args.q_stride = rowStride(d.q_stride, d.heads * d.head_dim);
+    args.k_stride = rowStride(d.k_stride, d.kv_heads * d.head_dim);
+    args.v_stride = rowStride(d.v_stride, d.kv_heads * d.head_dim);
+    const int texts = static_cast<int>(d.texts);
+    args.q_texts = {d.q_offsets, d.q_lengths, d.q_rows, texts, static_cast<int>(d.q_rows / d.texts)};
+    args.k_texts = {d.k_offsets, d.k_lengths, d.k_rows, texts, static_cast<int>(d.k_rows / d.texts)};
+    args.heads = d.heads;
+    args.group = d.heads / d.kv_heads;
+    args.head_dim = d.head_dim;
+    args.q_last = d.q_align == ZCGVS_ATTENTION_LAST ? 1 : 0;
+    args.causal = d.causal != 0 ? 1 : 0;
+    args.prefix = d.prefix_lengths;
+    args.scale = d.scale;
+    args.cap = d.cap;
+    args.slopes = d.slopes;
+    args.table = d.distance_bias;
+    args.max_distance = d.distance_bias == nullptr ? 0 : d.max_distance;
+    return args;
+}
+
+// Keys of a tile of the narrow shape.
+int narrowKeys(const zcgvs_attention_desc& d) {
+    const int bytes = paddedDim(d.head_dim) * elementBytes(d.dtype);
+    return bytes <= 64 ? 64 : bytes <= 128 || d.dtype != ZCGVS_DTYPE_F32 ? 32 : 16;
+}
+
+struct HostPlan {
+    AttentionShape shape;
+    int splits;
+};
+
+// By the mean rows and keys of a text: the narrow shape where a key head's query rows fit one workgroup's 16, or where the
+// others leave most CUs idle over long keys.
+HostPlan planAttention(const zcgvs_attention_desc& d) {
+    const long long units = deviceComputeUnits();
+    const int group = d.heads / d.kv_heads;
+    const double rows = static_cast<double>(d.q_rows) / static_cast<double>(d.texts);
+    const double keys = static_cast<double>(d.k_rows) / static_cast<double>(d.texts);
+    const double short_blocks = d.heads * (static_cast<double>(d.q_rows) / 64.0 + static_cast<double>(d.texts));
+    const long long table = d.distance_bias == nullptr ? 0 : 2ll * (d.max_distance + narrowKeys(d) + 16) + 1;
+    const bool fits = group * table <= kNarrowTableFloats && d.q_rows * group < (1ll << 30);
+    if (fits && (rows * group <= 16.0 || (short_blocks <= units / 2 && keys >= 512.0))) {
+        const double blocks = d.kv_heads * (static_cast<double>(d.q_rows) * group / 16.0 + static_cast<double>(d.texts));
+        // two workgroups a CU, and at least two tiles for each of a workgroup's wavefronts
+        const double most = keys / (8.0 * narrowKeys(d));
+        const double splits = std::min(2.0 * static_cast<double>(units) / blocks, most);
+        return {AttentionShape::kNarrow, std::max(1, std::min(128, static_cast<int>(splits)))};
+    }
+    return {rows <= 64.0 ? AttentionShape::kShort : AttentionShape::kLong, 1};
+}
+
+std::size_t partialFloats(const zcgvs_attention_desc& d, int splits, int each) {
+    return splits == 1 ? 0 : static_cast<std::size_t>(splits) * static_cast<std::size_t>(d.q_rows) * d.heads * each;
+}
+
+}  // namespace
+
+}  // namespace zcgvs_hip
+
+using namespace zcgvs_hip;
+
+extern "C" {
+
+int zcgvs_attention_max_head_dim(void) { return kAttentionMaxDim; }
+
+int zcgvs_attention_max_distance(void) { return kAttentionMaxDistance; }
+
+std::size_t zcgvs_attention_workspace_bytes(const zcgvs_attention_desc* desc) {
+    if (checkAttention(desc) != ZCGVS_OK) {
+        return 0;
+    }
+    clearError();
+    if (noWork(*desc)) {
+        return 256;
+    }
+    const int splits = planAttention(*desc).splits;
+    return std::max<std::size_t>(256, partialFloats(*desc, splits, paddedDim(desc->head_dim) + 2) * sizeof(float));
+}
+
+int zcgvs_attention(const zcgvs_attention_desc* desc, void* d_out, std::int64_t out_stride, float* d_lse,
+                    void* d_workspace, std::size_t workspace_bytes, zcgvs_stream_t stream) {
+    const int status = checkAttention(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_attention_desc& d = *desc;
+    const int width = d.heads * d.head_dim;
+    if (rowStride(out_stride, width) < width) {
+        return attentionInvalid("the output's row stride is smaller than its heads");
+    }
+    if (noWork(d)) {
+        return clearError();
+    }
+    if (d_out == nullptr) {
+        return attentionInvalid("null device pointer");
+    }
+    const HostPlan plan = planAttention(d);
+    const AttentionArgs args = attentionArgs(d);
+    AttentionOutput output{};
+    output.out = d_out;
+    output.out_stride = rowStride(out_stride, width);
+    output.lse = d_lse;
+    output.splits = plan.splits;
+    if (plan.splits > 1) {
+        if (d_workspace == nullptr || workspace_bytes < zcgvs_attention_workspace_bytes(desc)) {
+            return attentionInvalid("the workspace is too small");
+        }
+        if (!aligned16(d_workspace)) {
+            return attentionInvalid("the workspace must be aligned to 16 bytes");
+        }
+        output.partial_rows = static_cast<float*>(d_workspace);
+        output.partial_stats = output.partial_rows + partialFloats(d, plan.splits, paddedDim(d.head_dim));
+    }
+    const bool direct = directRows(d.k, args.k_stride, d.head_dim, d.dtype) && directRows(d.v, args.v_stride, d.head_dim, d.dtype);
+    const int launched = withElement(d.dtype, [&](auto element) {
+        return launchAttention<decltype(element)>({plan.shape, direct}, args, output, toStream(stream));
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+}  // extern "C"

@@ -1,0 +1,323 @@
+// What the attention's translation units share: arguments, the texts' rows, the tiles of keys in LDS.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.hpp"
+#include "elements.hpp"
+#include "lds_copy.hpp"
+#include "matrix_tile.hpp"
+
+namespace zcgvs_hip {
+
+constexpr int kAttentionMaxDim = 128;
+constexpr int kAttentionMaxDistance = 512;
+constexpr float kLog2E = 1.44269504f;
+constexpr float kLn2 = 0.69314718f;
+
+// Rows of a batch's texts: those of text t are offsets[t] .. offsets[t + 1] - 1 (null: `each` rows a text), the first
+// lengths[t] of them count (null: all).
+struct TextRows {
+    const std::int64_t* offsets;
+    const int* lengths;
+    std::int64_t total;
+    int texts;
+    int each;
+};
+
+struct AttentionArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    std::int64_t q_stride;
+    std::int64_t k_stride;
+    std::int64_t v_stride;
+    TextRows q_texts;
+    TextRows k_texts;
+    int heads;
+    int group;  // query heads to a key head
+    int head_dim;
+    int q_last;  // the query rows stand at the end of their text's keys
+    int causal;
+    const int* prefix;
+    float scale;
+    float cap;
+    const float* slopes;
+    const void* table;
+    int max_distance;
+};
+
+struct AttentionOutput {
+    void* out;
+    std::int64_t out_stride;
+    float* lse;
+    int slots;   // tiles of query rows, empty ones among them
+    int splits;  // parts of the keys, each with its own workgroups
+    float* partial_rows;   // [splits, q_rows * heads, padded head_dim] of unfinished rows (splits > 1)
+    float* partial_stats;  // [splits, q_rows * heads, 2]: the largest score and the sum of exponentials, base 2
+};
+
+// How attention.hip runs a call.
+enum class AttentionShape { kNarrow, kShort, kLong };  // 16 rows of a workgroup, 64, 128
+struct AttentionPlan {
+    AttentionShape shape;
+    bool direct;  // rows of whole aligned chunks
+};
+
+template <typename T>
+int launchAttention(const AttentionPlan& plan, const AttentionArgs& args, const AttentionOutput& output, hipStream_t stream);
+
+int attentionInvalid(const char* message);
+
+// The head's width in LDS and registers: zeros fill it up.
+inline int paddedDim(int head_dim) { return head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : 128; }
+
+// Keys of a wavefront's tile in the narrow shape: those of 4 KB, but whole turned fragments of them and at most 64.
+template <typename T, int kDim>
+constexpr int kNarrowKeys = kDim * static_cast<int>(sizeof(T)) <= 64    ? 64
+                            : kDim * static_cast<int>(sizeof(T)) <= 128 ? 32
+                            : sizeof(T) == 2                            ? 32
+                                                                        : 16;
+
+namespace {
+
+struct TextSpan {
+    std::int64_t first;
+    int rows;   // that there are
+    int count;  // that count
+};
+
+// Offsets out of order or out of range give spans within the rows all the same.
+__device__ __forceinline__ std::int64_t textStart(const TextRows& rows, int t) {
+    if (rows.offsets == nullptr) {
+        return static_cast<std::int64_t>(t) * rows.each;
+    }
+    const std::int64_t at = rows.offsets[t];
+    return at < 0 ? 0 : at < rows.total ? at : rows.total;
+}
+
+__device__ __forceinline__ TextSpan textSpan(const TextRows& rows, int t) {
+    TextSpan span;
+    span.first = textStart(rows, t);
+    const std::int64_t end = textStart(rows, t + 1);
+    span.rows = end > span.first ? static_cast<int>(end - span.first) : 0;
+    span.count = rows.lengths == nullptr ? span.rows : min(max(rows.lengths[t], 0), span.rows);
+    return span;
+}
+
+// Tiles of kTile rows never hold rows of two texts. Text t's begin at slot floor(first row / kTile) + t, so that they are
+// found without a list: the next text's begin at least as many slots on as this one has tiles.
+// The text of a slot (-1: none), by a search of all lanes at a time, the same in every lane. `weight`: tile rows
+// to a text's row.
+template <int kTile>
+__device__ __forceinline__ int textOfSlot(const TextRows& rows, int weight, int slot) {
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    int low = 0, high = rows.texts;
+    while (true) {
+        const int step = (high - low + kWave - 1) / kWave;
+        const int t = low + lane * step;
+        const bool at_or_before = t < high && textStart(rows, t) * weight / kTile + t <= slot;
+        const int count = __popcll(__ballot(at_or_before));
+        if (count == 0) {
+            return -1;
+        }
+        low += (count - 1) * step;
+        high = min(high, low + step);
+        if (step == 1) {
+            return __builtin_amdgcn_readfirstlane(low);
+        }
+    }
+}
+
+inline long long slotsOf(const TextRows& rows, int weight, int tile) { return rows.total * weight / tile + rows.texts; }
+
+// Position b of a launch of `total` blocks: blocks of one XCD (every eighth one) get neighbouring positions, so that tiles
+// of one head and text read its keys through one L2.
+__device__ __forceinline__ int positionOf(int block, int total) {
+    const int xcd = block % kXcds;
+    const int whole = total / kXcds;
+    return xcd * whole + min(xcd, total % kXcds) + block / kXcds;
+}
+
+// A row's 16-byte chunk from value `at` on, of which `left` exist; zeros past them.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::type loadRowChunk(const T* from, int left) {
+    typename Fragment<T>::type v = {};
+    if (left >= kChunk<T>) {
+        __builtin_memcpy(&v, from, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kChunk<T>; ++e) {
+            if (e < left) {
+                v[e] = from[e];
+            }
+        }
+    }
+    return v;
+}
+
+// kRows rows of kDim values in LDS, one behind the other. A row's chunk c stands in slot c ^ turn(row): the 16 rows of one
+// 16-byte read fall on 16 different columns of the 256 bytes that the banks hold, and so do the rows of a transposing
+// read's half wavefront (16-bit: eight rows, two chunks each; float32: four rows, four chunks each).
+template <typename T, int kRows, int kDim, int kTeam, bool kDirect>
+struct RowTile {
+    static constexpr int kRowBytes = kDim * static_cast<int>(sizeof(T));
+    static constexpr int kBytes = kRows * kRowBytes;
+    static constexpr int kRowChunks = kRowBytes / 16;
+    static constexpr int kCopies = kRows * kRowChunks / kTeam;
+    static constexpr int kSteps = kRowBytes / 64;  // matrix instruction steps over a row
+    static_assert(kRows * kRowChunks % kTeam == 0, "a tile splits over its threads");
+
+    static __device__ __forceinline__ int turn(int row) {
+        constexpr int kPerLine = kRowBytes >= 256 ? 1 : 256 / kRowBytes;
+        constexpr int kTurns = kRowChunks < 16 ? kRowChunks : 16;
+        const int p = (row / kPerLine) & (kTurns - 1);
+        if constexpr (sizeof(T) == 2) {
+            return ((p << 1) & (kTurns - 1)) | (p / (kTurns / 2));
+        } else {
+            return p;
+        }
+    }
+
+    const T* src[kCopies];
+    std::int64_t step;  // values from tile to tile
+    int rows_left;      // from the next tile's first row on
+    int width;          // values of a row that exist
+    u32x4 held[kDirect ? 1 : kCopies];
+
+    static __device__ __forceinline__ void placeOf(int i, int& row, int& chunk) {
+        const int slot = i * kTeam + static_cast<int>(threadIdx.x) % kTeam;
+        row = slot / kRowChunks;
+        chunk = (slot % kRowChunks) ^ turn(row);
+    }
+
+    // Rows `base`, base + stride, ..., `count` of them; tiles `tiles_apart` tiles apart.
+    __device__ __forceinline__ void begin(const T* base, std::int64_t stride, int count, int row_width, int tiles_apart) {
+        step = stride * kRows * tiles_apart;
+        rows_left = count;
+        width = row_width;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            int row, chunk;
+            placeOf(i, row, chunk);
+            src[i] = base + row * stride + chunk * kChunk<T>;
+        }
+    }
+    __device__ __forceinline__ bool exists(int i) const {
+        int row, chunk;
+        placeOf(i, row, chunk);
+        return row < rows_left && chunk * kChunk<T> < width;
+    }
+    // Starts the next tile's copies into `to` (direct).
+    __device__ __forceinline__ void issue(const std::uint8_t* to, int tiles_apart) {
+        const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) % kTeam / kWave);
+        const std::uint32_t base = ldsAddress(to) + static_cast<std::uint32_t>(wave * kWave * 16);
+        const bool whole = rows_left >= kRows && width == kDim;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const void* from = whole || exists(i) ? static_cast<const void*>(src[i]) : static_cast<const void*>(&zero_chunk);
+            copySharedToLds(from, __builtin_amdgcn_readfirstlane(base + i * kTeam * 16));
+            src[i] += step;
+        }
+        rows_left -= kRows * tiles_apart;
+    }
+    // Reads the next tile into registers, and later writes it to `to` (not direct).
+    __device__ __forceinline__ void fetch(int tiles_apart) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            int row, chunk;
+            placeOf(i, row, chunk);
+            const int left = row < rows_left ? width - chunk * kChunk<T> : 0;
+            held[i] = __builtin_bit_cast(u32x4, loadRowChunk(src[i], left));
+            src[i] += step;
+        }
+        rows_left -= kRows * tiles_apart;
+    }
+    __device__ __forceinline__ void put(std::uint8_t* to) const {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            *reinterpret_cast<u32x4*>(to + (i * kTeam + static_cast<int>(threadIdx.x) % kTeam) * 16) = held[i];
+        }
+    }
+
+    // The calling lane's fragment of rows 16 block .. + 15, values of step t along the row.
+    static __device__ __forceinline__ typename Fragment<T>::type read(const std::uint8_t* tile, int block, int t) {
+        const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+        const int row = 16 * block + (lane & 15);
+        const int slot = (4 * t + (lane >> 4)) ^ turn(row);
+        return *reinterpret_cast<const typename Fragment<T>::type*>(tile + row * kRowBytes + 16 * slot);
+    }
+    // The calling lane's fragment of columns 16 block .. + 15, contracted over rows: of lane group h the rows 4 h + e of
+    // row block `pair` (float32), or of the row blocks 2 pair and 2 pair + 1 (16-bit): the rows whose products a lane
+    // holds in its results, so that these are the other operand as they are.
+    static __device__ __forceinline__ typename Fragment<T>::type readTurned(const std::uint8_t* tile, int block, int pair) {
+        const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+        const int i = lane & 15;
+        const int h = lane >> 4;
+        if constexpr (sizeof(T) == 2) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* LdsPointer;
+            const int row = 32 * pair + 4 * h + (i >> 2);
+            const int chunk = 2 * block + ((i & 3) >> 1);
+            const std::uint32_t base = ldsAddress(tile) + static_cast<std::uint32_t>(8 * (i & 1));
+            const std::uint32_t low = base + static_cast<std::uint32_t>(row * kRowBytes + 16 * (chunk ^ turn(row)));
+            const std::uint32_t high =
+                base + static_cast<std::uint32_t>((row + 16) * kRowBytes + 16 * (chunk ^ turn(row + 16)));
+            const s16x4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(low));
+            const s16x4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(high));
+            return __builtin_bit_cast(typename Fragment<T>::type,
+                                      __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            typename Fragment<T>::type v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * pair + 4 * h + e;
+                const int chunk = (4 * block + (i >> 2)) ^ turn(row);
+                v[e] = *reinterpret_cast<const float*>(tile + row * kRowBytes + 16 * chunk + 4 * (i & 3));
+            }
+            return v;
+        }
+    }
+};
+
+// Row blocks that one turned fragment contracts over.
+template <typename T>
+constexpr int kBlocksTurned = sizeof(T) == 2 ? 2 : 1;
+
+// A lane's results for kBlocksTurned row blocks as the other operand of that contraction, rounded to T.
+template <typename T>
+__device__ __forceinline__ typename Fragment<T>::type resultFragment(const f32x4* blocks) {
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_convertvector(__builtin_shufflevector(blocks[0], blocks[1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                       typename Fragment<T>::type);
+    } else {
+        return blocks[0];
+    }
+}
+
+// Tiles that a team of threads (a workgroup, or a wavefront of its own) works through: the next one's copies are on their
+// way while this one is used.
+template <int kTeam>
+__device__ __forceinline__ void teamSync() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if constexpr (kTeam > kWave) {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float tanhOf(float y) {
+    if constexpr (sizeof(T) == 2) {
+        // within 2^-22 of 1, far below what the 16-bit operands have
+        return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2E * y));
+    } else {
+        return tanhf(y);
+    }
+}
+
+}  // namespace
+}  // namespace zcgvs_hip
