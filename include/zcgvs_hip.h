@@ -705,6 +705,19 @@ size_t zcgvs_attention_workspace_bytes(const zcgvs_attention_desc* desc);
 int zcgvs_attention(const zcgvs_attention_desc* desc, void* d_out, int64_t out_stride, float* d_lse,
                     void* d_workspace, size_t workspace_bytes, zcgvs_stream_t stream);
 
+/* The gradient of zcgvs_attention from that of its output, with what the forward call wrote (d_out with
+ * out_stride, d_lse). q_gradient, k_gradient and v_gradient have the shapes of q, k and v and desc->dtype;
+ * distance_bias_gradient (NULL: not wanted) that of distance_bias and desc->dtype. The softmax and its
+ * gradient are rounded to desc->dtype between the products (float16: to an infinity beyond 65504, so scale
+ * the loss as for stored tensors). A stride of 0 is the row's length. */
+size_t zcgvs_attention_gradient_workspace_bytes(const zcgvs_attention_desc* desc);
+int zcgvs_attention_gradient(const zcgvs_attention_desc* desc, const void* d_out, int64_t out_stride,
+                             const float* d_lse, const void* d_out_gradient, int64_t out_gradient_stride,
+                             void* d_q_gradient, int64_t q_gradient_stride, void* d_k_gradient,
+                             int64_t k_gradient_stride, void* d_v_gradient, int64_t v_gradient_stride,
+                             void* d_distance_bias_gradient, void* d_workspace, size_t workspace_bytes,
+                             zcgvs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,3 +138,65 @@ class Batch:
             finite = np.where(np.isfinite(text_lse), np.abs(text_lse), 0.0)
             lse_tolerance[rows] = (1.01 * worst[..., 0] + (n + 8) * STEP + 2.0 ** -21 * (finite + 1.0)).T
         return out, tolerance, lse, lse_tolerance
+
+    def gradient(self, g, out_stored):
+        """name -> (gradient, its tolerance), NaN in rows of no text and zeros in padding rows, from the output's gradient
+        g and the output as it is handed to the kernel."""
+        width = self.heads * self.head_dim
+        shapes = dict(q=(self.q_rows, width), k=self.k.shape, v=self.v.shape)
+        value = {n: np.full(s, np.nan) for n, s in shapes.items()}
+        error = {n: np.zeros(s) for n, s in shapes.items()}
+        unit, floor = UNIT[self.kind], FLOOR[self.kind]
+        inner, inner_floor = (0.0, 0.0) if self.kind == "f32" else (unit, floor)
+        bins = 2 * self.far + 1
+        table, table_error = np.zeros((self.heads, bins)), np.zeros((self.heads, bins))
+        ratio = self.heads // self.kv_heads
+        for t in range(self.texts):
+            q, k, v, distance, seen = self.of_text(t)
+            nq, nk = self.q_lens[t], self.k_lens[t]
+            rows = slice(self.q_starts[t], self.q_starts[t] + nq)
+            keys = slice(self.k_starts[t], self.k_starts[t] + nk)
+            dout = g[rows].reshape(nq, self.heads, self.head_dim).transpose(1, 0, 2)
+            out = out_stored[rows].reshape(nq, self.heads, self.head_dim).transpose(1, 0, 2)
+            scores, slope, s_error = self.scores(q, k, distance)
+            p, lse = self.softmax(scores, seen)
+            lse_size = np.where(np.isfinite(lse), np.abs(lse), 0.0)[..., None]
+            p_error = p * (1.02 * (s_error + 2.0 ** -21 * (lse_size + 1.0)))
+            dp = dout @ v.transpose(0, 2, 1)
+            delta = (p * dp).sum(2, keepdims=True)
+            dp_error = (self.head_dim + 2) * STEP * (np.abs(dout) @ np.abs(v).transpose(0, 2, 1))
+            # the output's own rounding is in the kernel's delta
+            exact_out = p @ v
+            delta_error = ((np.abs(dout) * (np.abs(out - exact_out) + (self.head_dim + 2) * STEP * np.abs(out))).sum(2, keepdims=True))
+            ds = p * (dp - delta)
+            ds_error = p_error * np.abs(dp - delta) + (p + p_error) * (dp_error + delta_error) + 4 * STEP * np.abs(ds)
+            dr = ds * slope
+            dr_error = ds_error * slope + (2.0 ** -18 * np.abs(ds) if self.cap else 0.0)
+            dr_error = dr_error + inner * (np.abs(dr) + dr_error) + inner_floor
+            p_rounded = p_error + inner * (p + p_error) + inner_floor
+            # masked places take no part
+            dr_error, p_rounded, ds_error = (np.where(seen, e, 0.0) for e in (dr_error, p_rounded, ds_error))
+            size = abs(self.scale)
+            results = dict(q=(dr @ k * self.scale, size * (dr_error @ np.abs(k) + (nk + 6) * STEP * (np.abs(dr) + dr_error) @ np.abs(k))))
+            turned = np.abs(dr).transpose(0, 2, 1) + dr_error.transpose(0, 2, 1)
+            results["k"] = (dr.transpose(0, 2, 1) @ q * self.scale,
+                            size * (dr_error.transpose(0, 2, 1) @ np.abs(q) + (nq * ratio + 6) * STEP * turned @ np.abs(q)))
+            turned = p.transpose(0, 2, 1) + p_rounded.transpose(0, 2, 1)
+            results["v"] = (p.transpose(0, 2, 1) @ dout,
+                            p_rounded.transpose(0, 2, 1) @ np.abs(dout) + (nq * ratio + 6) * STEP * turned @ np.abs(dout))
+            for name, (grad, own) in results.items():
+                n = nq if name == "q" else nk
+                if name != "q":  # summed over the heads of a key head
+                    grad, own = (x.reshape(self.kv_heads, ratio, n, self.head_dim).sum(1) for x in (grad, own))
+                own = own + unit * (np.abs(grad) + own) + floor
+                where = rows if name == "q" else keys
+                value[name][where] = grad.transpose(1, 0, 2).reshape(n, shapes[name][1])
+                error[name][where] = own.transpose(1, 0, 2).reshape(n, shapes[name][1])
+            if self.table is not None:
+                at = (np.clip(distance, -self.far, self.far) + self.far).ravel()
+                for i in range(self.heads):
+                    np.add.at(table[i], at, ds[i].ravel())
+                    np.add.at(table_error[i], at, (ds_error[i] + (nq + nk + 64) * STEP * np.abs(ds[i])).ravel())
+        if self.table is not None:
+            value["table"], error["table"] = table, table_error + unit * (np.abs(table) + table_error) + floor
+        return {name: (value[name], error[name]) for name in value}

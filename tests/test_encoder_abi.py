@@ -175,6 +175,30 @@ def test_attention_descriptor(capi, kw, match):
         capi.attention_workspace_bytes(_attention(capi, **kw))
     with pytest.raises(ValueError, match=match):
         capi.attention(_attention(capi, **kw), A, A, 1 << 30)
+    with pytest.raises(ValueError, match=match):
+        capi.attention_gradient_workspace_bytes(_attention(capi, **kw))
+    with pytest.raises(ValueError, match=match):
+        capi.attention_gradient(_attention(capi, **kw), A, A, A, A, A, A, A, 1 << 30)
+
+
+def test_attention_gradient_operands(capi):
+    for name in ("out_stride", "out_gradient_stride", "q_gradient_stride", "k_gradient_stride", "v_gradient_stride"):
+        with pytest.raises(ValueError, match="smaller than its heads"):
+            capi.attention_gradient(_attention(capi), A, A, A, A, A, A, A, 1 << 30, **{name: 15})
+    for i in range(6):
+        with pytest.raises(ValueError, match="null device pointer"):
+            capi.attention_gradient(_attention(capi), *(None if i == j else A for j in range(6)), A, 1 << 30)
+    with pytest.raises(ValueError, match="needs the distance bias"):
+        capi.attention_gradient(_attention(capi), A, A, A, A, A, A, A, 1 << 30, distance_bias_gradient=A)
+    need = capi.attention_gradient_workspace_bytes(_attention(capi))
+    with pytest.raises(ValueError, match="too small"):
+        capi.attention_gradient(_attention(capi), A, A, A, A, A, A, A, need - 1)
+    with pytest.raises(ValueError, match="too small"):
+        capi.attention_gradient(_attention(capi), A, A, A, A, A, A, None, need)
+    with pytest.raises(ValueError, match="16 bytes"):
+        capi.attention_gradient(_attention(capi), A, A, A, A, A, A, A + 4, need)
+    biased = _attention(capi, distance_bias=A, max_distance=100)
+    assert capi.attention_gradient_workspace_bytes(biased) > need
 
 
 def test_attention_operands(capi):
@@ -213,3 +237,4 @@ def test_empty_work_returns_ok(capi):
     capi.linear_gradient(_linear(capi, rows=0, x=None, weight=None), None, A, None, None, None, 0)
     for kw in (dict(texts=0), dict(q_rows=0), dict(texts=0, q_rows=0, k_rows=0, q=None, k=None, v=None)):
         capi.attention(_attention(capi, **kw), None, None, 0)
+    capi.attention_gradient(_attention(capi, texts=0, q_rows=0, k_rows=0), *(None,) * 6, None, 0)

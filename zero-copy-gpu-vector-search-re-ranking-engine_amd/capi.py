@@ -184,6 +184,9 @@ _SIGNATURES = {
     "zcgvs_attention_max_distance": (_i32, []),
     "zcgvs_attention_workspace_bytes": (_sz, [ctypes.POINTER(AttentionDesc)]),
     "zcgvs_attention": (_i32, [ctypes.POINTER(AttentionDesc), _vp, _i64, _vp, _vp, _sz, _vp]),
+    "zcgvs_attention_gradient_workspace_bytes": (_sz, [ctypes.POINTER(AttentionDesc)]),
+    "zcgvs_attention_gradient": (_i32, [ctypes.POINTER(AttentionDesc), _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                                        _i64, _vp, _vp, _sz, _vp]),
     "zcgvs_linear_gradient": (_i32, [ctypes.POINTER(LinearDesc), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp]),
 }
 
@@ -747,3 +750,16 @@ def attention(desc: AttentionDesc, out, workspace, workspace_bytes, *, lse=None,
     """Attention within each text; lse takes what attention_gradient needs of the softmax."""
     call("zcgvs_attention", ctypes.byref(desc), ptr(out), out_stride, ptr(lse), ptr(workspace), workspace_bytes,
          getattr(stream, "handle", stream))
+
+
+def attention_gradient_workspace_bytes(desc: AttentionDesc) -> int:
+    return _workspace_bytes("zcgvs_attention_gradient_workspace_bytes", desc)
+
+
+def attention_gradient(desc: AttentionDesc, out, lse, out_gradient, q_gradient, k_gradient, v_gradient, workspace,
+                       workspace_bytes, *, distance_bias_gradient=None, out_stride=0, out_gradient_stride=0,
+                       q_gradient_stride=0, k_gradient_stride=0, v_gradient_stride=0, stream=None) -> None:
+    """The gradients of attention, from what the forward call wrote (out, lse) and the gradient of its output."""
+    call("zcgvs_attention_gradient", ctypes.byref(desc), ptr(out), out_stride, ptr(lse), ptr(out_gradient),
+         out_gradient_stride, ptr(q_gradient), q_gradient_stride, ptr(k_gradient), k_gradient_stride, ptr(v_gradient),
+         v_gradient_stride, ptr(distance_bias_gradient), ptr(workspace), workspace_bytes, getattr(stream, "handle", stream))

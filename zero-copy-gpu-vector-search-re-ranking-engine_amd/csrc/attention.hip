@@ -129,6 +129,46 @@ std::size_t partialFloats(const zcgvs_attention_desc& d, int splits, int each) {
     return splits == 1 ? 0 : static_cast<std::size_t>(splits) * static_cast<std::size_t>(d.q_rows) * d.heads * each;
 }
 
+// ---- the gradient's workspace: the rows' statistics, the bias's partial sums -----------------------
+
+// Blocks of 16 rows of a wavefront by a text's mean rows: tiles of 128 where texts fill them. Two blocks of keys, their
+// values and both gradients do not fit the registers for float32 heads of 128.
+int gradientBlocks(std::int64_t rows, std::int64_t texts) { return rows <= 64 * texts ? 1 : 2; }
+
+int keyBlocks(const zcgvs_attention_desc& d) {
+    return d.dtype == ZCGVS_DTYPE_F32 && paddedDim(d.head_dim) == 128 ? 1 : gradientBlocks(d.k_rows, d.texts);
+}
+
+long long slotsFor(std::int64_t rows, std::int64_t texts, int blocks) { return rows / (64 * blocks) + texts; }
+
+std::size_t statsBytes(const zcgvs_attention_desc& d) {
+    return (static_cast<std::size_t>(d.q_rows) * d.heads * 2 * sizeof(float) + 255) / 256 * 256;
+}
+
+std::size_t tableBytes(const zcgvs_attention_desc& d) {
+    return d.distance_bias == nullptr ? 0
+                                      : static_cast<std::size_t>(slotsFor(d.k_rows, d.texts, keyBlocks(d))) * d.heads *
+                                            (2 * static_cast<std::size_t>(d.max_distance) + 1) * sizeof(float);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void clearTextRowsKernel(TextRows rows, int width, std::int64_t stride, T* out) {
+    const std::int64_t first = textStart(rows, 0), end = textStart(rows, rows.texts);
+    for (std::int64_t r = first + blockIdx.x; r < end; r += gridDim.x) {
+        for (int c = static_cast<int>(threadIdx.x); c < width; c += 256) {
+            out[r * stride + c] = static_cast<T>(0.0f);
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void clearTableKernel(int count, T* out) {
+    for (int i = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x); i < count;
+         i += static_cast<int>(gridDim.x) * 256) {
+        out[i] = static_cast<T>(0.0f);
+    }
+}
+
 }  // namespace
 
 }  // namespace zcgvs_hip
@@ -190,6 +230,113 @@ int zcgvs_attention(const zcgvs_attention_desc* desc, void* d_out, std::int64_t 
     const bool direct = directRows(d.k, args.k_stride, d.head_dim, d.dtype) && directRows(d.v, args.v_stride, d.head_dim, d.dtype);
     const int launched = withElement(d.dtype, [&](auto element) {
         return launchAttention<decltype(element)>({plan.shape, direct}, args, output, toStream(stream));
+    });
+    return launched == ZCGVS_OK ? clearError() : launched;
+}
+
+std::size_t zcgvs_attention_gradient_workspace_bytes(const zcgvs_attention_desc* desc) {
+    if (checkAttention(desc) != ZCGVS_OK) {
+        return 0;
+    }
+    clearError();
+    return desc->texts == 0 ? 256 : std::max<std::size_t>(256, statsBytes(*desc) + tableBytes(*desc));
+}
+
+int zcgvs_attention_gradient(const zcgvs_attention_desc* desc, const void* d_out, std::int64_t out_stride, const float* d_lse,
+                             const void* d_out_gradient, std::int64_t out_gradient_stride, void* d_q_gradient,
+                             std::int64_t q_gradient_stride, void* d_k_gradient, std::int64_t k_gradient_stride,
+                             void* d_v_gradient, std::int64_t v_gradient_stride, void* d_distance_bias_gradient,
+                             void* d_workspace, std::size_t workspace_bytes, zcgvs_stream_t stream) {
+    const int status = checkAttention(desc);
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const zcgvs_attention_desc& d = *desc;
+    const int q_width = d.heads * d.head_dim;
+    const int k_width = d.kv_heads * d.head_dim;
+    AttentionGradient more{};
+    more.out_stride = rowStride(out_stride, q_width);
+    more.out_gradient_stride = rowStride(out_gradient_stride, q_width);
+    more.q_gradient_stride = rowStride(q_gradient_stride, q_width);
+    more.k_gradient_stride = rowStride(k_gradient_stride, k_width);
+    more.v_gradient_stride = rowStride(v_gradient_stride, k_width);
+    if (more.out_stride < q_width || more.out_gradient_stride < q_width || more.q_gradient_stride < q_width ||
+        more.k_gradient_stride < k_width || more.v_gradient_stride < k_width) {
+        return attentionInvalid("a row stride is smaller than its heads");
+    }
+    if (d_distance_bias_gradient != nullptr && d.distance_bias == nullptr) {
+        return attentionInvalid("a gradient of the distance bias needs the distance bias");
+    }
+    const int table_count = d.heads * (2 * d.max_distance + 1);
+    if (d.texts == 0 || (d.q_rows == 0 && d.k_rows == 0)) {
+        if (d_distance_bias_gradient != nullptr) {
+            return withElement(d.dtype, [&](auto element) {
+                using T = decltype(element);
+                clearTableKernel<T><<<64, 256, 0, toStream(stream)>>>(table_count, static_cast<T*>(d_distance_bias_gradient));
+                ZCGVS_LAUNCH_CHECK("attention gradient");
+                return clearError();
+            });
+        }
+        return clearError();
+    }
+    if ((d.q_rows > 0 && (d_out == nullptr || d_lse == nullptr || d_out_gradient == nullptr || d_q_gradient == nullptr)) ||
+        (d.k_rows > 0 && (d_k_gradient == nullptr || d_v_gradient == nullptr))) {
+        return attentionInvalid("null device pointer");
+    }
+    if (d_workspace == nullptr || workspace_bytes < zcgvs_attention_gradient_workspace_bytes(desc)) {
+        return attentionInvalid("the workspace is too small");
+    }
+    if (!aligned16(d_workspace)) {
+        return attentionInvalid("the workspace must be aligned to 16 bytes");
+    }
+    const AttentionArgs args = attentionArgs(d);
+    more.out = d_out;
+    more.lse = d_lse;
+    more.out_gradient = d_out_gradient;
+    more.q_gradient = d_q_gradient;
+    more.k_gradient = d_k_gradient;
+    more.v_gradient = d_v_gradient;
+    more.table_gradient = d_distance_bias_gradient;
+    const int launched = withElement(d.dtype, [&](auto element) {
+        using T = decltype(element);
+        if (d.q_rows == 0 || d.k_rows == 0) {
+            // nothing sees anything: zeros for the rows of the texts
+            const TextRows& rows = d.q_rows == 0 ? args.k_texts : args.q_texts;
+            const int width = d.q_rows == 0 ? k_width : q_width;
+            if (d.q_rows == 0) {
+                clearTextRowsKernel<T><<<1024, 256, 0, toStream(stream)>>>(rows, width, more.k_gradient_stride,
+                                                                           static_cast<T*>(d_k_gradient));
+                clearTextRowsKernel<T><<<1024, 256, 0, toStream(stream)>>>(rows, width, more.v_gradient_stride,
+                                                                           static_cast<T*>(d_v_gradient));
+            } else {
+                clearTextRowsKernel<T><<<1024, 256, 0, toStream(stream)>>>(rows, width, more.q_gradient_stride,
+                                                                           static_cast<T*>(d_q_gradient));
+            }
+            if (d_distance_bias_gradient != nullptr) {
+                clearTableKernel<T><<<64, 256, 0, toStream(stream)>>>(table_count, static_cast<T*>(d_distance_bias_gradient));
+            }
+            ZCGVS_LAUNCH_CHECK("attention gradient");
+            return static_cast<int>(ZCGVS_OK);
+        }
+        AttentionGradientPlan plan{};
+        plan.key_blocks = keyBlocks(d);
+        plan.query_blocks = gradientBlocks(d.q_rows, d.texts);
+        const long long key_slots = slotsFor(d.k_rows, d.texts, plan.key_blocks);
+        const long long query_slots = slotsFor(d.q_rows, d.texts, plan.query_blocks);
+        if (key_slots * d.kv_heads > kMaxBlocks || query_slots * d.heads > kMaxBlocks) {
+            return attentionInvalid("more texts and rows than one launch can take");
+        }
+        more.key_slots = static_cast<int>(key_slots);
+        more.query_slots = static_cast<int>(query_slots);
+        more.stats = static_cast<float*>(d_workspace);
+        if (d_distance_bias_gradient != nullptr) {
+            more.table_partials = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + statsBytes(d));
+        }
+        plan.direct_rows = directRows(d.q, args.q_stride, d.head_dim, d.dtype) &&
+                           directRows(d_out_gradient, more.out_gradient_stride, d.head_dim, d.dtype);
+        plan.direct_keys = directRows(d.k, args.k_stride, d.head_dim, d.dtype) &&
+                           directRows(d.v, args.v_stride, d.head_dim, d.dtype);
+        return launchAttentionGradient<T>(plan, args, more, toStream(stream));
     });
     return launched == ZCGVS_OK ? clearError() : launched;
 }

@@ -70,6 +70,37 @@ struct AttentionPlan {
 template <typename T>
 int launchAttention(const AttentionPlan& plan, const AttentionArgs& args, const AttentionOutput& output, hipStream_t stream);
 
+struct AttentionGradient {
+    const void* out;
+    std::int64_t out_stride;
+    const float* lse;
+    const void* out_gradient;
+    std::int64_t out_gradient_stride;
+    void* q_gradient;
+    std::int64_t q_gradient_stride;
+    void* k_gradient;
+    std::int64_t k_gradient_stride;
+    void* v_gradient;
+    std::int64_t v_gradient_stride;
+    void* table_gradient;
+    float* stats;           // [heads, q_rows, 2]: lse in base 2, delta
+    float* table_partials;  // [heads, key_slots, 2 * max_distance + 1], or null: not wanted
+    int key_slots;          // tiles of keys, empty ones among them
+    int query_slots;
+};
+
+// Blocks of 16 keys (query rows) of a wavefront; rows of whole aligned chunks: of q and the output's gradient, of k and v.
+struct AttentionGradientPlan {
+    int key_blocks;
+    int query_blocks;
+    bool direct_rows;
+    bool direct_keys;
+};
+
+template <typename T>
+int launchAttentionGradient(const AttentionGradientPlan& plan, const AttentionArgs& args, const AttentionGradient& more,
+                            hipStream_t stream);
+
 int attentionInvalid(const char* message);
 
 // The head's width in LDS and registers: zeros fill it up.
@@ -167,9 +198,15 @@ struct RowTile {
     static constexpr int kRowBytes = kDim * static_cast<int>(sizeof(T));
     static constexpr int kBytes = kRows * kRowBytes;
     static constexpr int kRowChunks = kRowBytes / 16;
-    static constexpr int kCopies = kRows * kRowChunks / kTeam;
+    static constexpr int kChunks = kRows * kRowChunks;
+    static constexpr int kCopies = (kChunks + kTeam - 1) / kTeam;
     static constexpr int kSteps = kRowBytes / 64;  // matrix instruction steps over a row
-    static_assert(kRows * kRowChunks % kTeam == 0, "a tile splits over its threads");
+    static_assert(kChunks % kTeam == 0 || (kChunks < kTeam && kChunks % kWave == 0), "a tile splits over its wavefronts");
+
+    // Small tiles leave the last wavefronts without a copy.
+    static __device__ __forceinline__ bool hasCopy() {
+        return kChunks >= kTeam || __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) % kTeam / kWave) * kWave < kChunks;
+    }
 
     static __device__ __forceinline__ int turn(int row) {
         constexpr int kPerLine = kRowBytes >= 256 ? 1 : 256 / kRowBytes;
@@ -219,7 +256,9 @@ struct RowTile {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const void* from = whole || exists(i) ? static_cast<const void*>(src[i]) : static_cast<const void*>(&zero_chunk);
-            copySharedToLds(from, __builtin_amdgcn_readfirstlane(base + i * kTeam * 16));
+            if (hasCopy()) {
+                copySharedToLds(from, __builtin_amdgcn_readfirstlane(base + i * kTeam * 16));
+            }
             src[i] += step;
         }
         rows_left -= kRows * tiles_apart;
@@ -230,13 +269,16 @@ struct RowTile {
         for (int i = 0; i < kCopies; ++i) {
             int row, chunk;
             placeOf(i, row, chunk);
-            const int left = row < rows_left ? width - chunk * kChunk<T> : 0;
+            const int left = hasCopy() && row < rows_left ? width - chunk * kChunk<T> : 0;
             held[i] = __builtin_bit_cast(u32x4, loadRowChunk(src[i], left));
             src[i] += step;
         }
         rows_left -= kRows * tiles_apart;
     }
     __device__ __forceinline__ void put(std::uint8_t* to) const {
+        if (!hasCopy()) {
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             *reinterpret_cast<u32x4*>(to + (i * kTeam + static_cast<int>(threadIdx.x) % kTeam) * 16) = held[i];

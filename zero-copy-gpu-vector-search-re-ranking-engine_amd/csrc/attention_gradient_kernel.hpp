@@ -1,0 +1,741 @@
+// The gradient of attention over packed texts.
+//
+//     delta = dout . out (a row),  p = exp(s - lse),  dp = dout v^T,  ds = p (dp - delta)
+//     dbias = sums of ds along the diagonals,  dr = ds (1 - (c / cap)^2)
+//     dq = scale dr k,  dk = scale dr^T q,  dv = p^T dout
+//
+// Three launches (four with the bias's gradient), no atomics between workgroups: the same bits on every call.
+// 1. delta and the rows' lse in base 2, head by head.
+// 2. dk and dv: a wavefront keeps 16 or 32 keys and their values in registers and goes through the queries of all heads of
+//    its key head, in LDS tiles of 32 rows that the workgroup shares. Scores come out with a lane's four neighbouring query
+//    rows of one key, which is how the products over the rows take p and dr: they stay in registers.
+// 3. dq: a wavefront keeps 16 or 32 query rows and goes through the keys, as the forward kernel does.
+// So p is formed twice: seven products instead of five, for sums in one order and no float32 copy of dq.
+// The bias's gradient: every lane group of a wavefront adds to a table of its own in LDS (the 16 lanes of a group
+// always meet 16 different distances, so the order of its additions is the program's), with room for distances past
+// the table's ends; tiles that lie past them altogether add to two registers. A workgroup joins its tables and writes
+// one of partial sums a head, which the last launch adds in the order of the workgroups.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "attention.hpp"
+#include "column_sums.hpp"
+#include "matrix_plan.hpp"
+
+namespace zcgvs_hip {
+namespace {
+
+constexpr int kGradientWaves = 4;
+constexpr int kGradientThreads = kGradientWaves * kWave;
+constexpr int kQueryTile = 32;
+
+static __device__ const float no_row[2] = {INFINITY, 0.0f};  // p = 0
+
+// ---- rows: lse in base 2 and delta, [heads, q_rows, 2] -------------------------------------------
+
+constexpr int kStatsLanes = 16;  // of a row and head
+
+template <typename T>
+__global__ __launch_bounds__(kGradientThreads) void attentionStatsKernel(AttentionArgs args, AttentionGradient more) {
+    const int lane = static_cast<int>(threadIdx.x) % kStatsLanes;
+    const std::int64_t at =
+        static_cast<std::int64_t>(blockIdx.x) * (kGradientThreads / kStatsLanes) + threadIdx.x / kStatsLanes;
+    if (at >= args.q_texts.total * args.heads) {
+        return;  // (all lanes of a row and head)
+    }
+    const std::int64_t row = at / args.heads;
+    const int head = static_cast<int>(at % args.heads);
+    const T* out = static_cast<const T*>(more.out) + row * more.out_stride + head * args.head_dim;
+    const T* from = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim;
+    float sum = 0.0f;
+    for (int d = 4 * lane; d < args.head_dim; d += 4 * kStatsLanes) {
+        const f32x4 a = loadFour(out + d, args.head_dim - d);
+        const f32x4 b = loadFour(from + d, args.head_dim - d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            sum = fmaf(a[e], b[e], sum);
+        }
+    }
+#pragma unroll
+    for (int offset = kStatsLanes / 2; offset > 0; offset >>= 1) {
+        sum += waveXor(sum, offset);
+    }
+    if (lane == 0) {
+        const float lse = more.lse[at];
+        float* to = more.stats + 2 * (head * args.q_texts.total + row);
+        to[0] = lse == -INFINITY ? INFINITY : kLog2E * lse;
+        to[1] = lse == -INFINITY ? 0.0f : sum;
+    }
+}
+
+// ---- the scores' forms, shared by both kernels ---------------------------------------------------
+
+struct ScoreForm {
+    bool capped;
+    bool modified;
+    float factor;  // log2(e) |scale|
+    float unit;    // factor, or 1 where scores are formed first
+    float cap;     // log2(e) cap
+    float to_cap;  // |scale| / cap
+
+    __device__ __forceinline__ explicit ScoreForm(const AttentionArgs& args) {
+        capped = args.cap > 0.0f;
+        modified = capped || args.slopes != nullptr || args.table != nullptr || args.scale == 0.0f;
+        factor = kLog2E * fabsf(args.scale);
+        unit = modified ? 1.0f : factor;
+        cap = kLog2E * args.cap;
+        to_cap = capped ? fabsf(args.scale) / args.cap : 0.0f;
+    }
+};
+
+// Raw products -> scores in base 2 before the biases; tangent^2 of the cap goes to `bent`.
+template <typename T, int kCount>
+__device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCount], f32x4 (&bent)[kCount]) {
+    if (form.capped) {
+#pragma unroll
+        for (int b = 0; b < kCount; ++b) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float t = tanhOf<T>(s[b][e] * form.to_cap);
+                bent[b][e] = t * t;
+                s[b][e] = form.cap * t;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int b = 0; b < kCount; ++b) {
+            s[b] *= form.factor;
+        }
+    }
+}
+
+// The table of a head with `margin` copies of its end values on either side, base 2.
+template <typename T>
+__device__ __forceinline__ void loadTable(const AttentionArgs& args, int head, int margin, float* table) {
+    const int width = 2 * (args.max_distance + margin) + 1;
+    const T* from = static_cast<const T*>(args.table) + static_cast<std::int64_t>(head) * (2 * args.max_distance + 1);
+    for (int i = static_cast<int>(threadIdx.x); i < width; i += kGradientThreads) {
+        table[i] = kLog2E * static_cast<float>(from[min(max(i - margin, 0), 2 * args.max_distance)]);
+    }
+}
+
+// ---- dk, dv and the bias's partial sums ----------------------------------------------------------
+
+// kFar: the largest max_distance whose gradient is wanted (0: none).
+template <typename T, int kDim, int kBlocks, bool kDirect, int kFar>
+__global__ __launch_bounds__(kGradientThreads) void keyGradientKernel(AttentionArgs args, AttentionGradient more) {
+    using Rows = RowTile<T, kQueryTile, kDim, kGradientThreads, kDirect>;
+    constexpr int kWaveKeys = 16 * kBlocks;
+    constexpr int kKeys = kWaveKeys * kGradientWaves;
+    constexpr int kStageBytes = 2 * Rows::kBytes;  // queries, then the output's gradient
+    constexpr int kDimBlocks = kDim / 16;
+    constexpr int kRowBlocks = kQueryTile / 16;
+    constexpr int kTurned = kBlocksTurned<T>;
+    constexpr int kMargin = kQueryTile + kWaveKeys;
+    constexpr int kBins = kFar > 0 ? 2 * (kFar + kMargin) + 1 : 1;
+    __shared__ __attribute__((aligned(256))) std::uint8_t lds[2 * kStageBytes];
+    __shared__ __attribute__((aligned(256))) float stats[2][kQueryTile][2];
+    __shared__ float table[2 * (kAttentionMaxDistance + kMargin) + 1];
+    __shared__ float bins[kFar > 0 ? kGradientWaves * 4 : 1][kBins];
+
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int r16 = lane & 15;
+    const int h = lane >> 4;
+    const int position = positionOf(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    const int slot = position % more.key_slots;
+    const int key_head = position / more.key_slots;
+    const int table_columns = 2 * args.max_distance + 1;
+    auto partialTable = [&](int head) {
+        return more.table_partials + (static_cast<std::int64_t>(head) * more.key_slots + slot) * table_columns;
+    };
+    const int text = textOfSlot<kKeys>(args.k_texts, 1, slot);
+    TextSpan keys{0, 0, 0};
+    int tile_key = 0;
+    if (text >= 0) {
+        keys = textSpan(args.k_texts, text);
+        tile_key = (slot - (static_cast<int>(keys.first / kKeys) + text)) * kKeys;
+    }
+    if (text < 0 || tile_key < 0 || tile_key >= keys.rows) {
+        if constexpr (kFar > 0) {
+            for (int g = 0; g < args.group; ++g) {
+                for (int i = static_cast<int>(threadIdx.x); i < table_columns; i += kGradientThreads) {
+                    partialTable(key_head * args.group + g)[i] = 0.0f;
+                }
+            }
+        }
+        return;
+    }
+    const TextSpan queries = textSpan(args.q_texts, text);
+    const int prefix = args.prefix == nullptr ? 0 : args.prefix[text];
+    const int shift = args.q_last ? keys.count - queries.count : 0;
+    const ScoreForm form(args);
+
+    const int wave_key = tile_key + wave * kWaveKeys;
+    int key[kBlocks], seen_from[kBlocks];
+    bool valid[kBlocks];
+    typename Fragment<T>::type k[kBlocks][Rows::kSteps], v[kBlocks][Rows::kSteps];
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+        key[n] = wave_key + 16 * n + r16;
+        valid[n] = key[n] < keys.count;
+        seen_from[n] = !args.causal || key[n] < prefix ? INT32_MIN / 2 : key[n];
+        const std::int64_t row = keys.first + key[n];
+        const T* k_row = static_cast<const T*>(args.k) + row * args.k_stride + key_head * args.head_dim;
+        const T* v_row = static_cast<const T*>(args.v) + row * args.v_stride + key_head * args.head_dim;
+#pragma unroll
+        for (int t = 0; t < Rows::kSteps; ++t) {
+            const int d = (4 * t + h) * kChunk<T>;
+            k[n][t] = loadRowChunk(k_row + d, valid[n] ? args.head_dim - d : 0);
+            v[n][t] = loadRowChunk(v_row + d, valid[n] ? args.head_dim - d : 0);
+            if (args.scale < 0.0f) {
+                k[n][t] = -k[n][t];
+            }
+        }
+    }
+    f32x4 dk[kBlocks][kDimBlocks], dv[kBlocks][kDimBlocks];
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) {
+            dk[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            dv[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    // query rows from the first that sees one of the workgroup's keys on
+    const int query_begin = args.causal && tile_key >= prefix ? max(tile_key - shift, 0) : 0;
+    const bool any_key = wave_key < keys.count;
+    const int last_key = min(wave_key + kWaveKeys, keys.count) - 1;
+    const bool hidden_keys = args.causal && last_key >= prefix;  // some key of the wavefront is not seen by all
+
+    for (int g = 0; g < args.group; ++g) {
+        const int head = key_head * args.group + g;
+        const float slope = args.slopes != nullptr ? kLog2E * args.slopes[head] : 0.0f;
+        float past[2][kBlocks] = {};  // sums of ds at distances past the table's ends: before, behind
+        __syncthreads();              // the tables and tiles of the head before have been used
+        if (args.table != nullptr) {
+            loadTable<T>(args, head, kMargin, table);
+        }
+        if constexpr (kFar > 0) {
+            for (int i = static_cast<int>(threadIdx.x); i < kGradientWaves * 4 * kBins; i += kGradientThreads) {
+                (&bins[0][0])[i] = 0.0f;
+            }
+        }
+        const std::int64_t first = queries.first + query_begin;
+        Rows q_tile, d_tile;
+        q_tile.begin(static_cast<const T*>(args.q) + first * args.q_stride + head * args.head_dim, args.q_stride,
+                     queries.count - query_begin, args.head_dim, 1);
+        d_tile.begin(static_cast<const T*>(more.out_gradient) + first * more.out_gradient_stride + head * args.head_dim,
+                     more.out_gradient_stride, queries.count - query_begin, args.head_dim, 1);
+        const float* head_stats = more.stats + 2 * (head * args.q_texts.total + queries.first);
+        auto issueStats = [&](int row0, int buffer) {
+            // a dword for each lane of the first wavefront
+            if (wave == 0) {
+                const int row = row0 + (lane >> 1);
+                const float* from = row < queries.count ? head_stats + 2 * row + (lane & 1) : no_row + (lane & 1);
+                copyDwordToLds(from, __builtin_amdgcn_readfirstlane(ldsAddress(&stats[buffer][0][0])));
+            }
+        };
+        if (query_begin < queries.count) {
+            issueStats(query_begin, 0);
+            if constexpr (kDirect) {
+                q_tile.issue(lds, 1);
+                d_tile.issue(lds + Rows::kBytes, 1);
+            } else {
+                q_tile.fetch(1);
+                d_tile.fetch(1);
+                q_tile.put(lds);
+                d_tile.put(lds + Rows::kBytes);
+            }
+        }
+        int buffer = 0;
+        for (int row0 = query_begin; row0 < queries.count; row0 += kQueryTile) {
+            teamSync<kGradientThreads>();
+            const std::uint8_t* q_stage = lds + buffer * kStageBytes;
+            const std::uint8_t* d_stage = q_stage + Rows::kBytes;
+            const float* row_stats = &stats[buffer][0][0];
+            buffer ^= 1;
+            const bool next = row0 + kQueryTile < queries.count;
+            std::uint8_t* other = lds + buffer * kStageBytes;
+            if (next) {
+                issueStats(row0 + kQueryTile, buffer);
+                if constexpr (kDirect) {
+                    q_tile.issue(other, 1);
+                    d_tile.issue(other + Rows::kBytes, 1);
+                } else {
+                    q_tile.fetch(1);
+                    d_tile.fetch(1);
+                }
+            }
+            const int place0 = row0 + shift;  // of the tile's first row
+            if (any_key && !(hidden_keys && wave_key >= prefix && place0 + kQueryTile - 1 < wave_key)) {
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n) {
+                    f32x4 s[kRowBlocks], dp[kRowBlocks], bent[kRowBlocks] = {};
+#pragma unroll
+                    for (int m = 0; m < kRowBlocks; ++m) {
+                        s[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        dp[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int t = 0; t < Rows::kSteps; ++t) {
+                            s[m] = multiplyAdd(Rows::read(q_stage, m, t), k[n][t], s[m]);
+                            dp[m] = multiplyAdd(Rows::read(d_stage, m, t), v[n][t], dp[m]);
+                        }
+                    }
+                    const int distance = key[n] - place0 - 4 * h;  // of the lane's first row; one less a row
+                    bool before = false, behind = false;
+                    if (form.modified) {
+                        formScores<T>(form, s, bent);
+                        if (args.slopes != nullptr) {
+#pragma unroll
+                            for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    s[m][e] -= slope * fabsf(static_cast<float>(distance) - static_cast<float>(16 * m + e));
+                                }
+                            }
+                        }
+                        if (args.table != nullptr) {
+                            const int block_key = wave_key + 16 * n;
+                            before = block_key + 15 - place0 <= -args.max_distance;
+                            behind = block_key - (place0 + kQueryTile - 1) >= args.max_distance;
+                            if (before || behind) {
+                                const float end = table[before ? 0 : 2 * (args.max_distance + kMargin)];
+#pragma unroll
+                                for (int m = 0; m < kRowBlocks; ++m) {
+                                    s[m] += end;
+                                }
+                            } else {
+                                const float* from = table + distance + args.max_distance + kMargin;
+#pragma unroll
+                                for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        s[m][e] += from[-(16 * m + e)];
+                                    }
+                                }
+                            }
+                        }
+                    }
+                    const bool masked = hidden_keys && place0 < last_key;
+#pragma unroll
+                    for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int row = 16 * m + 4 * h + e;
+                            float p = __builtin_amdgcn_exp2f(fmaf(s[m][e], form.unit, -row_stats[2 * row]));
+                            if (masked) {
+                                p = place0 + row >= seen_from[n] ? p : 0.0f;
+                            }
+                            s[m][e] = p;
+                            dp[m][e] = p * (dp[m][e] - row_stats[2 * row + 1]);
+                        }
+                    }
+                    if constexpr (kFar > 0) {
+                        // (keys past the text's end have zeros as their operands, and scores)
+                        float* own = &bins[wave * 4 + h][0] + distance + args.max_distance + kMargin;
+                        if (before || behind) {
+                            float sum = 0.0f;
+#pragma unroll
+                            for (int m = 0; m < kRowBlocks; ++m) {
+                                sum += (dp[m][0] + dp[m][1]) + (dp[m][2] + dp[m][3]);
+                            }
+                            past[before ? 0 : 1][n] += valid[n] ? sum : 0.0f;
+                        } else if (valid[n]) {
+#pragma unroll
+                            for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    __hip_atomic_fetch_add(own - (16 * m + e), dp[m][e], __ATOMIC_RELAXED,
+                                                           __HIP_MEMORY_SCOPE_WORKGROUP);
+                                }
+                            }
+                        }
+                    }
+                    if (form.capped) {
+#pragma unroll
+                        for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                dp[m][e] -= dp[m][e] * bent[m][e];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int pair = 0; pair < kRowBlocks / kTurned; ++pair) {
+                        const auto p = resultFragment<T>(&s[pair * kTurned]);
+                        const auto dr = resultFragment<T>(&dp[pair * kTurned]);
+#pragma unroll
+                        for (int d = 0; d < kDimBlocks; ++d) {
+                            dv[n][d] = multiplyAdd(Rows::readTurned(d_stage, d, pair), p, dv[n][d]);
+                            dk[n][d] = multiplyAdd(Rows::readTurned(q_stage, d, pair), dr, dk[n][d]);
+                        }
+                    }
+                }
+            }
+            if constexpr (!kDirect) {
+                if (next) {
+                    q_tile.put(other);
+                    d_tile.put(other + Rows::kBytes);
+                }
+            }
+        }
+        if constexpr (kFar > 0) {
+            // the lanes' sums past the ends: over the wavefront, then to the ends of its first group's table
+            float ends[2];
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                ends[side] = past[side][0];
+#pragma unroll
+                for (int n = 1; n < kBlocks; ++n) {
+                    ends[side] += past[side][n];
+                }
+#pragma unroll
+                for (int offset = kWave / 2; offset > 0; offset >>= 1) {
+                    ends[side] += waveXor(ends[side], offset);
+                }
+            }
+            if (lane == 0) {
+                bins[wave * 4][kMargin] += ends[0];
+                bins[wave * 4][2 * args.max_distance + kMargin] += ends[1];
+            }
+            __syncthreads();
+            float* to = partialTable(head);
+            for (int i = static_cast<int>(threadIdx.x); i < table_columns; i += kGradientThreads) {
+                const int low = i == 0 ? 0 : i + kMargin;
+                const int high = i == table_columns - 1 ? i + 2 * kMargin : i + kMargin;
+                float sum = 0.0f;
+                for (int w = 0; w < kGradientWaves * 4; ++w) {
+                    for (int b = low; b <= high; ++b) {
+                        sum += bins[w][b];
+                    }
+                }
+                to[i] = sum;
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+        if (key[n] >= keys.rows) {
+            continue;
+        }
+        const std::int64_t row = keys.first + key[n];
+        T* k_to = static_cast<T*>(more.k_gradient) + row * more.k_gradient_stride + key_head * args.head_dim;
+        T* v_to = static_cast<T*>(more.v_gradient) + row * more.v_gradient_stride + key_head * args.head_dim;
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) {
+            const int column = 16 * d + 4 * h;
+            if (column < args.head_dim) {
+                storeFour(valid[n] ? dk[n][d] * args.scale : f32x4{}, k_to + column, args.head_dim - column);
+                storeFour(valid[n] ? dv[n][d] : f32x4{}, v_to + column, args.head_dim - column);
+            }
+        }
+    }
+}
+
+// ---- dq ------------------------------------------------------------------------------------------
+
+template <typename T, int kDim, int kBlocks, bool kDirect>
+__global__ __launch_bounds__(kGradientThreads) void queryGradientKernel(AttentionArgs args, AttentionGradient more) {
+    constexpr int kTileKeys = sizeof(T) == 2 ? 64 : 32;
+    using Keys = RowTile<T, kTileKeys, kDim, kGradientThreads, kDirect>;
+    constexpr int kWaveRows = 16 * kBlocks;
+    constexpr int kRows = kWaveRows * kGradientWaves;
+    constexpr int kStageBytes = 2 * Keys::kBytes;  // keys, then values
+    constexpr int kDimBlocks = kDim / 16;
+    constexpr int kTurned = kBlocksTurned<T>;
+    constexpr int kMargin = kTileKeys + kWaveRows;
+    __shared__ __attribute__((aligned(256))) std::uint8_t lds[2 * kStageBytes];
+    __shared__ float table[2 * (kAttentionMaxDistance + kMargin) + 1];
+
+    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int r16 = lane & 15;
+    const int h = lane >> 4;
+    const int position = positionOf(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    const int slot = position % more.query_slots;
+    const int head = position / more.query_slots;
+    const int key_head = head / args.group;
+    const int text = textOfSlot<kRows>(args.q_texts, 1, slot);
+    if (text < 0) {
+        return;
+    }
+    const TextSpan queries = textSpan(args.q_texts, text);
+    const int tile_row = (slot - (static_cast<int>(queries.first / kRows) + text)) * kRows;
+    if (tile_row < 0 || tile_row >= queries.rows) {
+        return;
+    }
+    const TextSpan keys = textSpan(args.k_texts, text);
+    const int prefix = args.prefix == nullptr ? 0 : args.prefix[text];
+    const int shift = args.q_last ? keys.count - queries.count : 0;
+    auto limitAt = [&](int at) { return args.causal ? min(keys.count, max(max(at + 1, prefix), 0)) : keys.count; };
+    const ScoreForm form(args);
+    const float slope = args.slopes != nullptr ? kLog2E * args.slopes[head] : 0.0f;
+
+    const int wave_row = tile_row + wave * kWaveRows;
+    int place[kBlocks], limit[kBlocks];
+    float lse[kBlocks], delta[kBlocks];
+    typename Fragment<T>::type q[kBlocks][Keys::kSteps], dout[kBlocks][Keys::kSteps];
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m) {
+        const int i = wave_row + 16 * m + r16;
+        const bool valid = i < queries.count;
+        const std::int64_t row = queries.first + i;
+        place[m] = i + shift;
+        limit[m] = valid ? limitAt(place[m]) : 0;
+        const float* row_stats = more.stats + 2 * (head * args.q_texts.total + row);
+        lse[m] = valid ? row_stats[0] : INFINITY;
+        delta[m] = valid ? row_stats[1] : 0.0f;
+        const T* q_row = static_cast<const T*>(args.q) + row * args.q_stride + head * args.head_dim;
+        const T* d_row = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim;
+#pragma unroll
+        for (int t = 0; t < Keys::kSteps; ++t) {
+            const int d = (4 * t + h) * kChunk<T>;
+            q[m][t] = loadRowChunk(q_row + d, valid ? args.head_dim - d : 0);
+            dout[m][t] = loadRowChunk(d_row + d, valid ? args.head_dim - d : 0);
+            if (args.scale < 0.0f) {
+                q[m][t] = -q[m][t];
+            }
+        }
+    }
+    const int last_row = min(wave_row + kWaveRows, queries.count) - 1;
+    const int first_place = wave_row + shift;
+    const int last_place = last_row + shift;
+    // a wavefront with rows that do not count has their limits of zero to mind
+    const int least_limit = last_row - wave_row + 1 == kWaveRows ? limitAt(first_place) : 0;
+    const int most_limit = last_row >= wave_row ? limitAt(last_place) : 0;
+    const int tile_last = min(tile_row + kRows, queries.count) - 1;
+    const int all_keys = tile_last >= tile_row ? limitAt(tile_last + shift) : 0;
+
+    if (args.table != nullptr) {
+        loadTable<T>(args, head, kMargin, table);
+    }
+    f32x4 dq[kBlocks][kDimBlocks];
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) {
+            dq[m][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    Keys k_tile, v_tile;
+    k_tile.begin(static_cast<const T*>(args.k) + keys.first * args.k_stride + key_head * args.head_dim, args.k_stride,
+                 keys.count, args.head_dim, 1);
+    v_tile.begin(static_cast<const T*>(args.v) + keys.first * args.v_stride + key_head * args.head_dim, args.v_stride,
+                 keys.count, args.head_dim, 1);
+    if (all_keys > 0) {
+        if constexpr (kDirect) {
+            k_tile.issue(lds, 1);
+            v_tile.issue(lds + Keys::kBytes, 1);
+        } else {
+            k_tile.fetch(1);
+            v_tile.fetch(1);
+            k_tile.put(lds);
+            v_tile.put(lds + Keys::kBytes);
+        }
+    }
+    int buffer = 0;
+    for (int key0 = 0; key0 < all_keys; key0 += kTileKeys) {
+        teamSync<kGradientThreads>();
+        const std::uint8_t* stage = lds + buffer * kStageBytes;
+        const std::uint8_t* values = stage + Keys::kBytes;
+        buffer ^= 1;
+        std::uint8_t* other = lds + buffer * kStageBytes;
+        const bool next = key0 + kTileKeys < all_keys;
+        if (next) {
+            if constexpr (kDirect) {
+                k_tile.issue(other, 1);
+                v_tile.issue(other + Keys::kBytes, 1);
+            } else {
+                k_tile.fetch(1);
+                v_tile.fetch(1);
+            }
+        }
+#pragma unroll
+        for (int pair = 0; pair < kTileKeys / 16 / kTurned; ++pair) {
+            const int pair_key = key0 + pair * 16 * kTurned;
+            if (pair_key >= most_limit) {
+                continue;
+            }
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+                f32x4 s[kTurned], dp[kTurned], bent[kTurned] = {};
+#pragma unroll
+                for (int b = 0; b < kTurned; ++b) {
+                    s[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    dp[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int t = 0; t < Keys::kSteps; ++t) {
+                        s[b] = multiplyAdd(Keys::read(stage, pair * kTurned + b, t), q[m][t], s[b]);
+                        dp[b] = multiplyAdd(Keys::read(values, pair * kTurned + b, t), dout[m][t], dp[b]);
+                    }
+                }
+                const int distance = pair_key + 4 * h - place[m];
+                if (form.modified) {
+                    formScores<T>(form, s, bent);
+                    if (args.slopes != nullptr) {
+#pragma unroll
+                        for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                s[b][e] -= slope * fabsf(static_cast<float>(distance) + static_cast<float>(16 * b + e));
+                            }
+                        }
+                    }
+                    if (args.table != nullptr) {
+                        const bool behind = pair_key - last_place >= args.max_distance;
+                        const bool before = pair_key + 16 * kTurned - 1 - first_place <= -args.max_distance;
+                        if (before || behind) {
+                            const float end = table[before ? 0 : 2 * (args.max_distance + kMargin)];
+#pragma unroll
+                            for (int b = 0; b < kTurned; ++b) {
+                                s[b] += end;
+                            }
+                        } else {
+                            // rows past the text's last one may reach beyond the margin
+                            const int at = max(distance + args.max_distance + kMargin, 0);
+#pragma unroll
+                            for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    s[b][e] += table[at + 16 * b + e];
+                                }
+                            }
+                        }
+                    }
+                }
+                const bool masked = pair_key + 16 * kTurned > least_limit;
+                const int left = limit[m] - pair_key - 4 * h;
+#pragma unroll
+                for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float p = __builtin_amdgcn_exp2f(fmaf(s[b][e], form.unit, -lse[m]));
+                        if (masked) {
+                            p = 16 * b + e < left ? p : 0.0f;
+                        }
+                        dp[b][e] = p * (dp[b][e] - delta[m]);
+                        if (form.capped) {
+                            dp[b][e] -= dp[b][e] * bent[b][e];
+                        }
+                    }
+                }
+                const auto dr = resultFragment<T>(dp);
+#pragma unroll
+                for (int d = 0; d < kDimBlocks; ++d) {
+                    dq[m][d] = multiplyAdd(Keys::readTurned(stage, d, pair), dr, dq[m][d]);
+                }
+            }
+        }
+        if constexpr (!kDirect) {
+            if (next) {
+                k_tile.put(other);
+                v_tile.put(other + Keys::kBytes);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m) {
+        const int i = wave_row + 16 * m + r16;
+        if (i >= queries.rows) {
+            continue;
+        }
+        T* to = static_cast<T*>(more.q_gradient) + (queries.first + i) * more.q_gradient_stride + head * args.head_dim;
+#pragma unroll
+        for (int d = 0; d < kDimBlocks; ++d) {
+            const int column = 16 * d + 4 * h;
+            if (column < args.head_dim) {
+                storeFour(i < queries.count ? dq[m][d] * args.scale : f32x4{}, to + column, args.head_dim - column);
+            }
+        }
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+template <typename T, int kDim, int kBlocks, bool kDirect>
+int launchKeyGradient(const AttentionArgs& args, const AttentionGradient& more, hipStream_t stream) {
+    const unsigned blocks = static_cast<unsigned>(more.key_slots * (args.heads / args.group));
+    if (more.table_partials == nullptr) {
+        keyGradientKernel<T, kDim, kBlocks, kDirect, 0><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+    } else if (args.max_distance <= 128) {
+        keyGradientKernel<T, kDim, kBlocks, kDirect, 128><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+    } else {
+        keyGradientKernel<T, kDim, kBlocks, kDirect, kAttentionMaxDistance><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+    }
+    ZCGVS_LAUNCH_CHECK("attention gradient");
+    return ZCGVS_OK;
+}
+
+template <typename T, int kDim>
+int launchGradientDim(const AttentionGradientPlan& plan, const AttentionArgs& args, const AttentionGradient& more,
+                      hipStream_t stream) {
+    int status = ZCGVS_OK;
+    constexpr bool kTwo = sizeof(T) == 2 || kDim < 128;  // (as attention.hip plans)
+    if (!kTwo || plan.key_blocks == 1) {
+        status = plan.direct_rows ? launchKeyGradient<T, kDim, 1, true>(args, more, stream)
+                                  : launchKeyGradient<T, kDim, 1, false>(args, more, stream);
+    } else if constexpr (kTwo) {
+        status = plan.direct_rows ? launchKeyGradient<T, kDim, 2, true>(args, more, stream)
+                                  : launchKeyGradient<T, kDim, 2, false>(args, more, stream);
+    }
+    if (status != ZCGVS_OK) {
+        return status;
+    }
+    const unsigned blocks = static_cast<unsigned>(more.query_slots * args.heads);
+    if (plan.query_blocks == 1) {
+        if (plan.direct_keys) {
+            queryGradientKernel<T, kDim, 1, true><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+        } else {
+            queryGradientKernel<T, kDim, 1, false><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+        }
+    } else if (plan.direct_keys) {
+        queryGradientKernel<T, kDim, 2, true><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+    } else {
+        queryGradientKernel<T, kDim, 2, false><<<blocks, kGradientThreads, 0, stream>>>(args, more);
+    }
+    ZCGVS_LAUNCH_CHECK("attention gradient");
+    return ZCGVS_OK;
+}
+
+// out [heads, columns] = the sums over the slots of partials [heads, slots, columns].
+template <typename T>
+__global__ __launch_bounds__(kColumnThreads) void joinTablesKernel(const float* __restrict__ partials, int slots, int columns,
+                                                                   T* __restrict__ out) {
+    joinColumns(partials + static_cast<std::int64_t>(blockIdx.y) * slots * columns, slots, columns,
+                out + static_cast<std::int64_t>(blockIdx.y) * columns);
+}
+
+}  // namespace
+
+template <typename T>
+int launchAttentionGradient(const AttentionGradientPlan& plan, const AttentionArgs& args, const AttentionGradient& more,
+                            hipStream_t stream) {
+    const std::int64_t rows = args.q_texts.total * args.heads;
+    constexpr int kStatsRows = kGradientThreads / kStatsLanes;
+    attentionStatsKernel<T><<<static_cast<unsigned>((rows + kStatsRows - 1) / kStatsRows), kGradientThreads, 0, stream>>>(args, more);
+    ZCGVS_LAUNCH_CHECK("attention gradient");
+    int status;
+    switch (paddedDim(args.head_dim)) {
+        case 32:
+            status = launchGradientDim<T, 32>(plan, args, more, stream);
+            break;
+        case 64:
+            status = launchGradientDim<T, 64>(plan, args, more, stream);
+            break;
+        default:
+            status = launchGradientDim<T, 128>(plan, args, more, stream);
+            break;
+    }
+    if (status == ZCGVS_OK && more.table_partials != nullptr) {
+        const int columns = 2 * args.max_distance + 1;
+        joinTablesKernel<T><<<dim3(static_cast<unsigned>(divideUp(columns, kJoinColumns)), static_cast<unsigned>(args.heads)),
+                              kColumnThreads, 0, stream>>>(more.table_partials, more.key_slots, columns,
+                                                           static_cast<T*>(more.table_gradient));
+        ZCGVS_LAUNCH_CHECK("attention gradient");
+    }
+    return status;
+}
+
+}  // namespace zcgvs_hip

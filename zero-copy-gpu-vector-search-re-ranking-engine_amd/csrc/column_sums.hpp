@@ -17,7 +17,7 @@ constexpr int kJoinColumns = 16;
 constexpr int kJoinLanes = kColumnThreads / kJoinColumns;
 
 template <typename T>
-__global__ __launch_bounds__(kColumnThreads) void joinColumnsKernel(const float* __restrict__ partials, int count, int dim,
+__device__ __forceinline__ void joinColumns(const float* __restrict__ partials, int count, int dim,
                                                                   T* __restrict__ out) {
     __shared__ float shared[kJoinLanes][kJoinColumns];
     const int column = static_cast<int>(threadIdx.x) % kJoinColumns;
@@ -39,6 +39,12 @@ __global__ __launch_bounds__(kColumnThreads) void joinColumnsKernel(const float*
         }
         out[c] = static_cast<T>(sum);
     }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kColumnThreads) void joinColumnsKernel(const float* __restrict__ partials, int count, int dim,
+                                                                    T* __restrict__ out) {
+    joinColumns(partials, count, dim, out);
 }
 
 template <typename T>
