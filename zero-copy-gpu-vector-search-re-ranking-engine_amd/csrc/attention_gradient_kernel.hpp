@@ -73,23 +73,20 @@ __global__ __launch_bounds__(kGradientThreads) void attentionStatsKernel(Attenti
 
 struct ScoreForm {
     bool capped;
-    bool modified;
     float factor;  // log2(e) |scale|
-    float unit;    // factor, or 1 where scores are formed first
     float cap;     // log2(e) cap
     float to_cap;  // |scale| / cap
 
     __device__ __forceinline__ explicit ScoreForm(const AttentionArgs& args) {
         capped = args.cap > 0.0f;
-        modified = capped || args.slopes != nullptr || args.table != nullptr || args.scale == 0.0f;
         factor = kLog2E * fabsf(args.scale);
-        unit = modified ? 1.0f : factor;
         cap = kLog2E * args.cap;
         to_cap = capped ? fabsf(args.scale) / args.cap : 0.0f;
     }
 };
 
-// Raw products -> scores in base 2 before the biases; tangent^2 of the cap goes to `bent`.
+// Raw products -> capped scores in base 2, the tangent's square to `bent`; scores of zero where scale is, which leaves no
+// infinities to the masks.
 template <typename T, int kCount>
 __device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCount], f32x4 (&bent)[kCount]) {
     if (form.capped) {
@@ -105,7 +102,7 @@ __device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCo
     } else {
 #pragma unroll
         for (int b = 0; b < kCount; ++b) {
-            s[b] *= form.factor;
+            s[b] *= 0.0f;
         }
     }
 }
@@ -122,9 +119,15 @@ __device__ __forceinline__ void loadTable(const AttentionArgs& args, int head, i
 
 // ---- dk, dv and the bias's partial sums ----------------------------------------------------------
 
+// Wavefronts of a SIMD that the registers do for; the bound also keeps sums out of the accumulation registers.
+template <typename T, int kDim, int kBlocks>
+constexpr int kKeyResident = kBlocks * kDim * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1;
+template <typename T, int kDim, int kBlocks>
+constexpr int kQueryResident = kBlocks * kDim * static_cast<int>(sizeof(T)) <= 512 ? 2 : 1;
+
 // kFar: the largest max_distance whose gradient is wanted (0: none).
 template <typename T, int kDim, int kBlocks, bool kDirect, int kFar>
-__global__ __launch_bounds__(kGradientThreads) void keyGradientKernel(AttentionArgs args, AttentionGradient more) {
+__global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>)) void keyGradientKernel(AttentionArgs args, AttentionGradient more) {
     using Rows = RowTile<T, kQueryTile, kDim, kGradientThreads, kDirect>;
     constexpr int kWaveKeys = 16 * kBlocks;
     constexpr int kKeys = kWaveKeys * kGradientWaves;
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(kGradientThreads) void keyGradientKernel(AttentionA
     for (int g = 0; g < args.group; ++g) {
         const int head = key_head * args.group + g;
         const float slope = args.slopes != nullptr ? kLog2E * args.slopes[head] : 0.0f;
-        float past[2][kBlocks] = {};  // sums of ds at distances past the table's ends: before, behind
+        float past[2] = {};  // sums of ds at distances past the table's ends: before, behind
         __syncthreads();              // the tables and tiles of the head before have been used
         if (args.table != nullptr) {
             loadTable<T>(args, head, kMargin, table);
@@ -270,106 +273,141 @@ __global__ __launch_bounds__(kGradientThreads) void keyGradientKernel(AttentionA
             }
             const int place0 = row0 + shift;  // of the tile's first row
             if (any_key && !(hidden_keys && wave_key >= prefix && place0 + kQueryTile - 1 < wave_key)) {
+                f32x4 s[kBlocks][kRowBlocks], dp[kBlocks][kRowBlocks], bent[kBlocks][kRowBlocks] = {};
 #pragma unroll
-                for (int n = 0; n < kBlocks; ++n) {
-                    f32x4 s[kRowBlocks], dp[kRowBlocks], bent[kRowBlocks] = {};
+                for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
-                    for (int m = 0; m < kRowBlocks; ++m) {
-                        s[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                        dp[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int n = 0; n < kBlocks; ++n) {
+                        s[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        dp[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
 #pragma unroll
-                        for (int t = 0; t < Rows::kSteps; ++t) {
-                            s[m] = multiplyAdd(Rows::read(q_stage, m, t), k[n][t], s[m]);
-                            dp[m] = multiplyAdd(Rows::read(d_stage, m, t), v[n][t], dp[m]);
+                    for (int t = 0; t < Rows::kSteps; ++t) {
+                        const auto q = Rows::read(q_stage, m, t);
+                        const auto d = Rows::read(d_stage, m, t);
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
+                            s[n][m] = multiplyAdd(q, k[n][t], s[n][m]);
+                            dp[n][m] = multiplyAdd(d, v[n][t], dp[n][m]);
                         }
                     }
-                    const int distance = key[n] - place0 - 4 * h;  // of the lane's first row; one less a row
-                    bool before = false, behind = false;
-                    if (form.modified) {
-                        formScores<T>(form, s, bent);
-                        if (args.slopes != nullptr) {
+                }
+                float score_factor = form.factor, score_offset = 0.0f;
+                if (form.capped || args.scale == 0.0f) {
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) {
+                        formScores<T>(form, s[n], bent[n]);
+                    }
+                    score_factor = 1.0f;
+                }
+                if (args.slopes != nullptr) {
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) {
+                        const float distance = static_cast<float>(key[n] - place0 - 4 * h);  // of the lane's first row
+#pragma unroll
+                        for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                s[n][m][e] = fmaf(-slope, fabsf(distance - static_cast<float>(16 * m + e)), s[n][m][e] * score_factor);
+                            }
+                        }
+                    }
+                    score_factor = 1.0f;
+                }
+                bool before = false, behind = false;
+                if (args.table != nullptr) {
+                    before = wave_key + kWaveKeys - 1 - place0 <= -args.max_distance;
+                    behind = wave_key - (place0 + kQueryTile - 1) >= args.max_distance;
+                    if (before || behind) {
+                        score_offset = table[before ? 0 : 2 * (args.max_distance + kMargin)];
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
+                            const float* from = table + key[n] - place0 - 4 * h + args.max_distance + kMargin;
 #pragma unroll
                             for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    s[m][e] -= slope * fabsf(static_cast<float>(distance) - static_cast<float>(16 * m + e));
+                                    s[n][m][e] = fmaf(s[n][m][e], score_factor, from[-(16 * m + e)]);
                                 }
                             }
                         }
-                        if (args.table != nullptr) {
-                            const int block_key = wave_key + 16 * n;
-                            before = block_key + 15 - place0 <= -args.max_distance;
-                            behind = block_key - (place0 + kQueryTile - 1) >= args.max_distance;
-                            if (before || behind) {
-                                const float end = table[before ? 0 : 2 * (args.max_distance + kMargin)];
-#pragma unroll
-                                for (int m = 0; m < kRowBlocks; ++m) {
-                                    s[m] += end;
-                                }
-                            } else {
-                                const float* from = table + distance + args.max_distance + kMargin;
-#pragma unroll
-                                for (int m = 0; m < kRowBlocks; ++m) {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        s[m][e] += from[-(16 * m + e)];
-                                    }
-                                }
-                            }
-                        }
+                        score_factor = 1.0f;
                     }
-                    const bool masked = hidden_keys && place0 < last_key;
+                }
+                const bool masked = hidden_keys && place0 < last_key;
 #pragma unroll
-                    for (int m = 0; m < kRowBlocks; ++m) {
+                for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int row = 16 * m + 4 * h + e;
-                            float p = __builtin_amdgcn_exp2f(fmaf(s[m][e], form.unit, -row_stats[2 * row]));
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = 16 * m + 4 * h + e;
+                        const float off = score_offset - row_stats[2 * row];
+                        const float delta = row_stats[2 * row + 1];
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
+                            float p = __builtin_amdgcn_exp2f(fmaf(s[n][m][e], score_factor, off));
                             if (masked) {
                                 p = place0 + row >= seen_from[n] ? p : 0.0f;
                             }
-                            s[m][e] = p;
-                            dp[m][e] = p * (dp[m][e] - row_stats[2 * row + 1]);
+                            s[n][m][e] = p;
+                            dp[n][m][e] = p * (dp[n][m][e] - delta);
                         }
                     }
-                    if constexpr (kFar > 0) {
-                        // (keys past the text's end have zeros as their operands, and scores)
-                        float* own = &bins[wave * 4 + h][0] + distance + args.max_distance + kMargin;
+                }
+                if constexpr (kFar > 0) {
+                    // (keys past the text's end have zeros as their operands, and scores)
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) {
                         if (before || behind) {
                             float sum = 0.0f;
 #pragma unroll
                             for (int m = 0; m < kRowBlocks; ++m) {
-                                sum += (dp[m][0] + dp[m][1]) + (dp[m][2] + dp[m][3]);
+                                sum += (dp[n][m][0] + dp[n][m][1]) + (dp[n][m][2] + dp[n][m][3]);
                             }
-                            past[before ? 0 : 1][n] += valid[n] ? sum : 0.0f;
+                            sum = valid[n] ? sum : 0.0f;
+                            past[0] += before ? sum : 0.0f;
+                            past[1] += before ? 0.0f : sum;
                         } else if (valid[n]) {
+                            float* own = &bins[wave * 4 + h][0] + key[n] - place0 - 4 * h + args.max_distance + kMargin;
 #pragma unroll
                             for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    __hip_atomic_fetch_add(own - (16 * m + e), dp[m][e], __ATOMIC_RELAXED,
+                                    __hip_atomic_fetch_add(own - (16 * m + e), dp[n][m][e], __ATOMIC_RELAXED,
                                                            __HIP_MEMORY_SCOPE_WORKGROUP);
                                 }
                             }
                         }
                     }
-                    if (form.capped) {
+                }
+                if (form.capped) {
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
                         for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                dp[m][e] -= dp[m][e] * bent[m][e];
+                                dp[n][m][e] = fmaf(-dp[n][m][e], bent[n][m][e], dp[n][m][e]);
                             }
                         }
                     }
+                }
 #pragma unroll
-                    for (int pair = 0; pair < kRowBlocks / kTurned; ++pair) {
-                        const auto p = resultFragment<T>(&s[pair * kTurned]);
-                        const auto dr = resultFragment<T>(&dp[pair * kTurned]);
+                for (int pair = 0; pair < kRowBlocks / kTurned; ++pair) {
+                    typename Fragment<T>::type p[kBlocks], dr[kBlocks];
 #pragma unroll
-                        for (int d = 0; d < kDimBlocks; ++d) {
-                            dv[n][d] = multiplyAdd(Rows::readTurned(d_stage, d, pair), p, dv[n][d]);
-                            dk[n][d] = multiplyAdd(Rows::readTurned(q_stage, d, pair), dr, dk[n][d]);
+                    for (int n = 0; n < kBlocks; ++n) {
+                        p[n] = resultFragment<T>(&s[n][pair * kTurned]);
+                        dr[n] = resultFragment<T>(&dp[n][pair * kTurned]);
+                    }
+#pragma unroll
+                    for (int d = 0; d < kDimBlocks; ++d) {
+                        const auto dout = Rows::readTurned(d_stage, d, pair);
+                        const auto q = Rows::readTurned(q_stage, d, pair);
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
+                            dv[n][d] = multiplyAdd(dout, p[n], dv[n][d]);
+                            dk[n][d] = multiplyAdd(q, dr[n], dk[n][d]);
                         }
                     }
                 }
@@ -386,11 +424,7 @@ __global__ __launch_bounds__(kGradientThreads) void keyGradientKernel(AttentionA
             float ends[2];
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
-                ends[side] = past[side][0];
-#pragma unroll
-                for (int n = 1; n < kBlocks; ++n) {
-                    ends[side] += past[side][n];
-                }
+                ends[side] = past[side];
 #pragma unroll
                 for (int offset = kWave / 2; offset > 0; offset >>= 1) {
                     ends[side] += waveXor(ends[side], offset);
@@ -437,7 +471,7 @@ __global__ __launch_bounds__(kGradientThreads) void keyGradientKernel(AttentionA
 // ---- dq ------------------------------------------------------------------------------------------
 
 template <typename T, int kDim, int kBlocks, bool kDirect>
-__global__ __launch_bounds__(kGradientThreads) void queryGradientKernel(AttentionArgs args, AttentionGradient more) {
+__global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>)) void queryGradientKernel(AttentionArgs args, AttentionGradient more) {
     constexpr int kTileKeys = sizeof(T) == 2 ? 64 : 32;
     using Keys = RowTile<T, kTileKeys, kDim, kGradientThreads, kDirect>;
     constexpr int kWaveRows = 16 * kBlocks;
@@ -558,73 +592,96 @@ __global__ __launch_bounds__(kGradientThreads) void queryGradientKernel(Attentio
             if (pair_key >= most_limit) {
                 continue;
             }
+            f32x4 s[kBlocks][kTurned], dp[kBlocks][kTurned], bent[kBlocks][kTurned] = {};
 #pragma unroll
-            for (int m = 0; m < kBlocks; ++m) {
-                f32x4 s[kTurned], dp[kTurned], bent[kTurned] = {};
+            for (int b = 0; b < kTurned; ++b) {
 #pragma unroll
-                for (int b = 0; b < kTurned; ++b) {
-                    s[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    dp[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int m = 0; m < kBlocks; ++m) {
+                    s[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    dp[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
 #pragma unroll
-                    for (int t = 0; t < Keys::kSteps; ++t) {
-                        s[b] = multiplyAdd(Keys::read(stage, pair * kTurned + b, t), q[m][t], s[b]);
-                        dp[b] = multiplyAdd(Keys::read(values, pair * kTurned + b, t), dout[m][t], dp[b]);
+                for (int t = 0; t < Keys::kSteps; ++t) {
+                    const auto k = Keys::read(stage, pair * kTurned + b, t);
+                    const auto v = Keys::read(values, pair * kTurned + b, t);
+#pragma unroll
+                    for (int m = 0; m < kBlocks; ++m) {
+                        s[m][b] = multiplyAdd(k, q[m][t], s[m][b]);
+                        dp[m][b] = multiplyAdd(v, dout[m][t], dp[m][b]);
                     }
                 }
-                const int distance = pair_key + 4 * h - place[m];
-                if (form.modified) {
-                    formScores<T>(form, s, bent);
-                    if (args.slopes != nullptr) {
+            }
+            float score_factor = form.factor, score_offset = 0.0f;
+            if (form.capped || args.scale == 0.0f) {
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    formScores<T>(form, s[m], bent[m]);
+                }
+                score_factor = 1.0f;
+            }
+            if (args.slopes != nullptr) {
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    const float distance = static_cast<float>(pair_key + 4 * h - place[m]);
+#pragma unroll
+                    for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[m][b][e] = fmaf(-slope, fabsf(distance + static_cast<float>(16 * b + e)), s[m][b][e] * score_factor);
+                        }
+                    }
+                }
+                score_factor = 1.0f;
+            }
+            if (args.table != nullptr) {
+                const bool behind = pair_key - last_place >= args.max_distance;
+                const bool before = pair_key + 16 * kTurned - 1 - first_place <= -args.max_distance;
+                if (before || behind) {
+                    score_offset = table[before ? 0 : 2 * (args.max_distance + kMargin)];
+                } else {
+#pragma unroll
+                    for (int m = 0; m < kBlocks; ++m) {
+                        // rows past the text's last one may reach beyond the margin
+                        const float* from = table + max(pair_key + 4 * h - place[m] + args.max_distance + kMargin, 0);
 #pragma unroll
                         for (int b = 0; b < kTurned; ++b) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                s[b][e] -= slope * fabsf(static_cast<float>(distance) + static_cast<float>(16 * b + e));
+                                s[m][b][e] = fmaf(s[m][b][e], score_factor, from[16 * b + e]);
                             }
                         }
                     }
-                    if (args.table != nullptr) {
-                        const bool behind = pair_key - last_place >= args.max_distance;
-                        const bool before = pair_key + 16 * kTurned - 1 - first_place <= -args.max_distance;
-                        if (before || behind) {
-                            const float end = table[before ? 0 : 2 * (args.max_distance + kMargin)];
-#pragma unroll
-                            for (int b = 0; b < kTurned; ++b) {
-                                s[b] += end;
-                            }
-                        } else {
-                            // rows past the text's last one may reach beyond the margin
-                            const int at = max(distance + args.max_distance + kMargin, 0);
-#pragma unroll
-                            for (int b = 0; b < kTurned; ++b) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    s[b][e] += table[at + 16 * b + e];
-                                }
-                            }
-                        }
-                    }
+                    score_factor = 1.0f;
                 }
-                const bool masked = pair_key + 16 * kTurned > least_limit;
+            }
+            const bool masked = pair_key + 16 * kTurned > least_limit;
+            typename Fragment<T>::type dr[kBlocks];
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
                 const int left = limit[m] - pair_key - 4 * h;
+                const float off = score_offset - lse[m];
 #pragma unroll
                 for (int b = 0; b < kTurned; ++b) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float p = __builtin_amdgcn_exp2f(fmaf(s[b][e], form.unit, -lse[m]));
+                        float p = __builtin_amdgcn_exp2f(fmaf(s[m][b][e], score_factor, off));
                         if (masked) {
                             p = 16 * b + e < left ? p : 0.0f;
                         }
-                        dp[b][e] = p * (dp[b][e] - delta[m]);
+                        dp[m][b][e] = p * (dp[m][b][e] - delta[m]);
                         if (form.capped) {
-                            dp[b][e] -= dp[b][e] * bent[b][e];
+                            dp[m][b][e] = fmaf(-dp[m][b][e], bent[m][b][e], dp[m][b][e]);
                         }
                     }
                 }
-                const auto dr = resultFragment<T>(dp);
+                dr[m] = resultFragment<T>(dp[m]);
+            }
 #pragma unroll
-                for (int d = 0; d < kDimBlocks; ++d) {
-                    dq[m][d] = multiplyAdd(Keys::readTurned(stage, d, pair), dr, dq[m][d]);
+            for (int d = 0; d < kDimBlocks; ++d) {
+                const auto k = Keys::readTurned(stage, d, pair);
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    dq[m][d] = multiplyAdd(k, dr[m], dq[m][d]);
                 }
             }
         }

@@ -44,6 +44,12 @@ struct AttentionTile {
     static constexpr int kTableFloats = kNarrow ? kNarrowTable : 2 * (kAttentionMaxDistance + kMargin) + 1;
 };
 
+// Wavefronts of a SIMD: two, for which the registers of all but wide float32 rows do. The bound also keeps the sums in
+// ordinary registers: with more of them to spend, tiles went through the accumulation registers and back
+// (768 us for 128 texts of 64 to 1024 tokens, 12 heads of 64, that take 306).
+template <typename T, int kDim, int kBlocks>
+constexpr int kAttentionResident = sizeof(T) == 4 && kDim == 128 && kBlocks == 2 ? 1 : 2;
+
 // The largest of a lane's value over the four lanes of its row.
 __device__ __forceinline__ float overGroups(float value) {
     value = fmaxf(value, waveXor(value, 16));
@@ -51,7 +57,7 @@ __device__ __forceinline__ float overGroups(float value) {
 }
 
 template <typename T, int kDim, int kBlocks, bool kNarrow, bool kDirect>
-__global__ __launch_bounds__(kAttentionThreads) void attentionKernel(AttentionArgs args, AttentionOutput output) {
+__global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBlocks>)) void attentionKernel(AttentionArgs args, AttentionOutput output) {
     using Tile = AttentionTile<T, kDim, kBlocks, kNarrow>;
     using Keys = RowTile<T, Tile::kTileKeys, kDim, Tile::kTeam, kDirect>;
     constexpr int kTeams = kNarrow ? kAttentionWaves : 1;
@@ -123,10 +129,7 @@ __global__ __launch_bounds__(kAttentionThreads) void attentionKernel(AttentionAr
     const int tile_end = min(tiles_all, (split + 1) * tiles_each);
 
     const bool capped = args.cap > 0.0f;
-    // (a factor of zero has no infinities to leave to the masks)
-    const bool modified = capped || args.slopes != nullptr || args.table != nullptr || args.scale == 0.0f;
     const float factor = kLog2E * fabsf(args.scale);
-    const float unit_factor = modified ? 1.0f : factor;
     const float cap = kLog2E * args.cap;
     const float to_cap = capped ? fabsf(args.scale) / args.cap : 0.0f;
     float slope[kBlocks];
@@ -189,68 +192,70 @@ __global__ __launch_bounds__(kAttentionThreads) void attentionKernel(AttentionAr
                 }
             }
         }
-        if (modified) {
-            if (capped) {
+        // scores are s * score_factor + score_offset in base 2
+        float score_factor = factor;
+        float score_offset[kBlocks] = {};
+        if (capped) {
 #pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[m][b][e] = cap * tanhOf<T>(s[m][b][e] * to_cap);
+                    }
+                }
+            }
+            score_factor = 1.0f;
+        } else if (args.scale == 0.0f) {
+            // a factor of zero leaves no infinities for the masks
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+                    s[m][b] *= 0.0f;
+                }
+            }
+            score_factor = 1.0f;
+        }
+        if (args.slopes != nullptr) {
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+                const float distance = static_cast<float>(key0 + 4 * h - place[m]);
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[m][b][e] = fmaf(-slope[m], fabsf(distance + static_cast<float>(16 * b + e)), s[m][b][e] * score_factor);
+                    }
+                }
+            }
+            score_factor = 1.0f;
+        }
+        if (args.table != nullptr) {
+            const int nearest = key0 - last_place;                          // the least distance of the tile
+            const int farthest = key0 + Tile::kTileKeys - 1 - first_place;  // the largest
+            const bool behind = nearest >= args.max_distance, before = farthest <= -args.max_distance;
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+                const int base = (kNarrow ? head[m] - unit * group : 0) * table_width;
+                if (behind || before) {
+                    score_offset[m] = table[base + (behind ? table_width - 1 : 0)];
+                } else {
+                    // rows past the text's last one may reach beyond the margin
+                    const int at = min(max(key0 + 4 * h - place[m] + args.max_distance + Tile::kMargin, 0),
+                                       table_width - Tile::kTileKeys + 12);
+                    const float* from = table + base + at;
 #pragma unroll
                     for (int b = 0; b < Tile::kKeyBlocks; ++b) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            s[m][b][e] = cap * tanhOf<T>(s[m][b][e] * to_cap);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
-#pragma unroll
-                    for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-                        s[m][b] *= factor;
-                    }
-                }
-            }
-            if (args.slopes != nullptr) {
-#pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
-                    const float distance = static_cast<float>(key0 + 4 * h - place[m]);
-#pragma unroll
-                    for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[m][b][e] -= slope[m] * fabsf(distance + static_cast<float>(16 * b + e));
+                            s[m][b][e] = fmaf(s[m][b][e], score_factor, from[16 * b + e]);
                         }
                     }
                 }
             }
-            if (args.table != nullptr) {
-                const int nearest = key0 - last_place;                       // the least distance of the tile
-                const int farthest = key0 + Tile::kTileKeys - 1 - first_place;  // the largest
-                const bool right = nearest >= args.max_distance, left = farthest <= -args.max_distance;
-#pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
-                    const int base = (kNarrow ? head[m] - unit * group : 0) * table_width;
-                    if (right || left) {
-                        const float end = table[base + (right ? table_width - 1 : 0)];
-#pragma unroll
-                        for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-                            s[m][b] += end;
-                        }
-                    } else {
-                        // rows past the text's last one may reach beyond the margin
-                        const int at = min(max(key0 + 4 * h - place[m] + args.max_distance + Tile::kMargin, 0),
-                                           table_width - Tile::kTileKeys + 12);
-                        const float* from = table + base + at;
-#pragma unroll
-                        for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                s[m][b][e] += from[16 * b + e];
-                            }
-                        }
-                    }
-                }
-            }
+            score_factor = behind || before ? score_factor : 1.0f;
         }
         if (key0 + Tile::kTileKeys > least_limit) {
 #pragma unroll
@@ -269,12 +274,15 @@ __global__ __launch_bounds__(kAttentionThreads) void attentionKernel(AttentionAr
         float peak[kBlocks];
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) {
-            peak[m] = fmaxf(fmaxf(s[m][0][0], s[m][0][1]), fmaxf(s[m][0][2], s[m][0][3]));
+            peak[m] = s[m][0][0];
 #pragma unroll
-            for (int b = 1; b < Tile::kKeyBlocks; ++b) {
-                peak[m] = fmaxf(fmaxf(peak[m], fmaxf(s[m][b][0], s[m][b][1])), fmaxf(s[m][b][2], s[m][b][3]));
+            for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    peak[m] = __builtin_elementwise_maximum(peak[m], s[m][b][e]);
+                }
             }
-            peak[m] = overGroups(peak[m]) * unit_factor;
+            peak[m] = fmaf(overGroups(peak[m]), score_factor, score_offset[m]);
             raise = raise || peak[m] > largest[m] + 8.0f;
         }
         if (__ballot(raise) != 0) {
@@ -294,12 +302,12 @@ __global__ __launch_bounds__(kAttentionThreads) void attentionKernel(AttentionAr
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m) {
             // a row that has seen no key yet has only scores of minus infinity
-            const float off = largest[m] == -INFINITY ? 0.0f : largest[m];
+            const float off = score_offset[m] - (largest[m] == -INFINITY ? 0.0f : largest[m]);
 #pragma unroll
             for (int b = 0; b < Tile::kKeyBlocks; ++b) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[m][b][e] = __builtin_amdgcn_exp2f(fmaf(s[m][b][e], unit_factor, -off));
+                    s[m][b][e] = __builtin_amdgcn_exp2f(fmaf(s[m][b][e], score_factor, off));
                     total[m] += s[m][b][e];
                 }
             }
