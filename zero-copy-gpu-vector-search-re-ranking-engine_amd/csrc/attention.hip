@@ -136,7 +136,7 @@ std::size_t partialFloats(const zcgvs_attention_desc& d, int splits, int each) {
 int gradientBlocks(std::int64_t rows, std::int64_t texts) { return rows <= 64 * texts ? 1 : 2; }
 
 int keyBlocks(const zcgvs_attention_desc& d) {
-    const char* E = getenv("KB"); return (d.dtype == ZCGVS_DTYPE_F32 || E) && paddedDim(d.head_dim) == 128 ? 1 : gradientBlocks(d.k_rows, d.texts);
+    return paddedDim(d.head_dim) == 128 ? 1 : gradientBlocks(d.k_rows, d.texts);
 }
 
 long long slotsFor(std::int64_t rows, std::int64_t texts, int blocks) { return rows / (64 * blocks) + texts; }

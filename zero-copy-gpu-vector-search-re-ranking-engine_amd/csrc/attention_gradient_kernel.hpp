@@ -11,9 +11,10 @@
 //    rows of one key, which is how the products over the rows take p and dr: they stay in registers.
 // 3. dq: a wavefront keeps 16 or 32 query rows and goes through the keys, as the forward kernel does.
 // So p is formed twice: seven products instead of five, for sums in one order and no float32 copy of dq.
-// The bias's gradient: every lane group of a wavefront adds to a table of its own in LDS (the 16 lanes of a group
-// always meet 16 different distances, so the order of its additions is the program's), with room for distances past
-// the table's ends; tiles that lie past them altogether add to two registers. A workgroup joins its tables and writes
+// The bias's gradient: a wavefront adds its tile up along the diagonals by moving rows along the lanes, and every lane
+// group adds the result to a table of its own in LDS (its 16 lanes always meet 16 different distances, so the order of
+// additions is the program's), with room for distances past the table's ends; tiles that lie past them altogether add
+// to two registers. A workgroup joins its tables and writes
 // one of partial sums a head, which the last launch adds in the order of the workgroups.
 #pragma once
 
@@ -34,38 +35,49 @@ static __device__ const float no_row[2] = {INFINITY, 0.0f};  // p = 0
 
 // ---- rows: lse in base 2 and delta, [heads, q_rows, 2] -------------------------------------------
 
-constexpr int kStatsLanes = 16;  // of a row and head
+// Workgroups of 16 rows and up to 64 heads, so that a head's rows are written together.
+constexpr int kStatsLanes = 8;  // of a row and head, 16 bytes each
+constexpr int kStatsRows = 16;
+constexpr int kStatsHeads = 64;
 
 template <typename T>
 __global__ __launch_bounds__(kGradientThreads) void attentionStatsKernel(AttentionArgs args, AttentionGradient more) {
+    __shared__ float shared[kStatsHeads][kStatsRows][2];
     const int lane = static_cast<int>(threadIdx.x) % kStatsLanes;
-    const std::int64_t at =
-        static_cast<std::int64_t>(blockIdx.x) * (kGradientThreads / kStatsLanes) + threadIdx.x / kStatsLanes;
-    if (at >= args.q_texts.total * args.heads) {
-        return;  // (all lanes of a row and head)
-    }
-    const std::int64_t row = at / args.heads;
-    const int head = static_cast<int>(at % args.heads);
-    const T* out = static_cast<const T*>(more.out) + row * more.out_stride + head * args.head_dim;
-    const T* from = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim;
-    float sum = 0.0f;
-    for (int d = 4 * lane; d < args.head_dim; d += 4 * kStatsLanes) {
-        const f32x4 a = loadFour(out + d, args.head_dim - d);
-        const f32x4 b = loadFour(from + d, args.head_dim - d);
+    const std::int64_t first_row = static_cast<std::int64_t>(blockIdx.x) * kStatsRows;
+    const int first_head = static_cast<int>(blockIdx.y) * kStatsHeads;
+    const int heads = min(args.heads - first_head, kStatsHeads);
+    const int rows = static_cast<int>(min<std::int64_t>(args.q_texts.total - first_row, kStatsRows));
+    for (int i = static_cast<int>(threadIdx.x) / kStatsLanes; i < rows * heads; i += kGradientThreads / kStatsLanes) {
+        const std::int64_t row = first_row + i / heads;
+        const int head = first_head + i % heads;
+        const T* out = static_cast<const T*>(more.out) + row * more.out_stride + head * args.head_dim;
+        const T* from = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim;
+        float sum = 0.0f;
+        for (int d = kChunk<T> * lane; d < args.head_dim; d += kChunk<T> * kStatsLanes) {
+            const auto a = loadRowChunk(out + d, args.head_dim - d);
+            const auto b = loadRowChunk(from + d, args.head_dim - d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            sum = fmaf(a[e], b[e], sum);
+            for (int e = 0; e < kChunk<T>; ++e) {
+                sum = fmaf(static_cast<float>(a[e]), static_cast<float>(b[e]), sum);
+            }
+        }
+#pragma unroll
+        for (int offset = kStatsLanes / 2; offset > 0; offset >>= 1) {
+            sum += waveXor(sum, offset);
+        }
+        if (lane == 0) {
+            const float lse = more.lse[row * args.heads + head];
+            float* to = shared[head - first_head][i / heads];
+            to[0] = lse == -INFINITY ? INFINITY : kLog2E * lse;
+            to[1] = lse == -INFINITY ? 0.0f : sum;
         }
     }
-#pragma unroll
-    for (int offset = kStatsLanes / 2; offset > 0; offset >>= 1) {
-        sum += waveXor(sum, offset);
-    }
-    if (lane == 0) {
-        const float lse = more.lse[at];
-        float* to = more.stats + 2 * (head * args.q_texts.total + row);
-        to[0] = lse == -INFINITY ? INFINITY : kLog2E * lse;
-        to[1] = lse == -INFINITY ? 0.0f : sum;
+    __syncthreads();
+    for (int i = static_cast<int>(threadIdx.x); i < heads * rows * 2; i += kGradientThreads) {
+        const int head = i / (2 * rows);
+        const int at = i - head * 2 * rows;
+        more.stats[2 * ((first_head + head) * args.q_texts.total + first_row) + at] = shared[head][at / 2][at % 2];
     }
 }
 
@@ -119,6 +131,16 @@ __device__ __forceinline__ void loadTable(const AttentionArgs& args, int head, i
 
 // ---- dk, dv and the bias's partial sums ----------------------------------------------------------
 
+// The value of the lane kBy lanes after (before) within a group of 16, zero past its end.
+template <int kBy>
+__device__ __forceinline__ float fromLaneAfter(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x100 + kBy, 0xF, 0xF, true));
+}
+template <int kBy>
+__device__ __forceinline__ float fromLaneBefore(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x110 + kBy, 0xF, 0xF, true));
+}
+
 // Wavefronts of a SIMD that the registers do for; the bound also keeps sums out of the accumulation registers.
 template <typename T, int kDim, int kBlocks>
 constexpr int kKeyResident = kBlocks * kDim * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1;
@@ -135,12 +157,15 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
     constexpr int kDimBlocks = kDim / 16;
     constexpr int kRowBlocks = kQueryTile / 16;
     constexpr int kTurned = kBlocksTurned<T>;
-    constexpr int kMargin = kQueryTile + kWaveKeys;
-    constexpr int kBins = kFar > 0 ? 2 * (kFar + kMargin) + 1 : 1;
+    constexpr int kMargin = kQueryTile + kWaveKeys + 16;
+    // the four groups of a wavefront add to 64 different banks
+    constexpr int kBins = kFar > 0 ? (2 * (kFar + kMargin) + 1 + 43) / 64 * 64 + 20 : 1;
+    static_assert(kFar == 0 || (kBins % 64 == 20 && kBins >= 2 * (kFar + kMargin) + 1), "a table holds its distances");
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[2 * kStageBytes];
     __shared__ __attribute__((aligned(256))) float stats[2][kQueryTile][2];
     __shared__ float table[2 * (kAttentionMaxDistance + kMargin) + 1];
     __shared__ float bins[kFar > 0 ? kGradientWaves * 4 : 1][kBins];
+    __shared__ float past_ends[2];
 
     const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -355,28 +380,52 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                     }
                 }
                 if constexpr (kFar > 0) {
-                    // (keys past the text's end have zeros as their operands, and scores)
+                    if (wave_key + kWaveKeys > keys.count) {
+                        // keys past the text's end have zeros as their operands, and scores
 #pragma unroll
-                    for (int n = 0; n < kBlocks; ++n) {
-                        if (before || behind) {
-                            float sum = 0.0f;
+                        for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+                            for (int m = 0; m < kRowBlocks; ++m) {
+                                dp[n][m] = valid[n] ? dp[n][m] : f32x4{};
+                            }
+                        }
+                    }
+                    if (before || behind) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
                             for (int m = 0; m < kRowBlocks; ++m) {
                                 sum += (dp[n][m][0] + dp[n][m][1]) + (dp[n][m][2] + dp[n][m][3]);
                             }
-                            sum = valid[n] ? sum : 0.0f;
-                            past[0] += before ? sum : 0.0f;
-                            past[1] += before ? 0.0f : sum;
-                        } else if (valid[n]) {
-                            float* own = &bins[wave * 4 + h][0] + key[n] - place0 - 4 * h + args.max_distance + kMargin;
+                        }
+                        past[0] += before ? sum : 0.0f;
+                        past[1] += before ? 0.0f : sum;
+                    } else {
+                        // Row e of a lane's four moved e lanes along: lane x then holds distance x - 4 h, and what moved
+                        // past the group's end the distance 16 less. Blocks on one diagonal add up before they go to
+                        // the table.
+                        float along[kBlocks + kRowBlocks] = {};  // at distances 16 (i - kRowBlocks) more
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
                             for (int m = 0; m < kRowBlocks; ++m) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    __hip_atomic_fetch_add(own - (16 * m + e), dp[n][m][e], __ATOMIC_RELAXED,
-                                                           __HIP_MEMORY_SCOPE_WORKGROUP);
-                                }
+                                float& here = along[n - m + kRowBlocks];
+                                float& less = along[n - m + kRowBlocks - 1];
+                                here += dp[n][m][0];
+                                here += fromLaneAfter<1>(dp[n][m][1]);
+                                here += fromLaneAfter<2>(dp[n][m][2]);
+                                here += fromLaneAfter<3>(dp[n][m][3]);
+                                less += fromLaneBefore<15>(dp[n][m][1]);
+                                less += fromLaneBefore<14>(dp[n][m][2]);
+                                less += fromLaneBefore<13>(dp[n][m][3]);
                             }
+                        }
+                        float* own = &bins[wave * 4 + h][0] + wave_key + r16 - place0 - 4 * h + args.max_distance + kMargin;
+#pragma unroll
+                        for (int i = 0; i < kBlocks + kRowBlocks; ++i) {
+                            __hip_atomic_fetch_add(own + 16 * (i - kRowBlocks), along[i], __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
                         }
                     }
                 }
@@ -435,16 +484,38 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                 bins[wave * 4][2 * args.max_distance + kMargin] += ends[1];
             }
             __syncthreads();
+            // the groups' tables one after the other, then what lies past either end by a wavefront
+            const int width = table_columns + 2 * kMargin;
+            for (int i = static_cast<int>(threadIdx.x); i < width; i += kGradientThreads) {
+                float sum = bins[0][i];
+#pragma unroll
+                for (int w = 1; w < kGradientWaves * 4; ++w) {
+                    sum += bins[w][i];
+                }
+                bins[0][i] = sum;
+            }
+            __syncthreads();
+            if (wave < 2) {
+                const int from = wave == 0 ? 0 : width - kMargin;
+                float sum = 0.0f;
+                for (int i = lane; i < kMargin; i += kWave) {
+                    sum += bins[0][from + i];
+                }
+#pragma unroll
+                for (int offset = kWave / 2; offset > 0; offset >>= 1) {
+                    sum += waveXor(sum, offset);
+                }
+                if (lane == 0) {
+                    // (one bin holds both ends where the table has one value)
+                    past_ends[wave] = sum;
+                }
+            }
+            __syncthreads();
             float* to = partialTable(head);
             for (int i = static_cast<int>(threadIdx.x); i < table_columns; i += kGradientThreads) {
-                const int low = i == 0 ? 0 : i + kMargin;
-                const int high = i == table_columns - 1 ? i + 2 * kMargin : i + kMargin;
-                float sum = 0.0f;
-                for (int w = 0; w < kGradientWaves * 4; ++w) {
-                    for (int b = low; b <= high; ++b) {
-                        sum += bins[w][b];
-                    }
-                }
+                float sum = bins[0][kMargin + i];
+                sum += i == 0 ? past_ends[0] : 0.0f;
+                sum += i == table_columns - 1 ? past_ends[1] : 0.0f;
                 to[i] = sum;
             }
         }
@@ -769,9 +840,9 @@ __global__ __launch_bounds__(kColumnThreads) void joinTablesKernel(const float* 
 template <typename T>
 int launchAttentionGradient(const AttentionGradientPlan& plan, const AttentionArgs& args, const AttentionGradient& more,
                             hipStream_t stream) {
-    const std::int64_t rows = args.q_texts.total * args.heads;
-    constexpr int kStatsRows = kGradientThreads / kStatsLanes;
-    attentionStatsKernel<T><<<static_cast<unsigned>((rows + kStatsRows - 1) / kStatsRows), kGradientThreads, 0, stream>>>(args, more);
+    const dim3 stats_grid(static_cast<unsigned>((args.q_texts.total + kStatsRows - 1) / kStatsRows),
+                          static_cast<unsigned>(divideUp(args.heads, kStatsHeads)));
+    attentionStatsKernel<T><<<stats_grid, kGradientThreads, 0, stream>>>(args, more);
     ZCGVS_LAUNCH_CHECK("attention gradient");
     int status;
     switch (paddedDim(args.head_dim)) {

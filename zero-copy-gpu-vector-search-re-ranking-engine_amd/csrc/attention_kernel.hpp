@@ -422,14 +422,13 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
                 sum += rows[(w * kDimBlocks + d) * kWave + lane];
             }
             const int column = 16 * d + 4 * h;
-            if (!exists[0] || column >= args.head_dim) {
+            if (!exists[0]) {
                 continue;
             }
             if (output.splits > 1) {
-                const std::int64_t at =
-                    (split * args.q_texts.total + row[0]) * args.heads + head[0];
+                const std::int64_t at = (split * args.q_texts.total + row[0]) * args.heads + head[0];
                 *reinterpret_cast<f32x4*>(output.partial_rows + at * kDim + column) = valid[0] ? sum : f32x4{};
-            } else {
+            } else if (column < args.head_dim) {
                 const float scale = valid[0] && total[0] != 0.0f ? 1.0f / total[0] : 0.0f;
                 const f32x4 result = valid[0] && total[0] != 0.0f ? sum * scale : f32x4{};
                 storeFour(result, static_cast<T*>(output.out) + row[0] * output.out_stride + head[0] * args.head_dim + column,
@@ -470,16 +469,16 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
     }
 }
 
-// Rows from the parts of their keys, a wavefront a row and head; parts of rows of no text are not written and not read.
+// Rows from the parts of their keys, a workgroup a row and head: its threads take four columns each of every
+// kJoinParts-th part. Parts of rows of no text are not written and not read.
 template <typename T, int kDim>
 __global__ __launch_bounds__(kAttentionThreads) void joinAttentionKernel(AttentionArgs args, AttentionOutput output) {
-    constexpr int kEach = kDim <= kWave ? 1 : kDim / kWave;
-    const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+    constexpr int kColumnThreads = kDim / 4;
+    constexpr int kJoinParts = kAttentionThreads / kColumnThreads;
+    __shared__ float maxima[kAttentionWaves], totals[kAttentionWaves];
+    __shared__ f32x4 sums[kJoinParts][kColumnThreads];
     const std::int64_t rows = args.q_texts.total * args.heads;
-    const std::int64_t at = static_cast<std::int64_t>(blockIdx.x) * kAttentionWaves + threadIdx.x / kWave;
-    if (at >= rows) {
-        return;
-    }
+    const std::int64_t at = blockIdx.x;
     const std::int64_t row = at / args.heads;
     const int head = static_cast<int>(at % args.heads);
     if (args.q_texts.offsets != nullptr) {
@@ -488,40 +487,64 @@ __global__ __launch_bounds__(kAttentionThreads) void joinAttentionKernel(Attenti
             return;
         }
     }
-    float now = -INFINITY;
-    for (int s = lane; s < output.splits; s += kWave) {
-        now = fmaxf(now, output.partial_stats[2 * (s * rows + at)]);
-    }
+    // (at most as many parts as threads)
+    const int thread = static_cast<int>(threadIdx.x);
+    const int wave = thread / kWave;
+    const float* stats = output.partial_stats + 2 * (thread * rows + at);
+    const float own_largest = thread < output.splits ? stats[0] : -INFINITY;
+    const float own_total = thread < output.splits ? stats[1] : 0.0f;
+    const int column = 4 * (thread % kColumnThreads);
+    const int part = thread / kColumnThreads;
+    float largest = own_largest;
 #pragma unroll
     for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-        now = fmaxf(now, waveXor(now, offset));
+        largest = fmaxf(largest, waveXor(largest, offset));
     }
-    float total = 0.0f, sum[kEach] = {};
-#pragma unroll 4
-    for (int s = 0; s < output.splits; ++s) {
-        const float largest = output.partial_stats[2 * (s * rows + at)];
-        const float keep = largest == now ? 1.0f : __builtin_amdgcn_exp2f(largest - now);
-        total = fmaf(output.partial_stats[2 * (s * rows + at) + 1], keep, total);
+    if (thread % kWave == 0) {
+        maxima[wave] = largest;
+    }
+    __syncthreads();
+    largest = maxima[0];
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int d = e * kWave + lane;
-            if (d < args.head_dim) {
-                sum[e] = fmaf(output.partial_rows[(s * rows + at) * kDim + d], keep, sum[e]);
-            }
-        }
+    for (int w = 1; w < kAttentionWaves; ++w) {
+        largest = fmaxf(largest, maxima[w]);
+    }
+    float total = own_total * (own_largest == largest ? 1.0f : __builtin_amdgcn_exp2f(own_largest - largest));
+#pragma unroll
+    for (int offset = kWave / 2; offset > 0; offset >>= 1) {
+        total += waveXor(total, offset);
+    }
+    if (thread % kWave == 0) {
+        totals[wave] = total;
+    }
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = part; s < output.splits; s += kJoinParts) {
+        const float at_part = output.partial_stats[2 * (s * rows + at)];
+        const float keep = at_part == largest ? 1.0f : __builtin_amdgcn_exp2f(at_part - largest);
+        sum += *reinterpret_cast<const f32x4*>(output.partial_rows + (s * rows + at) * kDim + column) * keep;
+    }
+    sums[part][thread % kColumnThreads] = sum;
+    __syncthreads();
+    if (part != 0) {
+        return;
+    }
+    total = totals[0];
+#pragma unroll
+    for (int w = 1; w < kAttentionWaves; ++w) {
+        total += totals[w];
+    }
+#pragma unroll
+    for (int p = 1; p < kJoinParts; ++p) {
+        sum += sums[p][thread];
     }
     const bool empty = total == 0.0f;
-    const float scale = empty ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int d = e * kWave + lane;
-        if (d < args.head_dim) {
-            static_cast<T*>(output.out)[row * output.out_stride + head * args.head_dim + d] =
-                static_cast<T>(empty ? 0.0f : sum[e] * scale);
-        }
+    if (column < args.head_dim) {
+        storeFour(empty ? f32x4{} : sum * (1.0f / total),
+                  static_cast<T*>(output.out) + row * output.out_stride + head * args.head_dim + column, args.head_dim - column);
     }
-    if (output.lse != nullptr && lane == 0) {
-        output.lse[at] = empty ? -INFINITY : kLn2 * (now + __builtin_amdgcn_logf(total));
+    if (output.lse != nullptr && thread == 0) {
+        output.lse[at] = empty ? -INFINITY : kLn2 * (largest + __builtin_amdgcn_logf(total));
     }
 }
 
@@ -541,8 +564,7 @@ int launchAttentionTiles(const AttentionArgs& args, AttentionOutput output, hipS
     ZCGVS_LAUNCH_CHECK("attention");
     if (output.splits > 1) {
         const std::int64_t rows = args.q_texts.total * args.heads;
-        joinAttentionKernel<T, kDim><<<static_cast<unsigned>((rows + kAttentionWaves - 1) / kAttentionWaves), kAttentionThreads,
-                                       0, stream>>>(args, output);
+        joinAttentionKernel<T, kDim><<<static_cast<unsigned>(rows), kAttentionThreads, 0, stream>>>(args, output);
         ZCGVS_LAUNCH_CHECK("attention");
     }
     return ZCGVS_OK;
