@@ -285,40 +285,61 @@ struct RowTile {
         }
     }
 
-    // The calling lane's fragment of rows 16 block .. + 15, values of step t along the row.
-    static __device__ __forceinline__ typename Fragment<T>::type read(const std::uint8_t* tile, int block, int t) {
-        const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-        const int row = 16 * block + (lane & 15);
-        const int slot = (4 * t + (lane >> 4)) ^ turn(row);
-        return *reinterpret_cast<const typename Fragment<T>::type*>(tile + row * kRowBytes + 16 * slot);
+    // Where the calling lane's fragments begin within a tile: what follows from the lane alone, so that a tile's reads
+    // differ by constants (turn() has the period of 16 rows).
+    struct Lane {
+        std::uint32_t plain[kSteps];
+        std::uint32_t turned[kDim / 16][sizeof(T) == 2 ? 1 : 4];
+
+        __device__ __forceinline__ Lane() {
+            const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+            const int i = lane & 15;
+            const int h = lane >> 4;
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t) {
+                plain[t] = static_cast<std::uint32_t>(i * kRowBytes + 16 * ((4 * t + h) ^ turn(i)));
+            }
+#pragma unroll
+            for (int d = 0; d < kDim / 16; ++d) {
+                if constexpr (sizeof(T) == 2) {
+                    const int row = 4 * h + (i >> 2);
+                    const int chunk = 2 * d + ((i & 3) >> 1);
+                    turned[d][0] = static_cast<std::uint32_t>(row * kRowBytes + 16 * (chunk ^ turn(row)) + 8 * (i & 1));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = 4 * h + e;
+                        turned[d][e] = static_cast<std::uint32_t>(row * kRowBytes + 16 * ((4 * d + (i >> 2)) ^ turn(row)) + 4 * (i & 3));
+                    }
+                }
+            }
+        }
+    };
+
+    // The calling lane's fragment of rows 16 block .. + 15, values of step t along the row. `tile`: an LDS address.
+    static __device__ __forceinline__ typename Fragment<T>::type read(std::uint32_t tile, const Lane& lane, int block, int t) {
+        typedef const __attribute__((address_space(3))) typename Fragment<T>::type* LdsPointer;
+        return *reinterpret_cast<LdsPointer>(tile + lane.plain[t] + 16 * block * kRowBytes);
     }
     // The calling lane's fragment of columns 16 block .. + 15, contracted over rows: of lane group h the rows 4 h + e of
     // row block `pair` (float32), or of the row blocks 2 pair and 2 pair + 1 (16-bit): the rows whose products a lane
     // holds in its results, so that these are the other operand as they are.
-    static __device__ __forceinline__ typename Fragment<T>::type readTurned(const std::uint8_t* tile, int block, int pair) {
-        const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
-        const int i = lane & 15;
-        const int h = lane >> 4;
+    static __device__ __forceinline__ typename Fragment<T>::type readTurned(std::uint32_t tile, const Lane& lane, int block,
+                                                                            int pair) {
         if constexpr (sizeof(T) == 2) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4* LdsPointer;
-            const int row = 32 * pair + 4 * h + (i >> 2);
-            const int chunk = 2 * block + ((i & 3) >> 1);
-            const std::uint32_t base = ldsAddress(tile) + static_cast<std::uint32_t>(8 * (i & 1));
-            const std::uint32_t low = base + static_cast<std::uint32_t>(row * kRowBytes + 16 * (chunk ^ turn(row)));
-            const std::uint32_t high =
-                base + static_cast<std::uint32_t>((row + 16) * kRowBytes + 16 * (chunk ^ turn(row + 16)));
+            const std::uint32_t low = tile + lane.turned[block][0] + 32 * pair * kRowBytes;
             const s16x4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(low));
-            const s16x4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(high));
+            const s16x4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPointer>(low + 16 * kRowBytes));
             return __builtin_bit_cast(typename Fragment<T>::type,
                                       __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
+            typedef const __attribute__((address_space(3))) float* LdsPointer;
             typename Fragment<T>::type v;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = 16 * pair + 4 * h + e;
-                const int chunk = (4 * block + (i >> 2)) ^ turn(row);
-                v[e] = *reinterpret_cast<const float*>(tile + row * kRowBytes + 16 * chunk + 4 * (i & 3));
+                v[e] = *reinterpret_cast<LdsPointer>(tile + lane.turned[block][e] + 16 * pair * kRowBytes);
             }
             return v;
         }

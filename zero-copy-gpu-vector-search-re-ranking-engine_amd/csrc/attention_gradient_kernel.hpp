@@ -112,6 +112,7 @@ __device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCo
             }
         }
     } else {
+        asm volatile("");  // stays a branch
 #pragma unroll
         for (int b = 0; b < kCount; ++b) {
             s[b] *= 0.0f;
@@ -142,14 +143,15 @@ __device__ __forceinline__ float fromLaneBefore(float x) {
 }
 
 // Wavefronts of a SIMD that the registers do for; the bound also keeps sums out of the accumulation registers.
-template <typename T, int kDim, int kBlocks>
-constexpr int kKeyResident = kBlocks * kDim * static_cast<int>(sizeof(T)) <= 256 ? 2 : 1;
+// (The largest tables leave LDS for one workgroup.)
+template <typename T, int kDim, int kBlocks, int kFar>
+constexpr int kKeyResident = kBlocks * kDim * static_cast<int>(sizeof(T)) <= 256 && kFar <= 128 ? 2 : 1;
 template <typename T, int kDim, int kBlocks>
 constexpr int kQueryResident = kBlocks * kDim * static_cast<int>(sizeof(T)) <= 512 ? 2 : 1;
 
 // kFar: the largest max_distance whose gradient is wanted (0: none).
 template <typename T, int kDim, int kBlocks, bool kDirect, int kFar>
-__global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>)) void keyGradientKernel(AttentionArgs args, AttentionGradient more) {
+__global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, kFar>)) void keyGradientKernel(AttentionArgs args, AttentionGradient more) {
     using Rows = RowTile<T, kQueryTile, kDim, kGradientThreads, kDirect>;
     constexpr int kWaveKeys = 16 * kBlocks;
     constexpr int kKeys = kWaveKeys * kGradientWaves;
@@ -231,6 +233,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
             dv[n][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
+    const typename Rows::Lane own_lane;
     // query rows from the first that sees one of the workgroup's keys on
     const int query_begin = args.causal && tile_key >= prefix ? max(tile_key - shift, 0) : 0;
     const bool any_key = wave_key < keys.count;
@@ -280,8 +283,8 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
         int buffer = 0;
         for (int row0 = query_begin; row0 < queries.count; row0 += kQueryTile) {
             teamSync<kGradientThreads>();
-            const std::uint8_t* q_stage = lds + buffer * kStageBytes;
-            const std::uint8_t* d_stage = q_stage + Rows::kBytes;
+            const std::uint32_t q_stage = ldsAddress(lds) + buffer * kStageBytes;
+            const std::uint32_t d_stage = q_stage + Rows::kBytes;
             const float* row_stats = &stats[buffer][0][0];
             buffer ^= 1;
             const bool next = row0 + kQueryTile < queries.count;
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
             }
             const int place0 = row0 + shift;  // of the tile's first row
             if (any_key && !(hidden_keys && wave_key >= prefix && place0 + kQueryTile - 1 < wave_key)) {
-                f32x4 s[kBlocks][kRowBlocks], dp[kBlocks][kRowBlocks], bent[kBlocks][kRowBlocks] = {};
+                f32x4 s[kBlocks][kRowBlocks], dp[kBlocks][kRowBlocks], bent[kBlocks][kRowBlocks];
 #pragma unroll
                 for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
@@ -308,8 +311,8 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                     }
 #pragma unroll
                     for (int t = 0; t < Rows::kSteps; ++t) {
-                        const auto q = Rows::read(q_stage, m, t);
-                        const auto d = Rows::read(d_stage, m, t);
+                        const auto q = Rows::read(q_stage, own_lane, m, t);
+                        const auto d = Rows::read(d_stage, own_lane, m, t);
 #pragma unroll
                         for (int n = 0; n < kBlocks; ++n) {
                             s[n][m] = multiplyAdd(q, k[n][t], s[n][m]);
@@ -319,6 +322,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                 }
                 float score_factor = form.factor, score_offset = 0.0f;
                 if (form.capped || args.scale == 0.0f) {
+                    asm volatile("");  // stays a branch
 #pragma unroll
                     for (int n = 0; n < kBlocks; ++n) {
                         formScores<T>(form, s[n], bent[n]);
@@ -360,22 +364,39 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                         score_factor = 1.0f;
                     }
                 }
-                const bool masked = hidden_keys && place0 < last_key;
 #pragma unroll
                 for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int row = 16 * m + 4 * h + e;
-                        const float off = score_offset - row_stats[2 * row];
-                        const float delta = row_stats[2 * row + 1];
+                        const float off = score_offset - row_stats[2 * (16 * m + 4 * h + e)];
 #pragma unroll
                         for (int n = 0; n < kBlocks; ++n) {
-                            float p = __builtin_amdgcn_exp2f(fmaf(s[n][m][e], score_factor, off));
-                            if (masked) {
-                                p = place0 + row >= seen_from[n] ? p : 0.0f;
+                            s[n][m][e] = __builtin_amdgcn_exp2f(fmaf(s[n][m][e], score_factor, off));
+                        }
+                    }
+                }
+                if (hidden_keys && place0 < last_key) {
+                    asm volatile("");  // stays a branch
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) {
+                        const int seen = seen_from[n] - place0 - 4 * h;
+#pragma unroll
+                        for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                s[n][m][e] = 16 * m + e >= seen ? s[n][m][e] : 0.0f;
                             }
-                            s[n][m][e] = p;
-                            dp[n][m][e] = p * (dp[n][m][e] - delta);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float delta = row_stats[2 * (16 * m + 4 * h + e) + 1];
+#pragma unroll
+                        for (int n = 0; n < kBlocks; ++n) {
+                            dp[n][m][e] = s[n][m][e] * (dp[n][m][e] - delta);
                         }
                     }
                 }
@@ -430,6 +451,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                     }
                 }
                 if (form.capped) {
+                    asm volatile("");  // stays a branch
 #pragma unroll
                     for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
@@ -451,8 +473,8 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks>))
                     }
 #pragma unroll
                     for (int d = 0; d < kDimBlocks; ++d) {
-                        const auto dout = Rows::readTurned(d_stage, d, pair);
-                        const auto q = Rows::readTurned(q_stage, d, pair);
+                        const auto dout = Rows::readTurned(d_stage, own_lane, d, pair);
+                        const auto q = Rows::readTurned(q_stage, own_lane, d, pair);
 #pragma unroll
                         for (int n = 0; n < kBlocks; ++n) {
                             dv[n][d] = multiplyAdd(dout, p[n], dv[n][d]);
@@ -624,6 +646,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
             dq[m][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
+    const typename Keys::Lane own_lane;
     Keys k_tile, v_tile;
     k_tile.begin(static_cast<const T*>(args.k) + keys.first * args.k_stride + key_head * args.head_dim, args.k_stride,
                  keys.count, args.head_dim, 1);
@@ -643,8 +666,8 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
     int buffer = 0;
     for (int key0 = 0; key0 < all_keys; key0 += kTileKeys) {
         teamSync<kGradientThreads>();
-        const std::uint8_t* stage = lds + buffer * kStageBytes;
-        const std::uint8_t* values = stage + Keys::kBytes;
+        const std::uint32_t stage = ldsAddress(lds) + buffer * kStageBytes;
+        const std::uint32_t values = stage + Keys::kBytes;
         buffer ^= 1;
         std::uint8_t* other = lds + buffer * kStageBytes;
         const bool next = key0 + kTileKeys < all_keys;
@@ -663,7 +686,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
             if (pair_key >= most_limit) {
                 continue;
             }
-            f32x4 s[kBlocks][kTurned], dp[kBlocks][kTurned], bent[kBlocks][kTurned] = {};
+            f32x4 s[kBlocks][kTurned], dp[kBlocks][kTurned], bent[kBlocks][kTurned];
 #pragma unroll
             for (int b = 0; b < kTurned; ++b) {
 #pragma unroll
@@ -673,8 +696,8 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
                 }
 #pragma unroll
                 for (int t = 0; t < Keys::kSteps; ++t) {
-                    const auto k = Keys::read(stage, pair * kTurned + b, t);
-                    const auto v = Keys::read(values, pair * kTurned + b, t);
+                    const auto k = Keys::read(stage, own_lane, pair * kTurned + b, t);
+                    const auto v = Keys::read(values, own_lane, pair * kTurned + b, t);
 #pragma unroll
                     for (int m = 0; m < kBlocks; ++m) {
                         s[m][b] = multiplyAdd(k, q[m][t], s[m][b]);
@@ -684,6 +707,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
             }
             float score_factor = form.factor, score_offset = 0.0f;
             if (form.capped || args.scale == 0.0f) {
+                asm volatile("");  // stays a branch
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
                     formScores<T>(form, s[m], bent[m]);
@@ -725,31 +749,62 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
                     score_factor = 1.0f;
                 }
             }
-            const bool masked = pair_key + 16 * kTurned > least_limit;
-            typename Fragment<T>::type dr[kBlocks];
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
-                const int left = limit[m] - pair_key - 4 * h;
                 const float off = score_offset - lse[m];
 #pragma unroll
                 for (int b = 0; b < kTurned; ++b) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float p = __builtin_amdgcn_exp2f(fmaf(s[m][b][e], score_factor, off));
-                        if (masked) {
-                            p = 16 * b + e < left ? p : 0.0f;
+                        s[m][b][e] = __builtin_amdgcn_exp2f(fmaf(s[m][b][e], score_factor, off));
+                    }
+                }
+            }
+            if (pair_key + 16 * kTurned > least_limit) {
+                asm volatile("");  // stays a branch
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    const int left = limit[m] - pair_key - 4 * h;
+#pragma unroll
+                    for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[m][b][e] = 16 * b + e < left ? s[m][b][e] : 0.0f;
                         }
-                        dp[m][b][e] = p * (dp[m][b][e] - delta[m]);
-                        if (form.capped) {
+                    }
+                }
+            }
+            typename Fragment<T>::type dr[kBlocks];
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        dp[m][b][e] = s[m][b][e] * (dp[m][b][e] - delta[m]);
+                    }
+                }
+            }
+            if (form.capped) {
+                asm volatile("");  // stays a branch
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                    for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
                             dp[m][b][e] = fmaf(-dp[m][b][e], bent[m][b][e], dp[m][b][e]);
                         }
                     }
                 }
+            }
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
                 dr[m] = resultFragment<T>(dp[m]);
             }
 #pragma unroll
             for (int d = 0; d < kDimBlocks; ++d) {
-                const auto k = Keys::readTurned(stage, d, pair);
+                const auto k = Keys::readTurned(stage, own_lane, d, pair);
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
                     dq[m][d] = multiplyAdd(k, dr[m], dq[m][d]);

@@ -47,8 +47,9 @@ struct AttentionTile {
 // Wavefronts of a SIMD: two, for which the registers of all but wide float32 rows do. The bound also keeps the sums in
 // ordinary registers: with more of them to spend, tiles went through the accumulation registers and back
 // (768 us for 128 texts of 64 to 1024 tokens, 12 heads of 64, that take 306).
-template <typename T, int kDim, int kBlocks>
-constexpr int kAttentionResident = sizeof(T) == 4 && kDim == 128 && kBlocks == 2 ? 1 : 2;
+// The narrow shape's tiles of wide rows leave LDS for one workgroup.
+template <typename T, int kDim, int kBlocks, bool kNarrow>
+constexpr int kAttentionResident = kDim == 128 && (kNarrow || (sizeof(T) == 4 && kBlocks == 2)) ? 1 : 2;
 
 // The largest of a lane's value over the four lanes of its row.
 __device__ __forceinline__ float overGroups(float value) {
@@ -57,7 +58,7 @@ __device__ __forceinline__ float overGroups(float value) {
 }
 
 template <typename T, int kDim, int kBlocks, bool kNarrow, bool kDirect>
-__global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBlocks>)) void attentionKernel(AttentionArgs args, AttentionOutput output) {
+__global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBlocks, kNarrow>)) void attentionKernel(AttentionArgs args, AttentionOutput output) {
     using Tile = AttentionTile<T, kDim, kBlocks, kNarrow>;
     using Keys = RowTile<T, Tile::kTileKeys, kDim, Tile::kTeam, kDirect>;
     constexpr int kTeams = kNarrow ? kAttentionWaves : 1;
@@ -175,7 +176,8 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
         }
     }
 
-    auto useTile = [&](const std::uint8_t* stage, int key0) {
+    const typename Keys::Lane own_lane;
+    auto useTile = [&](std::uint32_t stage, int key0) {
         f32x4 s[kBlocks][Tile::kKeyBlocks];
 #pragma unroll
         for (int b = 0; b < Tile::kKeyBlocks; ++b) {
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
             }
 #pragma unroll
             for (int t = 0; t < Keys::kSteps; ++t) {
-                const auto k = Keys::read(stage, b, t);
+                const auto k = Keys::read(stage, own_lane, b, t);
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
                     s[m][b] = multiplyAdd(k, q[m][t], s[m][b]);
@@ -208,6 +210,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
             }
             score_factor = 1.0f;
         } else if (args.scale == 0.0f) {
+            asm volatile("");  // stays a branch
             // a factor of zero leaves no infinities for the masks
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
@@ -258,6 +261,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
             score_factor = behind || before ? score_factor : 1.0f;
         }
         if (key0 + Tile::kTileKeys > least_limit) {
+            asm volatile("");  // stays a branch
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
                 const int left = limit[m] - key0 - 4 * h;
@@ -286,6 +290,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
             raise = raise || peak[m] > largest[m] + 8.0f;
         }
         if (__ballot(raise) != 0) {
+            asm volatile("");  // stays a branch
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
                 const float now = fmaxf(largest[m], peak[m]);
@@ -316,12 +321,12 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
                 p[m][b] = resultFragment<T>(&s[m][b * kBlocksTurned<T>]);
             }
         }
-        const std::uint8_t* values = stage + Keys::kBytes;
+        const std::uint32_t values = stage + Keys::kBytes;
 #pragma unroll
         for (int b = 0; b < Tile::kKeyBlocks / kBlocksTurned<T>; ++b) {
 #pragma unroll
             for (int d = 0; d < kDimBlocks; ++d) {
-                const auto v = Keys::readTurned(values, d, b);
+                const auto v = Keys::readTurned(values, own_lane, d, b);
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
                     sums[m][d] = multiplyAdd(v, p[m][b], sums[m][d]);
@@ -368,7 +373,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
         }
         const int key0 = tile * Tile::kTileKeys;
         if (key0 < most_limit) {
-            useTile(stage, key0);
+            useTile(ldsAddress(stage), key0);
         }
         if constexpr (!kDirect) {
             if (more) {
