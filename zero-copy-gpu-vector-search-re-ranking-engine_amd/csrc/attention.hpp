@@ -190,9 +190,10 @@ __device__ __forceinline__ typename Fragment<T>::type loadRowChunk(const T* from
     return v;
 }
 
-// kRows rows of kDim values in LDS, one behind the other. A row's chunk c stands in slot c ^ turn(row): the 16 rows of one
-// 16-byte read fall on 16 different columns of the 256 bytes that the banks hold, and so do the rows of a transposing
-// read's half wavefront (16-bit: eight rows, two chunks each; float32: four rows, four chunks each).
+// kRows rows of kDim values in LDS, one behind the other. A row's chunk c stands in slot c ^ turn(row), so that what is
+// read together falls on different columns of the 256 bytes that the banks hold. A 16-byte read takes 16 lanes at a time,
+// of a lane group and the next one: rows 0-3 and 12-15 of chunk c with rows 4-11 of chunk c + 1, or the others. A
+// transposing read (16-bit) takes half a wavefront: rows 0-7, or 8-15, two chunks of each.
 template <typename T, int kRows, int kDim, int kTeam, bool kDirect>
 struct RowTile {
     static constexpr int kRowBytes = kDim * static_cast<int>(sizeof(T));
@@ -213,7 +214,7 @@ struct RowTile {
         constexpr int kTurns = kRowChunks < 16 ? kRowChunks : 16;
         const int p = (row / kPerLine) & (kTurns - 1);
         if constexpr (sizeof(T) == 2) {
-            return ((p << 1) & (kTurns - 1)) | (p / (kTurns / 2));
+            return ((2 * p) & (kTurns - 1)) ^ (p / (kTurns / 2) * (kTurns / 2 + 1));
         } else {
             return p;
         }
@@ -350,6 +351,14 @@ struct RowTile {
 template <typename T>
 constexpr int kBlocksTurned = sizeof(T) == 2 ? 2 : 1;
 
+// The largest of a lane's value over the four lanes of its row (NaN where one is).
+__device__ __forceinline__ float overGroups(float value) {
+    const auto pairs = __builtin_amdgcn_permlane16_swap(__float_as_uint(value), __float_as_uint(value), false, false);
+    value = __builtin_elementwise_maximum(__uint_as_float(pairs[0]), __uint_as_float(pairs[1]));
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(value), __float_as_uint(value), false, false);
+    return __builtin_elementwise_maximum(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+
 // A lane's results for kBlocksTurned row blocks as the other operand of that contraction, rounded to T.
 template <typename T>
 __device__ __forceinline__ typename Fragment<T>::type resultFragment(const f32x4* blocks) {
@@ -372,11 +381,41 @@ __device__ __forceinline__ void teamSync() {
     }
 }
 
+// A head's values of the distance bias in LDS: `margin` copies of the end values on either side, times `factor`. Values of
+// -1e30 and less are minus infinity, and stay so.
+template <typename T>
+__device__ __forceinline__ float biasValue(T value, float factor) {
+    const float bias = static_cast<float>(value);
+    return bias <= -1.0e30f ? -INFINITY : factor * bias;
+}
+
+// How scores follow from the raw products. Without a cap, biases are where the products' sums begin (divided by scale, so
+// that one factor brings all to base 2); with a cap, or a scale too small to divide by, they are added to formed scores.
+struct ScoreForm {
+    bool capped;
+    bool formed;         // scores in base 2 are formed before the biases
+    float factor;        // log2(e) |scale| (the queries, or keys, carry scale's sign)
+    float bias_factor;   // of the table's values and the slopes
+    float cap;           // log2(e) cap
+    float to_cap;        // |scale| / cap (16-bit operands: times 2 log2(e))
+
+    __device__ __forceinline__ ScoreForm(const AttentionArgs& args, bool base_two) {
+        capped = args.cap > 0.0f;
+        const float scale = fabsf(args.scale);
+        formed = capped || scale < 0x1p-20f;
+        factor = kLog2E * scale;
+        bias_factor = formed ? kLog2E : 1.0f / scale;
+        cap = kLog2E * args.cap;
+        to_cap = capped ? (base_two ? 2.0f * kLog2E : 1.0f) * scale / args.cap : 0.0f;
+    }
+};
+
+// The tangent of a raw product times form.to_cap.
 template <typename T>
 __device__ __forceinline__ float tanhOf(float y) {
     if constexpr (sizeof(T) == 2) {
-        // within 2^-22 of 1, far below what the 16-bit operands have
-        return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2E * y));
+        // y in base 2 and doubled; within 2^-22 of 1, far below what the 16-bit operands have
+        return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y)), 1.0f);
     } else {
         return tanhf(y);
     }

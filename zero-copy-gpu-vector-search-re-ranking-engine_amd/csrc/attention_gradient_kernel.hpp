@@ -81,27 +81,13 @@ __global__ __launch_bounds__(kGradientThreads) void attentionStatsKernel(Attenti
     }
 }
 
-// ---- the scores' forms, shared by both kernels ---------------------------------------------------
+// ---- shared by both kernels ----------------------------------------------------------------------
 
-struct ScoreForm {
-    bool capped;
-    float factor;  // log2(e) |scale|
-    float cap;     // log2(e) cap
-    float to_cap;  // |scale| / cap
-
-    __device__ __forceinline__ explicit ScoreForm(const AttentionArgs& args) {
-        capped = args.cap > 0.0f;
-        factor = kLog2E * fabsf(args.scale);
-        cap = kLog2E * args.cap;
-        to_cap = capped ? fabsf(args.scale) / args.cap : 0.0f;
-    }
-};
-
-// Raw products -> capped scores in base 2, the tangent's square to `bent`; scores of zero where scale is, which leaves no
-// infinities to the masks.
+// Raw products -> formed scores in base 2 before the biases; the tangent's square to `bent`.
 template <typename T, int kCount>
 __device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCount], f32x4 (&bent)[kCount]) {
     if (form.capped) {
+        asm volatile("");  // stays a branch
 #pragma unroll
         for (int b = 0; b < kCount; ++b) {
 #pragma unroll
@@ -115,18 +101,18 @@ __device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCo
         asm volatile("");  // stays a branch
 #pragma unroll
         for (int b = 0; b < kCount; ++b) {
-            s[b] *= 0.0f;
+            s[b] *= form.factor;
         }
     }
 }
 
-// The table of a head with `margin` copies of its end values on either side, base 2.
+// The table of a head with `margin` copies of its end values on either side.
 template <typename T>
-__device__ __forceinline__ void loadTable(const AttentionArgs& args, int head, int margin, float* table) {
+__device__ __forceinline__ void loadTable(const AttentionArgs& args, int head, int margin, float factor, float* table) {
     const int width = 2 * (args.max_distance + margin) + 1;
     const T* from = static_cast<const T*>(args.table) + static_cast<std::int64_t>(head) * (2 * args.max_distance + 1);
     for (int i = static_cast<int>(threadIdx.x); i < width; i += kGradientThreads) {
-        table[i] = kLog2E * static_cast<float>(from[min(max(i - margin, 0), 2 * args.max_distance)]);
+        table[i] = biasValue(from[min(max(i - margin, 0), 2 * args.max_distance)], factor);
     }
 }
 
@@ -200,7 +186,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
     const TextSpan queries = textSpan(args.q_texts, text);
     const int prefix = args.prefix == nullptr ? 0 : args.prefix[text];
     const int shift = args.q_last ? keys.count - queries.count : 0;
-    const ScoreForm form(args);
+    const ScoreForm form(args, sizeof(T) == 2);
 
     const int wave_key = tile_key + wave * kWaveKeys;
     int key[kBlocks], seen_from[kBlocks];
@@ -242,11 +228,11 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
 
     for (int g = 0; g < args.group; ++g) {
         const int head = key_head * args.group + g;
-        const float slope = args.slopes != nullptr ? kLog2E * args.slopes[head] : 0.0f;
+        const float slope = args.slopes != nullptr ? form.bias_factor * args.slopes[head] : 0.0f;
         float past[2] = {};  // sums of ds at distances past the table's ends: before, behind
         __syncthreads();              // the tables and tiles of the head before have been used
         if (args.table != nullptr) {
-            loadTable<T>(args, head, kMargin, table);
+            loadTable<T>(args, head, kMargin, form.bias_factor, table);
         }
         if constexpr (kFar > 0) {
             for (int i = static_cast<int>(threadIdx.x); i < kGradientWaves * 4 * kBins; i += kGradientThreads) {
@@ -301,14 +287,53 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
             }
             const int place0 = row0 + shift;  // of the tile's first row
             if (any_key && !(hidden_keys && wave_key >= prefix && place0 + kQueryTile - 1 < wave_key)) {
+                float score_factor = form.factor, score_offset = 0.0f;
+                const bool before = wave_key + kWaveKeys - 1 - place0 <= -args.max_distance;
+                const bool behind = wave_key - (place0 + kQueryTile - 1) >= args.max_distance;
+                const bool in_table = args.table != nullptr && !before && !behind;
                 f32x4 s[kBlocks][kRowBlocks], dp[kBlocks][kRowBlocks], bent[kBlocks][kRowBlocks];
-#pragma unroll
-                for (int m = 0; m < kRowBlocks; ++m) {
+                auto loadBiases = [&](f32x4(&to)[kBlocks][kRowBlocks]) {
 #pragma unroll
                     for (int n = 0; n < kBlocks; ++n) {
+                        const float* from = table + key[n] - place0 - 4 * h + args.max_distance + kMargin;
+#pragma unroll
+                        for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                to[n][m][e] = from[-(16 * m + e)];
+                            }
+                        }
+                    }
+                };
+                auto addSlopes = [&](f32x4(&to)[kBlocks][kRowBlocks]) {
+#pragma unroll
+                    for (int n = 0; n < kBlocks; ++n) {
+                        const float distance = static_cast<float>(key[n] - place0 - 4 * h);  // of the lane's first row
+#pragma unroll
+                        for (int m = 0; m < kRowBlocks; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                to[n][m][e] = fmaf(-slope, fabsf(distance - static_cast<float>(16 * m + e)), to[n][m][e]);
+                            }
+                        }
+                    }
+                };
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+                    for (int m = 0; m < kRowBlocks; ++m) {
                         s[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                         dp[n][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                     }
+                }
+                if (in_table && !form.formed) {
+                    loadBiases(s);
+                }
+                if (args.slopes != nullptr && !form.formed) {
+                    addSlopes(s);
+                }
+#pragma unroll
+                for (int m = 0; m < kRowBlocks; ++m) {
 #pragma unroll
                     for (int t = 0; t < Rows::kSteps; ++t) {
                         const auto q = Rows::read(q_stage, own_lane, m, t);
@@ -320,49 +345,30 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
                         }
                     }
                 }
-                float score_factor = form.factor, score_offset = 0.0f;
-                if (form.capped || args.scale == 0.0f) {
+                if (form.formed) {
                     asm volatile("");  // stays a branch
 #pragma unroll
                     for (int n = 0; n < kBlocks; ++n) {
                         formScores<T>(form, s[n], bent[n]);
                     }
                     score_factor = 1.0f;
-                }
-                if (args.slopes != nullptr) {
-#pragma unroll
-                    for (int n = 0; n < kBlocks; ++n) {
-                        const float distance = static_cast<float>(key[n] - place0 - 4 * h);  // of the lane's first row
-#pragma unroll
-                        for (int m = 0; m < kRowBlocks; ++m) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                s[n][m][e] = fmaf(-slope, fabsf(distance - static_cast<float>(16 * m + e)), s[n][m][e] * score_factor);
-                            }
-                        }
-                    }
-                    score_factor = 1.0f;
-                }
-                bool before = false, behind = false;
-                if (args.table != nullptr) {
-                    before = wave_key + kWaveKeys - 1 - place0 <= -args.max_distance;
-                    behind = wave_key - (place0 + kQueryTile - 1) >= args.max_distance;
-                    if (before || behind) {
-                        score_offset = table[before ? 0 : 2 * (args.max_distance + kMargin)];
-                    } else {
+                    if (in_table) {
+                        f32x4 bias[kBlocks][kRowBlocks];
+                        loadBiases(bias);
 #pragma unroll
                         for (int n = 0; n < kBlocks; ++n) {
-                            const float* from = table + key[n] - place0 - 4 * h + args.max_distance + kMargin;
 #pragma unroll
                             for (int m = 0; m < kRowBlocks; ++m) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    s[n][m][e] = fmaf(s[n][m][e], score_factor, from[-(16 * m + e)]);
-                                }
+                                s[n][m] += bias[n][m];
                             }
                         }
-                        score_factor = 1.0f;
                     }
+                    if (args.slopes != nullptr) {
+                        addSlopes(s);
+                    }
+                }
+                if (args.table != nullptr && !in_table) {
+                    score_offset = score_factor * table[before ? 0 : 2 * (args.max_distance + kMargin)];
                 }
 #pragma unroll
                 for (int m = 0; m < kRowBlocks; ++m) {
@@ -443,10 +449,16 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
                             }
                         }
                         float* own = &bins[wave * 4 + h][0] + wave_key + r16 - place0 - 4 * h + args.max_distance + kMargin;
+                        // (no two lanes of a group, nor two diagonals, meet; LDS additions as one instruction took
+                        // 128 cycles each)
+                        float held[kBlocks + kRowBlocks];
 #pragma unroll
                         for (int i = 0; i < kBlocks + kRowBlocks; ++i) {
-                            __hip_atomic_fetch_add(own + 16 * (i - kRowBlocks), along[i], __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+                            held[i] = own[16 * (i - kRowBlocks)];
+                        }
+#pragma unroll
+                        for (int i = 0; i < kBlocks + kRowBlocks; ++i) {
+                            own[16 * (i - kRowBlocks)] = held[i] + along[i];
                         }
                     }
                 }
@@ -597,8 +609,8 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
     const int prefix = args.prefix == nullptr ? 0 : args.prefix[text];
     const int shift = args.q_last ? keys.count - queries.count : 0;
     auto limitAt = [&](int at) { return args.causal ? min(keys.count, max(max(at + 1, prefix), 0)) : keys.count; };
-    const ScoreForm form(args);
-    const float slope = args.slopes != nullptr ? kLog2E * args.slopes[head] : 0.0f;
+    const ScoreForm form(args, sizeof(T) == 2);
+    const float slope = args.slopes != nullptr ? form.bias_factor * args.slopes[head] : 0.0f;
 
     const int wave_row = tile_row + wave * kWaveRows;
     int place[kBlocks], limit[kBlocks];
@@ -636,7 +648,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
     const int all_keys = tile_last >= tile_row ? limitAt(tile_last + shift) : 0;
 
     if (args.table != nullptr) {
-        loadTable<T>(args, head, kMargin, table);
+        loadTable<T>(args, head, kMargin, form.bias_factor, table);
     }
     f32x4 dq[kBlocks][kDimBlocks];
 #pragma unroll
@@ -686,14 +698,54 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
             if (pair_key >= most_limit) {
                 continue;
             }
+            float score_factor = form.factor, score_offset = 0.0f;
+            const bool behind = pair_key - last_place >= args.max_distance;
+            const bool before = pair_key + 16 * kTurned - 1 - first_place <= -args.max_distance;
+            const bool in_table = args.table != nullptr && !before && !behind;
             f32x4 s[kBlocks][kTurned], dp[kBlocks][kTurned], bent[kBlocks][kTurned];
-#pragma unroll
-            for (int b = 0; b < kTurned; ++b) {
+            auto loadBiases = [&](f32x4(&to)[kBlocks][kTurned]) {
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
+                    // rows past the text's last one may reach beyond the margin
+                    const float* from = table + max(pair_key + 4 * h - place[m] + args.max_distance + kMargin, 0);
+#pragma unroll
+                    for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            to[m][b][e] = from[16 * b + e];
+                        }
+                    }
+                }
+            };
+            auto addSlopes = [&](f32x4(&to)[kBlocks][kTurned]) {
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    const float distance = static_cast<float>(pair_key + 4 * h - place[m]);
+#pragma unroll
+                    for (int b = 0; b < kTurned; ++b) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            to[m][b][e] = fmaf(-slope, fabsf(distance + static_cast<float>(16 * b + e)), to[m][b][e]);
+                        }
+                    }
+                }
+            };
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int b = 0; b < kTurned; ++b) {
                     s[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                     dp[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
+            }
+            if (in_table && !form.formed) {
+                loadBiases(s);
+            }
+            if (args.slopes != nullptr && !form.formed) {
+                addSlopes(s);
+            }
+#pragma unroll
+            for (int b = 0; b < kTurned; ++b) {
 #pragma unroll
                 for (int t = 0; t < Keys::kSteps; ++t) {
                     const auto k = Keys::read(stage, own_lane, pair * kTurned + b, t);
@@ -705,49 +757,30 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
                     }
                 }
             }
-            float score_factor = form.factor, score_offset = 0.0f;
-            if (form.capped || args.scale == 0.0f) {
+            if (form.formed) {
                 asm volatile("");  // stays a branch
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
                     formScores<T>(form, s[m], bent[m]);
                 }
                 score_factor = 1.0f;
-            }
-            if (args.slopes != nullptr) {
-#pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
-                    const float distance = static_cast<float>(pair_key + 4 * h - place[m]);
-#pragma unroll
-                    for (int b = 0; b < kTurned; ++b) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[m][b][e] = fmaf(-slope, fabsf(distance + static_cast<float>(16 * b + e)), s[m][b][e] * score_factor);
-                        }
-                    }
-                }
-                score_factor = 1.0f;
-            }
-            if (args.table != nullptr) {
-                const bool behind = pair_key - last_place >= args.max_distance;
-                const bool before = pair_key + 16 * kTurned - 1 - first_place <= -args.max_distance;
-                if (before || behind) {
-                    score_offset = table[before ? 0 : 2 * (args.max_distance + kMargin)];
-                } else {
+                if (in_table) {
+                    f32x4 bias[kBlocks][kTurned];
+                    loadBiases(bias);
 #pragma unroll
                     for (int m = 0; m < kBlocks; ++m) {
-                        // rows past the text's last one may reach beyond the margin
-                        const float* from = table + max(pair_key + 4 * h - place[m] + args.max_distance + kMargin, 0);
 #pragma unroll
                         for (int b = 0; b < kTurned; ++b) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                s[m][b][e] = fmaf(s[m][b][e], score_factor, from[16 * b + e]);
-                            }
+                            s[m][b] += bias[m][b];
                         }
                     }
-                    score_factor = 1.0f;
                 }
+                if (args.slopes != nullptr) {
+                    addSlopes(s);
+                }
+            }
+            if (args.table != nullptr && !in_table) {
+                score_offset = score_factor * table[before ? 0 : 2 * (args.max_distance + kMargin)];
             }
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {

@@ -51,12 +51,6 @@ struct AttentionTile {
 template <typename T, int kDim, int kBlocks, bool kNarrow>
 constexpr int kAttentionResident = kDim == 128 && (kNarrow || (sizeof(T) == 4 && kBlocks == 2)) ? 1 : 2;
 
-// The largest of a lane's value over the four lanes of its row.
-__device__ __forceinline__ float overGroups(float value) {
-    value = fmaxf(value, waveXor(value, 16));
-    return fmaxf(value, waveXor(value, 32));
-}
-
 template <typename T, int kDim, int kBlocks, bool kNarrow, bool kDirect>
 __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBlocks, kNarrow>)) void attentionKernel(AttentionArgs args, AttentionOutput output) {
     using Tile = AttentionTile<T, kDim, kBlocks, kNarrow>;
@@ -129,23 +123,20 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
     const int tile_begin = split * tiles_each + (kNarrow ? wave : 0);
     const int tile_end = min(tiles_all, (split + 1) * tiles_each);
 
-    const bool capped = args.cap > 0.0f;
-    const float factor = kLog2E * fabsf(args.scale);
-    const float cap = kLog2E * args.cap;
-    const float to_cap = capped ? fabsf(args.scale) / args.cap : 0.0f;
+    const ScoreForm form(args, sizeof(T) == 2);
     float slope[kBlocks];
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) {
-        slope[m] = args.slopes != nullptr && valid[m] ? kLog2E * args.slopes[head[m]] : 0.0f;
+        slope[m] = args.slopes != nullptr && valid[m] ? form.bias_factor * args.slopes[head[m]] : 0.0f;
     }
-    // the tables with kMargin copies of their end values on either side, base 2
+    // the tables with kMargin copies of their end values on either side
     const int table_width = 2 * (args.max_distance + Tile::kMargin) + 1;
     if (args.table != nullptr) {
         const T* from = static_cast<const T*>(args.table) +
                         static_cast<std::int64_t>(unit * group) * (2 * args.max_distance + 1);
         for (int i = static_cast<int>(threadIdx.x); i < group * table_width; i += kAttentionThreads) {
             const int distance = min(max(i % table_width - Tile::kMargin, 0), 2 * args.max_distance);
-            table[i] = kLog2E * static_cast<float>(from[i / table_width * (2 * args.max_distance + 1) + distance]);
+            table[i] = biasValue(from[i / table_width * (2 * args.max_distance + 1) + distance], form.bias_factor);
         }
         __syncthreads();
     }
@@ -178,13 +169,61 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
 
     const typename Keys::Lane own_lane;
     auto useTile = [&](std::uint32_t stage, int key0) {
+        // scores are s * score_factor + score_offset in base 2
+        float score_factor = form.factor;
+        float score_offset[kBlocks] = {};
+        const int nearest = key0 - last_place;                          // the least distance of the tile
+        const int farthest = key0 + Tile::kTileKeys - 1 - first_place;  // the largest
+        const bool behind = nearest >= args.max_distance, before = farthest <= -args.max_distance;
+        // biases of the tile, or zeros
         f32x4 s[kBlocks][Tile::kKeyBlocks];
-#pragma unroll
-        for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+        auto loadBiases = [&](f32x4(&to)[kBlocks][Tile::kKeyBlocks]) {
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
-                s[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                // rows past the text's last one may reach beyond the margin
+                const int at = min(max(key0 + 4 * h - place[m] + args.max_distance + Tile::kMargin, 0),
+                                   table_width - Tile::kTileKeys + 12);
+                const float* from = table + (kNarrow ? head[m] - unit * group : 0) * table_width + at;
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        to[m][b][e] = from[16 * b + e];
+                    }
+                }
             }
+        };
+        auto addSlopes = [&](f32x4(&to)[kBlocks][Tile::kKeyBlocks]) {
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+                const float distance = static_cast<float>(key0 + 4 * h - place[m]);
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        to[m][b][e] = fmaf(-slope[m], fabsf(distance + static_cast<float>(16 * b + e)), to[m][b][e]);
+                    }
+                }
+            }
+        };
+        const bool in_table = args.table != nullptr && !behind && !before;
+        const float offset_factor = form.formed ? 1.0f : form.factor;
+        if (in_table && !form.formed) {
+            loadBiases(s);
+        } else {
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+                    s[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
+        }
+        if (args.slopes != nullptr && !form.formed) {
+            addSlopes(s);
+        }
+#pragma unroll
+        for (int b = 0; b < Tile::kKeyBlocks; ++b) {
 #pragma unroll
             for (int t = 0; t < Keys::kSteps; ++t) {
                 const auto k = Keys::read(stage, own_lane, b, t);
@@ -194,71 +233,51 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
                 }
             }
         }
-        // scores are s * score_factor + score_offset in base 2
-        float score_factor = factor;
-        float score_offset[kBlocks] = {};
-        if (capped) {
-#pragma unroll
-            for (int m = 0; m < kBlocks; ++m) {
-#pragma unroll
-                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[m][b][e] = cap * tanhOf<T>(s[m][b][e] * to_cap);
-                    }
-                }
-            }
-            score_factor = 1.0f;
-        } else if (args.scale == 0.0f) {
+        if (form.capped) {
             asm volatile("");  // stays a branch
-            // a factor of zero leaves no infinities for the masks
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
-#pragma unroll
-                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-                    s[m][b] *= 0.0f;
-                }
-            }
-            score_factor = 1.0f;
-        }
-        if (args.slopes != nullptr) {
-#pragma unroll
-            for (int m = 0; m < kBlocks; ++m) {
-                const float distance = static_cast<float>(key0 + 4 * h - place[m]);
 #pragma unroll
                 for (int b = 0; b < Tile::kKeyBlocks; ++b) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        s[m][b][e] = fmaf(-slope[m], fabsf(distance + static_cast<float>(16 * b + e)), s[m][b][e] * score_factor);
+                        s[m][b][e] = tanhOf<T>(s[m][b][e] * form.to_cap);
                     }
                 }
             }
-            score_factor = 1.0f;
+            score_factor = form.cap;
         }
-        if (args.table != nullptr) {
-            const int nearest = key0 - last_place;                          // the least distance of the tile
-            const int farthest = key0 + Tile::kTileKeys - 1 - first_place;  // the largest
-            const bool behind = nearest >= args.max_distance, before = farthest <= -args.max_distance;
+        if (form.formed && (!form.capped || in_table || args.slopes != nullptr)) {
+            asm volatile("");  // stays a branch
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+                    s[m][b] *= score_factor;
+                }
+            }
+            score_factor = 1.0f;
+            if (in_table) {
+                f32x4 bias[kBlocks][Tile::kKeyBlocks];
+                loadBiases(bias);
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                    for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+                        s[m][b] += bias[m][b];
+                    }
+                }
+            }
+            if (args.slopes != nullptr) {
+                addSlopes(s);
+            }
+        }
+        if (args.table != nullptr && !in_table) {
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
                 const int base = (kNarrow ? head[m] - unit * group : 0) * table_width;
-                if (behind || before) {
-                    score_offset[m] = table[base + (behind ? table_width - 1 : 0)];
-                } else {
-                    // rows past the text's last one may reach beyond the margin
-                    const int at = min(max(key0 + 4 * h - place[m] + args.max_distance + Tile::kMargin, 0),
-                                       table_width - Tile::kTileKeys + 12);
-                    const float* from = table + base + at;
-#pragma unroll
-                    for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[m][b][e] = fmaf(s[m][b][e], score_factor, from[16 * b + e]);
-                        }
-                    }
-                }
+                score_offset[m] = offset_factor * table[base + (behind ? table_width - 1 : 0)];
             }
-            score_factor = behind || before ? score_factor : 1.0f;
         }
         if (key0 + Tile::kTileKeys > least_limit) {
             asm volatile("");  // stays a branch
@@ -293,7 +312,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
             asm volatile("");  // stays a branch
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
-                const float now = fmaxf(largest[m], peak[m]);
+                const float now = __builtin_elementwise_maximum(largest[m], peak[m]);
                 const float keep = now == largest[m] ? 1.0f : __builtin_amdgcn_exp2f(largest[m] - now);
                 largest[m] = now;
                 total[m] *= keep;
