@@ -190,6 +190,26 @@ __device__ __forceinline__ typename Fragment<T>::type loadRowChunk(const T* from
     return v;
 }
 
+// The calling lane's fragments of a row along its kSteps matrix instruction steps: `width` values exist (0: no row).
+template <typename T, int kSteps>
+__device__ __forceinline__ void loadRowFragments(const T* row, int width, bool whole_chunks, typename Fragment<T>::type (&to)[kSteps]) {
+    const int h = (static_cast<int>(threadIdx.x) & (kWave - 1)) >> 4;
+    if (whole_chunks) {
+        // every chunk is there or not: all loads at once
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) {
+            const int d = (4 * t + h) * kChunk<T>;
+            __builtin_memcpy(&to[t], d < width ? static_cast<const void*>(row + d) : static_cast<const void*>(&zero_chunk), 16);
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) {
+            const int d = (4 * t + h) * kChunk<T>;
+            to[t] = loadRowChunk(row + d, width - d);
+        }
+    }
+}
+
 // kRows rows of kDim values in LDS, one behind the other. A row's chunk c stands in slot c ^ turn(row), so that what is
 // read together falls on different columns of the 256 bytes that the banks hold. A 16-byte read takes 16 lanes at a time,
 // of a lane group and the next one: rows 0-3 and 12-15 of chunk c with rows 4-11 of chunk c + 1, or the others. A
@@ -357,6 +377,21 @@ __device__ __forceinline__ float overGroups(float value) {
     value = __builtin_elementwise_maximum(__uint_as_float(pairs[0]), __uint_as_float(pairs[1]));
     const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(value), __float_as_uint(value), false, false);
     return __builtin_elementwise_maximum(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+
+// Asks the scheduler for kReads LDS reads, each with kEach matrix instructions, in an order that keeps four reads ahead:
+// left to itself it reads late and waits for every read.
+template <int kReads, int kEach>
+__device__ __forceinline__ void scheduleProducts() {
+    constexpr int kAhead = kReads < 4 ? kReads : 4;
+    constexpr int kMatrix = 0x8, kLdsRead = 0x100;
+    __builtin_amdgcn_sched_group_barrier(kLdsRead, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < kReads - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMatrix, kEach, 0);
+        __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMatrix, kAhead * kEach, 0);
 }
 
 // A lane's results for kBlocksTurned row blocks as the other operand of that contraction, rounded to T.

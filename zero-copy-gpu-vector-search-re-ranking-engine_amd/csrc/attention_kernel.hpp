@@ -60,7 +60,6 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
     constexpr int kJoinBytes = kNarrow ? kAttentionWaves * (kDim / 16 * kWave * 16 + 2 * 16 * 4) : 0;
     constexpr int kTileBytes = kTeams * 2 * kStageBytes;
     constexpr int kDimBlocks = kDim / 16;
-    constexpr int kChunkValues = kChunk<T>;
     __shared__ __attribute__((aligned(256))) std::uint8_t lds[kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes];
     __shared__ float table[Tile::kTableFloats];
 
@@ -123,6 +122,26 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
     const int tile_begin = split * tiles_each + (kNarrow ? wave : 0);
     const int tile_end = min(tiles_all, (split + 1) * tiles_each);
 
+    std::uint8_t* own = lds + (kNarrow ? wave * 2 * kStageBytes : 0);
+    Keys k_tile, v_tile;
+    if (tile_begin < tile_end) {
+        const int key0 = tile_begin * Tile::kTileKeys;
+        const std::int64_t first = keys.first + key0;
+        k_tile.begin(static_cast<const T*>(args.k) + first * args.k_stride + key_head * args.head_dim, args.k_stride,
+                     keys.count - key0, args.head_dim, kTeams);
+        v_tile.begin(static_cast<const T*>(args.v) + first * args.v_stride + key_head * args.head_dim, args.v_stride,
+                     keys.count - key0, args.head_dim, kTeams);
+        if constexpr (kDirect) {
+            k_tile.issue(own, kTeams);
+            v_tile.issue(own + Keys::kBytes, kTeams);
+        } else {
+            k_tile.fetch(kTeams);
+            v_tile.fetch(kTeams);
+            k_tile.put(own);
+            v_tile.put(own + Keys::kBytes);
+        }
+    }
+
     const ScoreForm form(args, sizeof(T) == 2);
     float slope[kBlocks];
 #pragma unroll
@@ -142,14 +161,17 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
     }
 
     typename Fragment<T>::type q[kBlocks][Keys::kSteps];
+    const bool whole_chunks = args.head_dim % kChunk<T> == 0;
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) {
         const T* from = static_cast<const T*>(args.q) + row[m] * args.q_stride + head[m] * args.head_dim;
+        loadRowFragments(from, valid[m] ? args.head_dim : 0, whole_chunks, q[m]);
+    }
+    if (args.scale < 0.0f) {
 #pragma unroll
-        for (int t = 0; t < Keys::kSteps; ++t) {
-            const int d = (4 * t + h) * kChunkValues;
-            q[m][t] = loadRowChunk(from + d, valid[m] ? args.head_dim - d : 0);
-            if (args.scale < 0.0f) {
+        for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+            for (int t = 0; t < Keys::kSteps; ++t) {
                 q[m][t] = -q[m][t];
             }
         }
@@ -208,30 +230,38 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
         };
         const bool in_table = args.table != nullptr && !behind && !before;
         const float offset_factor = form.formed ? 1.0f : form.factor;
-        if (in_table && !form.formed) {
-            loadBiases(s);
-        } else {
+        auto products = [&](auto from_zero) {
 #pragma unroll
-            for (int m = 0; m < kBlocks; ++m) {
+            for (int b = 0; b < Tile::kKeyBlocks; ++b) {
 #pragma unroll
-                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-                    s[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int t = 0; t < Keys::kSteps; ++t) {
+                    const auto k = Keys::read(stage, own_lane, b, t);
+#pragma unroll
+                    for (int m = 0; m < kBlocks; ++m) {
+                        s[m][b] = multiplyAdd(k, q[m][t], decltype(from_zero)::value && t == 0 ? f32x4{} : s[m][b]);
+                    }
                 }
             }
-        }
-        if (args.slopes != nullptr && !form.formed) {
-            addSlopes(s);
-        }
-#pragma unroll
-        for (int b = 0; b < Tile::kKeyBlocks; ++b) {
-#pragma unroll
-            for (int t = 0; t < Keys::kSteps; ++t) {
-                const auto k = Keys::read(stage, own_lane, b, t);
+            scheduleProducts<Tile::kKeyBlocks * Keys::kSteps, kBlocks * (sizeof(T) == 2 ? 1 : 4)>();
+        };
+        if (form.formed || (!in_table && args.slopes == nullptr)) {
+            products(std::true_type{});
+        } else {
+            if (in_table) {
+                loadBiases(s);
+            } else {
 #pragma unroll
                 for (int m = 0; m < kBlocks; ++m) {
-                    s[m][b] = multiplyAdd(k, q[m][t], s[m][b]);
+#pragma unroll
+                    for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+                        s[m][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
                 }
             }
+            if (args.slopes != nullptr) {
+                addSlopes(s);
+            }
+            products(std::false_type{});
         }
         if (form.capped) {
             asm volatile("");  // stays a branch
@@ -354,25 +384,8 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
         }
     };
 
-    std::uint8_t* own = lds + (kNarrow ? wave * 2 * kStageBytes : 0);
-    Keys k_tile, v_tile;
-    if (tile_begin < tile_end) {
-        const int key0 = tile_begin * Tile::kTileKeys;
-        const std::int64_t first = keys.first + key0;
-        k_tile.begin(static_cast<const T*>(args.k) + first * args.k_stride + key_head * args.head_dim, args.k_stride,
-                     keys.count - key0, args.head_dim, kTeams);
-        v_tile.begin(static_cast<const T*>(args.v) + first * args.v_stride + key_head * args.head_dim, args.v_stride,
-                     keys.count - key0, args.head_dim, kTeams);
-        if constexpr (kDirect) {
-            k_tile.issue(own, kTeams);
-            v_tile.issue(own + Keys::kBytes, kTeams);
-        } else {
-            k_tile.fetch(kTeams);
-            v_tile.fetch(kTeams);
-            k_tile.put(own);
-            v_tile.put(own + Keys::kBytes);
-        }
-    }
+    // the queries have arrived as well: a wait for them within the loop would be one for the next tile too
+    __builtin_amdgcn_s_waitcnt(vmcntOnly(0));
     int buffer = 0;
     for (int tile = tile_begin; tile < tile_end; tile += kTeams) {
         // this tile has arrived, and every wavefront of the team has read the other buffer
