@@ -191,6 +191,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
     const int wave_key = tile_key + wave * kWaveKeys;
     int key[kBlocks], seen_from[kBlocks];
     bool valid[kBlocks];
+    const bool whole_chunks = args.head_dim % kChunk<T> == 0;
     typename Fragment<T>::type k[kBlocks][Rows::kSteps], v[kBlocks][Rows::kSteps];
 #pragma unroll
     for (int n = 0; n < kBlocks; ++n) {
@@ -198,18 +199,21 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
         valid[n] = key[n] < keys.count;
         seen_from[n] = !args.causal || key[n] < prefix ? INT32_MIN / 2 : key[n];
         const std::int64_t row = keys.first + key[n];
-        const T* k_row = static_cast<const T*>(args.k) + row * args.k_stride + key_head * args.head_dim;
-        const T* v_row = static_cast<const T*>(args.v) + row * args.v_stride + key_head * args.head_dim;
+        const int width = valid[n] ? args.head_dim : 0;
+        loadRowFragments(static_cast<const T*>(args.k) + row * args.k_stride + key_head * args.head_dim, width, whole_chunks, k[n]);
+        loadRowFragments(static_cast<const T*>(args.v) + row * args.v_stride + key_head * args.head_dim, width, whole_chunks, v[n]);
+    }
+    if (args.scale < 0.0f) {
 #pragma unroll
-        for (int t = 0; t < Rows::kSteps; ++t) {
-            const int d = (4 * t + h) * kChunk<T>;
-            k[n][t] = loadRowChunk(k_row + d, valid[n] ? args.head_dim - d : 0);
-            v[n][t] = loadRowChunk(v_row + d, valid[n] ? args.head_dim - d : 0);
-            if (args.scale < 0.0f) {
+        for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+            for (int t = 0; t < Rows::kSteps; ++t) {
                 k[n][t] = -k[n][t];
             }
         }
     }
+    // they have arrived before the loop: a wait within it would be one for the next tile too
+    __builtin_amdgcn_s_waitcnt(vmcntOnly(0));
     f32x4 dk[kBlocks][kDimBlocks], dv[kBlocks][kDimBlocks];
 #pragma unroll
     for (int n = 0; n < kBlocks; ++n) {
@@ -613,6 +617,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
     const float slope = args.slopes != nullptr ? form.bias_factor * args.slopes[head] : 0.0f;
 
     const int wave_row = tile_row + wave * kWaveRows;
+    const bool whole_chunks = args.head_dim % kChunk<T> == 0;
     int place[kBlocks], limit[kBlocks];
     float lse[kBlocks], delta[kBlocks];
     typename Fragment<T>::type q[kBlocks][Keys::kSteps], dout[kBlocks][Keys::kSteps];
@@ -626,14 +631,16 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
         const float* row_stats = more.stats + 2 * (head * args.q_texts.total + row);
         lse[m] = valid ? row_stats[0] : INFINITY;
         delta[m] = valid ? row_stats[1] : 0.0f;
-        const T* q_row = static_cast<const T*>(args.q) + row * args.q_stride + head * args.head_dim;
-        const T* d_row = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim;
+        const int width = valid ? args.head_dim : 0;
+        loadRowFragments(static_cast<const T*>(args.q) + row * args.q_stride + head * args.head_dim, width, whole_chunks, q[m]);
+        loadRowFragments(static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim, width,
+                         whole_chunks, dout[m]);
+    }
+    if (args.scale < 0.0f) {
 #pragma unroll
-        for (int t = 0; t < Keys::kSteps; ++t) {
-            const int d = (4 * t + h) * kChunk<T>;
-            q[m][t] = loadRowChunk(q_row + d, valid ? args.head_dim - d : 0);
-            dout[m][t] = loadRowChunk(d_row + d, valid ? args.head_dim - d : 0);
-            if (args.scale < 0.0f) {
+        for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+            for (int t = 0; t < Keys::kSteps; ++t) {
                 q[m][t] = -q[m][t];
             }
         }
@@ -675,6 +682,8 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
             v_tile.put(lds + Keys::kBytes);
         }
     }
+    // the rows have arrived as well: a wait for them within the loop would be one for the next tile too
+    __builtin_amdgcn_s_waitcnt(vmcntOnly(0));
     int buffer = 0;
     for (int key0 = 0; key0 < all_keys; key0 += kTileKeys) {
         teamSync<kGradientThreads>();
