@@ -929,7 +929,7 @@ template <typename T>
 __global__ __launch_bounds__(kColumnThreads) void joinTablesKernel(const float* __restrict__ partials, int slots, int columns,
                                                                    T* __restrict__ out) {
     joinColumns(partials + static_cast<std::int64_t>(blockIdx.y) * slots * columns, slots, columns,
-                out + static_cast<std::int64_t>(blockIdx.y) * columns);
+                out + static_cast<std::int64_t>(blockIdx.y) * columns, static_cast<int>(blockIdx.x));
 }
 
 }  // namespace

@@ -17,12 +17,12 @@ constexpr int kJoinColumns = 16;
 constexpr int kJoinLanes = kColumnThreads / kJoinColumns;
 
 template <typename T>
-__device__ __forceinline__ void joinColumns(const float* __restrict__ partials, int count, int dim,
-                                                                  T* __restrict__ out) {
+__device__ __forceinline__ void joinColumns(const float* __restrict__ partials, int count, int dim, T* __restrict__ out,
+                                            int block) {
     __shared__ float shared[kJoinLanes][kJoinColumns];
     const int column = static_cast<int>(threadIdx.x) % kJoinColumns;
     const int part = static_cast<int>(threadIdx.x) / kJoinColumns;
-    const int c = static_cast<int>(blockIdx.x) * kJoinColumns + column;
+    const int c = block * kJoinColumns + column;
     float sum = 0.0f;
     if (c < dim) {
 #pragma unroll 8
@@ -44,7 +44,7 @@ __device__ __forceinline__ void joinColumns(const float* __restrict__ partials, 
 template <typename T>
 __global__ __launch_bounds__(kColumnThreads) void joinColumnsKernel(const float* __restrict__ partials, int count, int dim,
                                                                     T* __restrict__ out) {
-    joinColumns(partials, count, dim, out);
+    joinColumns(partials, count, dim, out, static_cast<int>(blockIdx.x));
 }
 
 template <typename T>

@@ -250,10 +250,7 @@ int formGradients(const zcgvs_linear_desc& d, const void* out_gradient, std::int
                               stream>>>(static_cast<const T*>(dz), dz_stride, static_cast<int>(d.rows), d.out_dim, bias_partials);
         ZCGVS_LAUNCH_CHECK("linear gradient");
     }
-    if (status == ZCGVS_OK && bias_gradient != nullptr) {
-        status = launchJoinColumns<T>(bias_partials, bias_rows, d.out_dim, bias_gradient, stream);
-    }
-    if (status != ZCGVS_OK || (input.out == nullptr && weight.out == nullptr)) {
+    if (status != ZCGVS_OK) {
         return status;
     }
     const bool direct_dz = directRows(dz, dz_stride, dz_columns, d.dtype);
@@ -266,7 +263,8 @@ int formGradients(const zcgvs_linear_desc& d, const void* out_gradient, std::int
     input.a_columns = weight.a_columns = dz_columns;
     splitProduct(input_plan, input);
     splitProduct(weight_plan, weight);
-    return launchLinearProducts<T>(input_plan, direct_input, input, weight_plan, direct_weight, weight, stream);
+    const ColumnJoin bias{bias_partials, bias_rows, d.out_dim, bias_gradient};
+    return launchLinearProducts<T>(input_plan, direct_input, input, weight_plan, direct_weight, weight, bias, stream);
 }
 
 }  // namespace

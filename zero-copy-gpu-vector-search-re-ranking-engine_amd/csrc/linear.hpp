@@ -59,6 +59,14 @@ struct ProductArgs {
 constexpr int kThinStageBytes = 1024;  // of k that a workgroup of the kernel for few rows takes at a time
 constexpr int kThinMostRows = 4096;
 
+// The bias's gradient: out [columns] = the sums over `rows` rows of partials, by a launch's last blocks (out null: none).
+struct ColumnJoin {
+    const float* partials;
+    int rows;
+    int columns;
+    void* out;
+};
+
 // How linear.hip runs a call.
 struct LinearPlan {
     ProductPlan product;
@@ -73,10 +81,10 @@ template <typename T>
 int launchLinear(const LinearPlan& plan, int activation, LinearArgs args, hipStream_t stream);
 template <typename T>
 int launchLinearSlope(const LinearPlan& plan, int activation, LinearArgs args, hipStream_t stream);
-// dx = dz weight, dW = dz^T x; a null `out` is not wanted.
+// dx = dz weight, dW = dz^T x and what is left of the bias's gradient; a null `out` is not wanted.
 template <typename T>
 int launchLinearProducts(ProductPlan input_plan, bool input_direct, ProductArgs input, ProductPlan weight_plan,
-                         bool weight_direct, ProductArgs weight, hipStream_t stream);
+                         bool weight_direct, ProductArgs weight, ColumnJoin bias, hipStream_t stream);
 
 int linearInvalid(const char* message);
 

@@ -4,5 +4,6 @@
 namespace zcgvs_hip {
 template int launchLinear<float>(const LinearPlan&, int, LinearArgs, hipStream_t);
 template int launchLinearSlope<float>(const LinearPlan&, int, LinearArgs, hipStream_t);
-template int launchLinearProducts<float>(ProductPlan, bool, ProductArgs, ProductPlan, bool, ProductArgs, hipStream_t);
+template int launchLinearProducts<float>(ProductPlan, bool, ProductArgs, ProductPlan, bool, ProductArgs,
+                                          ColumnJoin, hipStream_t);
 }  // namespace zcgvs_hip

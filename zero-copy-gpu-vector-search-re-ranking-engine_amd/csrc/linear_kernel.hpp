@@ -17,10 +17,10 @@
 #include <type_traits>
 
 #include "activation.hpp"
+#include "column_sums.hpp"
 #include "common.hpp"
 #include "elements.hpp"
 #include "linear.hpp"
-#include "matrix_join.hpp"
 #include "matrix_plan.hpp"
 #include "matrix_split.hpp"
 #include "matrix_tile.hpp"
@@ -420,14 +420,17 @@ __global__ __launch_bounds__(Tile::kThreads) void productKernel(ProductArgs args
 // `input_blocks` blocks form dx.
 template <class InputTile, class WeightTile>
 __global__ __launch_bounds__(InputTile::kThreads) void bothProductsKernel(ProductArgs input, ProductArgs weight,
-                                                                          int input_blocks) {
-    static_assert(InputTile::kThreads == WeightTile::kThreads, "one workgroup size");
+                                                                          int input_blocks, int weight_blocks, ColumnJoin bias) {
+    static_assert(InputTile::kThreads == WeightTile::kThreads && InputTile::kThreads == kColumnThreads, "one workgroup size");
     __shared__ __attribute__((aligned(256))) std::uint8_t
         lds[InputTile::kLdsBytes > WeightTile::kLdsBytes ? InputTile::kLdsBytes : WeightTile::kLdsBytes];
     const int block = static_cast<int>(blockIdx.x);
     if (block < input_blocks) {
         const int tiles = input.tiles_m * input.tiles_n;
         formProduct<InputTile, false>(input, lds, block % tiles, block / tiles);
+    } else if (block >= input_blocks + weight_blocks) {
+        joinColumns(bias.partials, bias.rows, bias.columns, static_cast<typename InputTile::T*>(bias.out),
+                    block - input_blocks - weight_blocks);
     } else {
         const int tiles = weight.tiles_m * weight.tiles_n;
         formProduct<WeightTile, true>(weight, lds, (block - input_blocks) % tiles, (block - input_blocks) / tiles);
@@ -504,27 +507,74 @@ int launchProduct(const ProductPlan& plan, bool direct, ProductArgs args, hipStr
 }
 
 template <class InputTile, class WeightTile>
-int launchBothProducts(ProductArgs input, ProductArgs weight, hipStream_t stream) {
+int launchBothProducts(ProductArgs input, ProductArgs weight, ColumnJoin bias, hipStream_t stream) {
     input.tiles_m = divideUp(input.m, InputTile::kM);
     input.tiles_n = divideUp(input.n, InputTile::kN);
     weight.tiles_m = divideUp(weight.m, WeightTile::kM);
     weight.tiles_n = divideUp(weight.n, WeightTile::kN);
     const long long input_blocks = static_cast<long long>(input.tiles_m) * input.tiles_n * input.splits;
     const long long weight_blocks = static_cast<long long>(weight.tiles_m) * weight.tiles_n * weight.splits;
-    if (input_blocks + weight_blocks > kMaxBlocks) {
+    const long long bias_blocks = bias.out == nullptr ? 0 : divideUp(bias.columns, kJoinColumns);
+    if (input_blocks + weight_blocks + bias_blocks > kMaxBlocks) {
         return linearInvalid("more output than one launch can write");
     }
-    bothProductsKernel<InputTile, WeightTile><<<static_cast<unsigned>(input_blocks + weight_blocks), InputTile::kThreads,
-                                                0, stream>>>(input, weight, static_cast<int>(input_blocks));
+    bothProductsKernel<InputTile, WeightTile><<<static_cast<unsigned>(input_blocks + weight_blocks + bias_blocks),
+                                                InputTile::kThreads, 0, stream>>>(
+        input, weight, static_cast<int>(input_blocks), static_cast<int>(weight_blocks), bias);
     ZCGVS_LAUNCH_CHECK("linear gradient");
     return ZCGVS_OK;
 }
 
+// The sums of both products' splits and the bias's, whichever there are, in one launch: the first blocks take packs of
+// four values of the products, the last ones 16 columns of the bias.
 template <typename T>
-int joinSplits(const ProductArgs& args, hipStream_t stream) {
-    return args.splits == 1 ? static_cast<int>(ZCGVS_OK)
-                            : launchJoin<T>(args.partials, args.splits, args.m, args.n, args.m, args.out, nullptr,
-                                            args.out_stride, stream);
+__global__ __launch_bounds__(kColumnThreads) void joinProductsKernel(ProductArgs input, ProductArgs weight, int input_blocks,
+                                                                     int weight_blocks, ColumnJoin bias) {
+    const int block = static_cast<int>(blockIdx.x);
+    if (block >= input_blocks + weight_blocks) {
+        joinColumns(bias.partials, bias.rows, bias.columns, static_cast<T*>(bias.out), block - input_blocks - weight_blocks);
+        return;
+    }
+    const bool first = block < input_blocks;
+    const ProductArgs& args = first ? input : weight;
+    const int blocks = first ? input_blocks : weight_blocks;
+    const int packs_per_row = (args.n + 3) / 4;
+    const long long packs = static_cast<long long>(args.m) * packs_per_row;
+    const long long split_values = static_cast<long long>(args.m) * args.n;
+    for (long long p = static_cast<long long>(first ? block : block - input_blocks) * kColumnThreads + threadIdx.x; p < packs;
+         p += static_cast<long long>(blocks) * kColumnThreads) {
+        const long long row = p / packs_per_row;
+        const int column = 4 * static_cast<int>(p - row * packs_per_row);
+        const int left = args.n - column;
+        const float* from = args.partials + row * args.n + column;
+        f32x4 sum = loadFour(from, left);
+#pragma unroll 4
+        for (int s = 1; s < args.splits; ++s) {
+            sum += loadFour(from + s * split_values, left);
+        }
+        storeFour(sum, static_cast<T*>(args.out) + row * args.out_stride + column, left);
+    }
+}
+
+inline int joinBlocks(const ProductArgs& args) {
+    const long long packs = static_cast<long long>(args.m) * ((args.n + 3) / 4);
+    return args.out == nullptr || args.splits == 1
+               ? 0
+               : static_cast<int>(std::min(4096ll, (packs + kColumnThreads - 1) / kColumnThreads));
+}
+
+template <typename T>
+int launchJoins(const ProductArgs& input, const ProductArgs& weight, const ColumnJoin& bias, hipStream_t stream) {
+    const int input_blocks = joinBlocks(input);
+    const int weight_blocks = joinBlocks(weight);
+    const int bias_blocks = bias.out == nullptr ? 0 : divideUp(bias.columns, kJoinColumns);
+    if (input_blocks + weight_blocks + bias_blocks == 0) {
+        return ZCGVS_OK;
+    }
+    joinProductsKernel<T><<<static_cast<unsigned>(input_blocks + weight_blocks + bias_blocks), kColumnThreads, 0, stream>>>(
+        input, weight, input_blocks, weight_blocks, bias);
+    ZCGVS_LAUNCH_CHECK("linear gradient");
+    return ZCGVS_OK;
 }
 
 }  // namespace
@@ -541,7 +591,7 @@ int launchLinearSlope(const LinearPlan& plan, int activation, LinearArgs args, h
 
 template <typename T>
 int launchLinearProducts(ProductPlan input_plan, bool input_direct, ProductArgs input, ProductPlan weight_plan,
-                         bool weight_direct, ProductArgs weight, hipStream_t stream) {
+                         bool weight_direct, ProductArgs weight, ColumnJoin bias, hipStream_t stream) {
     const bool wants_input = input.out != nullptr;
     const bool wants_weight = weight.out != nullptr;
     int status = ZCGVS_OK;
@@ -549,14 +599,15 @@ int launchLinearProducts(ProductPlan input_plan, bool input_direct, ProductArgs 
         weight_plan.shape == TileShape::k64x64) {
         if constexpr (std::is_same_v<T, float>) {
             status = launchBothProducts<SplitTile<64, 64, 2, 2, false, true>, SplitTile<64, 64, 2, 2, true, true>>(
-                input, weight, stream);
+                input, weight, bias, stream);
         } else if (input_direct) {
             status = launchBothProducts<MatrixTile<T, 64, 64, 2, 2, false, true, true>,
-                                        MatrixTile<T, 64, 64, 2, 2, true, true, true>>(input, weight, stream);
+                                        MatrixTile<T, 64, 64, 2, 2, true, true, true>>(input, weight, bias, stream);
         } else {
             status = launchBothProducts<MatrixTile<T, 64, 64, 2, 2, false, true, false>,
-                                        MatrixTile<T, 64, 64, 2, 2, true, true, false>>(input, weight, stream);
+                                        MatrixTile<T, 64, 64, 2, 2, true, true, false>>(input, weight, bias, stream);
         }
+        bias.out = nullptr;
     } else {
         if (wants_input) {
             status = launchProduct<T, false>(input_plan, input_direct, input, stream);
@@ -565,11 +616,8 @@ int launchLinearProducts(ProductPlan input_plan, bool input_direct, ProductArgs 
             status = launchProduct<T, true>(weight_plan, weight_direct, weight, stream);
         }
     }
-    if (status == ZCGVS_OK && wants_input) {
-        status = joinSplits<T>(input, stream);
-    }
-    if (status == ZCGVS_OK && wants_weight) {
-        status = joinSplits<T>(weight, stream);
+    if (status == ZCGVS_OK) {
+        status = launchJoins<T>(input, weight, bias, stream);
     }
     return status;
 }
