@@ -16,6 +16,9 @@ what the call returns); calls may follow each other without a wait, also on chan
 
 The reference's QueryEmbedder (include/zcgvs/embed/query_embedder.hpp:8-15) returns one text's vector on
 the host instead. `gradient` gives what training the table and the gated block needs.
+
+With `encoder`, an EncoderBlocks, each token's row (table[id] times `scale`) goes through its blocks, where it meets the
+other tokens of its text, before the mean is taken; padding and ids out of range are left out of the texts first.
 """
 
 from __future__ import annotations
@@ -60,7 +63,7 @@ class DeviceEmbedder:
     optionally ranks [n] and scales [n]."""
 
     def __init__(self, table, gate, up, projection, *, dtype, scale=1.0, padding_id=-1, activation=capi.ACT_SILU,
-                 adapters=None):
+                 adapters=None, encoder=None):
         self.dtype, self.scale, self.padding_id, self.activation = dtype, scale, padding_id, activation
         if dtype not in _STORAGE:
             _refuse("dtype must be F32, F16 or BF16")
@@ -72,6 +75,9 @@ class DeviceEmbedder:
         up = _matrix("up", up, (self.hidden, self.dim), element)
         projection = _matrix("projection", projection, (None, self.hidden), element)
         self.width = projection.shape[0]
+        if encoder is not None and (encoder.dim != self.dim or encoder.dtype != dtype):
+            _refuse(f"the encoder's rows are [{encoder.dim}] of dtype {encoder.dtype}, not [{self.dim}] of {dtype}")
+        self.encoder = encoder
         parts = {}
         if adapters is not None:
             if adapters.get("down") is None or adapters.get("up") is None:
@@ -138,21 +144,44 @@ class DeviceEmbedder:
             _refuse("offsets must ascend from 0 or more to at most the number of ids")
         return ids, offsets
 
-    def _forward(self, ids, offsets, stream, **more):
-        """The lookup and the gated block; `more`: further host arrays of the call, name=(values, type), copied
-        beside the ids."""
+    def _without_padding(self, ids, offsets):
+        """The tokens of the texts that count, one text directly behind the other."""
+        ids, offsets = ids[offsets[0]:offsets[-1]], offsets - offsets[0]
+        held = (ids >= 0) & (ids < self.vocab) & (ids != self.padding_id)
+        return ids[held], np.concatenate([[0], np.cumsum(held, dtype=np.int64)])[offsets]
+
+    def _encode(self, d_ids, d_offsets, d_order, texts, tokens, stream, keep):
+        """The token rows through the encoder, and the descriptors of their lookup and of their mean by text."""
+        lookup = capi.embedding_desc(self.table, self.vocab, self.dim, self.dtype, d_ids, tokens, scale=self.scale)
+        x = self._buffer("token rows", (tokens, self.dim), self._element)
+        capi.embedding_lookup(lookup, x, self.dtype, stream=stream)
+        encoded, kept = self.encoder.forward(self._buffer, x, d_offsets, texts, tokens, stream, keep)
+        pooled = capi.embedding_desc(encoded, tokens, self.dim, self.dtype, d_order, tokens, bag_offsets=d_offsets,
+                                     bag_count=texts, reduce=capi.EMBEDDING_MEAN)
+        return pooled, dict(lookup=lookup, kept=kept, tokens=tokens)
+
+    def _forward(self, ids, offsets, stream, keep=False, **more):
+        """The lookup (with an encoder: the mean of its rows) and the gated block; `more`: further host arrays of the
+        call, name=(values, type), copied beside the ids."""
+        if self.encoder is not None:
+            ids, offsets = self._without_padding(ids, offsets)
+            more = dict(more, order=(np.arange(len(ids)), np.int32))
         texts, tokens = len(offsets) - 1, len(ids)
         self._enter(stream)
         d_ids, d_offsets = self._upload("ids", ids, np.int32), self._upload("offsets", offsets, np.int64)
         uploaded = {name: self._upload(name, *values) for name, values in more.items()}
         self._settle()
-        lookup = self._lookup_desc(d_ids, d_offsets, texts, tokens)
+        encoded = None
+        if self.encoder is not None and tokens:
+            lookup, encoded = self._encode(d_ids, d_offsets, uploaded["order"], texts, tokens, stream, keep)
+        else:
+            lookup = self._lookup_desc(d_ids, d_offsets, texts, tokens)
         rows = self._buffer("rows", (texts, self.dim), self._element)
         hidden = self._buffer("hidden", (texts, self.hidden), self._element)
         capi.embedding_lookup(lookup, rows, self.dtype, stream=stream)
         gated = capi.gated_desc(rows, texts, self.dim, self.gate, self.up, self.hidden, self.dtype, self.activation)
         capi.gated_projection(gated, hidden, stream=stream)
-        return lookup, gated, hidden, uploaded
+        return lookup, gated, hidden, dict(uploaded, encoded=encoded)
 
     def embed(self, ids, offsets, adapter_ids=None, stream=None) -> capi.DeviceArray:
         """Queries of the texts ids[offsets[t]:offsets[t + 1]], each through adapter adapter_ids[t] (-1: none):
@@ -168,7 +197,7 @@ class DeviceEmbedder:
                 _refuse("one adapter id per text")
             more = dict(adapter_ids=(adapter_ids, np.int32))
         _, _, hidden, uploaded = self._forward(ids, offsets, stream, **more)
-        extra = dict(self._adapters, **uploaded) if uploaded else {}
+        extra = dict(self._adapters, adapter_ids=uploaded["adapter_ids"]) if more else {}
         desc = capi.adapted_desc(hidden, texts, self.hidden, self.projection, self.width, self.dtype, **extra)
         size = capi.adapted_projection_workspace_bytes(desc)
         workspace = self._buffer("workspace", (size,), np.uint8)
@@ -188,19 +217,31 @@ class DeviceEmbedder:
 
     def gradient(self, ids, offsets, hidden_gradient, stream=None) -> dict:
         """The gradients of the table (float32) and of gate and up (their type), as device arrays, from the
-        gradient of the hidden rows (host [texts, hidden], of the model's type: no other is converted)."""
+        gradient of the hidden rows (host [texts, hidden], of the model's type: no other is converted). With an
+        encoder also `encoder`: dict(blocks=[{name: array}], final_norm=array), None where no text has a token."""
         ids, offsets = self._lists(ids, offsets)
         texts = len(offsets) - 1
         hidden_gradient = _matrix("hidden_gradient", hidden_gradient, (texts, self.hidden), self._element)
-        lookup, gated, _, uploaded = self._forward(ids, offsets, stream, hidden_gradient=(hidden_gradient, self._element))
+        lookup, gated, _, uploaded = self._forward(ids, offsets, stream, keep=True,
+                                                   hidden_gradient=(hidden_gradient, self._element))
         d_hidden = uploaded["hidden_gradient"]
         rows = self._buffer("rows_gradient", (texts, self.dim), self._element)
         gate, up = (capi.DeviceArray((self.hidden, self.dim), self._element) for _ in range(2))
         size = capi.gated_gradient_workspace_bytes(gated)
         capi.gated_gradient(gated, d_hidden, rows, gate, up, self._buffer("gated_workspace", (size,), np.uint8), size,
                             stream=stream)
-        table = capi.DeviceArray((self.vocab, self.dim), np.float32)
+        table, more = capi.DeviceArray((self.vocab, self.dim), np.float32), {}
+        if self.encoder is not None:
+            more = dict(encoder=None)
+        if uploaded["encoded"] is not None:
+            saved, tokens = uploaded["encoded"], uploaded["encoded"]["tokens"]
+            mean = self._buffer("encoded gradient", (tokens, self.dim), self._element)
+            size = capi.embedding_gradient_workspace_bytes(lookup)
+            capi.embedding_gradient(lookup, rows, self.dtype, mean, self.dtype,
+                                    self._buffer("mean workspace", (size,), np.uint8), size, stream=stream)
+            rows, more["encoder"] = self.encoder.gradient(self._buffer, saved["kept"], mean, tokens, stream)
+            lookup = saved["lookup"]
         size = capi.embedding_gradient_workspace_bytes(lookup)
         capi.embedding_gradient(lookup, rows, self.dtype, table, capi.F32,
                                 self._buffer("table_workspace", (size,), np.uint8), size, stream=stream)
-        return dict(table=table, gate=gate, up=up)
+        return dict(table=table, gate=gate, up=up, **more)
