@@ -658,7 +658,8 @@ enum zcgvs_attention_align { ZCGVS_ATTENTION_FIRST = 0, ZCGVS_ATTENTION_LAST = 1
  *     s_j = c - slopes[h] * |j - p| + distance_bias[h][clamp(j - p, -max_distance, max_distance) + max_distance]
  *     out_i = sum_j softmax(s)_j v_j   over the keys that i sees.
  * A query row sees the keys of its own text; with `causal` those at j <= p and, where prefix_lengths is
- * given, those at j < prefix_lengths[t] as well. A row that sees no key gives zeros.
+ * given, those at j < prefix_lengths[t] as well. A distance_bias of -1e30 or less leaves the keys at its distances
+ * out, as minus infinity does. A row that sees no key gives zeros.
  * The rows of text t are q_offsets[t] .. q_offsets[t + 1] - 1 (offsets ascend and lie in [0, q_rows]), or
  * with q_offsets NULL t * (q_rows / texts) on (q_rows a multiple of texts): one query row a text, or a padded
  * batch. Of these the first q_lengths[t] count (clamped to [0, the text's rows]; NULL: all); the rest are padding:

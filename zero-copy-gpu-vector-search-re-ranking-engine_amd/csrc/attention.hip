@@ -267,7 +267,7 @@ int zcgvs_attention_gradient(const zcgvs_attention_desc* desc, const void* d_out
     if (d_distance_bias_gradient != nullptr && d.distance_bias == nullptr) {
         return attentionInvalid("a gradient of the distance bias needs the distance bias");
     }
-    const int table_count = d.heads * (2 * d.max_distance + 1);
+    const int table_count = d.distance_bias == nullptr ? 0 : d.heads * (2 * d.max_distance + 1);
     if (d.texts == 0 || (d.q_rows == 0 && d.k_rows == 0)) {
         if (d_distance_bias_gradient != nullptr) {
             return withElement(d.dtype, [&](auto element) {
@@ -323,7 +323,7 @@ int zcgvs_attention_gradient(const zcgvs_attention_desc* desc, const void* d_out
         plan.query_blocks = gradientBlocks(d.q_rows, d.texts);
         const long long key_slots = slotsFor(d.k_rows, d.texts, plan.key_blocks);
         const long long query_slots = slotsFor(d.q_rows, d.texts, plan.query_blocks);
-        if (key_slots * d.kv_heads > kMaxBlocks || query_slots * d.heads > kMaxBlocks) {
+        if (key_slots * d.kv_heads > kMaxAttentionBlocks || query_slots * d.heads > kMaxAttentionBlocks) {
             return attentionInvalid("more texts and rows than one launch can take");
         }
         more.key_slots = static_cast<int>(key_slots);

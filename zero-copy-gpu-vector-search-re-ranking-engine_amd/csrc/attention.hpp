@@ -15,6 +15,7 @@ namespace zcgvs_hip {
 
 constexpr int kAttentionMaxDim = 128;
 constexpr int kAttentionMaxDistance = 512;
+constexpr long long kMaxAttentionBlocks = (1ll << 24) - 1;  // a launch has less than 2^32 threads, of 256 a block
 constexpr float kLog2E = 1.44269504f;
 constexpr float kLn2 = 0.69314718f;
 

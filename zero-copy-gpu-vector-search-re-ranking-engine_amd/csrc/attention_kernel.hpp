@@ -592,7 +592,7 @@ int launchAttentionTiles(const AttentionArgs& args, AttentionOutput output, hipS
     using Tile = AttentionTile<T, kDim, kBlocks, kNarrow>;
     const int units = kNarrow ? args.heads / args.group : args.heads;
     const long long slots = slotsOf(args.q_texts, kNarrow ? args.group : 1, Tile::kRows);
-    if (slots * units * output.splits > kMaxBlocks) {
+    if (slots * units * output.splits > kMaxAttentionBlocks) {
         return attentionInvalid("more texts and rows than one launch can take");
     }
     output.slots = static_cast<int>(slots);
