@@ -4,7 +4,9 @@ at once on two streams, biases that leave keys out, int8 rows from the norm to t
 import numpy as np
 import pytest
 
+from attention_helpers import Batch
 from operator_helpers import from_bits, kind_code, to_bits
+from test_gpu_attention_gradient import check
 
 pytestmark = pytest.mark.gpu
 
@@ -313,3 +315,19 @@ def test_int8_rows_into_the_product(gpu, kind, rows):
     # the scales' product, the sum's conversion and product, two additions: a float32 rounding each
     allowed = 5 * 2.0 ** -24 * (np.abs(product) + np.abs(from_bits(bias, kind)) + np.abs(from_bits(residual, kind)))
     assert np.all(np.abs(out.to_host() - want) <= allowed)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(3, 1, 33), (16, 2, 64), (7, 1, 20), (6, 2, 1), (5, 5, 40)])
+def test_key_heads_of_many_query_heads(gpu, kind, heads, kv_heads, head_dim):
+    """Few keys under many query heads, whose parts are formed apart and added: the formula's gradients, and rows of no
+    text left as they were."""
+    batch = Batch(gpu, kind, [30, 0, 77, 1], heads=heads, kv_heads=kv_heads, head_dim=head_dim, mask="causal", bias="table", far=4,
+                  lead=5, tail=3, pad=1)
+    grad, got = check(batch, pad=3, shift=1)
+    for name in ("q", "k", "v"):
+        assert np.all(got[name][:5] == 7.0) and np.all(got[name][-3:] == 7.0), name
+    first = {name: values.copy() for name, values in got.items()}
+    grad.call()
+    gpu.synchronize()
+    assert all(np.array_equal(first[name], values) for name, values in grad.read().items())

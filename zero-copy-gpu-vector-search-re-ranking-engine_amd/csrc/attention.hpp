@@ -87,6 +87,8 @@ struct AttentionGradient {
     float* stats;           // [heads, q_rows, 2]: lse in base 2, delta
     float* table_partials;  // [heads, key_slots, 2 * max_distance + 1], or null: not wanted
     int key_slots;          // tiles of keys, empty ones among them
+    int key_parts;          // of a key head's query heads, each with its own workgroups
+    float* key_partials;    // [2 (dk, dv), key_parts, k_rows, kv_heads * head_dim] (key_parts > 1)
     int query_slots;
 };
 

@@ -4,11 +4,12 @@
 //     dbias = sums of ds along the diagonals,  dr = ds (1 - (c / cap)^2)
 //     dq = scale dr k,  dk = scale dr^T q,  dv = p^T dout
 //
-// Three launches (four with the bias's gradient), no atomics between workgroups: the same bits on every call.
+// Three launches (one more each with the bias's gradient and with few keys), no atomics between workgroups: the same bits on every call.
 // 1. delta and the rows' lse in base 2, head by head.
 // 2. dk and dv: a wavefront keeps 16 or 32 keys and their values in registers and goes through the queries of all heads of
 //    its key head, in LDS tiles of 32 rows that the workgroup shares. Scores come out with a lane's four neighbouring query
 //    rows of one key, which is how the products over the rows take p and dr: they stay in registers.
+//    Where that leaves CUs idle, the query heads are split over workgroups and one more launch adds the parts.
 // 3. dq: a wavefront keeps 16 or 32 query rows and goes through the keys, as the forward kernel does.
 // So p is formed twice: seven products instead of five, for sums in one order and no float32 copy of dq.
 // The bias's gradient: a wavefront adds its tile up along the diagonals by moving rows along the lanes, and every lane
@@ -19,6 +20,8 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "attention.hpp"
 #include "column_sums.hpp"
@@ -161,7 +164,11 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
     const int h = lane >> 4;
     const int position = positionOf(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
     const int slot = position % more.key_slots;
-    const int key_head = position / more.key_slots;
+    const int key_heads = args.heads / args.group;
+    const int key_head = position / more.key_slots % key_heads;
+    const int part = position / more.key_slots / key_heads;
+    const int first_head = part * args.group / more.key_parts;  // of the part, within the key head's
+    const int end_head = (part + 1) * args.group / more.key_parts;
     const int table_columns = 2 * args.max_distance + 1;
     auto partialTable = [&](int head) {
         return more.table_partials + (static_cast<std::int64_t>(head) * more.key_slots + slot) * table_columns;
@@ -175,7 +182,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
     }
     if (text < 0 || tile_key < 0 || tile_key >= keys.rows) {
         if constexpr (kFar > 0) {
-            for (int g = 0; g < args.group; ++g) {
+            for (int g = first_head; g < end_head; ++g) {
                 for (int i = static_cast<int>(threadIdx.x); i < table_columns; i += kGradientThreads) {
                     partialTable(key_head * args.group + g)[i] = 0.0f;
                 }
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
     const int last_key = min(wave_key + kWaveKeys, keys.count) - 1;
     const bool hidden_keys = args.causal && last_key >= prefix;  // some key of the wavefront is not seen by all
 
-    for (int g = 0; g < args.group; ++g) {
+    for (int g = first_head; g < end_head; ++g) {
         const int head = key_head * args.group + g;
         const float slope = args.slopes != nullptr ? form.bias_factor * args.slopes[head] : 0.0f;
         float past[2] = {};  // sums of ds at distances past the table's ends: before, behind
@@ -564,6 +571,20 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
             continue;
         }
         const std::int64_t row = keys.first + key[n];
+        if (more.key_parts > 1) {
+            const std::int64_t width = static_cast<std::int64_t>(key_heads) * args.head_dim;
+            float* to = more.key_partials + (part * args.k_texts.total + row) * width + key_head * args.head_dim;
+            const std::int64_t values_on = more.key_parts * args.k_texts.total * width;
+#pragma unroll
+            for (int d = 0; d < kDimBlocks; ++d) {
+                const int column = 16 * d + 4 * h;
+                if (column < args.head_dim) {
+                    storeFour(valid[n] ? dk[n][d] * args.scale : f32x4{}, to + column, args.head_dim - column);
+                    storeFour(valid[n] ? dv[n][d] : f32x4{}, to + values_on + column, args.head_dim - column);
+                }
+            }
+            continue;
+        }
         T* k_to = static_cast<T*>(more.k_gradient) + row * more.k_gradient_stride + key_head * args.head_dim;
         T* v_to = static_cast<T*>(more.v_gradient) + row * more.v_gradient_stride + key_head * args.head_dim;
 #pragma unroll
@@ -574,6 +595,31 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
                 storeFour(valid[n] ? dv[n][d] : f32x4{}, v_to + column, args.head_dim - column);
             }
         }
+    }
+}
+
+// dk and dv from the parts of their query heads, in their order; rows of no text are left as they are.
+template <typename T>
+__global__ __launch_bounds__(kGradientThreads) void joinKeyPartsKernel(AttentionArgs args, AttentionGradient more) {
+    const int width = args.heads / args.group * args.head_dim;
+    const int packs = (width + 3) / 4;
+    const std::int64_t first = textStart(args.k_texts, 0), end = textStart(args.k_texts, args.k_texts.texts);
+    const std::int64_t part_values = args.k_texts.total * width;
+    const bool values = blockIdx.y == 1;
+    const float* partials = more.key_partials + (values ? more.key_parts * part_values : 0);
+    T* out = static_cast<T*>(values ? more.v_gradient : more.k_gradient);
+    const std::int64_t stride = values ? more.v_gradient_stride : more.k_gradient_stride;
+    for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * kGradientThreads + threadIdx.x; i < (end - first) * packs;
+         i += static_cast<std::int64_t>(gridDim.x) * kGradientThreads) {
+        const std::int64_t row = first + i / packs;
+        const int column = 4 * static_cast<int>(i % packs);
+        const float* from = partials + row * width + column;
+        f32x4 sum = loadFour(from, width - column);
+#pragma unroll 4
+        for (int p = 1; p < more.key_parts; ++p) {
+            sum += loadFour(from + p * part_values, width - column);
+        }
+        storeFour(sum, out + row * stride + column, width - column);
     }
 }
 
@@ -881,7 +927,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
 
 template <typename T, int kDim, int kBlocks, bool kDirect>
 int launchKeyGradient(const AttentionArgs& args, const AttentionGradient& more, hipStream_t stream) {
-    const unsigned blocks = static_cast<unsigned>(more.key_slots * (args.heads / args.group));
+    const unsigned blocks = static_cast<unsigned>(more.key_slots * (args.heads / args.group) * more.key_parts);
     if (more.table_partials == nullptr) {
         keyGradientKernel<T, kDim, kBlocks, kDirect, 0><<<blocks, kGradientThreads, 0, stream>>>(args, more);
     } else if (args.max_distance <= 128) {
@@ -890,6 +936,12 @@ int launchKeyGradient(const AttentionArgs& args, const AttentionGradient& more, 
         keyGradientKernel<T, kDim, kBlocks, kDirect, kAttentionMaxDistance><<<blocks, kGradientThreads, 0, stream>>>(args, more);
     }
     ZCGVS_LAUNCH_CHECK("attention gradient");
+    if (more.key_parts > 1) {
+        const long long packs = args.k_texts.total * ((args.heads / args.group * args.head_dim + 3) / 4);
+        const unsigned join_blocks = static_cast<unsigned>(std::min(4096ll, (packs + kGradientThreads - 1) / kGradientThreads));
+        joinKeyPartsKernel<T><<<dim3(join_blocks, 2), kGradientThreads, 0, stream>>>(args, more);
+        ZCGVS_LAUNCH_CHECK("attention gradient");
+    }
     return ZCGVS_OK;
 }
 
