@@ -17,6 +17,9 @@
 // additions is the program's), with room for distances past the table's ends; tiles that lie past them altogether add
 // to two registers. A workgroup joins its tables and writes
 // one of partial sums a head, which the last launch adds in the order of the workgroups.
+// Bound by the vector units (exponentials, the bias's sums) beside seven products. Measured, bfloat16: 128 texts of 64 to 512, 12 heads
+// of 64, a learned bias and its gradient 380-395 us (keys 251, queries 136, rows 26 at memory's rate); 8 texts of 4096, 8 heads
+// of 64 on 2 1040 us, of 128 2130. 3 texts of 20 to 77 float32 27.2 us (the launches).
 #pragma once
 
 #include <hip/hip_runtime.h>

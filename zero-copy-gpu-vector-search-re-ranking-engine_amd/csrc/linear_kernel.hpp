@@ -10,6 +10,11 @@
 // Few rows (linearThinKernel) are bound by latency and by reading W once: a workgroup takes 16 columns and 16 or 32
 // rows, its eight wavefronts every eighth 128 bytes of k, straight from memory into registers, and joins their sums
 // through LDS. No LDS stages, no splits over workgroups, one launch.
+//
+// Measured: one row 768 -> 768 float16 6.6 us (the launch); 8192 rows 1024 -> 4096 int8, GELU by tanh 55-58 us (1.2 POP/s), bfloat16
+// 84-87 (0.8 PFLOP/s); 8192 cubed bfloat16 1015 us (1.08 PFLOP/s, a library product 1.45); the gradient of 16,384 rows 768 -> 2048
+// bfloat16 216 us (dz 91, dW 66, dx 55, joins 8). Bound by the product loop, dz also by its loads and stores between the
+// tiles' products.
 #pragma once
 
 #include <hip/hip_runtime.h>

