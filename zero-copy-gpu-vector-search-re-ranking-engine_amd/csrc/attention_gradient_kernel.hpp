@@ -4,13 +4,14 @@
 //     dbias = sums of ds along the diagonals,  dr = ds (1 - (c / cap)^2)
 //     dq = scale dr k,  dk = scale dr^T q,  dv = p^T dout
 //
-// Three launches (one more each with the bias's gradient and with few keys), no atomics between workgroups: the same bits on every call.
-// 1. delta and the rows' lse in base 2, head by head.
+// Two launches (one more each with the bias's gradient and with few keys), no atomics between workgroups: the same bits on
+// every call.
+// 1. dq: a wavefront keeps 16 or 32 query rows and goes through the keys, as the forward kernel does. Before, it forms delta
+//    and the rows' lse in base 2, for itself and the second launch (in a launch of their own 392 us instead of the 376 below).
 // 2. dk and dv: a wavefront keeps 16 or 32 keys and their values in registers and goes through the queries of all heads of
 //    its key head, in LDS tiles of 32 rows that the workgroup shares. Scores come out with a lane's four neighbouring query
 //    rows of one key, which is how the products over the rows take p and dr: they stay in registers.
 //    Where that leaves CUs idle, the query heads are split over workgroups and one more launch adds the parts.
-// 3. dq: a wavefront keeps 16 or 32 query rows and goes through the keys, as the forward kernel does.
 // So p is formed twice: seven products instead of five, for sums in one order and no float32 copy of dq.
 // The bias's gradient: a wavefront adds its tile up along the diagonals by moving rows along the lanes, and every lane
 // group adds the result to a table of its own in LDS (its 16 lanes always meet 16 different distances, so the order of
@@ -18,8 +19,8 @@
 // to two registers. A workgroup joins its tables and writes
 // one of partial sums a head, which the last launch adds in the order of the workgroups.
 // Bound by the vector units (exponentials, the bias's sums) beside seven products. Measured, bfloat16: 128 texts of 64 to 512, 12 heads
-// of 64, a learned bias and its gradient 380-395 us (keys 251, queries 136, rows 26 at memory's rate); 8 texts of 4096, 8 heads
-// of 64 on 2 1040 us, of 128 2130. 3 texts of 20 to 77 float32 27.2 us (the launches).
+// of 64, a learned bias and its gradient 376 us (queries 147, keys 257 under the profiler); 8 texts of 4096, 8 heads of 64 on 2
+// 1035 us, of 128 2055. 3 texts of 20 to 77 float32, 6 heads of 32 on 2 24.5 us (the launches).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -38,54 +39,6 @@ constexpr int kGradientThreads = kGradientWaves * kWave;
 constexpr int kQueryTile = 32;
 
 static __device__ const float no_row[2] = {INFINITY, 0.0f};  // p = 0
-
-// ---- rows: lse in base 2 and delta, [heads, q_rows, 2] -------------------------------------------
-
-// Workgroups of 16 rows and up to 64 heads, so that a head's rows are written together.
-constexpr int kStatsLanes = 8;  // of a row and head, 16 bytes each
-constexpr int kStatsRows = 16;
-constexpr int kStatsHeads = 64;
-
-template <typename T>
-__global__ __launch_bounds__(kGradientThreads) void attentionStatsKernel(AttentionArgs args, AttentionGradient more) {
-    __shared__ float shared[kStatsHeads][kStatsRows][2];
-    const int lane = static_cast<int>(threadIdx.x) % kStatsLanes;
-    const std::int64_t first_row = static_cast<std::int64_t>(blockIdx.x) * kStatsRows;
-    const int first_head = static_cast<int>(blockIdx.y) * kStatsHeads;
-    const int heads = min(args.heads - first_head, kStatsHeads);
-    const int rows = static_cast<int>(min<std::int64_t>(args.q_texts.total - first_row, kStatsRows));
-    for (int i = static_cast<int>(threadIdx.x) / kStatsLanes; i < rows * heads; i += kGradientThreads / kStatsLanes) {
-        const std::int64_t row = first_row + i / heads;
-        const int head = first_head + i % heads;
-        const T* out = static_cast<const T*>(more.out) + row * more.out_stride + head * args.head_dim;
-        const T* from = static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim;
-        float sum = 0.0f;
-        for (int d = kChunk<T> * lane; d < args.head_dim; d += kChunk<T> * kStatsLanes) {
-            const auto a = loadRowChunk(out + d, args.head_dim - d);
-            const auto b = loadRowChunk(from + d, args.head_dim - d);
-#pragma unroll
-            for (int e = 0; e < kChunk<T>; ++e) {
-                sum = fmaf(static_cast<float>(a[e]), static_cast<float>(b[e]), sum);
-            }
-        }
-#pragma unroll
-        for (int offset = kStatsLanes / 2; offset > 0; offset >>= 1) {
-            sum += waveXor(sum, offset);
-        }
-        if (lane == 0) {
-            const float lse = more.lse[row * args.heads + head];
-            float* to = shared[head - first_head][i / heads];
-            to[0] = lse == -INFINITY ? INFINITY : kLog2E * lse;
-            to[1] = lse == -INFINITY ? 0.0f : sum;
-        }
-    }
-    __syncthreads();
-    for (int i = static_cast<int>(threadIdx.x); i < heads * rows * 2; i += kGradientThreads) {
-        const int head = i / (2 * rows);
-        const int at = i - head * 2 * rows;
-        more.stats[2 * ((first_head + head) * args.q_texts.total + first_row) + at] = shared[head][at / 2][at % 2];
-    }
-}
 
 // ---- shared by both kernels ----------------------------------------------------------------------
 
@@ -669,7 +622,7 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
     const bool whole_chunks = args.head_dim % kChunk<T> == 0;
     int place[kBlocks], limit[kBlocks];
     float lse[kBlocks], delta[kBlocks];
-    typename Fragment<T>::type q[kBlocks][Keys::kSteps], dout[kBlocks][Keys::kSteps];
+    typename Fragment<T>::type q[kBlocks][Keys::kSteps], dout[kBlocks][Keys::kSteps], out[kBlocks][Keys::kSteps];
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) {
         const int i = wave_row + 16 * m + r16;
@@ -677,10 +630,9 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
         const std::int64_t row = queries.first + i;
         place[m] = i + shift;
         limit[m] = valid ? limitAt(place[m]) : 0;
-        const float* row_stats = more.stats + 2 * (head * args.q_texts.total + row);
-        lse[m] = valid ? row_stats[0] : INFINITY;
-        delta[m] = valid ? row_stats[1] : 0.0f;
         const int width = valid ? args.head_dim : 0;
+        lse[m] = valid ? more.lse[row * args.heads + head] : -INFINITY;
+        loadRowFragments(static_cast<const T*>(more.out) + row * more.out_stride + head * args.head_dim, width, whole_chunks, out[m]);
         loadRowFragments(static_cast<const T*>(args.q) + row * args.q_stride + head * args.head_dim, width, whole_chunks, q[m]);
         loadRowFragments(static_cast<const T*>(more.out_gradient) + row * more.out_gradient_stride + head * args.head_dim, width,
                          whole_chunks, dout[m]);
@@ -731,8 +683,32 @@ __global__ __launch_bounds__(kGradientThreads, (kQueryResident<T, kDim, kBlocks>
             v_tile.put(lds + Keys::kBytes);
         }
     }
-    // the rows have arrived as well: a wait for them within the loop would be one for the next tile too
+    // delta, from the chunks of the row's four lanes, and lse in base 2, here and for the launch of the keys (a wait for the
+    // rows within the loop would be one for the next tile too)
     __builtin_amdgcn_s_waitcnt(vmcntOnly(0));
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < Keys::kSteps; ++t) {
+#pragma unroll
+            for (int e = 0; e < kChunk<T>; ++e) {
+                sum = fmaf(static_cast<float>(out[m][t][e]), static_cast<float>(dout[m][t][e]), sum);
+            }
+        }
+        sum += waveXor(sum, 16);
+        sum += waveXor(sum, 32);
+        // a row that sees no key: p = 0
+        const bool empty = lse[m] == -INFINITY;
+        lse[m] = empty ? INFINITY : kLog2E * lse[m];
+        delta[m] = empty ? 0.0f : sum;
+        const int i = wave_row + 16 * m + r16;
+        if (h == 0 && i < queries.count) {
+            float* row_stats = more.stats + 2 * (head * args.q_texts.total + queries.first + i);
+            row_stats[0] = lse[m];
+            row_stats[1] = delta[m];
+        }
+    }
     int buffer = 0;
     for (int key0 = 0; key0 < all_keys; key0 += kTileKeys) {
         teamSync<kGradientThreads>();
@@ -951,18 +927,6 @@ int launchKeyGradient(const AttentionArgs& args, const AttentionGradient& more, 
 template <typename T, int kDim>
 int launchGradientDim(const AttentionGradientPlan& plan, const AttentionArgs& args, const AttentionGradient& more,
                       hipStream_t stream) {
-    int status = ZCGVS_OK;
-    constexpr bool kTwo = sizeof(T) == 2 || kDim < 128;  // (as attention.hip plans)
-    if (!kTwo || plan.key_blocks == 1) {
-        status = plan.direct_rows ? launchKeyGradient<T, kDim, 1, true>(args, more, stream)
-                                  : launchKeyGradient<T, kDim, 1, false>(args, more, stream);
-    } else if constexpr (kTwo) {
-        status = plan.direct_rows ? launchKeyGradient<T, kDim, 2, true>(args, more, stream)
-                                  : launchKeyGradient<T, kDim, 2, false>(args, more, stream);
-    }
-    if (status != ZCGVS_OK) {
-        return status;
-    }
     const unsigned blocks = static_cast<unsigned>(more.query_slots * args.heads);
     if (plan.query_blocks == 1) {
         if (plan.direct_keys) {
@@ -976,7 +940,15 @@ int launchGradientDim(const AttentionGradientPlan& plan, const AttentionArgs& ar
         queryGradientKernel<T, kDim, 2, false><<<blocks, kGradientThreads, 0, stream>>>(args, more);
     }
     ZCGVS_LAUNCH_CHECK("attention gradient");
-    return ZCGVS_OK;
+    constexpr bool kTwo = sizeof(T) == 2 || kDim < 128;  // (as attention.hip plans)
+    if constexpr (kTwo) {
+        if (plan.key_blocks == 2) {
+            return plan.direct_rows ? launchKeyGradient<T, kDim, 2, true>(args, more, stream)
+                                    : launchKeyGradient<T, kDim, 2, false>(args, more, stream);
+        }
+    }
+    return plan.direct_rows ? launchKeyGradient<T, kDim, 1, true>(args, more, stream)
+                            : launchKeyGradient<T, kDim, 1, false>(args, more, stream);
 }
 
 // out [heads, columns] = the sums over the slots of partials [heads, slots, columns].
@@ -992,10 +964,6 @@ __global__ __launch_bounds__(kColumnThreads) void joinTablesKernel(const float* 
 template <typename T>
 int launchAttentionGradient(const AttentionGradientPlan& plan, const AttentionArgs& args, const AttentionGradient& more,
                             hipStream_t stream) {
-    const dim3 stats_grid(static_cast<unsigned>((args.q_texts.total + kStatsRows - 1) / kStatsRows),
-                          static_cast<unsigned>(divideUp(args.heads, kStatsHeads)));
-    attentionStatsKernel<T><<<stats_grid, kGradientThreads, 0, stream>>>(args, more);
-    ZCGVS_LAUNCH_CHECK("attention gradient");
     int status;
     switch (paddedDim(args.head_dim)) {
         case 32:
