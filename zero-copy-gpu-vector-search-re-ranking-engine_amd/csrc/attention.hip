@@ -117,9 +117,11 @@ HostPlan planAttention(const zcgvs_attention_desc& d) {
     const bool fits = group * table <= kNarrowTableFloats && d.q_rows * group < (1ll << 30);
     if (fits && (rows * group <= 16.0 || (short_blocks <= units / 2 && keys >= 512.0))) {
         const double blocks = d.kv_heads * (static_cast<double>(d.q_rows) * group / 16.0 + static_cast<double>(d.texts));
-        // two workgroups a CU, and at least two tiles for each of a workgroup's wavefronts
-        const double most = keys / (8.0 * narrowKeys(d));
-        const double splits = std::min(2.0 * static_cast<double>(units) / blocks, most);
+        // A workgroup a CU, and tiles for two of its wavefronts at least. The last of 32,000 rows, 16 heads of 128 on 4
+        // float16: 20.3 us, 25.0 with two workgroups a CU (one of which wide heads leave LDS for); of 1500 float32 13.4, 17.1
+        // with two tiles for every wavefront; of 8193 14.0, 14.0.
+        const double most = keys / (2.0 * narrowKeys(d));
+        const double splits = std::min(static_cast<double>(units) / blocks, most);
         return {AttentionShape::kNarrow, std::max(1, std::min(128, static_cast<int>(splits)))};
     }
     return {rows <= 64.0 ? AttentionShape::kShort : AttentionShape::kLong, 1};
