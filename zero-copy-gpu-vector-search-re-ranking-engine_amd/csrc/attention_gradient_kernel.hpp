@@ -480,7 +480,8 @@ __global__ __launch_bounds__(kGradientThreads, (kKeyResident<T, kDim, kBlocks, k
                     ends[side] += waveXor(ends[side], offset);
                 }
             }
-            if (lane == 0) {
+            // (without a tile of rows the sums are zeros, and no barrier stands behind the tables' clearing yet)
+            if (lane == 0 && query_begin < queries.count) {
                 bins[wave * 4][kMargin] += ends[0];
                 bins[wave * 4][2 * args.max_distance + kMargin] += ends[1];
             }
