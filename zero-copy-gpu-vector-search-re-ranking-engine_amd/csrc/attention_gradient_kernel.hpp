@@ -46,16 +46,17 @@ static __device__ const float no_row[2] = {INFINITY, 0.0f};  // p = 0
 template <typename T, int kCount>
 __device__ __forceinline__ void formScores(const ScoreForm& form, f32x4 (&s)[kCount], f32x4 (&bent)[kCount]) {
     if (form.capped) {
-        asm volatile("");  // stays a branch
+        withTanh<T>(form, [&](auto fine) {
 #pragma unroll
-        for (int b = 0; b < kCount; ++b) {
+            for (int b = 0; b < kCount; ++b) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float t = tanhOf<T>(s[b][e] * form.to_cap);
-                bent[b][e] = t * t;
-                s[b][e] = form.cap * t;
+                for (int e = 0; e < 4; ++e) {
+                    const float t = tanhOf<T, decltype(fine)::value>(s[b][e] * form.to_cap);
+                    bent[b][e] = t * t;
+                    s[b][e] = form.cap * t;
+                }
             }
-        }
+        });
     } else {
         asm volatile("");  // stays a branch
 #pragma unroll

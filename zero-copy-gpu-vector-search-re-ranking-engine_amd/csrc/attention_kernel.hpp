@@ -267,17 +267,18 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
             products(std::false_type{});
         }
         if (form.capped) {
-            asm volatile("");  // stays a branch
+            withTanh<T>(form, [&](auto fine) {
 #pragma unroll
-            for (int m = 0; m < kBlocks; ++m) {
+                for (int m = 0; m < kBlocks; ++m) {
 #pragma unroll
-                for (int b = 0; b < Tile::kKeyBlocks; ++b) {
+                    for (int b = 0; b < Tile::kKeyBlocks; ++b) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[m][b][e] = tanhOf<T>(s[m][b][e] * form.to_cap);
+                        for (int e = 0; e < 4; ++e) {
+                            s[m][b][e] = tanhOf<T, decltype(fine)::value>(s[m][b][e] * form.to_cap);
+                        }
                     }
                 }
-            }
+            });
             score_factor = form.cap;
         }
         if (form.formed && (!form.capped || in_table || args.slopes != nullptr)) {
