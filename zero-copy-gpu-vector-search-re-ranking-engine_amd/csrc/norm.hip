@@ -29,6 +29,7 @@ namespace {
 constexpr int kNormThreads = 256;
 constexpr int kNormWaves = kNormThreads / kWave;
 constexpr int kNormMaxDim = 16384;
+constexpr long long kNormMaxBlocks = (1ll << 24) - 1;  // a launch has less than 2^32 threads, of 256 a block
 
 // Values of 16 bytes, which a thread takes at a time.
 template <typename T>
@@ -98,6 +99,7 @@ struct NormArgs {
     std::int64_t residual_stride;
     const void* weight;
     long long rows;
+    long long first;  // row of the launch's first workgroup
     int dim;
     float weight_offset;
     float eps;
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(kNormThreads) void residualNormKernel(NormArgs args
     constexpr int kPack = kNormPack<T>;
     __shared__ float shared[2][kNormWaves];
     const int lane = static_cast<int>(threadIdx.x) % kThreads;
-    const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / kThreads) + threadIdx.x / kThreads;
+    const long long row = args.first + static_cast<long long>(blockIdx.x) * (blockDim.x / kThreads) + threadIdx.x / kThreads;
     if (row >= args.rows) {
         return;  // (a whole row's threads, and the whole workgroup where they share memory)
     }
@@ -504,16 +506,19 @@ int zcgvs_residual_norm(const zcgvs_norm_desc* desc, void* d_out, std::int64_t o
             // a wavefront's rows in workgroups of four, or of one where that leaves CUs without one
             const int rows_each =
                 kThreads > kWave || d.rows <= kNormWaves * static_cast<std::int64_t>(deviceComputeUnits()) ? 1 : kNormWaves;
-            const unsigned blocks = static_cast<unsigned>((d.rows + rows_each - 1) / rows_each);
             const unsigned block_threads = static_cast<unsigned>(rows_each * kThreads);
-            if (codes) {
-                residualNormKernel<T, std::int8_t, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
-            } else if (out_dtype == d.dtype) {
-                residualNormKernel<T, T, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
-            } else {
-                residualNormKernel<T, float, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+            for (args.first = 0; args.first < d.rows; args.first += kNormMaxBlocks * rows_each) {
+                const unsigned blocks =
+                    static_cast<unsigned>(std::min<long long>(kNormMaxBlocks, (d.rows - args.first + rows_each - 1) / rows_each));
+                if (codes) {
+                    residualNormKernel<T, std::int8_t, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+                } else if (out_dtype == d.dtype) {
+                    residualNormKernel<T, T, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+                } else {
+                    residualNormKernel<T, float, kThreads, kVectors><<<blocks, block_threads, 0, toStream(stream)>>>(args);
+                }
+                ZCGVS_LAUNCH_CHECK("residual norm");
             }
-            ZCGVS_LAUNCH_CHECK("residual norm");
             return static_cast<int>(ZCGVS_OK);
         });
     });
