@@ -13,6 +13,8 @@ namespace {
 
 constexpr int kConvertThreads = 256;
 constexpr std::size_t kMaxConvertBlocks = 65535;
+// Rows of a launch that takes four of them (a wavefront each) or more to a workgroup: a launch has less than 2^32 threads.
+constexpr int kMaxLaunchRows = 4 * ((1 << 24) - 1);
 constexpr int kConvertUnroll = 4;  // 16-byte loads in flight per lane of the elementwise conversions
 
 unsigned convertBlocks(std::size_t count) {
@@ -330,17 +332,24 @@ __global__ __launch_bounds__(256) void generateKernel(float* __restrict__ out, l
 int launchQuantizeRows(const float* src, int rows, int dim, std::int8_t* dst, float* scales,
                        hipStream_t stream) {
     const bool vectors = dim % 4 == 0 && aligned16(src) && (reinterpret_cast<std::uintptr_t>(dst) & 3u) == 0;
-    if (vectors && dim <= 256) {
-        launchQuantizeVectors<16>(src, rows, dim, dst, scales, stream);
-    } else if (vectors && dim <= 512) {
-        launchQuantizeVectors<32>(src, rows, dim, dst, scales, stream);
-    } else if (vectors && dim <= 1024) {
-        launchQuantizeVectors<64>(src, rows, dim, dst, scales, stream);
-    } else {
-        const unsigned blocks = static_cast<unsigned>((static_cast<long long>(rows) + 3) / 4);
-        quantizeAnyRowsKernel<<<blocks, kConvertThreads, 0, stream>>>(src, rows, dim, dst, scales);
+    while (rows > 0) {
+        const int part = std::min(rows, kMaxLaunchRows);
+        if (vectors && dim <= 256) {
+            launchQuantizeVectors<16>(src, part, dim, dst, scales, stream);
+        } else if (vectors && dim <= 512) {
+            launchQuantizeVectors<32>(src, part, dim, dst, scales, stream);
+        } else if (vectors && dim <= 1024) {
+            launchQuantizeVectors<64>(src, part, dim, dst, scales, stream);
+        } else {
+            const unsigned blocks = static_cast<unsigned>((static_cast<long long>(part) + 3) / 4);
+            quantizeAnyRowsKernel<<<blocks, kConvertThreads, 0, stream>>>(src, part, dim, dst, scales);
+        }
+        ZCGVS_LAUNCH_CHECK("quantize rows");
+        src += static_cast<std::size_t>(part) * dim;
+        dst += static_cast<std::size_t>(part) * dim;
+        scales += part;
+        rows -= part;
     }
-    ZCGVS_LAUNCH_CHECK("quantize rows");
     return ZCGVS_OK;
 }
 
@@ -429,12 +438,11 @@ int zcgvs_generate_normalized(float* d_out, std::int64_t rows, int dim, std::uin
     if (d_out == nullptr) {
         return setError(ZCGVS_ERR_INVALID_ARGUMENT, "zcgvs generate: null device pointer");
     }
-    const long long blocks = (rows + 3) / 4;
-    if (blocks > 0x7FFFFFFFLL) {
-        return setError(ZCGVS_ERR_INVALID_ARGUMENT, "zcgvs generate: too many rows per call");
+    for (std::int64_t first = 0; first < rows; first += kMaxLaunchRows) {
+        const std::int64_t part = std::min<std::int64_t>(rows - first, kMaxLaunchRows);
+        generateKernel<<<static_cast<unsigned>((part + 3) / 4), 256, 0, toStream(stream)>>>(
+            d_out + first * dim, part, dim, seed, row_offset + first);
     }
-    generateKernel<<<static_cast<unsigned>(blocks), 256, 0, toStream(stream)>>>(
-        d_out, rows, dim, seed, row_offset);
     ZCGVS_LAUNCH_CHECK("generate");
     return clearError();
 }
