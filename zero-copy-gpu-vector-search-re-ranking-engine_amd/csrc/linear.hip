@@ -32,8 +32,6 @@ int linearWaveRows(const LinearPlan& plan, int dtype, std::int64_t rows) {
 
 namespace {
 
-constexpr int kMaxCodes = 131072;  // 127 * 127 of them stay below 2^31
-
 // Column sums of a matrix [rows, columns]: workgroup (c, p) those of columns 32 c on and every kSumChunks-th stretch of
 // rows, to partials [kSumChunks, columns].
 constexpr int kSumColumns = 32;

@@ -56,6 +56,7 @@ struct ProductArgs {
     std::int64_t out_stride;
 };
 
+constexpr int kMaxCodes = 131072;  // of an int8 row: products of -128 add up to 2^31 (exactSum)
 constexpr int kThinStageBytes = 1024;  // of k that a workgroup of the kernel for few rows takes at a time
 constexpr int kThinMostRows = 4096;
 

@@ -97,6 +97,15 @@ __device__ __forceinline__ void storeResult(const LinearArgs& args, const f32x4&
     }
 }
 
+// kMaxCodes products of -128 and -128 are 2^31, which wraps to -2^31; no other codes give that (-128 times 127 is more). The
+// integer below 2^31 is the same float32.
+__device__ __forceinline__ void exactSum(i32x4& sum) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        sum[e] = sum[e] == INT32_MIN ? INT32_MAX : sum[e];
+    }
+}
+
 // z of four neighbouring columns n of row m from their sum of products.
 template <typename T, typename Sum>
 __device__ __forceinline__ f32x4 beforeActivation(const Sum& sum, float x_scale, const f32x4& weight_scales,
@@ -141,6 +150,17 @@ __global__ __launch_bounds__(Tile::kThreads) void linearKernel(LinearArgs args) 
                 begin(index + static_cast<int>(gridDim.x));
             }
         });
+        if constexpr (std::is_same_v<T, std::int8_t>) {
+            if (args.dim == kMaxCodes) {
+#pragma unroll
+                for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+                    for (int j = 0; j < Tile::kBlocksN; ++j) {
+                        exactSum(sums[i][j]);
+                    }
+                }
+            }
+        }
         int tile_m, tile_n;
         tileOf(index, args.tiles_m, args.tiles_n, tile_m, tile_n);
         const int m0 = tile_m * Tile::kM + Tile::waveM() * Tile::kBlocksM * 16 + (lane & 15);
@@ -346,9 +366,19 @@ __global__ __launch_bounds__(kThinThreads) void linearThinKernel(LinearArgs args
     }
     // wavefront i joins and finishes the rows of block i
     Sum sum = shared[0][wave][lane];
+    if constexpr (std::is_same_v<T, std::int8_t>) {
+        u32x4 wrapping = __builtin_bit_cast(u32x4, sum);
 #pragma unroll
-    for (int w = 1; w < kThinWaves; ++w) {
-        sum += shared[w][wave][lane];
+        for (int w = 1; w < kThinWaves; ++w) {
+            wrapping += __builtin_bit_cast(u32x4, shared[w][wave][lane]);
+        }
+        sum = __builtin_bit_cast(Sum, wrapping);
+        exactSum(sum);
+    } else {
+#pragma unroll
+        for (int w = 1; w < kThinWaves; ++w) {
+            sum += shared[w][wave][lane];
+        }
     }
     const int m = m0 + wave * 16 + r16;
     const int n = n0 + 4 * h;
