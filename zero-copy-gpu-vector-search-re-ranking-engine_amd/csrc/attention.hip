@@ -18,8 +18,6 @@ int attentionInvalid(const char* message) {
 
 namespace {
 
-constexpr int kNarrowTableFloats = 4096;  // of the heads' tables that the narrow shape holds in LDS
-
 int checkAttention(const zcgvs_attention_desc* desc) {
     if (desc == nullptr) {
         return attentionInvalid("null descriptor");
@@ -94,12 +92,6 @@ AttentionArgs attentionArgs(const zcgvs_attention_desc& d) {
     return args;
 }
 
-// Keys of a tile of the narrow shape.
-int narrowKeys(const zcgvs_attention_desc& d) {
-    const int bytes = paddedDim(d.head_dim) * elementBytes(d.dtype);
-    return bytes <= 64 ? 64 : bytes <= 128 || d.dtype != ZCGVS_DTYPE_F32 ? 32 : 16;
-}
-
 struct HostPlan {
     AttentionShape shape;
     int splits;
@@ -113,14 +105,15 @@ HostPlan planAttention(const zcgvs_attention_desc& d) {
     const double rows = static_cast<double>(d.q_rows) / static_cast<double>(d.texts);
     const double keys = static_cast<double>(d.k_rows) / static_cast<double>(d.texts);
     const double short_blocks = d.heads * (static_cast<double>(d.q_rows) / 64.0 + static_cast<double>(d.texts));
-    const long long table = d.distance_bias == nullptr ? 0 : 2ll * (d.max_distance + narrowKeys(d) + 16) + 1;
-    const bool fits = group * table <= kNarrowTableFloats && d.q_rows * group < (1ll << 30);
+    const int tile_keys = narrowKeys(paddedDim(d.head_dim), elementBytes(d.dtype));
+    const long long table = d.distance_bias == nullptr ? 0 : biasTableWidth(d.max_distance, tile_keys + kNarrowRows);
+    const bool fits = group * table <= kNarrowTable && d.q_rows * group < (1ll << 30);
     if (fits && (rows * group <= 16.0 || (short_blocks <= units / 2 && keys >= 512.0))) {
         const double blocks = d.kv_heads * (static_cast<double>(d.q_rows) * group / 16.0 + static_cast<double>(d.texts));
         // A workgroup a CU, and tiles for two of its wavefronts at least. The last of 32,000 rows, 16 heads of 128 on 4
         // float16: 20.3 us, 25.0 with two workgroups a CU (one of which wide heads leave LDS for); of 1500 float32 13.4, 17.1
         // with two tiles for every wavefront; of 8193 14.0, 14.0.
-        const double most = keys / (2.0 * narrowKeys(d));
+        const double most = keys / (2.0 * tile_keys);
         const double splits = std::min(static_cast<double>(units) / blocks, most);
         return {AttentionShape::kNarrow, std::max(1, std::min(128, static_cast<int>(splits)))};
     }

@@ -110,12 +110,14 @@ int attentionInvalid(const char* message);
 // The head's width in LDS and registers: zeros fill it up.
 inline int paddedDim(int head_dim) { return head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : 128; }
 
-// Keys of a wavefront's tile in the narrow shape: those of 4 KB, but whole turned fragments of them and at most 64.
-template <typename T, int kDim>
-constexpr int kNarrowKeys = kDim * static_cast<int>(sizeof(T)) <= 64    ? 64
-                            : kDim * static_cast<int>(sizeof(T)) <= 128 ? 32
-                            : sizeof(T) == 2                            ? 32
-                                                                        : 16;
+// The narrow shape: keys of a wavefront's tile, those of 4 KB, but whole turned fragments of them and at most 64; floats of the
+// tables of a key head's query heads that LDS holds, each with a margin on either side.
+constexpr int narrowKeys(int padded_dim, int element_bytes) {
+    return padded_dim * element_bytes <= 64 ? 64 : padded_dim * element_bytes <= 128 || element_bytes == 2 ? 32 : 16;
+}
+constexpr int kNarrowRows = 16;
+constexpr int kNarrowTable = 4096;
+constexpr int biasTableWidth(int max_distance, int margin) { return 2 * (max_distance + margin) + 1; }
 
 namespace {
 

@@ -33,18 +33,18 @@ namespace {
 
 constexpr int kAttentionWaves = 4;
 constexpr int kAttentionThreads = kAttentionWaves * kWave;
-constexpr int kNarrowTable = 4096;  // floats of the heads' tables that the narrow shape holds
 
 template <typename T, int kDim, int kBlocks, bool kNarrow>
 struct AttentionTile {
-    static constexpr int kTileKeys = kNarrow ? kNarrowKeys<T, kDim> : sizeof(T) == 2 ? 64 : 32;
+    static constexpr int kTileKeys = kNarrow ? narrowKeys(kDim, sizeof(T)) : sizeof(T) == 2 ? 64 : 32;
     static constexpr int kTeam = kNarrow ? kWave : kAttentionThreads;
     static constexpr int kWaveRows = 16 * kBlocks;
     static constexpr int kRows = kNarrow ? kWaveRows : kWaveRows * kAttentionWaves;
     static constexpr int kKeyBlocks = kTileKeys / 16;
     // distances past the table's ends that a tile which reaches into it can hold, on either side
     static constexpr int kMargin = kTileKeys + kWaveRows;
-    static constexpr int kTableFloats = kNarrow ? kNarrowTable : 2 * (kAttentionMaxDistance + kMargin) + 1;
+    static constexpr int kTableFloats = kNarrow ? kNarrowTable : biasTableWidth(kAttentionMaxDistance, kMargin);
+    static_assert(!kNarrow || kWaveRows == kNarrowRows, "the margin that attention.hip plans with");
 };
 
 // Wavefronts of a SIMD: two, for which the registers of all but wide float32 rows do. The bound also keeps the sums in
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(kAttentionThreads, (kAttentionResident<T, kDim, kBl
         slope[m] = args.slopes != nullptr && valid[m] ? form.bias_factor * args.slopes[head[m]] : 0.0f;
     }
     // the tables with kMargin copies of their end values on either side
-    const int table_width = 2 * (args.max_distance + Tile::kMargin) + 1;
+    const int table_width = biasTableWidth(args.max_distance, Tile::kMargin);
     if (args.table != nullptr) {
         const T* from = static_cast<const T*>(args.table) +
                         static_cast<std::int64_t>(unit * group) * (2 * args.max_distance + 1);
