@@ -36,8 +36,17 @@ class EncoderBlocks:
         final_norm = _matrix("final_norm", final_norm, (None,), element)
         self.dim, self.heads, self.kv_heads = final_norm.shape[0], heads, kv_heads or heads
         self.dtype, self.activation, self.eps, self.causal, self.cap = dtype, activation, eps, causal, cap
-        if self.heads < 1 or self.kv_heads < 1 or self.heads % self.kv_heads:
-            _refuse("heads must be a multiple of kv_heads")
+        if not 1 <= self.heads <= 1024 or self.kv_heads < 1 or self.heads % self.kv_heads:
+            _refuse("heads must lie in [1, 1024] and be a multiple of kv_heads")
+        limits = capi.library()
+        self._limits = dict(dim=limits.zcgvs_residual_norm_max_dim(), head_dim=limits.zcgvs_attention_max_head_dim(),
+                            max_distance=limits.zcgvs_attention_max_distance())
+        if not 1 <= self.dim <= self._limits["dim"]:
+            _refuse(f"final_norm must have 1 to {self._limits['dim']} values")
+        if not (np.isfinite(eps) and eps >= 0 and np.isfinite(cap) and cap >= 0):
+            _refuse("eps and cap must be finite and at least 0")
+        if activation not in (capi.ACT_SILU, capi.ACT_GELU, capi.ACT_GELU_TANH):
+            _refuse("unknown activation")
         self.head_dim = 0
         self.blocks = [self._block(block, element) for block in blocks]
         self.final_norm = capi.DeviceArray.from_host(final_norm)
@@ -57,6 +66,8 @@ class EncoderBlocks:
         if self.head_dim and out.shape[1] != self.heads * self.head_dim:
             _refuse("all blocks must have one head_dim")
         self.head_dim = out.shape[1] // self.heads
+        if self.head_dim > self._limits["head_dim"]:
+            _refuse(f"heads hold at most {self._limits['head_dim']} values, not {self.head_dim}")
         wide = (self.heads + 2 * self.kv_heads) * self.head_dim
         hidden = _matrix("a block's gate", block["gate"], (None, self.dim), element).shape[0]
         shapes = dict(norm1=(self.dim,), norm2=(self.dim,), qkv=(wide, self.dim), out=out.shape, gate=(hidden, self.dim),
@@ -65,6 +76,8 @@ class EncoderBlocks:
                 for name, values in block.items() if values is not None}
         if "distance_bias" in held and held["distance_bias"].shape[1] % 2 == 0:
             _refuse("distance_bias must have 2 max_distance + 1 columns")
+        if "distance_bias" in held and held["distance_bias"].shape[1] // 2 > self._limits["max_distance"]:
+            _refuse(f"distance_bias reaches to distances of at most {self._limits['max_distance']}")
         return {name: capi.DeviceArray.from_host(values) for name, values in held.items()}
 
     def _attention_desc(self, block, qkv, offsets, texts, tokens):
