@@ -99,3 +99,13 @@ def test_scores_of_zero_under_any_cap(gpu, kind, cap):
     allowed = 2 * (UNIT[kind] + 48 * STEP) * np.abs(from_bits(v, kind)).mean(0)
     assert np.all(np.abs(from_bits(out.to_host(), kind) - mean) <= allowed)
     assert np.allclose(lse.to_host(), np.log(rows), rtol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("mask", ["full", "causal"])
+def test_one_long_text_among_short_ones(gpu, kind, mask):
+    """The kernel for few rows is chosen by the mean of a text's rows: it takes a long text as well."""
+    b = Batch(gpu, kind, [1] * 40 + [700] + [0, 2] * 30, heads=2, head_dim=64, mask=mask, bias="table", far=9)
+    assert b.q_rows / b.texts <= 16
+    forward(b)
+    check(b)
