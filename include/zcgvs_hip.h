@@ -666,8 +666,10 @@ enum zcgvs_attention_align { ZCGVS_ATTENTION_FIRST = 0, ZCGVS_ATTENTION_LAST = 1
  * their output rows are zeros, and so are the gradients of padding rows. Rows of no text (before the first
  * offset, behind the last) are neither read nor written. Likewise for the keys.
  * Padding rows, rows of no text and other texts may hold anything, infinities and NaN included. A key of the
- * row's own text that only the causal mask hides must be finite, as must the queries that do not see a key
- * for that key's gradient. */
+ * row's own text that only the causal mask or a bias hides must be finite, as must the queries that do not see
+ * a key for that key's gradient.
+ * A call may take (q_rows / 64 + 2 * texts) * heads workgroups, its gradient also (k_rows / 64 + texts) * kv_heads:
+ * calls that need 2^24 of either are refused. */
 typedef struct zcgvs_attention_desc {
     const void* q;             /* [q_rows, heads, head_dim]                                     */
     int64_t q_stride;          /* elements from row to row; 0: heads * head_dim                 */
@@ -690,7 +692,7 @@ typedef struct zcgvs_attention_desc {
     int causal;
     const int* prefix_lengths; /* [texts] (causal), or NULL                                     */
     float scale;               /* finite                                                        */
-    float cap;                 /* 0: none                                                       */
+    float cap;                 /* 0: none. 16-bit: c within 2^-21 cap up to caps of 64, 2^-19 c above */
     const float* slopes;       /* [heads], or NULL: none                                        */
     const void* distance_bias; /* [heads, 2 * max_distance + 1], or NULL: none                  */
     int max_distance;          /* at most zcgvs_attention_max_distance()                        */
@@ -709,8 +711,9 @@ int zcgvs_attention(const zcgvs_attention_desc* desc, void* d_out, int64_t out_s
 /* The gradient of zcgvs_attention from that of its output, with what the forward call wrote (d_out with
  * out_stride, d_lse). q_gradient, k_gradient and v_gradient have the shapes of q, k and v and desc->dtype;
  * distance_bias_gradient (NULL: not wanted) that of distance_bias and desc->dtype. The softmax and its
- * gradient are rounded to desc->dtype between the products (float16: to an infinity beyond 65504, so scale
- * the loss as for stored tensors). A stride of 0 is the row's length. */
+ * gradient are rounded to desc->dtype between the products (float16: to an infinity beyond 65504 and to
+ * multiples of 2^-24 below 2^-14, so scale the loss as for stored tensors; probabilities over more than 2^14
+ * keys lose bits). A stride of 0 is the row's length. */
 size_t zcgvs_attention_gradient_workspace_bytes(const zcgvs_attention_desc* desc);
 int zcgvs_attention_gradient(const zcgvs_attention_desc* desc, const void* d_out, int64_t out_stride,
                              const float* d_lse, const void* d_out_gradient, int64_t out_gradient_stride,

@@ -38,3 +38,13 @@ def test_rows_wider_than_the_norm_takes(capi, with_blocks):  # noqa: F811
 def test_the_largest_are_taken(capi, with_blocks):  # noqa: F811
     _encoder(capi, _block(**_heads(128), distance_bias=np.ones((4, 1025), np.float32)), cap=50.0, eps=0.0,
              activation=capi.ACT_GELU)
+
+
+@pytest.mark.parametrize("texts,rows,heads", [(1 << 24, 1 << 24, 1), (1, 1 << 28, 1024)])
+def test_attention_of_more_workgroups_than_a_launch_takes(capi, texts, rows, heads):
+    at = 1 << 20  # an address that nothing reads here
+    desc = capi.attention_desc(at, at, at, texts, rows, rows, heads, 8, capi.F16)
+    with pytest.raises(ValueError, match="more texts and rows than one launch"):
+        capi.attention(desc, at, at, 1 << 50)
+    with pytest.raises(ValueError, match="more texts and rows than one launch"):
+        capi.attention_gradient(desc, at, at, at, at, at, at, at, 1 << 60)

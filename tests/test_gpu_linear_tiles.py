@@ -18,3 +18,9 @@ def test_int8(gpu, act):
 def test_projection_and_gradient(gpu, kind, act):
     linear.test_projection(gpu, (kind, 2050, 64, 4096, act, 0, 0), False)
     linear.test_gradient(gpu, (kind, 2050, 64, 4096, act, 0, 0))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_gradient_on_the_widest(gpu, kind, act):
+    linear.test_gradient(gpu, (kind, 4200, 64, 3000, act, 0, 0))

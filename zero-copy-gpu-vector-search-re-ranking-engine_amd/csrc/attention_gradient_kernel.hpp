@@ -7,7 +7,7 @@
 // Two launches (one more each with the bias's gradient and with few keys), no atomics between workgroups: the same bits on
 // every call.
 // 1. dq: a wavefront keeps 16 or 32 query rows and goes through the keys, as the forward kernel does. Before, it forms delta
-//    and the rows' lse in base 2, for itself and the second launch (in a launch of their own 392 us instead of the 376 below).
+//    and the rows' lse in base 2, for itself and the second launch (in a launch of their own 16 us more than the 378 below).
 // 2. dk and dv: a wavefront keeps 16 or 32 keys and their values in registers and goes through the queries of all heads of
 //    its key head, in LDS tiles of 32 rows that the workgroup shares. Scores come out with a lane's four neighbouring query
 //    rows of one key, which is how the products over the rows take p and dr: they stay in registers.
@@ -18,9 +18,13 @@
 // additions is the program's), with room for distances past the table's ends; tiles that lie past them altogether add
 // to two registers. A workgroup joins its tables and writes
 // one of partial sums a head, which the last launch adds in the order of the workgroups.
-// Bound by the vector units (exponentials, the bias's sums) beside seven products. Measured, bfloat16: 128 texts of 64 to 512, 12 heads
-// of 64, a learned bias and its gradient 376 us (queries 147, keys 257 under the profiler); 8 texts of 4096, 8 heads of 64 on 2
-// 1035 us, of 128 2055. 3 texts of 20 to 77 float32, 6 heads of 32 on 2 24.5 us (the launches).
+// 16-bit p and dr are rounded for the products over them, whose matrix instructions take 16-bit operands; the bias's gradient
+// is the sum of the unrounded ds.
+// Bound by waits: wavefronts, about two of them on a SIMD, stand half of their time at tiles whose copies were started one tile
+// before. Counted for the 128 texts below, of all SIMD cycles: keys 36% vector and 14% matrix instructions, 1.6 wavefronts a SIMD;
+// queries 46%, 19% and 2.3. Measured, bfloat16: 128 texts of 64 to 512, 12 heads of 64, a learned bias and its gradient 378-380 us
+// (queries 149, keys 253 under the profiler), without a bias 321, float32 1963; 8 texts of 4096, 8 heads of 64 on 2 1046 us,
+// of 128 2070. 3 texts of 20 to 77 float32, 6 heads of 32 on 2 23.5-24.5 us (the launches).
 #pragma once
 
 #include <hip/hip_runtime.h>

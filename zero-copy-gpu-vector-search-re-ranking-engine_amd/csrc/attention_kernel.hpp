@@ -15,12 +15,16 @@
 // read once; the four wavefronts take every fourth tile each, from LDS of their own without a barrier, and the keys
 // may be split over workgroups as well. The parts are joined by their maxima and sums.
 //
-// Bound: per score of a 64-wide head 1/2 matrix instruction cycle against about one cycle of vector work (of which the
-// exponential is more than half), so by the vector units up to heads of 64 and by both at 128; the narrow shape by reading the
-// keys once.
-// Measured, bfloat16: 128 texts of 64 to 1024 tokens, 12 heads of 64, a learned bias 266-300 us (500-550 TFLOP/s of the pairs' four
-// products' operations); 8 texts of 4096, 8 heads of 64 350 us (785), of 128 570 (965). The last of 8193 rows, 16 heads of 128 on 4
-// float16 13.2 us (17 MB of keys, two launches).
+// 16-bit exponentials are rounded for the product with v, since its matrix instructions take 16-bit operands (float32 ones have
+// a sixteenth of their rate); their sum is that of the unrounded ones.
+//
+// Bound: by the vector units' issue up to heads of 64. Counted for heads of 64, SIMD cycles a score: over 8 texts of 4096 vector
+// instructions 0.59 (76% of all cycles) and matrix instructions 0.25 of 0.77; over texts of 64 to 1024 with a learned bias 0.77
+// (67%) and 0.27 of 1.15, wavefronts waiting a third of their time. The narrow shape by reading the keys once.
+// Measured, bfloat16: 128 texts of 64 to 1024 tokens, 12 heads of 64, a learned bias 271-281 us (520-540 TFLOP/s of the pairs' four
+// products' operations), without it 259, float32 1452; 8 texts of 4096, 8 heads of 64 346 us (790), of 80 and 96 (padded to 128)
+// 541 and 550, of 128 580 (950), float32 of 64 2240. The last of 8193 rows, 16 heads of 128 on 4 float16 13.4 us (17 MB of keys,
+// two launches).
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -11,9 +11,9 @@
 // rows, its eight wavefronts every eighth 128 bytes of k, straight from memory into registers, and joins their sums
 // through LDS. No LDS stages, no splits over workgroups, one launch.
 //
-// Measured: one row 768 -> 768 float16 6.6 us (the launch); 8192 rows 1024 -> 4096 int8, GELU by tanh 55-58 us (1.2 POP/s), bfloat16
-// 84-87 (0.8 PFLOP/s); 8192 cubed bfloat16 1015 us (1.08 PFLOP/s, a library product 1.45); the gradient of 16,384 rows 768 -> 2048
-// bfloat16 216 us (dz 91, dW 66, dx 55, joins 8). Bound by the product loop, dz also by its loads and stores between the
+// Measured: one row 768 -> 768 float16 6.6 us (the launch); 8192 rows 1024 -> 4096 int8, GELU by tanh 60-68 us (1.0-1.1 POP/s), bfloat16
+// 84-95 (0.7-0.8 PFLOP/s); 8192 cubed bfloat16 1015-1034 us (1.07 PFLOP/s, a library product 1.45); the gradient of 16,384 rows
+// 768 -> 2048 bfloat16 216-222 us (dz 91, dW 66, dx 55, joins 8). Bound by the product loop, dz also by its loads and stores between the
 // tiles' products.
 #pragma once
 
